@@ -79,7 +79,9 @@ void mmhip_destroy(mmhip_ctx* ctx);
  * a failed grid-wide wait of an earlier one-launch MoE decode
  * (mmhip_moe_ffn_dev): MMHIP_ERR_HIP with the reason, once, and the status
  * is cleared. A caller that synchronises the raw stream from mmhip_stream()
- * instead never sees that error. */
+ * instead never sees that error. Then it reports, as MMHIP_ERR_INVALID and
+ * once, what a call of the operators between the products (below) met in
+ * device data. */
 int mmhip_synchronize(mmhip_ctx* ctx);
 /* The context's hipStream_t, as an opaque pointer. */
 void* mmhip_stream(mmhip_ctx* ctx);
@@ -90,7 +92,7 @@ int mmhip_num_cu(mmhip_ctx* ctx);
  * stream around every launch of the hot kernels; mmhip_profile_read sums
  * them per kernel family ("gemv_q", "gemv_float", "qmm", "quantize",
  * "moe_router", "moe_route", "moe_quantize", "moe_gateup", "moe_down", "moe_decode",
- * "moe_combine"). This fills the role
+ * "moe_combine", "rms_norm", "rope", "kv_store", "attention", "logprobs"). This fills the role
  * of the per-op GPU timings the reference leaves empty
  * (op_perf_db.zig:88-97). Enabling resets the accumulators. */
 int mmhip_profile_enable(mmhip_ctx* ctx, int enable);
@@ -314,6 +316,185 @@ int mmhip_qmm_dev(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat,
 int mmhip_qmm_dev_noalloc(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat,
                           const float* x_dev, float* y_dev, uint64_t batch,
                           int out_layout);
+
+/* ======================================================================
+ * Between the products of a decode step: the norms, rotary positions, the
+ * paged latent key-value cache, its attention, and log probabilities. They
+ * take the place of math.rmsNorm (src/math.zig:7-35), RoPECache
+ * (src/math.zig:197-240), KVCache.put (src/kv_cache.zig:279-362) and the
+ * cached part of mlaAttention / mlaAttentionBatch (src/inference.zig:456-883)
+ * on device buffers, so that hidden states, the cache and the logits stay on
+ * the device from one product to the next.
+ *
+ * All of them are asynchronous on mmhip_stream(ctx), allocate nothing and
+ * can be captured into a HIP graph. Where a workspace is needed the caller
+ * gives it, for as long as the work may run: two calls (or two graphs) that
+ * can run at the same time need one each. Arguments are checked before the
+ * context is. What only the device can see (slots, page numbers, lengths,
+ * positions, tokens) is bounds-checked there and never read or written out
+ * of bounds; where it is wrong, the next mmhip_synchronize returns
+ * MMHIP_ERR_INVALID and says what was met, once (the last, of several).
+ * ====================================================================== */
+
+/* Root-mean-square norm of n_rows rows of cols values, with a residual added
+ * first:
+ *     s = x + residual                      (s = x where residual_dev is NULL)
+ *     y = (s * r) * weight,  r = 1 / sqrt(mean(s^2) + eps)
+ * s and the two products are f32 operations; the sum of squares and r are
+ * computed in 64 bits and r is rounded to f32 once, so a row's result does not
+ * depend on how its sum was split. sum_dev (NULL: not wanted) receives s, the
+ * next residual. y_type: MMHIP_TYPE_F32, MMHIP_TYPE_F16 (rounded to nearest
+ * even), or MMHIP_TYPE_Q8_0 (ceil(cols / 32) blocks of 34 bytes per row, the
+ * rows back to back, each block as mmhip_quantize_q8_0 gives it; y_dev 2-byte
+ * aligned, y_stride unused). Strides in elements, at least cols.
+ * Each output may be one of the inputs themselves (same address and stride,
+ * f32), but y_dev and sum_dev must differ; buffers must not overlap
+ * otherwise. eps >= 0; a row of zeros with eps = 0 gives NaN. */
+int mmhip_rms_norm_dev(mmhip_ctx* ctx, void* y_dev, uint32_t y_type, uint64_t y_stride, float* sum_dev,
+                       uint64_t sum_stride, const float* x_dev, uint64_t x_stride, const float* residual_dev,
+                       uint64_t residual_stride, const float* weight_dev, uint64_t n_rows, uint32_t cols, float eps);
+
+/* Rotary positions. Pair i < dims / 2 of a head's rotated dims is turned by
+ * the angle position * f_i:
+ *     (a, b) -> (a cos - b sin, a sin + b cos) * magnitude
+ * with f_i = base^(-2 i / dims), scaled for long contexts:
+ *   MMHIP_ROPE_LINEAR  f_i / factor;
+ *   MMHIP_ROPE_YARN    f_i (1 - r_i) + f_i / factor * r_i, where r_i rises from
+ *                      0 at pair low to 1 at pair high: at(n) = dims
+ *                      ln(original_context / (2 pi n)) / (2 ln base), low =
+ *                      floor(at(beta_fast)) and high = ceil(at(beta_slow)),
+ *                      both kept within [0, dims - 1].
+ * magnitude 0 stands for 0.1 ln(factor) + 1 with YaRN and for 1 otherwise.
+ * Angles are reduced in 64 bits, so positions up to 2^32 - 1 keep an angle
+ * error below 2e-6 (below 1e-9 up to 2^20); cosines and sines are rounded to
+ * f32 once, and the products and sums are f32 operations. */
+#define MMHIP_ROPE_INTERLEAVED 0u /* pair i: dims 2 i and 2 i + 1 */
+#define MMHIP_ROPE_HALF 1u        /* pair i: dims i and i + dims / 2 */
+#define MMHIP_ROPE_NONE 0u
+#define MMHIP_ROPE_LINEAR 1u
+#define MMHIP_ROPE_YARN 2u
+#define MMHIP_ROPE_MAX_DIMS 256u
+typedef struct {
+    uint32_t dims;             /* even, 2..MMHIP_ROPE_MAX_DIMS */
+    uint32_t layout;           /* MMHIP_ROPE_INTERLEAVED or MMHIP_ROPE_HALF */
+    uint32_t scaling;          /* MMHIP_ROPE_NONE, _LINEAR or _YARN */
+    uint32_t original_context; /* YaRN: positions the model was trained on */
+    float base;                /* > 1 */
+    float factor;              /* linear, YaRN: > 0 */
+    float beta_fast, beta_slow; /* YaRN: turns over original_context, > 0 */
+    float magnitude;
+} mmhip_rope_params;
+typedef struct mmhip_rope mmhip_rope;
+int mmhip_rope_create(mmhip_ctx* ctx, const mmhip_rope_params* params, mmhip_rope** out_rope);
+void mmhip_rope_destroy(mmhip_ctx* ctx, mmhip_rope* rope);
+/* The frequency of each pair in radians per position (dims / 2 values) and the
+ * magnitude, from the parameters alone: no device needed. */
+int mmhip_rope_frequencies(const mmhip_rope_params* params, double* out, double* magnitude);
+/* x [n_tokens][n_heads][head_dim] -> y, dims [first, first + rope.dims) of
+ * every head turned by its token's position and the others copied. Strides in
+ * floats (head strides at least head_dim). y_dev may be x_dev with the same
+ * strides (the other dims are then left alone); otherwise the two must not
+ * overlap. */
+int mmhip_rope_dev(mmhip_ctx* ctx, const mmhip_rope* rope, float* y_dev, uint64_t y_token_stride,
+                   uint64_t y_head_stride, const float* x_dev, uint64_t x_token_stride, uint64_t x_head_stride,
+                   const uint32_t* positions_dev, uint64_t n_tokens, uint32_t n_heads, uint32_t head_dim,
+                   uint32_t first);
+
+/* A layer's paged latent cache (KVCache's blocks, src/kv_cache.zig:14-140) in
+ * a pool that the caller owns. A position's row holds rank latent values and
+ * rope_dims rotary ones. Pages hold page_tokens rows:
+ *   MMHIP_TYPE_F16   [page_tokens][rank + rope_dims] f16;
+ *   MMHIP_TYPE_Q8_0  [page_tokens][rank + rope_dims] i8 codes, then
+ *                    [page_tokens][(rank + rope_dims) / 32] f16 scales: the
+ *                    codes and scales of mmhip_quantize_q8_0's blocks, kept
+ *                    apart so that codes are read 16 bytes at a time.
+ * rank is a multiple of 32 up to MMHIP_KV_MAX_RANK, rope_dims one up to
+ * MMHIP_KV_MAX_ROPE (or 0), page_tokens a power of two from 16 to 1024,
+ * n_pages * page_tokens below 2^31; pool_dev is 16-byte aligned. */
+#define MMHIP_KV_MAX_RANK 512u
+#define MMHIP_KV_MAX_ROPE 64u
+typedef struct {
+    void* pool_dev;
+    uint32_t type; /* MMHIP_TYPE_F16 or MMHIP_TYPE_Q8_0 */
+    uint32_t rank, rope_dims;
+    uint32_t page_tokens, n_pages;
+} mmhip_kv_cache;
+/* Bytes of one page (the pool holds n_pages of them); 0 if the cache's type
+ * or sizes are not supported. pool_dev is not looked at. */
+uint64_t mmhip_kv_page_bytes(const mmhip_kv_cache* cache);
+/* Writes n_tokens positions: kv_dev rows of rank + rope_dims floats (the
+ * kv_a projection's output, kv_stride floats apart) -> row slots[t] of the
+ * pool (page slots[t] / page_tokens). The latent part is normed with
+ * norm_weight_dev [rank] and eps as mmhip_rms_norm_dev does (NULL: stored as
+ * it is), the rotary part turned by positions_dev[t] as mmhip_rope_dev does
+ * (rope NULL: stored as it is, positions unused; else rope.dims = rope_dims).
+ * A negative slot skips its token. Slots of one call must differ: a row named
+ * twice ends with some values of either token. Values beyond f16's range
+ * become infinities in an F16 cache. */
+int mmhip_kv_store_dev(mmhip_ctx* ctx, const mmhip_kv_cache* cache, const float* kv_dev, uint64_t kv_stride,
+                       const float* norm_weight_dev, float eps, const mmhip_rope* rope, const uint32_t* positions_dev,
+                       const int32_t* slots_dev, uint64_t n_tokens);
+
+/* Attention of single tokens over the paged latent cache, in the latent space
+ * (k_b folded into the query, v_b applied to the result):
+ *     score_p = scale * (q . latent_p + q_pe . pe_p)   p < lens[t]
+ *     out     = sum_p softmax(score)_p * latent_p
+ *     lse     = ln(sum_p exp(score_p))
+ * for each token t and head. Token t reads row table_of[t] (t where
+ * table_of_dev is NULL) of the page tables: position p lies in page
+ * tables[row][p / page_tokens], at row p % page_tokens. A prompt's chunk is
+ * one table with lens[t] = position + 1. lens[t] = 0 gives out = 0 and lse =
+ * -infinity. Rows of the last page behind the length may hold anything, NaN
+ * too. A length beyond the table's pages is cut there, a page number that the
+ * pool does not have is left out like a masked one, and a row number that the
+ * tables do not have counts as length 0; each is reported (above).
+ * Scores, softmax statistics and sums are f32; queries and probabilities enter
+ * the matrix cores as two f16 parts each (22 bits), cached values exactly.
+ * Queries beyond 1e30 in size or not finite give NaN. The work is split
+ * over the positions and joined, in an order that depends on the call's
+ * shape and lengths alone, so a call repeated gives the same bits. */
+typedef struct {
+    mmhip_kv_cache cache;
+    const float* q_dev;      /* [n_tokens][n_heads][rank] */
+    const float* q_pe_dev;   /* [n_tokens][n_heads][rope_dims]; unused where rope_dims = 0 */
+    float* out_dev;          /* [n_tokens][n_heads][rank] */
+    float* lse_dev;          /* [n_tokens][n_heads], contiguous; NULL: not wanted */
+    uint64_t q_token_stride, q_head_stride;       /* in floats */
+    uint64_t q_pe_token_stride, q_pe_head_stride;
+    uint64_t out_token_stride, out_head_stride;
+    const int32_t* tables_dev;     /* [n_tables][table_stride], table_pages of each used */
+    uint64_t table_stride;
+    uint32_t n_tables, table_pages;
+    const uint32_t* table_of_dev;  /* [n_tokens] or NULL */
+    const uint32_t* lens_dev;      /* [n_tokens] */
+    uint32_t n_tokens, n_heads;
+    float scale;
+    void* workspace_dev;           /* 16-byte aligned */
+    uint64_t workspace_bytes;      /* at least mmhip_mla_attention_workspace */
+} mmhip_mla_attention;
+uint64_t mmhip_mla_attention_workspace(mmhip_ctx* ctx, uint32_t n_tokens, uint32_t n_heads, uint32_t rank);
+int mmhip_mla_attention_dev(mmhip_ctx* ctx, const mmhip_mla_attention* args);
+
+/* Log probabilities of each row's logits (computeLogits' output), beside
+ * mmhip_argmax_dev:
+ *     token_logprobs[r][i] = logits[r][tokens[r][i]] - lse(logits[r])
+ *     entropy[r]           = -sum_v p_v ln p_v            (nats)
+ *     top_ids[r][j], top_logprobs[r][j]  the `top` largest logits, largest
+ *                          first, equal ones by the lower id
+ * Masked logits (-infinity) have probability 0. A row that holds a NaN, a
+ * +infinity, or nothing but -infinity has no probabilities: its log
+ * probabilities and entropy are NaN; its ids still follow the logits, NaN
+ * after every number. A token outside the vocabulary gets NaN and is
+ * reported (above). n_given may be 0 (tokens and their outputs unused), and
+ * so may top (ids and log probabilities unused; top_logprobs_dev may be NULL
+ * too); entropy_dev may be NULL. top <= MMHIP_LOGPROBS_MAX_TOP, top <= vocab,
+ * 1 <= vocab < 2^31, n_given < 2^31. Outputs are contiguous. */
+#define MMHIP_LOGPROBS_MAX_TOP 32u
+uint64_t mmhip_logprobs_workspace(mmhip_ctx* ctx, uint64_t n_rows, uint64_t vocab, uint32_t top);
+int mmhip_logprobs_dev(mmhip_ctx* ctx, const float* logits_dev, uint64_t stride, uint64_t n_rows, uint64_t vocab,
+                       const uint32_t* tokens_dev, uint64_t n_given, float* token_logprobs_dev, float* entropy_dev,
+                       uint32_t top, uint32_t* top_ids_dev, float* top_logprobs_dev, void* workspace_dev,
+                       uint64_t workspace_bytes);
 
 /* ======================================================================
  * MoE FFN layer: replaces moeFFN (src/inference.zig:886-1010) with

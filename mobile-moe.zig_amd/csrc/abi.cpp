@@ -134,7 +134,7 @@ int mmhip_init(mmhip_ctx** out_ctx, int device) {
         delete ctx;
         return hip_fail(e, "init: scratch symbol address");
     }
-    e = hipHostMalloc((void**)&ctx->status, sizeof(uint32_t), hipHostMallocDefault);
+    e = hipHostMalloc((void**)&ctx->status, 2 * sizeof(uint32_t), hipHostMallocDefault);
     if (e == hipSuccess) e = hipHostGetDevicePointer((void**)&ctx->status_dev, ctx->status, 0);
     if (e != hipSuccess) {
         if (ctx->status) (void)hipHostFree(ctx->status);
@@ -142,7 +142,7 @@ int mmhip_init(mmhip_ctx** out_ctx, int device) {
         delete ctx;
         return hip_fail(e, "init: status word");
     }
-    *ctx->status = 0;
+    ctx->status[0] = ctx->status[1] = 0;
     *out_ctx = ctx;
     return MMHIP_OK;
 }
@@ -169,7 +169,8 @@ int mmhip_synchronize(mmhip_ctx* ctx) {
     if (int rc = require_ctx(ctx)) return rc;
     hipError_t e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) return hip_fail(e, "synchronize");
-    return check_device_status(ctx, "synchronize");
+    if (int rc = check_device_status(ctx, "synchronize")) return rc;
+    return check_step_status(ctx, "synchronize");
 }
 
 void* mmhip_stream(mmhip_ctx* ctx) { return ctx ? (void*)ctx->stream : nullptr; }

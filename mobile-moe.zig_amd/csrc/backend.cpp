@@ -35,6 +35,21 @@ int check_device_status(mmhip_ctx* ctx, const char* what) {
     return MMHIP_ERR_HIP;
 }
 
+int check_step_status(mmhip_ctx* ctx, const char* what) {
+    const uint32_t st = ctx->status ? __atomic_load_n(ctx->status + 1, __ATOMIC_ACQUIRE) : 0u;
+    if (st == 0) return MMHIP_OK;
+    __atomic_store_n(ctx->status + 1, 0u, __ATOMIC_RELEASE);
+    static const char* const met[] = {"",
+                                      "kv_store: a slot that the pool does not have (its token was not stored)",
+                                      "mla_attention: a table row that does not exist (its token saw nothing)",
+                                      "mla_attention: a length beyond its table's pages (cut there)",
+                                      "mla_attention: a page that the pool does not have (left out)",
+                                      "logprobs: a token outside the vocabulary (NaN)"};
+    set_error(MMHIP_ERR_INVALID, std::string(what) + ": an earlier call met " +
+                                     (st < sizeof(met) / sizeof(met[0]) ? met[st] : "an unknown fault"));
+    return MMHIP_ERR_INVALID;
+}
+
 uint64_t block_size(uint32_t type) {
     switch (type) {
         case kF32: case kF16: return 1;

@@ -85,8 +85,11 @@ struct mmhip_ctx {
     void* noalloc = nullptr;  // this device's fixed QMM scratch (mmhip_qmm_dev_noalloc)
     // Pinned host word that device code sets when a grid-wide wait of the
     // one-launch decode MoE layer timed out (0: none); read after a sync.
+    // The second word is for what the operators between the products meet in
+    // device data (StepStatus), reported by mmhip_synchronize.
     uint32_t* status = nullptr;
     uint32_t* status_dev = nullptr;
+    uint32_t* step_status_dev() const { return status_dev + 1; }
     KernelTimer timer;
 };
 
@@ -110,6 +113,8 @@ namespace mmhip {
 // failure in the context's status word since the last check (which clears
 // it). Call after the context's stream has been synchronised.
 int check_device_status(mmhip_ctx* ctx, const char* what);
+// The same for the second word: MMHIP_ERR_INVALID.
+int check_step_status(mmhip_ctx* ctx, const char* what);
 
 // Upload helpers shared by the ABI and the MoE layer.
 int weight_create(mmhip_ctx* ctx, const void* raw, bool raw_on_device, uint32_t type, uint64_t rows,

@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "paged.hpp"
+
 namespace mmhip {
 
 enum TileFormat : uint32_t { kFmtQ8 = 0, kFmtIq2 = 1 };
@@ -335,5 +337,101 @@ uint32_t route_max_work(uint32_t n_tokens, uint32_t n_experts, uint32_t item_row
 hipError_t launch_combine(const float* eo, const int32_t* assign_slot, const float* assign_w,
                           const int32_t* shared_slot, const uint32_t* deferred, const float* bias, float* out,
                           uint32_t n_tokens, uint32_t hidden, hipStream_t s);
+
+// ---- Between the products of a decode step (norm.hip, mla.hip, logprobs.hip) ----
+
+constexpr uint32_t kRopeMaxPairs = 128, kKvMaxRank = 512, kKvMaxRope = 64, kLogprobsMaxTop = 32;
+
+// What device code met in device data (a host-visible word, 0: nothing), for
+// the next synchronisation to report.
+enum StepStatus : uint32_t { kBadSlot = 1, kBadTableRow, kBadLength, kBadPage, kBadToken };
+#if defined(__HIPCC__)
+__device__ __forceinline__ void report(uint32_t* status, uint32_t code) {
+    __hip_atomic_store(status, code, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+#endif
+
+struct NormArgs {
+    void* y;
+    uint64_t y_stride;
+    float* sum;             // or null
+    uint64_t sum_stride;
+    const float* x;
+    uint64_t x_stride;
+    const float* residual;  // or null
+    uint64_t residual_stride;
+    const float* weight;
+    uint32_t cols;
+    float eps;
+    bool vec;               // set by the launcher: 16-byte accesses fit
+};
+// out: 0 f32, 1 f16, 2 Q8_0.
+hipError_t launch_rms_norm(const NormArgs& a, uint32_t out, uint64_t n_rows, hipStream_t s);
+
+struct RopeArgs {
+    float* y;
+    const float* x;
+    uint64_t y_token_stride, y_head_stride, x_token_stride, x_head_stride;
+    const uint32_t* positions;
+    const double* turns;    // [dims / 2]: turns per position
+    double magnitude;
+    uint32_t dims, half, n_heads, head_dim, first;
+    uint32_t copy;          // 1: the other dims are copied (y is not x)
+};
+hipError_t launch_rope(const RopeArgs& a, uint64_t n_tokens, hipStream_t s);
+
+struct StoreArgs {
+    uint8_t* pool;
+    PagedGeom geom;
+    const float* kv;
+    uint64_t kv_stride;
+    const float* weight;    // or null
+    float eps;
+    const double* turns;    // or null
+    double magnitude;
+    uint32_t half;
+    const uint32_t* positions;
+    const int32_t* slots;
+    uint32_t* status;
+    bool vec;               // set by the launcher
+};
+hipError_t launch_kv_store(const StoreArgs& a, uint64_t n_tokens, hipStream_t s);
+
+struct MlaArgs {
+    const uint8_t* pool;
+    PagedGeom geom;
+    const float *q, *q_pe;
+    float *out, *lse;       // lse or null
+    uint64_t q_token_stride, q_head_stride, q_pe_token_stride, q_pe_head_stride, out_token_stride, out_head_stride;
+    const int32_t* tables;
+    uint64_t table_stride;
+    uint32_t n_tables, table_pages;
+    const uint32_t* table_of;  // or null
+    const uint32_t* lens;
+    uint32_t n_tokens, n_heads;
+    float scale;
+    void* work;
+    uint32_t* status;
+    int num_cu;
+};
+uint64_t mla_workspace_bytes(uint32_t n_tokens, uint32_t n_heads, uint32_t rank, int num_cu);
+hipError_t launch_mla(const MlaArgs& a, hipStream_t s);
+
+struct LogprobsArgs {
+    const float* logits;
+    uint64_t stride;
+    uint32_t vocab;
+    const uint32_t* tokens;
+    uint64_t n_given;
+    float* token_logprobs;
+    float* entropy;         // or null
+    uint32_t top;
+    uint32_t* top_ids;
+    float* top_logprobs;    // or null
+    void* work;
+    uint32_t* status;
+};
+uint64_t logprobs_workspace_bytes(uint64_t n_rows, uint64_t vocab, uint32_t top);
+hipError_t launch_logprobs(const LogprobsArgs& a, uint64_t n_rows, hipStream_t s);
 
 }  // namespace mmhip

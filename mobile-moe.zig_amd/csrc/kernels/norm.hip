@@ -1,0 +1,271 @@
+// Root-mean-square norm, rotary positions and the paged cache's writer
+// (math.rmsNorm, math.zig:7-35; RoPECache, 197-240; KVCache.put,
+// kv_cache.zig:279-362) on gfx950. All three are bound by HBM for many rows and
+// by one launch's latency for few.
+//
+// Norm: a row's sum of squares and the inverse root are in f64 and the root is
+// rounded to f32 once; every other operation is one f32 operation per value,
+// never contracted. So a value depends on its row alone, not on how threads
+// shared the sum, and the cache writer stores the bits that norm and codec
+// would give one after the other. The f64 sum costs a conversion and an FMA
+// per value, hidden behind the row's loads.
+#include "device_common.hpp"
+#include "kernels.hpp"
+#include "q8_ops.hpp"
+
+namespace mmhip {
+
+namespace {
+
+constexpr int kNormThreads = 256;
+enum NormOut : uint32_t { kOutF32 = 0, kOutF16 = 1, kOutQ8 = 2 };
+
+// Four values from p + c, those at or past `cols` absent (0).
+__device__ __forceinline__ void load4(float (&v)[4], const float* p, uint32_t c, uint32_t cols, bool vec) {
+    if (vec && c + 4 <= cols) {
+        const float4 q = *reinterpret_cast<const float4*>(p + c);
+        v[0] = q.x;
+        v[1] = q.y;
+        v[2] = q.z;
+        v[3] = q.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c + e < cols ? p[c + e] : 0.0f;
+    }
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4], uint32_t c, uint32_t cols, bool vec) {
+    if (vec && c + 4 <= cols) {
+        *reinterpret_cast<float4*>(p + c) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < cols) p[c + e] = v[e];
+    }
+}
+
+__device__ __forceinline__ uint32_t half_bits(float v) { return __half_as_ushort(__float2half_rn(v)); }
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+
+// 1 / sqrt(mean + eps), rounded to f32.
+__device__ __forceinline__ float inverse_root(double sum, uint32_t cols, float eps) {
+    return (float)(1.0 / sqrt(sum / (double)cols + (double)eps));
+}
+
+// One workgroup per row; thread t has columns 4 (t + 256 i).. of it.
+template <uint32_t OUT>
+__global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(NormArgs a) {
+    __shared__ double part[kNormThreads / 64];
+    const uint64_t row = blockIdx.x;
+    const float* x = a.x + row * a.x_stride;
+    const float* res = a.residual ? a.residual + row * a.residual_stride : nullptr;
+    float* sum = a.sum ? a.sum + row * a.sum_stride : nullptr;
+    double acc = 0.0;
+    for (uint32_t c = threadIdx.x * 4; c < a.cols; c += kNormThreads * 4) {
+        float v[4], w[4];
+        load4(v, x, c, a.cols, a.vec);
+        if (res) {
+            load4(w, res, c, a.cols, a.vec);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __fadd_rn(v[e], w[e]);
+        }
+        if (sum) store4(sum, v, c, a.cols, a.vec);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = fma((double)v[e], (double)v[e], acc);
+    }
+    acc = wave_sum(acc);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    acc = 0.0;
+#pragma unroll
+    for (int i = 0; i < kNormThreads / 64; ++i) acc += part[i];
+    const float r = inverse_root(acc, a.cols, a.eps);
+    // Every thread takes every step, so that a Q8_0 block's 8 lanes are together.
+    const uint32_t steps = (a.cols + kNormThreads * 4 - 1) / (kNormThreads * 4);
+    for (uint32_t i = 0; i < steps; ++i) {
+        const uint32_t c = (threadIdx.x + i * kNormThreads) * 4;
+        float v[4], w[4];
+        // A sum that replaced its input is read back, by the thread that wrote it.
+        load4(v, sum ? sum : x, c, a.cols, a.vec);
+        if (res && !sum) {
+            load4(w, res, c, a.cols, a.vec);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __fadd_rn(v[e], w[e]);
+        }
+        load4(w, a.weight, c, a.cols, a.vec);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], r), w[e]);
+        if constexpr (OUT == kOutF32) {
+            store4(static_cast<float*>(a.y) + row * a.y_stride, v, c, a.cols, a.vec);
+        } else if constexpr (OUT == kOutF16) {
+            uint16_t* y = static_cast<uint16_t*>(a.y) + row * a.y_stride;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < a.cols) y[c + e] = (uint16_t)half_bits(v[e]);
+        } else {
+            float d;
+            const uint32_t q4 = q8_quad(v, c < a.cols ? min(a.cols - c, 4u) : 0u, d);
+            const uint32_t blocks = (a.cols + 31) / 32;
+            if (c / 32 < blocks) {
+                uint16_t* y = static_cast<uint16_t*>(a.y) + (row * blocks + c / 32) * 17;
+                const uint32_t j = (c / 4) & 7;
+                y[1 + 2 * j] = (uint16_t)(q4 & 0xFFFFu);
+                y[2 + 2 * j] = (uint16_t)(q4 >> 16);
+                if (j == 0) y[0] = (uint16_t)f32_to_f16_scale(d);
+            }
+        }
+    }
+}
+
+// Cosine and sine of position * frequency, times the magnitude, from the
+// angle in turns: its whole turns are dropped in f64, so far positions keep
+// their angle.
+__device__ __forceinline__ float2 turn(double turns_per_position, double magnitude, uint32_t position) {
+    double t = (double)position * turns_per_position;
+    t -= rint(t);
+    double s, c;
+    sincospi(2.0 * t, &s, &c);
+    return make_float2((float)(c * magnitude), (float)(s * magnitude));
+}
+
+// One rotated value: dim `i` of the rotated dims, `v` its value, `o` its
+// partner's. The products and the sum are rounded one by one.
+__device__ __forceinline__ float rotate(float v, float o, float2 cs, bool second) {
+#pragma clang fp contract(off)
+    return second ? o * cs.y + v * cs.x : v * cs.x - o * cs.y;
+}
+
+constexpr int kRopeThreads = 256;
+
+// One workgroup per token: its pairs' cosines once, then all heads. A thread
+// handles a pair (both values), or a value of the other dims.
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
+    __shared__ float2 cs[kRopeMaxPairs];
+    const uint64_t t = blockIdx.x;
+    const uint32_t pairs = a.dims / 2;
+    if (threadIdx.x < pairs) cs[threadIdx.x] = turn(a.turns[threadIdx.x], a.magnitude, a.positions[t]);
+    __syncthreads();
+    const float* x = a.x + t * a.x_token_stride;
+    float* y = a.y + t * a.y_token_stride;
+    const uint32_t rest = a.copy ? a.head_dim - a.dims : 0, per_head = pairs + rest;
+    const uint64_t n = (uint64_t)a.n_heads * per_head;
+    for (uint64_t i = threadIdx.x; i < n; i += kRopeThreads) {
+        const uint32_t h = (uint32_t)(i / per_head), j = (uint32_t)(i - (uint64_t)h * per_head);
+        const float* xh = x + h * a.x_head_stride;
+        float* yh = y + h * a.y_head_stride;
+        if (j < pairs) {
+            const uint32_t ia = a.first + (a.half ? j : 2 * j), ib = ia + (a.half ? pairs : 1);
+            const float va = xh[ia], vb = xh[ib];
+            yh[ia] = rotate(va, vb, cs[j], false);
+            yh[ib] = rotate(vb, va, cs[j], true);
+        } else {
+            const uint32_t k = j - pairs, c = k < a.first ? k : k + a.dims;
+            yh[c] = xh[c];
+        }
+    }
+}
+
+// One workgroup per position: thread t has values 4t.. of the row.
+constexpr int kStoreThreads = 192;
+static_assert(kStoreThreads * 4 >= kKvMaxRank + kKvMaxRope, "a row fits one pass");
+__global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(StoreArgs a) {
+    __shared__ double part[kStoreThreads / 64];
+    __shared__ float2 cs[kKvMaxRope / 2];
+    const uint64_t t = blockIdx.x;
+    const PagedGeom g = a.geom;
+    const int32_t slot = a.slots[t];
+    uint32_t page, at;
+    if (!paged_slot(g, slot, page, at)) {
+        if (slot >= 0 && threadIdx.x == 0) report(a.status, kBadSlot);
+        return;
+    }
+    const float* x = a.kv + t * a.kv_stride;
+    const uint32_t c = threadIdx.x * 4, pe = g.width - g.rank;
+    const bool live = c < g.width, latent = c < g.rank;
+    float v[4];
+    load4(v, x, live ? c : 0, live ? g.width : 0, a.vec);
+    if (a.turns && threadIdx.x < pe / 2) cs[threadIdx.x] = turn(a.turns[threadIdx.x], a.magnitude, a.positions[t]);
+    double acc = 0.0;
+    if (latent && a.weight) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = fma((double)v[e], (double)v[e], acc);
+    }
+    acc = wave_sum(acc);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    if (latent && a.weight) {
+        acc = 0.0;
+#pragma unroll
+        for (int i = 0; i < kStoreThreads / 64; ++i) acc += part[i];
+        const float r = inverse_root(acc, g.rank, a.eps);
+        float w[4];
+        load4(w, a.weight, c, g.rank, a.vec);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], r), w[e]);
+    } else if (live && !latent && a.turns) {
+        const uint32_t k = c - g.rank, half = pe / 2;
+        if (a.half) {
+            float o[4];
+            const bool second = k >= half;
+            load4(o, x, second ? c - half : c + half, g.width, a.vec);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = rotate(v[e], o[e], cs[(second ? k - half : k) + e], second);
+        } else {
+            const float2 c0 = cs[k / 2], c1 = cs[k / 2 + 1];
+            const float w[4] = {rotate(v[0], v[1], c0, false), rotate(v[1], v[0], c0, true),
+                                rotate(v[2], v[3], c1, false), rotate(v[3], v[2], c1, true)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = w[e];
+        }
+    }
+    if (g.q8) {
+        float d;
+        const uint32_t q4 = q8_quad(v, live ? 4u : 0u, d);
+        if (live) {
+            *reinterpret_cast<uint32_t*>(a.pool + paged_row(g, page, at) + c) = q4;
+            if ((threadIdx.x & 7) == 0)
+                *reinterpret_cast<uint16_t*>(a.pool + paged_scales(g, page, at) + c / 32 * 2) = (uint16_t)f32_to_f16_scale(d);
+        }
+    } else if (live) {
+        *reinterpret_cast<uint2*>(a.pool + paged_row(g, page, at) + 2 * c) =
+            make_uint2(half_bits(v[0]) | half_bits(v[1]) << 16, half_bits(v[2]) | half_bits(v[3]) << 16);
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+
+hipError_t launch_rms_norm(const NormArgs& in, uint32_t out, uint64_t n_rows, hipStream_t s) {
+    if (n_rows == 0) return hipSuccess;
+    NormArgs a = in;
+    a.vec = aligned16(a.x) && a.x_stride % 4 == 0 && aligned16(a.weight) &&
+            (!a.residual || (aligned16(a.residual) && a.residual_stride % 4 == 0)) &&
+            (!a.sum || (aligned16(a.sum) && a.sum_stride % 4 == 0)) &&
+            (out != kOutF32 || (aligned16(a.y) && a.y_stride % 4 == 0));
+    const unsigned grid = (unsigned)n_rows;
+    if (out == kOutF32) rms_norm_kernel<kOutF32><<<grid, kNormThreads, 0, s>>>(a);
+    else if (out == kOutF16) rms_norm_kernel<kOutF16><<<grid, kNormThreads, 0, s>>>(a);
+    else rms_norm_kernel<kOutQ8><<<grid, kNormThreads, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+hipError_t launch_rope(const RopeArgs& a, uint64_t n_tokens, hipStream_t s) {
+    if (n_tokens == 0 || a.n_heads == 0) return hipSuccess;
+    rope_kernel<<<(unsigned)n_tokens, kRopeThreads, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_store(const StoreArgs& in, uint64_t n_tokens, hipStream_t s) {
+    if (n_tokens == 0) return hipSuccess;
+    StoreArgs a = in;
+    a.vec = aligned16(a.kv) && a.kv_stride % 4 == 0 && aligned16(a.weight);
+    kv_store_kernel<<<(unsigned)n_tokens, kStoreThreads, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace mmhip

@@ -84,6 +84,27 @@ class GgufTensor(ctypes.Structure):
                 ("n_elements", _u64), ("n_bytes", _u64), ("data", _c_void_p)]
 
 
+class RopeParams(ctypes.Structure):
+    _fields_ = [("dims", _u32), ("layout", _u32), ("scaling", _u32), ("original_context", _u32),
+                ("base", ctypes.c_float), ("factor", ctypes.c_float), ("beta_fast", ctypes.c_float),
+                ("beta_slow", ctypes.c_float), ("magnitude", ctypes.c_float)]
+
+
+class KvCacheDesc(ctypes.Structure):
+    _fields_ = [("pool_dev", _c_void_p), ("type", _u32), ("rank", _u32), ("rope_dims", _u32), ("page_tokens", _u32),
+                ("n_pages", _u32)]
+
+
+class MlaAttention(ctypes.Structure):
+    _fields_ = [("cache", KvCacheDesc), ("q_dev", _c_void_p), ("q_pe_dev", _c_void_p), ("out_dev", _c_void_p),
+                ("lse_dev", _c_void_p), ("q_token_stride", _u64), ("q_head_stride", _u64),
+                ("q_pe_token_stride", _u64), ("q_pe_head_stride", _u64), ("out_token_stride", _u64),
+                ("out_head_stride", _u64), ("tables_dev", _c_void_p), ("table_stride", _u64), ("n_tables", _u32),
+                ("table_pages", _u32), ("table_of_dev", _c_void_p), ("lens_dev", _c_void_p), ("n_tokens", _u32),
+                ("n_heads", _u32), ("scale", ctypes.c_float), ("workspace_dev", _c_void_p),
+                ("workspace_bytes", _u64)]
+
+
 _SIGS = {
     "mmhip_last_error": (ctypes.c_char_p, []),
     "mmhip_is_available": (ctypes.c_int, []),
@@ -124,6 +145,21 @@ _SIGS = {
                                               _c_void_p, _u64]),
     "mmhip_qmm_dev": (ctypes.c_int, [_c_void_p, _c_void_p, _u64, _c_void_p, _c_void_p, _u64, ctypes.c_int]),
     "mmhip_qmm_dev_noalloc": (ctypes.c_int, [_c_void_p, _c_void_p, _u64, _c_void_p, _c_void_p, _u64, ctypes.c_int]),
+    "mmhip_rms_norm_dev": (ctypes.c_int, [_c_void_p, _c_void_p, _u32, _u64, _c_void_p, _u64, _c_void_p, _u64,
+                                          _c_void_p, _u64, _c_void_p, _u64, _u32, ctypes.c_float]),
+    "mmhip_rope_create": (ctypes.c_int, [_c_void_p, ctypes.POINTER(RopeParams), ctypes.POINTER(_c_void_p)]),
+    "mmhip_rope_destroy": (None, [_c_void_p, _c_void_p]),
+    "mmhip_rope_frequencies": (ctypes.c_int, [ctypes.POINTER(RopeParams), _c_void_p, ctypes.POINTER(ctypes.c_double)]),
+    "mmhip_rope_dev": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _u64, _u64, _c_void_p, _u64, _u64, _c_void_p,
+                                      _u64, _u32, _u32, _u32]),
+    "mmhip_kv_page_bytes": (_u64, [ctypes.POINTER(KvCacheDesc)]),
+    "mmhip_kv_store_dev": (ctypes.c_int, [_c_void_p, ctypes.POINTER(KvCacheDesc), _c_void_p, _u64, _c_void_p,
+                                          ctypes.c_float, _c_void_p, _c_void_p, _c_void_p, _u64]),
+    "mmhip_mla_attention_workspace": (_u64, [_c_void_p, _u32, _u32, _u32]),
+    "mmhip_mla_attention_dev": (ctypes.c_int, [_c_void_p, ctypes.POINTER(MlaAttention)]),
+    "mmhip_logprobs_workspace": (_u64, [_c_void_p, _u64, _u64, _u32]),
+    "mmhip_logprobs_dev": (ctypes.c_int, [_c_void_p, _c_void_p, _u64, _u64, _u64, _c_void_p, _u64, _c_void_p,
+                                          _c_void_p, _u32, _c_void_p, _c_void_p, _c_void_p, _u64]),
     "mmhip_moe_layer_create": (ctypes.c_int, [_c_void_p, ctypes.POINTER(MoeWeights), ctypes.POINTER(_c_void_p)]),
     "mmhip_moe_layer_destroy": (None, [_c_void_p, _c_void_p]),
     "mmhip_moe_ffn": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _u32,
@@ -427,6 +463,128 @@ class Context:
         check(self.lib.mmhip_dequantize_q8_0_rows_dev(self.handle, out.ptr + out_offset, out_stride,
                                                       blocks.ptr + blocks_offset, n_rows, row_len),
               "mmhip_dequantize_q8_0_rows_dev")
+
+
+    # -- between the products of a decode step --
+    def rms_norm_dev(self, y, x, weight, n_rows: int, cols: int, eps: float = 1e-5, y_type: int = F32,
+                     y_stride: Optional[int] = None, x_stride: Optional[int] = None, residual=None,
+                     residual_stride: Optional[int] = None, sum_out=None, sum_stride: Optional[int] = None):
+        """mmhip_rms_norm_dev: y = norm(x + residual) * weight, sum_out = x + residual. Strides default to cols."""
+        check(self.lib.mmhip_rms_norm_dev(
+            self.handle, y.ptr, y_type, cols if y_stride is None else y_stride, None if sum_out is None else sum_out.ptr,
+            cols if sum_stride is None else sum_stride, x.ptr, cols if x_stride is None else x_stride,
+            None if residual is None else residual.ptr, cols if residual_stride is None else residual_stride,
+            weight.ptr, n_rows, cols, eps), "mmhip_rms_norm_dev")
+
+    def rope_dev(self, rope: "Rope", y, x, positions, n_tokens: int, n_heads: int, head_dim: int, first: int = 0,
+                 y_strides=None, x_strides=None, y_offset: int = 0, x_offset: int = 0):
+        """mmhip_rope_dev: dims [first, first + rope.dims) of every head turned by its token's position. Strides are
+        (token, head) in floats, by default those of [n_tokens][n_heads][head_dim]; offsets are in bytes."""
+        ys = y_strides or (n_heads * head_dim, head_dim)
+        xs = x_strides or (n_heads * head_dim, head_dim)
+        check(self.lib.mmhip_rope_dev(self.handle, rope.handle, y.ptr + y_offset, ys[0], ys[1], x.ptr + x_offset, xs[0],
+                                      xs[1], positions.ptr, n_tokens, n_heads, head_dim, first), "mmhip_rope_dev")
+
+    def kv_store_dev(self, cache: "KvCache", kv, slots, n_tokens: int, kv_stride: Optional[int] = None,
+                     norm_weight=None, eps: float = 1e-5, rope: Optional["Rope"] = None, positions=None,
+                     kv_offset: int = 0):
+        """mmhip_kv_store_dev: KVCache.put for n_tokens positions, norm and rope included."""
+        check(self.lib.mmhip_kv_store_dev(
+            self.handle, ctypes.byref(cache.desc), kv.ptr + kv_offset, cache.width if kv_stride is None else kv_stride,
+            None if norm_weight is None else norm_weight.ptr, eps, None if rope is None else rope.handle,
+            None if positions is None else positions.ptr, slots.ptr, n_tokens), "mmhip_kv_store_dev")
+
+    def mla_attention_workspace(self, n_tokens: int, n_heads: int, rank: int) -> int:
+        return self.lib.mmhip_mla_attention_workspace(self.handle, n_tokens, n_heads, rank)
+
+    def mla_attention_args(self, cache: "KvCache", *, q, q_pe=None, out, lens, tables, n_tables: int, table_pages: int,
+                           n_tokens: int, n_heads: int, scale: float, workspace, lse=None, table_of=None,
+                           table_stride: Optional[int] = None, q_strides=None, q_pe_strides=None, out_strides=None,
+                           q_offset: int = 0, q_pe_offset: int = 0, out_offset: int = 0) -> MlaAttention:
+        """The mmhip_mla_attention that mla_attention_dev takes (built once, reusable; it keeps the buffers alive).
+        Strides are (token, head) in floats, by default those of contiguous [n_tokens][n_heads][row]; offsets are in
+        bytes."""
+        d = cache.desc
+        a = MlaAttention()
+        a.cache = d
+        a.q_dev, a.out_dev = q.ptr + q_offset, out.ptr + out_offset
+        a.q_pe_dev = None if q_pe is None else q_pe.ptr + q_pe_offset
+        a.lse_dev = None if lse is None else lse.ptr
+        a.q_token_stride, a.q_head_stride = q_strides or (n_heads * d.rank, d.rank)
+        a.q_pe_token_stride, a.q_pe_head_stride = q_pe_strides or (n_heads * d.rope_dims, d.rope_dims)
+        a.out_token_stride, a.out_head_stride = out_strides or (n_heads * d.rank, d.rank)
+        a.tables_dev, a.table_stride = tables.ptr, table_pages if table_stride is None else table_stride
+        a.n_tables, a.table_pages = n_tables, table_pages
+        a.table_of_dev = None if table_of is None else table_of.ptr
+        a.lens_dev, a.n_tokens, a.n_heads, a.scale = lens.ptr, n_tokens, n_heads, scale
+        a.workspace_dev, a.workspace_bytes = workspace.ptr, workspace.nbytes
+        a._keep = (cache, q, q_pe, out, lse, tables, table_of, lens, workspace)
+        return a
+
+    def mla_attention_dev(self, args: MlaAttention):
+        """mmhip_mla_attention_dev: attention of single tokens over the paged latent cache."""
+        check(self.lib.mmhip_mla_attention_dev(self.handle, ctypes.byref(args)), "mmhip_mla_attention_dev")
+
+    def logprobs_workspace(self, n_rows: int, vocab: int, top: int) -> int:
+        return self.lib.mmhip_logprobs_workspace(self.handle, n_rows, vocab, top)
+
+    def logprobs_dev(self, logits, n_rows: int, vocab: int, *, stride: Optional[int] = None, tokens=None,
+                     n_given: int = 0, token_logprobs=None, entropy=None, top: int = 0, top_ids=None,
+                     top_logprobs=None, workspace=None):
+        """mmhip_logprobs_dev: log probabilities of the given tokens, entropy and the largest alternatives."""
+        p = [None if b is None else b.ptr for b in (tokens, token_logprobs, entropy, top_ids, top_logprobs, workspace)]
+        check(self.lib.mmhip_logprobs_dev(self.handle, logits.ptr, vocab if stride is None else stride, n_rows, vocab,
+                                          p[0], n_given, p[1], p[2], top, p[3], p[4], p[5],
+                                          0 if workspace is None else workspace.nbytes), "mmhip_logprobs_dev")
+
+
+ROPE_LAYOUT = dict(interleaved=0, half=1)
+ROPE_SCALING = dict(none=0, linear=1, yarn=2)
+
+
+def rope_params(dims: int, base: float = 10000.0, layout: str = "interleaved", scaling: str = "none",
+                factor: float = 1.0, original_context: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                magnitude: float = 0.0) -> RopeParams:
+    return RopeParams(dims, ROPE_LAYOUT[layout], ROPE_SCALING[scaling], original_context, base, factor, beta_fast,
+                      beta_slow, magnitude)
+
+
+def rope_frequencies(params: RopeParams):
+    """mmhip_rope_frequencies: (radians per position of each pair, magnitude); host only."""
+    lib = load_library()
+    out, m = np.empty(max(1, params.dims // 2), dtype=np.float64), ctypes.c_double()
+    check(lib.mmhip_rope_frequencies(ctypes.byref(params), _ptr(out), ctypes.byref(m)), "mmhip_rope_frequencies")
+    return out, m.value
+
+
+class Rope:
+    """A rotary plan (RoPECache's role, math.zig:197-240): frequencies on the device."""
+
+    def __init__(self, ctx: "Context", **params):
+        self.ctx, self.params = ctx, rope_params(**params)
+        h = _c_void_p()
+        check(ctx.lib.mmhip_rope_create(ctx.handle, ctypes.byref(self.params), ctypes.byref(h)), "mmhip_rope_create")
+        self.handle = h.value
+
+    def free(self):
+        if self.handle:
+            self.ctx.lib.mmhip_rope_destroy(self.ctx.handle, self.handle)
+            self.handle = None
+
+
+class KvCache:
+    """A layer's paged latent cache in a pool the caller owns (mmhip_kv_cache)."""
+
+    def __init__(self, pool, ggml_type: int, *, rank: int, rope_dims: int, page_tokens: int, n_pages: int):
+        self.pool = pool
+        self.desc = KvCacheDesc(pool.ptr, ggml_type, rank, rope_dims, page_tokens, n_pages)
+        self.width = rank + rope_dims
+
+    @staticmethod
+    def page_bytes(ggml_type: int, rank: int, rope_dims: int, page_tokens: int) -> int:
+        """Bytes of one page; 0 if the library does not support such a cache."""
+        return load_library().mmhip_kv_page_bytes(ctypes.byref(KvCacheDesc(None, ggml_type, rank, rope_dims,
+                                                                           page_tokens, 1)))
 
 
 class Gguf:

@@ -109,6 +109,58 @@ pub const GgufTensor = extern struct {
     data: ?*const anyopaque = null,
 };
 
+pub const mmhip_rope = opaque {};
+pub const RopeHandle = mmhip_rope;
+
+pub const mmhip_rope_params = extern struct {
+    dims: u32,
+    layout: u32 = 0,
+    scaling: u32 = 0,
+    original_context: u32 = 0,
+    base: f32,
+    factor: f32 = 1.0,
+    beta_fast: f32 = 32.0,
+    beta_slow: f32 = 1.0,
+    magnitude: f32 = 0.0,
+};
+pub const RopeParams = mmhip_rope_params;
+
+pub const mmhip_kv_cache = extern struct {
+    pool_dev: ?*anyopaque,
+    type_: u32,
+    rank: u32,
+    rope_dims: u32,
+    page_tokens: u32,
+    n_pages: u32,
+};
+pub const LatentCache = mmhip_kv_cache;
+
+pub const mmhip_mla_attention = extern struct {
+    cache: mmhip_kv_cache,
+    q_dev: ?[*]const f32,
+    q_pe_dev: ?[*]const f32 = null,
+    out_dev: ?[*]f32,
+    lse_dev: ?[*]f32 = null,
+    q_token_stride: u64,
+    q_head_stride: u64,
+    q_pe_token_stride: u64 = 0,
+    q_pe_head_stride: u64 = 0,
+    out_token_stride: u64,
+    out_head_stride: u64,
+    tables_dev: ?[*]const i32,
+    table_stride: u64,
+    n_tables: u32,
+    table_pages: u32,
+    table_of_dev: ?[*]const u32 = null,
+    lens_dev: ?[*]const u32,
+    n_tokens: u32,
+    n_heads: u32,
+    scale: f32,
+    workspace_dev: ?*anyopaque,
+    workspace_bytes: u64,
+};
+pub const MlaAttention = mmhip_mla_attention;
+
 pub const max_moe_tokens: u32 = 256;
 
 extern fn mmhip_last_error() [*:0]const u8;
@@ -160,6 +212,17 @@ extern fn mmhip_gemv_batched_dev(ctx: *Ctx, w: *const Weight, first: u64, n_mats
 extern fn mmhip_gemv_grouped_dev(ctx: *Ctx, groups: [*]const GemvGroup, n_groups: u32) c_int;
 extern fn mmhip_qmm_dev(ctx: *Ctx, w: *const Weight, mat: u64, x_dev: ?[*]const f32, y_dev: ?[*]f32, batch: u64, out_layout: c_int) c_int;
 extern fn mmhip_qmm_dev_noalloc(ctx: *Ctx, w: *const Weight, mat: u64, x_dev: ?[*]const f32, y_dev: ?[*]f32, batch: u64, out_layout: c_int) c_int;
+extern fn mmhip_rms_norm_dev(ctx: *Ctx, y_dev: ?*anyopaque, y_type: u32, y_stride: u64, sum_dev: ?[*]f32, sum_stride: u64, x_dev: ?[*]const f32, x_stride: u64, residual_dev: ?[*]const f32, residual_stride: u64, weight_dev: ?[*]const f32, n_rows: u64, cols: u32, eps: f32) c_int;
+extern fn mmhip_rope_create(ctx: *Ctx, params: *const mmhip_rope_params, out_rope: *?*mmhip_rope) c_int;
+extern fn mmhip_rope_destroy(ctx: *Ctx, rope: ?*mmhip_rope) void;
+extern fn mmhip_rope_frequencies(params: *const mmhip_rope_params, out: [*]f64, magnitude: *f64) c_int;
+extern fn mmhip_rope_dev(ctx: *Ctx, rope: *const mmhip_rope, y_dev: ?[*]f32, y_token_stride: u64, y_head_stride: u64, x_dev: ?[*]const f32, x_token_stride: u64, x_head_stride: u64, positions_dev: ?[*]const u32, n_tokens: u64, n_heads: u32, head_dim: u32, first: u32) c_int;
+extern fn mmhip_kv_page_bytes(cache: *const mmhip_kv_cache) u64;
+extern fn mmhip_kv_store_dev(ctx: *Ctx, cache: *const mmhip_kv_cache, kv_dev: ?[*]const f32, kv_stride: u64, norm_weight_dev: ?[*]const f32, eps: f32, rope: ?*const mmhip_rope, positions_dev: ?[*]const u32, slots_dev: ?[*]const i32, n_tokens: u64) c_int;
+extern fn mmhip_mla_attention_workspace(ctx: *Ctx, n_tokens: u32, n_heads: u32, rank: u32) u64;
+extern fn mmhip_mla_attention_dev(ctx: *Ctx, args: *const mmhip_mla_attention) c_int;
+extern fn mmhip_logprobs_workspace(ctx: *Ctx, n_rows: u64, vocab: u64, top: u32) u64;
+extern fn mmhip_logprobs_dev(ctx: *Ctx, logits_dev: ?[*]const f32, stride: u64, n_rows: u64, vocab: u64, tokens_dev: ?[*]const u32, n_given: u64, token_logprobs_dev: ?[*]f32, entropy_dev: ?[*]f32, top: u32, top_ids_dev: ?[*]u32, top_logprobs_dev: ?[*]f32, workspace_dev: ?*anyopaque, workspace_bytes: u64) c_int;
 extern fn mmhip_moe_layer_create(ctx: *Ctx, wts: *const MoeWeights, out_layer: *?*MoeLayerHandle) c_int;
 extern fn mmhip_moe_layer_destroy(ctx: *Ctx, layer: ?*MoeLayerHandle) void;
 extern fn mmhip_moe_ffn(ctx: *Ctx, layer: *MoeLayerHandle, hidden_host: [*]const f32, out_host: [*]f32, n_tokens: u32, rp: ?*const RouteParams, route_ids_host: ?[*]u32, route_weights_host: ?[*]f32) c_int;
@@ -298,6 +361,57 @@ pub const HipBackend = struct {
     /// n_rows device rows at once.
     pub fn dequantizeRowsQ8_0Dev(self: *Self, out_dev: [*]f32, out_stride: u64, blocks_dev: *const anyopaque, n_rows: u64, row_len: u32) !void {
         try check(mmhip_dequantize_q8_0_rows_dev(self.ctx, out_dev, out_stride, blocks_dev, n_rows, row_len));
+    }
+
+    /// math.rmsNorm (math.zig:7-35) of contiguous device rows with the
+    /// residual added first: sum_dev (may be residual_dev itself) receives
+    /// x + residual, y_dev the normed rows.
+    pub fn rmsNormDev(self: *Self, y_dev: [*]f32, sum_dev: ?[*]f32, x_dev: [*]const f32, residual_dev: ?[*]const f32, weight_dev: [*]const f32, n_rows: u64, cols: u32, eps: f32) !void {
+        try check(mmhip_rms_norm_dev(self.ctx, @ptrCast(y_dev), 0, cols, sum_dev, cols, x_dev, cols, residual_dev, cols, weight_dev, n_rows, cols, eps));
+    }
+
+    /// RoPECache's role (math.zig:197-240): frequencies kept on the device.
+    pub fn createRope(self: *Self, params: RopeParams) !*RopeHandle {
+        var h: ?*RopeHandle = null;
+        try check(mmhip_rope_create(self.ctx, &params, &h));
+        return h.?;
+    }
+
+    pub fn destroyRope(self: *Self, rope: *RopeHandle) void {
+        mmhip_rope_destroy(self.ctx, rope);
+    }
+
+    /// Turns the last dims of every head in place, e.g. the 64 rotary ones of
+    /// q_b's 192 per head; x_dev [n_tokens][n_heads][head_dim].
+    pub fn ropeDev(self: *Self, rope: *const RopeHandle, x_dev: [*]f32, positions_dev: [*]const u32, n_tokens: u64, n_heads: u32, head_dim: u32, first: u32) !void {
+        const row: u64 = @as(u64, n_heads) * head_dim;
+        try check(mmhip_rope_dev(self.ctx, rope, x_dev, row, head_dim, x_dev, row, head_dim, positions_dev, n_tokens, n_heads, head_dim, first));
+    }
+
+    /// KVCache.put (kv_cache.zig:279-362) for n_tokens positions: kv_a's rows
+    /// normed, turned, rounded and written to their slots of the paged cache.
+    pub fn kvStoreDev(self: *Self, cache: *const LatentCache, kv_dev: [*]const f32, kv_stride: u64, norm_weight_dev: ?[*]const f32, eps: f32, rope: ?*const RopeHandle, positions_dev: ?[*]const u32, slots_dev: [*]const i32, n_tokens: u64) !void {
+        try check(mmhip_kv_store_dev(self.ctx, cache, kv_dev, kv_stride, norm_weight_dev, eps, rope, positions_dev, slots_dev, n_tokens));
+    }
+
+    /// The cached part of mlaAttention (inference.zig:539-660) for single
+    /// tokens, in the latent space.
+    pub fn mlaAttentionDev(self: *Self, args: *const MlaAttention) !void {
+        try check(mmhip_mla_attention_dev(self.ctx, args));
+    }
+
+    pub fn mlaAttentionWorkspace(self: *Self, n_tokens: u32, n_heads: u32, rank: u32) u64 {
+        return mmhip_mla_attention_workspace(self.ctx, n_tokens, n_heads, rank);
+    }
+
+    /// Log probabilities of given tokens and of the `top` largest logits, and
+    /// the entropy, for contiguous rows of device logits.
+    pub fn logprobsDev(self: *Self, logits_dev: [*]const f32, n_rows: u64, vocab: u64, tokens_dev: ?[*]const u32, n_given: u64, token_logprobs_dev: ?[*]f32, entropy_dev: ?[*]f32, top: u32, top_ids_dev: ?[*]u32, top_logprobs_dev: ?[*]f32, workspace_dev: ?*anyopaque, workspace_bytes: u64) !void {
+        try check(mmhip_logprobs_dev(self.ctx, logits_dev, vocab, n_rows, vocab, tokens_dev, n_given, token_logprobs_dev, entropy_dev, top, top_ids_dev, top_logprobs_dev, workspace_dev, workspace_bytes));
+    }
+
+    pub fn logprobsWorkspace(self: *Self, n_rows: u64, vocab: u64, top: u32) u64 {
+        return mmhip_logprobs_workspace(self.ctx, n_rows, vocab, top);
     }
 
     /// Drops the resident copy of a weight (e.g. before unmapping the file).
