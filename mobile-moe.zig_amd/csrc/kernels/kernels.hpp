@@ -414,6 +414,18 @@ struct MlaArgs {
     uint32_t* status;
     int num_cu;
 };
+// How a call is cut and where its pieces go (set by the launcher).
+constexpr uint32_t kMlaMostGroups = 1024;
+struct MlaPlan {
+    uint32_t groups;      // workgroups that share the list of tiles
+    uint32_t rows;        // heads per head tile: 16 or 32
+    uint32_t head_tiles;
+    uint32_t part_rows;   // rows of a piece in the workspace: min(rows, n_heads)
+    float* parts;         // [groups][2][part_rows][rank]: a piece that begins its item is the second
+    float2* part_ml;      // [groups][2][rows]: its maximum (base 2) and sum
+    void* splits;         // [groups]
+    bool vec_q, vec_out;  // 16-byte accesses fit
+};
 uint64_t mla_workspace_bytes(uint32_t n_tokens, uint32_t n_heads, uint32_t rank, int num_cu);
 hipError_t launch_mla(const MlaArgs& a, hipStream_t s);
 

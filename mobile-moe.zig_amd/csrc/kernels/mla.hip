@@ -1,5 +1,37 @@
 // Attention of single tokens over the paged latent cache (mlaAttention's
-// cached part, inference.zig:539-660) on gfx950.
+// cached part, inference.zig:539-660) on gfx950: for every token and head,
+// out = sum_p softmax_p(scale (q . c_p + q_pe . k_p)) c_p over the rows (c, k)
+// that the token's page table names. One pass over the rows with the running
+// maximum and sum of the softmax; all heads of a token share the read rows.
+//
+// Bound: HBM. A row of 512 + 64 values is 1152 B in f16 (612 B in Q8_0) and
+// costs 2 x 20 x 1088 operations. The matrix work is up to four times that
+// (heads padded to 32, and the f32 operands of each product in two f16 parts,
+// 22 bits; the cached values are exact in f16), still below the rows' time.
+//
+// A workgroup is four waves and takes tiles of 32 positions. Wave w owns the
+// latent columns 128 w .. 128 w + 127 and 16 of the rotary ones, both as keys
+// and as values, so cached data never crosses waves: a wave stages its slice
+// of the next tile in registers while it works on the current one, and keeps
+// it in its own part of LDS, from which it is read as keys in rows and as
+// values transposed (ds_read_b64_tr_b16). Per tile:
+//   S^T partial = K Q^T over the wave's columns     (rows are positions)
+//   exchange: the four partials are added, each wave takes a quarter of the
+//             heads through the softmax and leaves P
+//   O^T += V^T P^T for the wave's columns           (rows are columns)
+// with two barriers. S^T leaves the matrix cores with four consecutive
+// positions per lane, and P is stored in the order in which O^T's operand takes
+// positions, so both are 16-byte accesses.
+//
+// Q8_0: codes become f16 integers on their way to LDS. A score is summed block
+// by block, each block's product times the position's block scale. In O the
+// scale is folded into P, block by block, times a power of two that keeps
+// the largest scale seen (running, like the softmax's maximum) within f16.
+//
+// Work is cut evenly, whatever the lengths: the tiles of all tokens and head
+// tiles form one list, of which every workgroup takes an equal run, two
+// workgroups per CU. A run may end inside a token; such pieces leave their
+// sums in the workspace and mla_join_kernel adds them in the list's order.
 #include "device_common.hpp"
 #include "kernels.hpp"
 
@@ -7,86 +39,769 @@ namespace mmhip {
 
 namespace {
 
-constexpr int kMlaThreads = 256;
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
 
-// One workgroup per token and head; positions in tiles of 256.
-__global__ __launch_bounds__(kMlaThreads) void mla_simple_kernel(MlaArgs a) {
-    __shared__ float q[kKvMaxRank + kKvMaxRope];
-    __shared__ float p[kMlaThreads];
-    __shared__ uint64_t at_row[kMlaThreads], at_scale[kMlaThreads];
-    __shared__ float red[kMlaThreads / 64];
+constexpr int kMlaThreads = 256, kMlaWaves = 4;
+constexpr uint32_t kMlaTile = 32;       // positions per tile
+constexpr uint32_t kMlaCols = 128;      // latent columns per wave
+constexpr uint32_t kMlaPe = 16;         // rotary columns per wave
+constexpr uint32_t kSpLd = 36;          // floats between rows of the score partials
+constexpr float kPScale = 32768.0f;     // P in [0, 1] uses f16's upper range: parts down to 2^-39 survive
+constexpr int kJoinThreads = 1024;
+
+// A begun and unfinished item of a workgroup: the item, and how many pieces it
+// has (this workgroup's and the first ones of the following); pieces 0: none.
+struct MlaSplit {
+    uint32_t item, pieces;
+};
+
+template <bool Q8, int HT>
+struct MlaLds {
+    uint8_t kv[kMlaWaves][kMlaTile * 256];  // f16 [position][128], 16-byte chunks swizzled by the position
+    uint8_t pe[kMlaWaves][kMlaTile * 32];   // f16 [position][16]
+    float sp[kMlaWaves][16 * HT][kSpLd];
+    // P: f16 parts (hi, lo) in rows of 40, or f32 in rows of 36
+    uint32_t p[Q8 ? 16 * HT * 36 : 2 * 16 * HT * 20];
+    float ds[Q8 ? kMlaWaves : 1][5][kMlaTile];  // block scales of the keys
+    float dv[Q8 ? kMlaWaves : 1][4][kMlaTile];  // of the values, scaled into range
+    float alpha[16 * HT], factor[16 * HT], qmax[kMlaWaves][16 * HT];
+    float2 ml[16 * HT];
+    uint64_t scan[kMlaWaves];
+    uint64_t start_off;
+    uint32_t start_token;
+};
+
+__device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (uint32_t)(((uint64_t)len + kMlaTile - 1) / kMlaTile); }
+
+__device__ __forceinline__ uint32_t seen(const MlaArgs& a, uint32_t t, uint32_t& row, uint32_t& bad) {
+    row = a.table_of ? a.table_of[t] : t;
+    return paged_seen(a.geom, a.lens[t], row, a.n_tables, a.table_pages, bad);
+}
+
+// Two codes (bytes i, i + 1 of u = code + 128) as f16 integers: 0x6400 | u is
+// 1024 + u.
+__device__ __forceinline__ uint32_t codes2(uint32_t u, uint32_t sel) {
+    const uint32_t h = __builtin_amdgcn_perm(0x64646464u, u, sel);
+    const v2h v = __builtin_bit_cast(v2h, h) - (v2h){(_Float16)1152.0f, (_Float16)1152.0f};
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ uint4 codes8(uint32_t a, uint32_t b) {
+    const uint32_t x = a ^ 0x80808080u, y = b ^ 0x80808080u;
+    return make_uint4(codes2(x, 0x04010400u), codes2(x, 0x04030402u), codes2(y, 0x04010400u), codes2(y, 0x04030402u));
+}
+
+// Two values as f16 parts: hi + lo is the value to 22 bits (hi truncated, lo
+// the rest).
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    const auto l = __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]);
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, l);
+}
+
+__device__ __forceinline__ v8h half8(const uint4& v) { return __builtin_bit_cast(v8h, v); }
+
+// 2^e, e within f32's normal exponents.
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+template <bool Q8, int HT, bool FULL>
+__global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, MlaPlan pl) {
+    constexpr int kRows = 16 * HT;
+    __shared__ __align__(16) MlaLds<Q8, HT> s;
     const PagedGeom g = a.geom;
-    const uint32_t t = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads;
-    const uint32_t row = a.table_of ? a.table_of[t] : t;
-    uint32_t bad;
-    const uint32_t len = paged_seen(g, a.lens[t], row, a.n_tables, a.table_pages, bad);
-    if (bad && threadIdx.x == 0) report(a.status, bad == 1 ? kBadTableRow : kBadLength);
-    for (uint32_t c = threadIdx.x; c < g.width; c += kMlaThreads)
-        q[c] = a.scale * (c < g.rank ? a.q[t * a.q_token_stride + h * a.q_head_stride + c]
-                                     : a.q_pe[t * a.q_pe_token_stride + h * a.q_pe_head_stride + c - g.rank]);
-    float m = -INFINITY, l = 0.0f, o[2] = {0.0f, 0.0f};
-    for (uint32_t p0 = 0; p0 < len; p0 += kMlaThreads) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t n16 = lane & 15, grp = lane >> 4;
+    const uint32_t wg = blockIdx.x;
+    MlaSplit* const splits = reinterpret_cast<MlaSplit*>(pl.splits);
+
+    // ---- this workgroup's run of the list ----
+    uint64_t f, end, total;
+    {
+        const uint32_t per = (a.n_tokens + kMlaThreads - 1) / kMlaThreads;
+        const uint64_t t0 = (uint64_t)tid * per;
+        uint64_t mine = 0;
+        for (uint64_t t = t0; t < t0 + per && t < a.n_tokens; ++t) {
+            uint32_t row, bad;
+            mine += tiles_of(seen(a, (uint32_t)t, row, bad));
+        }
+        mine *= pl.head_tiles;
+        uint64_t incl = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint64_t o = __shfl_up((unsigned long long)incl, off, 64);
+            if ((int)lane >= off) incl += o;
+        }
+        if (lane == 63) s.scan[wave] = incl;
         __syncthreads();
-        const uint32_t pos = p0 + threadIdx.x;
-        float s = -INFINITY;
-        uint64_t ro = ~0ull, so = 0;
-        if (pos < len) {
-            const int32_t id = a.tables[row * a.table_stride + (pos >> g.page_shift)];
-            if (paged_has(g, id)) {
-                const uint32_t at = pos & ((1u << g.page_shift) - 1);
-                ro = paged_row(g, (uint32_t)id, at);
-                so = paged_scales(g, (uint32_t)id, at);
-                s = 0.0f;
-                for (uint32_t c = 0; c < g.width; ++c)
-                    s += q[c] * (g.q8 ? (float)(int8_t)a.pool[ro + c] * f16_scale(*reinterpret_cast<const uint16_t*>(a.pool + so + c / 32 * 2))
-                                      : f16_scale(*reinterpret_cast<const uint16_t*>(a.pool + ro + 2 * c)));
+        total = 0;
+        uint64_t before = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kMlaWaves; ++w) {
+            if (w < wave) before += s.scan[w];
+            total += s.scan[w];
+        }
+        incl += before;
+        const uint64_t chunk = (total + pl.groups - 1) / pl.groups;
+        f = wg * chunk;
+        end = f + chunk < total ? f + chunk : total;
+        if (f < end && incl - mine <= f && f < incl) {
+            uint64_t at = incl - mine;
+            uint32_t t = (uint32_t)t0;
+            for (; t + 1 < a.n_tokens; ++t) {
+                uint32_t row, bad;
+                const uint64_t n = (uint64_t)tiles_of(seen(a, t, row, bad)) * pl.head_tiles;
+                if (f < at + n) break;
+                at += n;
+            }
+            s.start_token = t;
+            s.start_off = f - at;
+        }
+        __syncthreads();
+    }
+    MlaSplit begun{0, 0};
+    const uint64_t chunk = (total + pl.groups - 1) / pl.groups;
+
+    const uint32_t row_bytes = Q8 ? g.width : 2 * g.width, at_mask = (1u << g.page_shift) - 1;
+    const uint32_t blocks = FULL ? 4u : (g.rank / 32 > 4 * wave ? min(g.rank / 32 - 4 * wave, 4u) : 0u);
+    const bool has_pe = FULL || kMlaPe * wave < g.width - g.rank;
+
+    uint32_t token = f < end ? s.start_token : 0;
+    uint64_t off = f < end ? s.start_off : 0;
+    while (f < end && token < a.n_tokens) {
+        uint32_t row, bad;
+        const uint32_t len = __builtin_amdgcn_readfirstlane(seen(a, token, row, bad));
+        const uint32_t n_tiles = tiles_of(len);
+        if (n_tiles == 0) {
+            ++token;
+            continue;
+        }
+        row = __builtin_amdgcn_readfirstlane(row);
+        const uint32_t ht_index = (uint32_t)(off / n_tiles), tile0 = (uint32_t)(off - (uint64_t)ht_index * n_tiles);
+        const uint32_t count = (uint32_t)(end - f < n_tiles - tile0 ? end - f : n_tiles - tile0);
+        const uint32_t head0 = ht_index * kRows;
+        const int32_t* table = a.tables + (uint64_t)row * a.table_stride;
+
+        // ---- loads of a tile: page numbers one tile before its rows ----
+        int32_t id[2];
+        auto load_ids = [&](uint32_t tile) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint64_t p = (uint64_t)tile * kMlaTile + 16 * h;
+                id[h] = p < len ? table[p >> g.page_shift] : -1;
+            }
+        };
+        uint4 pre[Q8 ? 4 : 8], pre_pe;
+        uint2 pre_d;
+        uint32_t pre_dpe = 0, live = 0;
+        pre_pe = make_uint4(0, 0, 0, 0);
+        pre_d = make_uint2(0, 0);
+        auto load_rows = [&](uint32_t tile) {
+            const uint8_t* base[2];
+            const uint8_t* base_d[2];
+            live = 0;
+            const uint32_t p0 = tile * kMlaTile;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int32_t page = __builtin_amdgcn_readfirstlane(id[h]);
+                const uint32_t p = p0 + 16 * h;
+                const bool want = p < len, ok = want && paged_has(g, page);
+                if (ok) live |= (len - p >= 16 ? 0xFFFFu : (1u << (len - p)) - 1) << (16 * h);
+                else if (want && tid == 0) report(a.status, kBadPage);
+                // A page that is not there is read as page 0 and left out.
+                base[h] = a.pool + paged_row(g, ok ? (uint32_t)page : 0u, p & at_mask);
+                if constexpr (Q8) base_d[h] = a.pool + paged_scales(g, ok ? (uint32_t)page : 0u, p & at_mask);
+            }
+            if constexpr (Q8) {
+                if (FULL || blocks) {
+                    uint32_t c = lane & 7;
+                    if (!FULL) c = min(c, 2 * blocks - 1);
+                    const uint32_t o = (lane >> 3) * row_bytes + wave * kMlaCols + c * 16;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        pre[j] = *reinterpret_cast<const uint4*>(base[j >> 1] + (8 * (j & 1)) * row_bytes + o);
+                    const uint8_t* d = (lane & 16 ? base_d[1] : base_d[0]) + n16 * (g.width / 32 * 2) + wave * 8;
+                    if constexpr (FULL) {
+                        pre_d.x = reinterpret_cast<const uint32_t*>(d)[0];
+                        pre_d.y = reinterpret_cast<const uint32_t*>(d)[1];
+                    } else {
+                        uint32_t v[4];
+#pragma unroll
+                        for (uint32_t b = 0; b < 4; ++b) v[b] = reinterpret_cast<const uint16_t*>(d)[min(b, blocks - 1)];
+                        pre_d = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+                    }
+                }
+                if (has_pe) {
+                    const uint8_t* r = (lane & 16 ? base[1] : base[0]) + n16 * row_bytes + g.rank + wave * kMlaPe;
+                    pre_pe = *reinterpret_cast<const uint4*>(r);
+                    const uint8_t* d = (lane & 16 ? base_d[1] : base_d[0]) + n16 * (g.width / 32 * 2) + (g.rank / 32 + wave / 2) * 2;
+                    pre_dpe = *reinterpret_cast<const uint16_t*>(d);
+                }
             } else {
-                report(a.status, kBadPage);
+                if (FULL || blocks) {
+                    uint32_t c = n16;
+                    if (!FULL) c = min(c, 4 * blocks - 1);
+                    const uint32_t o = grp * row_bytes + wave * (2 * kMlaCols) + c * 16;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        pre[j] = *reinterpret_cast<const uint4*>(base[j >> 2] + (4 * (j & 3)) * row_bytes + o);
+                }
+                if (has_pe)
+                    pre_pe = *reinterpret_cast<const uint4*>((lane & 32 ? base[1] : base[0]) + ((lane >> 1) & 15) * row_bytes +
+                                                             2 * g.rank + wave * (2 * kMlaPe) + (lane & 1) * 16);
+            }
+        };
+        load_ids(tile0);
+        load_rows(tile0);
+        load_ids(tile0 + 1);
+
+        // ---- the queries, scaled by a power of two per head, in two parts ----
+        v8h qh[HT][4], ql[HT][4];
+        v4h peh[HT], pel[HT];
+        {
+            float q[HT][4][8], pe[HT][4], top[HT];
+#pragma unroll
+            for (int ht = 0; ht < HT; ++ht) {
+                const uint32_t h = head0 + ht * 16 + n16;
+                const bool there = h < a.n_heads;
+                const float* src = a.q + (uint64_t)token * a.q_token_stride + (uint64_t)(there ? h : 0) * a.q_head_stride +
+                                   wave * kMlaCols + 8 * grp;
+                const float* src_pe = a.q_pe + (uint64_t)token * a.q_pe_token_stride +
+                                      (uint64_t)(there ? h : 0) * a.q_pe_head_stride + wave * kMlaPe + 4 * grp;
+                top[ht] = 0.0f;
+#pragma unroll
+                for (uint32_t b = 0; b < 4; ++b) {
+                    if (there && (FULL || b < blocks)) {
+                        if (pl.vec_q) {
+                            const float4 x = *reinterpret_cast<const float4*>(src + 32 * b);
+                            const float4 y = *reinterpret_cast<const float4*>(src + 32 * b + 4);
+                            q[ht][b][0] = x.x, q[ht][b][1] = x.y, q[ht][b][2] = x.z, q[ht][b][3] = x.w;
+                            q[ht][b][4] = y.x, q[ht][b][5] = y.y, q[ht][b][6] = y.z, q[ht][b][7] = y.w;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) q[ht][b][e] = src[32 * b + e];
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) q[ht][b][e] = 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pe[ht][e] = there && has_pe ? src_pe[e] : 0.0f;
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top[ht] = fmaxf(top[ht], fabsf(q[ht][b][e]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[ht] = fmaxf(top[ht], fabsf(pe[ht][e]));
+                top[ht] = fmaxf(top[ht], __shfl_xor(top[ht], 16, 64));
+                top[ht] = fmaxf(top[ht], __shfl_xor(top[ht], 32, 64));
+                if (grp == 0) s.qmax[wave][ht * 16 + n16] = top[ht];
+            }
+            lds_barrier();
+#pragma unroll
+            for (int ht = 0; ht < HT; ++ht) {
+                const uint32_t r = ht * 16 + n16;
+                const float m = fmaxf(fmaxf(s.qmax[0][r], s.qmax[1][r]), fmaxf(s.qmax[2][r], s.qmax[3][r]));
+                // m 2^e in [2^13, 2^14) for m within f32's middle range
+                const int e = m > 0.0f ? min(max(140 - (int)(__float_as_uint(m) >> 23), -115), 115) : 0;
+                const float sc = pow2(e);
+                if (wave == 0 && grp == 0) s.factor[r] = a.scale * 1.44269504088896f * pow2(-e);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) split2(q[ht][b][2 * i] * sc, q[ht][b][2 * i + 1] * sc, h[i], l[i]);
+                    qh[ht][b] = half8(make_uint4(h[0], h[1], h[2], h[3]));
+                    ql[ht][b] = half8(make_uint4(l[0], l[1], l[2], l[3]));
+                }
+                uint32_t h[2], l[2];
+                split2(pe[ht][0] * sc, pe[ht][1] * sc, h[0], l[0]);
+                split2(pe[ht][2] * sc, pe[ht][3] * sc, h[1], l[1]);
+                peh[ht] = __builtin_bit_cast(v4h, make_uint2(h[0], h[1]));
+                pel[ht] = __builtin_bit_cast(v4h, make_uint2(l[0], l[1]));
             }
         }
-        at_row[threadIdx.x] = ro;
-        at_scale[threadIdx.x] = so;
-        float top = s;
-        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float m2 = fmaxf(m, top), base = m2 == -INFINITY ? 0.0f : m2;
-        const float f = expf(m - base);
-        p[threadIdx.x] = expf(s - base);
-        float sum = p[threadIdx.x];
-        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
-        __syncthreads();
-        l = l * f + ((red[0] + red[1]) + (red[2] + red[3]));
-        m = m2;
-        const uint32_t n = min(len - p0, (uint32_t)kMlaThreads);
-        for (int e = 0; e < 2; ++e) {
-            const uint32_t c = threadIdx.x + e * kMlaThreads;
-            o[e] *= f;
-            if (c >= g.rank) continue;
-            for (uint32_t i = 0; i < n; ++i) {
-                if (at_row[i] == ~0ull) continue;
-                o[e] += p[i] * (g.q8 ? (float)(int8_t)a.pool[at_row[i] + c] * f16_scale(*reinterpret_cast<const uint16_t*>(a.pool + at_scale[i] + c / 32 * 2))
-                                     : f16_scale(*reinterpret_cast<const uint16_t*>(a.pool + at_row[i] + 2 * c)));
+
+        v4f o[8][HT];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+#pragma unroll
+            for (int ht = 0; ht < HT; ++ht) o[c][ht] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        // Softmax state: this wave's rows 4 HT w .., kPer positions per lane.
+        constexpr uint32_t kPer = 2 * HT, kLanes = kMlaTile / kPer;
+        const uint32_t srow = wave * (4 * HT) + lane / kLanes, spos = (lane % kLanes) * kPer;
+        float m_run = -INFINITY, l_run = 0.0f;
+        int e_run = -100;  // Q8_0: scales so far are below 2^e_run
+
+        for (uint32_t i = 0; i < count; ++i) {
+            // ---- the wave's slice into LDS ----
+            uint8_t* const kv = s.kv[wave];
+            const uint32_t mask = live;
+            if constexpr (Q8) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t p = 8 * j + (lane >> 3), c = 2 * (lane & 7);
+                    uint4 x = codes8(pre[j].x, pre[j].y), y = codes8(pre[j].z, pre[j].w);
+                    if (mask != 0xFFFFFFFFu && !((mask >> p) & 1)) x = y = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(kv + p * 256 + ((c ^ (p & 15)) << 4)) = x;
+                    *reinterpret_cast<uint4*>(kv + p * 256 + (((c + 1) ^ (p & 15)) << 4)) = y;
+                }
+                float d[5];
+                const uint32_t p = lane & 31;
+                const bool dead = !((mask >> p) & 1);
+                d[0] = f16_scale((uint16_t)(pre_d.x & 0xFFFFu));
+                d[1] = f16_scale((uint16_t)(pre_d.x >> 16));
+                d[2] = f16_scale((uint16_t)(pre_d.y & 0xFFFFu));
+                d[3] = f16_scale((uint16_t)(pre_d.y >> 16));
+                d[4] = f16_scale((uint16_t)pre_dpe);
+                float top = 0.0f;
+#pragma unroll
+                for (int b = 0; b < 5; ++b) {
+                    if (dead) d[b] = 0.0f;
+                    if (b < 4) top = fmaxf(top, fabsf(d[b]));
+                }
+#pragma unroll
+                for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+                // f16 scales are below 2^16 (17: infinity).
+                const uint32_t tb = __builtin_amdgcn_readfirstlane(__float_as_uint(top));
+                const int e = tb == 0 ? -100 : min((int)(tb >> 23) - 126, 17);
+                if (e > e_run) {
+                    const float f2 = e_run == -100 ? 1.0f : pow2(e_run - e);
+                    e_run = e;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) o[c][ht] *= f2;
+                }
+                const float sv = pow2(14 - e_run);
+                if (lane < 32) {
+#pragma unroll
+                    for (int b = 0; b < 5; ++b) {
+                        s.ds[wave][b][p] = d[b];
+                        if (b < 4) s.dv[wave][b][p] = d[b] * sv;
+                    }
+                    uint4 x = codes8(pre_pe.x, pre_pe.y), y = codes8(pre_pe.z, pre_pe.w);
+                    if (dead) x = y = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(s.pe[wave] + p * 32) = x;
+                    *reinterpret_cast<uint4*>(s.pe[wave] + p * 32 + 16) = y;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t p = 4 * j + grp;
+                    uint4 x = pre[j];
+                    if (mask != 0xFFFFFFFFu && !((mask >> p) & 1)) x = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(kv + p * 256 + ((n16 ^ (p & 15)) << 4)) = x;
+                }
+                uint4 x = pre_pe;
+                if (!((mask >> (lane >> 1)) & 1)) x = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(s.pe[wave] + (lane >> 1) * 32 + (lane & 1) * 16) = x;
+            }
+            // The slice is read back through other types, by this wave alone.
+            asm volatile("" ::: "memory");
+            if (i + 1 < count) {
+                load_rows(tile0 + i + 1);
+                load_ids(tile0 + i + 2);
+            }
+
+            // ---- S^T partial ----
+#pragma unroll
+            for (int pt = 0; pt < 2; ++pt) {
+                v4f sc[HT];
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht) sc[ht] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+                const uint32_t p = pt * 16 + n16;
+#pragma unroll
+                for (uint32_t b = 0; b < 4; ++b) {
+                    if (!FULL && b >= blocks) continue;
+                    const v8h k = half8(*reinterpret_cast<const uint4*>(kv + p * 256 + (((4 * b + grp) ^ n16) << 4)));
+                    if constexpr (Q8) {
+                        const v4f d = *reinterpret_cast<const v4f*>(&s.ds[wave][b][pt * 16 + 4 * grp]);
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) {
+                            v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+                            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[ht][b], x, 0, 0, 0);
+                            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[ht][b], x, 0, 0, 0);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) sc[ht][e] = fmaf(d[e], x[e], sc[ht][e]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) {
+                            sc[ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[ht][b], sc[ht], 0, 0, 0);
+                            sc[ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[ht][b], sc[ht], 0, 0, 0);
+                        }
+                    }
+                }
+                if (has_pe) {
+                    const v4h k = __builtin_bit_cast(v4h, *reinterpret_cast<const uint2*>(s.pe[wave] + p * 32 + 8 * grp));
+                    if constexpr (Q8) {
+                        const v4f d = *reinterpret_cast<const v4f*>(&s.ds[wave][4][pt * 16 + 4 * grp]);
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) {
+                            v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+                            x = __builtin_amdgcn_mfma_f32_16x16x16f16(k, pel[ht], x, 0, 0, 0);
+                            x = __builtin_amdgcn_mfma_f32_16x16x16f16(k, peh[ht], x, 0, 0, 0);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) sc[ht][e] = fmaf(d[e], x[e], sc[ht][e]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) {
+                            sc[ht] = __builtin_amdgcn_mfma_f32_16x16x16f16(k, pel[ht], sc[ht], 0, 0, 0);
+                            sc[ht] = __builtin_amdgcn_mfma_f32_16x16x16f16(k, peh[ht], sc[ht], 0, 0, 0);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht)
+                    *reinterpret_cast<v4f*>(&s.sp[wave][ht * 16 + n16][pt * 16 + 4 * grp]) = sc[ht];
+            }
+            lds_barrier();
+
+            // ---- softmax of this wave's rows ----
+            {
+                const float fac = s.factor[srow];
+                float x[kPer], top = -INFINITY;
+#pragma unroll
+                for (uint32_t e = 0; e < kPer; ++e) x[e] = s.sp[0][srow][spos + e];
+#pragma unroll
+                for (uint32_t w = 1; w < kMlaWaves; ++w)
+#pragma unroll
+                    for (uint32_t e = 0; e < kPer; ++e) x[e] += s.sp[w][srow][spos + e];
+                const uint32_t lv = mask >> spos;
+#pragma unroll
+                for (uint32_t e = 0; e < kPer; ++e) {
+                    x[e] = (lv >> e) & 1 ? x[e] * fac : -INFINITY;
+                    top = fmaxf(top, x[e]);
+                }
+#pragma unroll
+                for (uint32_t d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+                const float m_new = fmaxf(m_run, top), base = m_new == -INFINITY ? 0.0f : m_new;
+                const float al = __builtin_amdgcn_exp2f(m_run - base);
+                float sum = 0.0f;
+#pragma unroll
+                for (uint32_t e = 0; e < kPer; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(x[e] - base);
+                    sum += x[e];
+                }
+#pragma unroll
+                for (uint32_t d = 1; d < kLanes; d <<= 1) sum += __shfl_xor(sum, d, 64);
+                l_run = l_run * al + sum;
+                m_run = m_new;
+                if (lane % kLanes == 0) s.alpha[srow] = al;
+                // position 16 h + 4 g + e is O^T's operand element 4 h + e of group g
+                const uint32_t at = ((spos >> 2) & 3) * 8 + (spos >> 4) * 4 + (spos & 3);
+                if constexpr (Q8) {
+                    float* dst = reinterpret_cast<float*>(s.p) + srow * 36 + at;
+#pragma unroll
+                    for (uint32_t e = 0; e < kPer; ++e) dst[e] = x[e];
+                } else {
+                    uint32_t* hi = s.p + srow * 20 + at / 2;
+                    uint32_t* lo = hi + kRows * 20;
+#pragma unroll
+                    for (uint32_t e = 0; e < kPer; e += 2) split2(x[e] * kPScale, x[e + 1] * kPScale, hi[e / 2], lo[e / 2]);
+                }
+            }
+            lds_barrier();
+
+            // ---- O^T += V^T P^T ----
+            {
+                float al[HT];
+                bool same = true;
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht) {
+                    al[ht] = s.alpha[ht * 16 + n16];
+                    same = same && al[ht] == 1.0f;
+                }
+                if (!__all(same)) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) o[c][ht] *= al[ht];
+                }
+                const auto values = [&](uint32_t c) {  // 16 columns, all 32 positions
+                    v4s t[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t p = 16 * h + 4 * grp + (n16 >> 2);
+                        const uint8_t* src = kv + p * 256 + (((2 * c + ((n16 >> 1) & 1)) ^ (p & 15)) << 4) + (n16 & 1) * 8;
+                        t[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)src);
+                    }
+                    const uint2 x = __builtin_bit_cast(uint2, t[0]), y = __builtin_bit_cast(uint2, t[1]);
+                    return half8(make_uint4(x.x, x.y, y.x, y.y));
+                };
+                if constexpr (Q8) {
+                    float p[HT][8];
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht) {
+                        const float* src = reinterpret_cast<const float*>(s.p) + (ht * 16 + n16) * 36 + grp * 8;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) p[ht][e] = src[e];
+                    }
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b) {
+                        if (!FULL && b >= blocks) continue;
+                        const v4f d0 = *reinterpret_cast<const v4f*>(&s.dv[wave][b][4 * grp]);
+                        const v4f d1 = *reinterpret_cast<const v4f*>(&s.dv[wave][b][16 + 4 * grp]);
+                        v8h ph[HT], plo[HT];
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) {
+                            uint32_t h[4], l[4];
+                            split2(p[ht][0] * d0[0], p[ht][1] * d0[1], h[0], l[0]);
+                            split2(p[ht][2] * d0[2], p[ht][3] * d0[3], h[1], l[1]);
+                            split2(p[ht][4] * d1[0], p[ht][5] * d1[1], h[2], l[2]);
+                            split2(p[ht][6] * d1[2], p[ht][7] * d1[3], h[3], l[3]);
+                            ph[ht] = half8(make_uint4(h[0], h[1], h[2], h[3]));
+                            plo[ht] = half8(make_uint4(l[0], l[1], l[2], l[3]));
+                        }
+#pragma unroll
+                        for (uint32_t c = 2 * b; c < 2 * b + 2; ++c) {
+                            const v8h v = values(c);
+#pragma unroll
+                            for (int ht = 0; ht < HT; ++ht) {
+                                o[c][ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, plo[ht], o[c][ht], 0, 0, 0);
+                                o[c][ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ht], o[c][ht], 0, 0, 0);
+                            }
+                        }
+                    }
+                } else {
+                    v8h ph[HT], plo[HT];
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht) {
+                        const uint32_t* src = s.p + (ht * 16 + n16) * 20 + grp * 4;
+                        ph[ht] = half8(*reinterpret_cast<const uint4*>(src));
+                        plo[ht] = half8(*reinterpret_cast<const uint4*>(src + kRows * 20));
+                    }
+#pragma unroll
+                    for (uint32_t c = 0; c < 8; ++c) {
+                        if (!FULL && c >= 2 * blocks) continue;
+                        const v8h v = values(c);
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) {
+                            o[c][ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, plo[ht], o[c][ht], 0, 0, 0);
+                            o[c][ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ht], o[c][ht], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+        }
+
+        // ---- the piece's result ----
+        if (lane % kLanes == 0) s.ml[srow] = make_float2(m_run, l_run);
+        lds_barrier();
+        const bool first = tile0 == 0, whole = first && count == n_tiles;
+        const float back = Q8 ? (e_run == -100 ? 0.0f : pow2(e_run - 14)) : 1.0f / kPScale;
+        const uint64_t slot = (uint64_t)wg * 2 + (first ? 1 : 0);
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht) {
+            const uint32_t r = ht * 16 + n16, h = head0 + r;
+            if (h >= a.n_heads) continue;
+            const float2 ml = s.ml[r];
+            float f2 = back;
+            float* dst;
+            if (whole) {
+                f2 = ml.y == 0.0f ? 0.0f : back / ml.y;
+                dst = a.out + (uint64_t)token * a.out_token_stride + (uint64_t)h * a.out_head_stride;
+                if (a.lse && wave == 0 && grp == 0)
+                    a.lse[(uint64_t)token * a.n_heads + h] =
+                        ml.y == 0.0f ? -INFINITY : 0.69314718055995f * (ml.x + __builtin_amdgcn_logf(ml.y));
+            } else {
+                dst = pl.parts + (slot * pl.part_rows + r) * g.rank;
+                if (wave == 0 && grp == 0) pl.part_ml[slot * kRows + r] = ml;
+            }
+            dst += wave * kMlaCols + 4 * grp;
+            const bool vec = whole ? pl.vec_out : true;
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c) {
+                if (!FULL && c >= 2 * blocks) continue;
+                const v4f v = o[c][ht] * f2;
+                if (vec) {
+                    *reinterpret_cast<v4f*>(dst + 16 * c) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dst[16 * c + e] = v[e];
+                }
+            }
+        }
+        if (first && !whole) {
+            begun.item = token * pl.head_tiles + ht_index;
+            begun.pieces = (uint32_t)((f + n_tiles - 1) / chunk) - wg + 1;
+        }
+        f += count;
+        off += count;
+        if (off == (uint64_t)n_tiles * pl.head_tiles) {
+            off = 0;
+            ++token;
+        }
+        lds_barrier();
+    }
+    if (tid == 0) splits[wg] = begun;
+
+    // ---- tokens that see nothing, 256 at a time ----
+    for (uint64_t t0 = (uint64_t)wg * kMlaThreads; t0 < a.n_tokens; t0 += (uint64_t)pl.groups * kMlaThreads) {
+        uint32_t row, bad = 0;
+        bool none = false;
+        if (t0 + tid < a.n_tokens) none = seen(a, (uint32_t)(t0 + tid), row, bad) == 0;
+        if (bad) report(a.status, bad == 1 ? kBadTableRow : kBadLength);
+        for (uint64_t todo = __ballot(none); todo; todo &= todo - 1) {
+            const uint64_t t = t0 + wave * 64 + __builtin_ctzll(todo);
+            for (uint32_t h = 0; h < a.n_heads; ++h) {
+                float* dst = a.out + t * a.out_token_stride + (uint64_t)h * a.out_head_stride;
+                for (uint32_t c = lane; c < g.rank; c += 64) dst[c] = 0.0f;
+                if (a.lse && lane == 0) a.lse[t * a.n_heads + h] = -INFINITY;
             }
         }
     }
-    for (int e = 0; e < 2; ++e) {
-        const uint32_t c = threadIdx.x + e * kMlaThreads;
-        if (c < g.rank) a.out[t * a.out_token_stride + h * a.out_head_stride + c] = l == 0.0f ? 0.0f : o[e] / l;
+}
+
+// Joins the pieces of split items, in order: out = sum_k w_k O_k / sum_k w_k l_k
+// with w_k = 2^(m_k - max m). Half-waves of 32 lanes take 128 columns of a
+// head each (16 bytes per lane); for an item of many pieces up to 32
+// half-waves share them and add their sums through LDS.
+__global__ __launch_bounds__(kJoinThreads) void mla_join_kernel(MlaArgs a, MlaPlan pl) {
+    __shared__ float sums[32][128];
+    __shared__ uint32_t list[kMlaMostGroups];
+    __shared__ uint32_t n_list;
+    const MlaSplit* splits = reinterpret_cast<const MlaSplit*>(pl.splits);
+    const uint32_t tid = threadIdx.x, hw = tid >> 5, l32 = tid & 31;
+    if (tid < 64) {  // the workgroups that begun an item they did not finish
+        uint32_t n = 0;
+        for (uint32_t g0 = 0; g0 < pl.groups; g0 += 64) {
+            const bool is = g0 + tid < pl.groups && splits[g0 + tid].pieces != 0;
+            const uint64_t b = __ballot(is);
+            if (is) list[n + __popcll(b & ((1ull << tid) - 1))] = g0 + tid;
+            n += __popcll(b);
+        }
+        if (tid == 0) n_list = n;
     }
-    if (a.lse && threadIdx.x == 0) a.lse[(uint64_t)t * a.n_heads + h] = l == 0.0f ? -INFINITY : m + logf(l);
+    __syncthreads();
+    const uint32_t rank = a.geom.rank, parts = (rank + 127) / 128;
+    uint32_t job = blockIdx.x;
+    for (uint32_t k = 0; k < n_list; ++k) {
+        const uint32_t g0 = list[k];
+        const MlaSplit sp = splits[g0];
+        const uint32_t token = sp.item / pl.head_tiles, head0 = (sp.item % pl.head_tiles) * pl.rows;
+        const uint32_t heads = min(pl.rows, a.n_heads - head0);
+        uint32_t share = 1;  // half-waves per head and 128 columns
+        while (share < 32 && share * 8 < sp.pieces) share *= 2;
+        const uint32_t per_wg = 32 / share, units = heads * parts, jobs = (units + per_wg - 1) / per_wg;
+        for (; job < jobs; job += gridDim.x) {
+            const uint32_t unit = job * per_wg + hw / share, mine = hw % share;
+            const bool on = unit < units;
+            const uint32_t r = on ? unit / parts : 0, c = (on ? unit % parts : 0) * 128 + l32 * 4;
+            float top = -INFINITY;
+            for (uint32_t p = 0; p < sp.pieces; p += 32) {
+                const uint32_t q = p + l32;
+                if (q < sp.pieces) top = fmaxf(top, pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + r].x);
+            }
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+            const float base = top == -INFINITY ? 0.0f : top;
+            float l = 0.0f;
+            v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t p = 0; p < sp.pieces; ++p) {
+                const uint64_t slot = (uint64_t)(g0 + p) * 2 + (p == 0);
+                const float2 ml = pl.part_ml[slot * pl.rows + r];
+                const float w = __builtin_amdgcn_exp2f(ml.x - base);
+                l += w * ml.y;
+                if (p % share == mine && on && c < rank) {
+                    const v4f v = *reinterpret_cast<const v4f*>(pl.parts + (slot * pl.part_rows + r) * rank + c);
+                    acc += v * w;
+                }
+            }
+            if (share > 1) {
+                __syncthreads();
+                *reinterpret_cast<v4f*>(&sums[hw][l32 * 4]) = acc;
+                __syncthreads();
+                if (mine == 0)
+                    for (uint32_t i = 1; i < share; ++i) acc += *reinterpret_cast<const v4f*>(&sums[hw + i][l32 * 4]);
+            }
+            if (mine == 0 && on && c < rank) {
+                const v4f v = l == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc / l;
+                float* dst = a.out + (uint64_t)token * a.out_token_stride + (uint64_t)(head0 + r) * a.out_head_stride + c;
+                if (pl.vec_out) {
+                    *reinterpret_cast<v4f*>(dst) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dst[e] = v[e];
+                }
+                if (a.lse && c == 0)
+                    a.lse[(uint64_t)token * a.n_heads + head0 + r] =
+                        l == 0.0f ? -INFINITY : 0.69314718055995f * (top + __builtin_amdgcn_logf(l));
+            }
+        }
+        job -= jobs;
+    }
+}
+
+// Two workgroups per CU, whatever the call: its lengths are known on the
+// device alone.
+uint32_t mla_groups(int num_cu) { return num_cu * 2 < (int)kMlaMostGroups ? (uint32_t)num_cu * 2 : kMlaMostGroups; }
+uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
+
+struct MlaLayout {
+    uint32_t groups, rows, head_tiles, part_rows;
+    uint64_t parts, ml, splits, bytes;
+};
+MlaLayout mla_layout(uint32_t n_heads, uint32_t rank, int num_cu) {
+    MlaLayout w;
+    w.groups = mla_groups(num_cu);
+    w.rows = n_heads <= 16 ? 16 : 32;
+    w.head_tiles = (n_heads + w.rows - 1) / w.rows;
+    w.part_rows = n_heads < w.rows ? n_heads : w.rows;
+    w.parts = 0;
+    w.ml = up256(2ull * w.groups * w.part_rows * rank * 4);
+    w.splits = w.ml + up256(2ull * w.groups * w.rows * 8);
+    w.bytes = w.splits + up256(w.groups * sizeof(MlaSplit));
+    return w;
+}
+
+template <bool Q8>
+void launch_split(const MlaArgs& a, const MlaPlan& p, hipStream_t s) {
+    const bool full = a.geom.rank == 512 && a.geom.width == 576;
+    if (p.rows == 16) {
+        if (full) mla_split_kernel<Q8, 1, true><<<p.groups, kMlaThreads, 0, s>>>(a, p);
+        else mla_split_kernel<Q8, 1, false><<<p.groups, kMlaThreads, 0, s>>>(a, p);
+    } else {
+        if (full) mla_split_kernel<Q8, 2, true><<<p.groups, kMlaThreads, 0, s>>>(a, p);
+        else mla_split_kernel<Q8, 2, false><<<p.groups, kMlaThreads, 0, s>>>(a, p);
+    }
 }
 
 }  // namespace
 
-uint64_t mla_workspace_bytes(uint32_t, uint32_t, uint32_t, int) { return 0; }
+uint64_t mla_workspace_bytes(uint32_t n_tokens, uint32_t n_heads, uint32_t rank, int num_cu) {
+    if (n_tokens == 0 || n_heads == 0 || rank == 0) return 0;
+    return mla_layout(n_heads, rank, num_cu).bytes;
+}
 
 hipError_t launch_mla(const MlaArgs& a, hipStream_t s) {
     if (a.n_tokens == 0 || a.n_heads == 0) return hipSuccess;
-    mla_simple_kernel<<<a.n_tokens * a.n_heads, kMlaThreads, 0, s>>>(a);
+    const MlaLayout w = mla_layout(a.n_heads, a.geom.rank, a.num_cu);
+    char* base = static_cast<char*>(a.work);
+    MlaPlan p{};
+    p.groups = w.groups;
+    p.rows = w.rows;
+    p.head_tiles = w.head_tiles;
+    p.part_rows = w.part_rows;
+    p.parts = reinterpret_cast<float*>(base + w.parts);
+    p.part_ml = reinterpret_cast<float2*>(base + w.ml);
+    p.splits = base + w.splits;
+    const auto aligned = [](const void* q, uint64_t s0, uint64_t s1) {
+        return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && s0 % 4 == 0 && s1 % 4 == 0;
+    };
+    p.vec_q = aligned(a.q, a.q_token_stride, a.q_head_stride);
+    p.vec_out = aligned(a.out, a.out_token_stride, a.out_head_stride);
+    if (a.geom.q8) launch_split<true>(a, p, s);
+    else launch_split<false>(a, p, s);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    mla_join_kernel<<<a.num_cu, kJoinThreads, 0, s>>>(a, p);
     return hipGetLastError();
 }
 
