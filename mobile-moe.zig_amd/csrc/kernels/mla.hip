@@ -72,7 +72,7 @@ struct MlaLds {
     float2 ml[16 * HT];
     uint64_t scan[kMlaWaves];
     uint64_t start_off;
-    uint32_t start_token;
+    uint32_t start_token, start_row, start_len;
 };
 
 __device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (uint32_t)(((uint64_t)len + kMlaTile - 1) / kMlaTile); }
@@ -124,9 +124,11 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         const uint32_t per = (a.n_tokens + kMlaThreads - 1) / kMlaThreads;
         const uint64_t t0 = (uint64_t)tid * per;
         uint64_t mine = 0;
+        uint32_t last_row = 0, last_len = 0;
         for (uint64_t t = t0; t < t0 + per && t < a.n_tokens; ++t) {
-            uint32_t row, bad;
-            mine += tiles_of(seen(a, (uint32_t)t, row, bad));
+            uint32_t bad;
+            last_len = seen(a, (uint32_t)t, last_row, bad);
+            mine += tiles_of(last_len);
         }
         mine *= pl.head_tiles;
         uint64_t incl = mine;
@@ -150,14 +152,19 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         end = f + chunk < total ? f + chunk : total;
         if (f < end && incl - mine <= f && f < incl) {
             uint64_t at = incl - mine;
-            uint32_t t = (uint32_t)t0;
-            for (; t + 1 < a.n_tokens; ++t) {
-                uint32_t row, bad;
-                const uint64_t n = (uint64_t)tiles_of(seen(a, t, row, bad)) * pl.head_tiles;
-                if (f < at + n) break;
-                at += n;
+            uint32_t t = (uint32_t)t0, row = last_row, len = last_len;
+            if (per > 1) {
+                uint32_t bad;
+                for (;; ++t) {
+                    len = seen(a, t, row, bad);
+                    const uint64_t n = (uint64_t)tiles_of(len) * pl.head_tiles;
+                    if (f < at + n || t + 1 >= a.n_tokens) break;
+                    at += n;
+                }
             }
             s.start_token = t;
+            s.start_row = row;
+            s.start_len = len;
             s.start_off = f - at;
         }
         __syncthreads();
@@ -171,15 +178,20 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 
     uint32_t token = f < end ? s.start_token : 0;
     uint64_t off = f < end ? s.start_off : 0;
+    uint32_t row = s.start_row, len = s.start_len, of_token = token;
     while (f < end && token < a.n_tokens) {
-        uint32_t row, bad;
-        const uint32_t len = __builtin_amdgcn_readfirstlane(seen(a, token, row, bad));
+        if (token != of_token) {
+            uint32_t bad;
+            len = seen(a, token, row, bad);
+            of_token = token;
+        }
+        len = __builtin_amdgcn_readfirstlane(len);
+        row = __builtin_amdgcn_readfirstlane(row);
         const uint32_t n_tiles = tiles_of(len);
         if (n_tiles == 0) {
             ++token;
             continue;
         }
-        row = __builtin_amdgcn_readfirstlane(row);
         const uint32_t ht_index = (uint32_t)(off / n_tiles), tile0 = (uint32_t)(off - (uint64_t)ht_index * n_tiles);
         const uint32_t count = (uint32_t)(end - f < n_tiles - tile0 ? end - f : n_tiles - tile0);
         const uint32_t head0 = ht_index * kRows;
@@ -255,51 +267,86 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             }
         };
         load_ids(tile0);
-        load_rows(tile0);
-        load_ids(tile0 + 1);
 
         // ---- the queries, scaled by a power of two per head, in two parts ----
         v8h qh[HT][4], ql[HT][4];
         v4h peh[HT], pel[HT];
         {
-            float q[HT][4][8], pe[HT][4], top[HT];
+            // Every load is issued whether its head exists or not (the last
+            // head's again, zeroed below): a load under a branch would be
+            // waited for at the branch's end, together with the rows.
+            float q[HT][4][8], pe[HT][4];
+            const float *src[HT], *src_pe[HT];
 #pragma unroll
             for (int ht = 0; ht < HT; ++ht) {
-                const uint32_t h = head0 + ht * 16 + n16;
-                const bool there = h < a.n_heads;
-                const float* src = a.q + (uint64_t)token * a.q_token_stride + (uint64_t)(there ? h : 0) * a.q_head_stride +
-                                   wave * kMlaCols + 8 * grp;
-                const float* src_pe = a.q_pe + (uint64_t)token * a.q_pe_token_stride +
-                                      (uint64_t)(there ? h : 0) * a.q_pe_head_stride + wave * kMlaPe + 4 * grp;
-                top[ht] = 0.0f;
+                const uint32_t h = min(head0 + ht * 16 + n16, a.n_heads - 1);
+                src[ht] = a.q + (uint64_t)token * a.q_token_stride + (uint64_t)h * a.q_head_stride + wave * kMlaCols + 8 * grp;
+                src_pe[ht] = a.q_pe + (uint64_t)token * a.q_pe_token_stride + (uint64_t)h * a.q_pe_head_stride + wave * kMlaPe + 4 * grp;
+            }
 #pragma unroll
-                for (uint32_t b = 0; b < 4; ++b) {
-                    if (there && (FULL || b < blocks)) {
-                        if (pl.vec_q) {
-                            const float4 x = *reinterpret_cast<const float4*>(src + 32 * b);
-                            const float4 y = *reinterpret_cast<const float4*>(src + 32 * b + 4);
-                            q[ht][b][0] = x.x, q[ht][b][1] = x.y, q[ht][b][2] = x.z, q[ht][b][3] = x.w;
-                            q[ht][b][4] = y.x, q[ht][b][5] = y.y, q[ht][b][6] = y.z, q[ht][b][7] = y.w;
-                        } else {
+            for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) q[ht][b][e] = src[32 * b + e];
-                        }
-                    } else {
+                for (int e = 0; e < 4; ++e) pe[ht][e] = 0.0f;
+            if (!FULL) {
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) q[ht][b][e] = 0.0f;
+            }
+            if (pl.vec_q) {
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b) {
+                        if (!FULL && b >= blocks) continue;
+                        const float4 x = *reinterpret_cast<const float4*>(src[ht] + 32 * b);
+                        const float4 y = *reinterpret_cast<const float4*>(src[ht] + 32 * b + 4);
+                        q[ht][b][0] = x.x, q[ht][b][1] = x.y, q[ht][b][2] = x.z, q[ht][b][3] = x.w;
+                        q[ht][b][4] = y.x, q[ht][b][5] = y.y, q[ht][b][6] = y.z, q[ht][b][7] = y.w;
+                    }
+                    if (has_pe) {
+                        const float4 x = *reinterpret_cast<const float4*>(src_pe[ht]);
+                        pe[ht][0] = x.x, pe[ht][1] = x.y, pe[ht][2] = x.z, pe[ht][3] = x.w;
                     }
                 }
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) pe[ht][e] = there && has_pe ? src_pe[e] : 0.0f;
+                for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b) {
+                        if (!FULL && b >= blocks) continue;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) q[ht][b][e] = src[ht][32 * b + e];
+                    }
+                    if (has_pe) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) pe[ht][e] = src_pe[ht][e];
+                    }
+                }
+            }
+            load_rows(tile0);
+            load_ids(tile0 + 1);
+#pragma unroll
+            for (int ht = 0; ht < HT; ++ht) {
+                const bool there = head0 + ht * 16 + n16 < a.n_heads;
+                float top = 0.0f;
 #pragma unroll
                 for (int b = 0; b < 4; ++b)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top[ht] = fmaxf(top[ht], fabsf(q[ht][b][e]));
+                    for (int e = 0; e < 8; ++e) {
+                        q[ht][b][e] = there ? q[ht][b][e] : 0.0f;
+                        top = fmaxf(top, fabsf(q[ht][b][e]));
+                    }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top[ht] = fmaxf(top[ht], fabsf(pe[ht][e]));
-                top[ht] = fmaxf(top[ht], __shfl_xor(top[ht], 16, 64));
-                top[ht] = fmaxf(top[ht], __shfl_xor(top[ht], 32, 64));
-                if (grp == 0) s.qmax[wave][ht * 16 + n16] = top[ht];
+                for (int e = 0; e < 4; ++e) {
+                    pe[ht][e] = there ? pe[ht][e] : 0.0f;
+                    top = fmaxf(top, fabsf(pe[ht][e]));
+                }
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                if (grp == 0) s.qmax[wave][ht * 16 + n16] = top;
             }
             lds_barrier();
 #pragma unroll
@@ -664,56 +711,86 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 // head each (16 bytes per lane); for an item of many pieces up to 32
 // half-waves share them and add their sums through LDS.
 __global__ __launch_bounds__(kJoinThreads) void mla_join_kernel(MlaArgs a, MlaPlan pl) {
-    __shared__ float sums[32][128];
-    __shared__ uint32_t list[kMlaMostGroups];
-    __shared__ uint32_t n_list;
-    const MlaSplit* splits = reinterpret_cast<const MlaSplit*>(pl.splits);
-    const uint32_t tid = threadIdx.x, hw = tid >> 5, l32 = tid & 31;
-    if (tid < 64) {  // the workgroups that begun an item they did not finish
-        uint32_t n = 0;
-        for (uint32_t g0 = 0; g0 < pl.groups; g0 += 64) {
-            const bool is = g0 + tid < pl.groups && splits[g0 + tid].pieces != 0;
-            const uint64_t b = __ballot(is);
-            if (is) list[n + __popcll(b & ((1ull << tid) - 1))] = g0 + tid;
-            n += __popcll(b);
-        }
-        if (tid == 0) n_list = n;
-    }
-    __syncthreads();
+    __shared__ __align__(16) float sums[32][128];
+    // A job's rows times its pieces: at most 32 / (4 share) + 2 rows of 8 share
+    // pieces (parts = 4), 32 / share + 1 rows (parts = 1), or one row of all.
+    __shared__ float weights[kMlaMostGroups];
+    __shared__ float2 row_ml[33];
+    __shared__ uint32_t scan[kJoinThreads / 64];
+    __shared__ uint32_t cur[4];
+    const uint32_t tid = threadIdx.x, hw = tid >> 5, l32 = tid & 31, wave = tid >> 6;
     const uint32_t rank = a.geom.rank, parts = (rank + 127) / 128;
-    uint32_t job = blockIdx.x;
-    for (uint32_t k = 0; k < n_list; ++k) {
-        const uint32_t g0 = list[k];
-        const MlaSplit sp = splits[g0];
-        const uint32_t token = sp.item / pl.head_tiles, head0 = (sp.item % pl.head_tiles) * pl.rows;
-        const uint32_t heads = min(pl.rows, a.n_heads - head0);
-        uint32_t share = 1;  // half-waves per head and 128 columns
-        while (share < 32 && share * 8 < sp.pieces) share *= 2;
-        const uint32_t per_wg = 32 / share, units = heads * parts, jobs = (units + per_wg - 1) / per_wg;
-        for (; job < jobs; job += gridDim.x) {
+    // Thread g knows the item that workgroup g began and did not finish, and
+    // which of the call's jobs are that item's.
+    MlaSplit sp{0, 0};
+    if (tid < pl.groups) sp = reinterpret_cast<const MlaSplit*>(pl.splits)[tid];
+    uint32_t share = 1;  // half-waves per head and 128 columns
+    while (share < 32 && share * 8 < sp.pieces) share *= 2;
+    const uint32_t heads_of = min(pl.rows, a.n_heads - (sp.item % pl.head_tiles) * pl.rows);
+    const uint32_t my_jobs = sp.pieces ? (heads_of * parts * share + 31) / 32 : 0;
+    uint32_t end = my_jobs;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t o = __shfl_up(end, off, 64);
+        if ((int)(tid & 63) >= off) end += o;
+    }
+    if ((tid & 63) == 63) scan[wave] = end;
+    __syncthreads();
+    uint32_t total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kJoinThreads / 64; ++w) {
+        if (w < wave) end += scan[w];
+        total += scan[w];
+    }
+    for (uint32_t all_job = blockIdx.x; all_job < total; all_job += gridDim.x) {
+        __syncthreads();
+        if (all_job < end && all_job >= end - my_jobs) {
+            cur[0] = tid;
+            cur[1] = sp.item;
+            cur[2] = sp.pieces;
+            cur[3] = all_job - (end - my_jobs);
+        }
+        __syncthreads();
+        {
+            const uint32_t g0 = cur[0], item = cur[1], pieces = cur[2], job = cur[3];
+            const uint32_t token = item / pl.head_tiles, head0 = (item % pl.head_tiles) * pl.rows;
+            const uint32_t heads = min(pl.rows, a.n_heads - head0);
+            uint32_t share = 1;
+            while (share < 32 && share * 8 < pieces) share *= 2;
+            const uint32_t per_wg = 32 / share, units = heads * parts;
             const uint32_t unit = job * per_wg + hw / share, mine = hw % share;
             const bool on = unit < units;
-            const uint32_t r = on ? unit / parts : 0, c = (on ? unit % parts : 0) * 128 + l32 * 4;
-            float top = -INFINITY;
-            for (uint32_t p = 0; p < sp.pieces; p += 32) {
-                const uint32_t q = p + l32;
-                if (q < sp.pieces) top = fmaxf(top, pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + r].x);
-            }
+            const uint32_t r0 = job * per_wg / parts, r1 = min((job + 1) * per_wg - 1, units - 1) / parts;
+            const uint32_t r = on ? unit / parts : r0, c = (on ? unit % parts : 0) * 128 + l32 * 4;
+            // The weights of this job's rows, a half-wave each.
+            for (uint32_t i = r0 + hw; i <= r1; i += 32) {
+                float top = -INFINITY, l = 0.0f;
+                for (uint32_t q = l32; q < pieces; q += 32)
+                    top = fmaxf(top, pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + i].x);
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-            const float base = top == -INFINITY ? 0.0f : top;
-            float l = 0.0f;
-            v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (uint32_t p = 0; p < sp.pieces; ++p) {
-                const uint64_t slot = (uint64_t)(g0 + p) * 2 + (p == 0);
-                const float2 ml = pl.part_ml[slot * pl.rows + r];
-                const float w = __builtin_amdgcn_exp2f(ml.x - base);
-                l += w * ml.y;
-                if (p % share == mine && on && c < rank) {
-                    const v4f v = *reinterpret_cast<const v4f*>(pl.parts + (slot * pl.part_rows + r) * rank + c);
-                    acc += v * w;
+                for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+                const float base = top == -INFINITY ? 0.0f : top;
+                for (uint32_t q = l32; q < pieces; q += 32) {
+                    const float2 ml = pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + i];
+                    const float w = __builtin_amdgcn_exp2f(ml.x - base);
+                    weights[(i - r0) * pieces + q] = w;
+                    l += w * ml.y;
                 }
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) l += __shfl_xor(l, d, 64);
+                if (l32 == 0) row_ml[i - r0] = make_float2(top, l);
             }
+            __syncthreads();
+            v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (on && c < rank) {
+                const float* src = pl.parts + ((uint64_t)g0 * 2 * pl.part_rows + r) * rank + c;
+                const uint64_t step = 2ull * pl.part_rows * rank, own = (uint64_t)pl.part_rows * rank;
+                const float* w = weights + (r - r0) * pieces;
+#pragma unroll 8
+                for (uint32_t p = mine; p < pieces; p += share)
+                    acc += *reinterpret_cast<const v4f*>(src + p * step + (p == 0 ? own : 0)) * w[p];
+            }
+            const float top = row_ml[r - r0].x, l = row_ml[r - r0].y;
             if (share > 1) {
                 __syncthreads();
                 *reinterpret_cast<v4f*>(&sums[hw][l32 * 4]) = acc;
@@ -735,7 +812,6 @@ __global__ __launch_bounds__(kJoinThreads) void mla_join_kernel(MlaArgs a, MlaPl
                         l == 0.0f ? -INFINITY : 0.69314718055995f * (top + __builtin_amdgcn_logf(l));
             }
         }
-        job -= jobs;
     }
 }
 
@@ -795,7 +871,8 @@ hipError_t launch_mla(const MlaArgs& a, hipStream_t s) {
     const auto aligned = [](const void* q, uint64_t s0, uint64_t s1) {
         return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && s0 % 4 == 0 && s1 % 4 == 0;
     };
-    p.vec_q = aligned(a.q, a.q_token_stride, a.q_head_stride);
+    p.vec_q = aligned(a.q, a.q_token_stride, a.q_head_stride) &&
+              (a.geom.width == a.geom.rank || aligned(a.q_pe, a.q_pe_token_stride, a.q_pe_head_stride));
     p.vec_out = aligned(a.out, a.out_token_stride, a.out_head_stride);
     if (a.geom.q8) launch_split<true>(a, p, s);
     else launch_split<false>(a, p, s);
