@@ -418,7 +418,7 @@ struct MlaArgs {
 constexpr uint32_t kMlaMostGroups = 1024;
 struct MlaPlan {
     uint32_t groups;      // workgroups that share the list of tiles
-    uint32_t rows;        // heads per head tile: 16 or 32
+    uint32_t rows;        // heads per head tile
     uint32_t head_tiles;
     uint32_t part_rows;   // rows of a piece in the workspace: min(rows, n_heads)
     float* parts;         // [groups][2][part_rows][rank]: a piece that begins its item is the second

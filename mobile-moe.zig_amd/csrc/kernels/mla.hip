@@ -5,9 +5,12 @@
 // maximum and sum of the softmax; all heads of a token share the read rows.
 //
 // Bound: HBM. A row of 512 + 64 values is 1152 B in f16 (612 B in Q8_0) and
-// costs 2 x 20 x 1088 operations. The matrix work is up to four times that
-// (heads padded to 32, and the f32 operands of each product in two f16 parts,
-// 22 bits; the cached values are exact in f16), still below the rows' time.
+// costs 2 x 20 x 1088 operations. The matrix work is more than that: the f32
+// operand of each product enters as two f16 parts (22 bits; the cached values
+// are exact in f16), and heads come in tiles of 16. From 17 to 24 heads the
+// second tile holds up to 8 heads' high parts in its first half and their low
+// parts in the other, one product in place of two (kPacked): a quarter of the
+// matrix work and of the queries' registers less at 20 heads.
 //
 // A workgroup is four waves and takes tiles of 32 positions. Wave w owns the
 // latent columns 128 w .. 128 w + 127 and 16 of the rotary ones, both as keys
@@ -40,7 +43,6 @@ namespace mmhip {
 namespace {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
@@ -59,17 +61,23 @@ struct MlaSplit {
     uint32_t item, pieces;
 };
 
-template <bool Q8, int HT>
+// Heads per head tile: one product tile of 16, two, or one and a packed one.
+enum MlaMode : int { kOne = 0, kTwo = 1, kPacked = 2 };
+constexpr int mode_tiles(int mode) { return mode == kOne ? 1 : 2; }
+constexpr uint32_t mode_rows(int mode) { return mode == kOne ? 16 : mode == kTwo ? 32 : 24; }
+
+template <bool Q8, int MODE>
 struct MlaLds {
+    static constexpr int NT = mode_tiles(MODE);
     uint8_t kv[kMlaWaves][kMlaTile * 256];  // f16 [position][128], 16-byte chunks swizzled by the position
     uint8_t pe[kMlaWaves][kMlaTile * 32];   // f16 [position][16]
-    float sp[kMlaWaves][16 * HT][kSpLd];
-    // P: f16 parts (hi, lo) in rows of 40, or f32 in rows of 36
-    uint32_t p[Q8 ? 16 * HT * 36 : 2 * 16 * HT * 20];
+    float sp[kMlaWaves][16 * NT][kSpLd];    // score partials, a row per product column
+    // P: f16 in rows of 40 (per tile high parts, low parts; packed as it is), or f32 per head in rows of 36
+    uint32_t p[Q8 ? mode_rows(MODE) * 36 : (MODE == kTwo ? 4 : MODE == kPacked ? 3 : 2) * 16 * 20];
     float ds[Q8 ? kMlaWaves : 1][5][kMlaTile];  // block scales of the keys
     float dv[Q8 ? kMlaWaves : 1][4][kMlaTile];  // of the values, scaled into range
-    float alpha[16 * HT], factor[16 * HT], qmax[kMlaWaves][16 * HT];
-    float2 ml[16 * HT];
+    float alpha[16 * NT], factor[16 * NT], qmax[kMlaWaves][16 * NT];
+    float2 ml[16 * NT];
     uint64_t scan[kMlaWaves];
     uint64_t start_off;
     uint32_t start_token, start_row, start_len;
@@ -108,18 +116,23 @@ __device__ __forceinline__ v8h half8(const uint4& v) { return __builtin_bit_cast
 // 2^e, e within f32's normal exponents.
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-template <bool Q8, int HT, bool FULL>
+template <bool Q8, int MODE, bool FULL>
 __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, MlaPlan pl) {
-    constexpr int kRows = 16 * HT;
-    __shared__ __align__(16) MlaLds<Q8, HT> s;
+    constexpr int NT = mode_tiles(MODE);       // product tiles of 16 columns
+    constexpr uint32_t kHeads = mode_rows(MODE);
+    __shared__ __align__(256) MlaLds<Q8, MODE> s;
     const PagedGeom g = a.geom;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t n16 = lane & 15, grp = lane >> 4;
     const uint32_t wg = blockIdx.x;
     MlaSplit* const splits = reinterpret_cast<MlaSplit*>(pl.splits);
+    // The head (of the head tile) behind column n16 of product tile t; in a
+    // packed tile column 8 + k has head k's low parts.
+    const bool low_half = n16 >= 8;
+    const auto head_of = [&](int t) { return MODE == kPacked && t == 1 ? 16 + (n16 & 7) : 16 * t + n16; };
 
     // ---- this workgroup's run of the list ----
-    uint64_t f, end, total;
+    uint64_t f, end, total, chunk;
     {
         const uint32_t per = (a.n_tokens + kMlaThreads - 1) / kMlaThreads;
         const uint64_t t0 = (uint64_t)tid * per;
@@ -147,7 +160,8 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             total += s.scan[w];
         }
         incl += before;
-        const uint64_t chunk = (total + pl.groups - 1) / pl.groups;
+        // (a 64-bit division is some 150 instructions)
+        chunk = total < 0x80000000u ? ((uint32_t)total + pl.groups - 1) / pl.groups : (total + pl.groups - 1) / pl.groups;
         f = wg * chunk;
         end = f + chunk < total ? f + chunk : total;
         if (f < end && incl - mine <= f && f < incl) {
@@ -170,7 +184,6 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         __syncthreads();
     }
     MlaSplit begun{0, 0};
-    const uint64_t chunk = (total + pl.groups - 1) / pl.groups;
 
     const uint32_t row_bytes = Q8 ? g.width : 2 * g.width, at_mask = (1u << g.page_shift) - 1;
     const uint32_t blocks = FULL ? 4u : (g.rank / 32 > 4 * wave ? min(g.rank / 32 - 4 * wave, 4u) : 0u);
@@ -192,9 +205,10 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             ++token;
             continue;
         }
-        const uint32_t ht_index = (uint32_t)(off / n_tiles), tile0 = (uint32_t)(off - (uint64_t)ht_index * n_tiles);
+        const uint32_t ht_index = pl.head_tiles == 1 ? 0u : (uint32_t)(off / n_tiles);
+        const uint32_t tile0 = (uint32_t)(off - (uint64_t)ht_index * n_tiles);
         const uint32_t count = (uint32_t)(end - f < n_tiles - tile0 ? end - f : n_tiles - tile0);
-        const uint32_t head0 = ht_index * kRows;
+        const uint32_t head0 = ht_index * kHeads;
         const int32_t* table = a.tables + (uint64_t)row * a.table_stride;
 
         // ---- loads of a tile: page numbers one tile before its rows ----
@@ -266,151 +280,40 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                                                              2 * g.rank + wave * (2 * kMlaPe) + (lane & 1) * 16);
             }
         };
-        load_ids(tile0);
-
-        // ---- the queries, scaled by a power of two per head, in two parts ----
-        v8h qh[HT][4], ql[HT][4];
-        v4h peh[HT], pel[HT];
-        {
-            // Every load is issued whether its head exists or not (the last
-            // head's again, zeroed below): a load under a branch would be
-            // waited for at the branch's end, together with the rows.
-            float q[HT][4][8], pe[HT][4];
-            const float *src[HT], *src_pe[HT];
-#pragma unroll
-            for (int ht = 0; ht < HT; ++ht) {
-                const uint32_t h = min(head0 + ht * 16 + n16, a.n_heads - 1);
-                src[ht] = a.q + (uint64_t)token * a.q_token_stride + (uint64_t)h * a.q_head_stride + wave * kMlaCols + 8 * grp;
-                src_pe[ht] = a.q_pe + (uint64_t)token * a.q_pe_token_stride + (uint64_t)h * a.q_pe_head_stride + wave * kMlaPe + 4 * grp;
-            }
-#pragma unroll
-            for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) pe[ht][e] = 0.0f;
-            if (!FULL) {
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                    for (int b = 0; b < 4; ++b)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) q[ht][b][e] = 0.0f;
-            }
-            if (pl.vec_q) {
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht) {
-#pragma unroll
-                    for (uint32_t b = 0; b < 4; ++b) {
-                        if (!FULL && b >= blocks) continue;
-                        const float4 x = *reinterpret_cast<const float4*>(src[ht] + 32 * b);
-                        const float4 y = *reinterpret_cast<const float4*>(src[ht] + 32 * b + 4);
-                        q[ht][b][0] = x.x, q[ht][b][1] = x.y, q[ht][b][2] = x.z, q[ht][b][3] = x.w;
-                        q[ht][b][4] = y.x, q[ht][b][5] = y.y, q[ht][b][6] = y.z, q[ht][b][7] = y.w;
-                    }
-                    if (has_pe) {
-                        const float4 x = *reinterpret_cast<const float4*>(src_pe[ht]);
-                        pe[ht][0] = x.x, pe[ht][1] = x.y, pe[ht][2] = x.z, pe[ht][3] = x.w;
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht) {
-#pragma unroll
-                    for (uint32_t b = 0; b < 4; ++b) {
-                        if (!FULL && b >= blocks) continue;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) q[ht][b][e] = src[ht][32 * b + e];
-                    }
-                    if (has_pe) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) pe[ht][e] = src_pe[ht][e];
-                    }
-                }
-            }
-            load_rows(tile0);
-            load_ids(tile0 + 1);
-#pragma unroll
-            for (int ht = 0; ht < HT; ++ht) {
-                const bool there = head0 + ht * 16 + n16 < a.n_heads;
-                float top = 0.0f;
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        q[ht][b][e] = there ? q[ht][b][e] : 0.0f;
-                        top = fmaxf(top, fabsf(q[ht][b][e]));
-                    }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    pe[ht][e] = there ? pe[ht][e] : 0.0f;
-                    top = fmaxf(top, fabsf(pe[ht][e]));
-                }
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                if (grp == 0) s.qmax[wave][ht * 16 + n16] = top;
-            }
-            lds_barrier();
-#pragma unroll
-            for (int ht = 0; ht < HT; ++ht) {
-                const uint32_t r = ht * 16 + n16;
-                const float m = fmaxf(fmaxf(s.qmax[0][r], s.qmax[1][r]), fmaxf(s.qmax[2][r], s.qmax[3][r]));
-                // m 2^e in [2^13, 2^14) for m within f32's middle range
-                const int e = m > 0.0f ? min(max(140 - (int)(__float_as_uint(m) >> 23), -115), 115) : 0;
-                const float sc = pow2(e);
-                if (wave == 0 && grp == 0) s.factor[r] = a.scale * 1.44269504088896f * pow2(-e);
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    uint32_t h[4], l[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) split2(q[ht][b][2 * i] * sc, q[ht][b][2 * i + 1] * sc, h[i], l[i]);
-                    qh[ht][b] = half8(make_uint4(h[0], h[1], h[2], h[3]));
-                    ql[ht][b] = half8(make_uint4(l[0], l[1], l[2], l[3]));
-                }
-                uint32_t h[2], l[2];
-                split2(pe[ht][0] * sc, pe[ht][1] * sc, h[0], l[0]);
-                split2(pe[ht][2] * sc, pe[ht][3] * sc, h[1], l[1]);
-                peh[ht] = __builtin_bit_cast(v4h, make_uint2(h[0], h[1]));
-                pel[ht] = __builtin_bit_cast(v4h, make_uint2(l[0], l[1]));
-            }
-        }
-
-        v4f o[8][HT];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-#pragma unroll
-            for (int ht = 0; ht < HT; ++ht) o[c][ht] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-        // Softmax state: this wave's rows 4 HT w .., kPer positions per lane.
-        constexpr uint32_t kPer = 2 * HT, kLanes = kMlaTile / kPer;
-        const uint32_t srow = wave * (4 * HT) + lane / kLanes, spos = (lane % kLanes) * kPer;
-        float m_run = -INFINITY, l_run = 0.0f;
+        // The wave's slice of the tile in registers -> LDS, in f16. Positions
+        // that count for nothing (past the length, on a page that is not
+        // there) become zeros: their bytes may be anything.
+        uint8_t* const kv = s.kv[wave];
+        uint32_t mask = 0;
+        v4f o[8][NT];
         int e_run = -100;  // Q8_0: scales so far are below 2^e_run
-
-        for (uint32_t i = 0; i < count; ++i) {
-            // ---- the wave's slice into LDS ----
-            uint8_t* const kv = s.kv[wave];
-            const uint32_t mask = live;
+        auto stage = [&]() {
+            mask = live;
             if constexpr (Q8) {
+                if (mask != 0xFFFFFFFFu) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t keep = 0u - ((mask >> (8 * j + (lane >> 3))) & 1u);
+                        pre[j].x &= keep, pre[j].y &= keep, pre[j].z &= keep, pre[j].w &= keep;
+                    }
+                    const uint32_t keep = 0u - ((mask >> (lane & 31)) & 1u);
+                    pre_pe.x &= keep, pre_pe.y &= keep, pre_pe.z &= keep, pre_pe.w &= keep;
+                    pre_d.x &= keep, pre_d.y &= keep, pre_dpe &= keep;
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t p = 8 * j + (lane >> 3), c = 2 * (lane & 7);
-                    uint4 x = codes8(pre[j].x, pre[j].y), y = codes8(pre[j].z, pre[j].w);
-                    if (mask != 0xFFFFFFFFu && !((mask >> p) & 1)) x = y = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(kv + p * 256 + ((c ^ (p & 15)) << 4)) = x;
-                    *reinterpret_cast<uint4*>(kv + p * 256 + (((c + 1) ^ (p & 15)) << 4)) = y;
+                    uint8_t* dst = kv + p * 256;
+                    *reinterpret_cast<uint4*>(dst + ((c ^ (p & 15)) << 4)) = codes8(pre[j].x, pre[j].y);
+                    *reinterpret_cast<uint4*>(dst + ((c ^ (p & 15) ^ 1) << 4)) = codes8(pre[j].z, pre[j].w);
                 }
                 float d[5];
-                const uint32_t p = lane & 31;
-                const bool dead = !((mask >> p) & 1);
                 d[0] = f16_scale((uint16_t)(pre_d.x & 0xFFFFu));
                 d[1] = f16_scale((uint16_t)(pre_d.x >> 16));
                 d[2] = f16_scale((uint16_t)(pre_d.y & 0xFFFFu));
                 d[3] = f16_scale((uint16_t)(pre_d.y >> 16));
                 d[4] = f16_scale((uint16_t)pre_dpe);
-                float top = 0.0f;
-#pragma unroll
-                for (int b = 0; b < 5; ++b) {
-                    if (dead) d[b] = 0.0f;
-                    if (b < 4) top = fmaxf(top, fabsf(d[b]));
-                }
+                float top = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
 #pragma unroll
                 for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
                 // f16 scales are below 2^16 (17: infinity).
@@ -422,96 +325,236 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
 #pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) o[c][ht] *= f2;
+                        for (int t = 0; t < NT; ++t) o[c][t] *= f2;
                 }
                 const float sv = pow2(14 - e_run);
+                const uint32_t p = lane & 31;
                 if (lane < 32) {
 #pragma unroll
                     for (int b = 0; b < 5; ++b) {
                         s.ds[wave][b][p] = d[b];
                         if (b < 4) s.dv[wave][b][p] = d[b] * sv;
                     }
-                    uint4 x = codes8(pre_pe.x, pre_pe.y), y = codes8(pre_pe.z, pre_pe.w);
-                    if (dead) x = y = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(s.pe[wave] + p * 32) = x;
-                    *reinterpret_cast<uint4*>(s.pe[wave] + p * 32 + 16) = y;
+                    *reinterpret_cast<uint4*>(s.pe[wave] + p * 32) = codes8(pre_pe.x, pre_pe.y);
+                    *reinterpret_cast<uint4*>(s.pe[wave] + p * 32 + 16) = codes8(pre_pe.z, pre_pe.w);
                 }
             } else {
+                if (mask != 0xFFFFFFFFu) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t p = 4 * j + grp;
-                    uint4 x = pre[j];
-                    if (mask != 0xFFFFFFFFu && !((mask >> p) & 1)) x = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(kv + p * 256 + ((n16 ^ (p & 15)) << 4)) = x;
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t keep = 0u - ((mask >> (4 * j + grp)) & 1u);
+                        pre[j].x &= keep, pre[j].y &= keep, pre[j].z &= keep, pre[j].w &= keep;
+                    }
+                    const uint32_t keep = 0u - ((mask >> (lane >> 1)) & 1u);
+                    pre_pe.x &= keep, pre_pe.y &= keep, pre_pe.z &= keep, pre_pe.w &= keep;
                 }
-                uint4 x = pre_pe;
-                if (!((mask >> (lane >> 1)) & 1)) x = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(s.pe[wave] + (lane >> 1) * 32 + (lane & 1) * 16) = x;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    *reinterpret_cast<uint4*>(kv + j * 1024 + grp * 256 + (((n16 ^ grp) << 4) ^ ((j & 3) << 6))) = pre[j];
+                *reinterpret_cast<uint4*>(s.pe[wave] + lane * 16) = pre_pe;
             }
             // The slice is read back through other types, by this wave alone.
             asm volatile("" ::: "memory");
-            if (i + 1 < count) {
-                load_rows(tile0 + i + 1);
-                load_ids(tile0 + i + 2);
-            }
+        };
 
+        load_ids(tile0);
+        load_rows(tile0);
+        load_ids(tile0 + 1);
+
+        // ---- the queries, scaled by a power of two per head, in two parts ----
+        // (packed tile: each lane has the part of its half)
+        v8h qh[NT][4], ql[MODE == kTwo ? 2 : 1][4];
+        // The 16 rotary columns fill one product of 32: their keys stand twice,
+        // against the high parts and the low parts.
+        v8h pe2[NT];
+        {
+            // Every load is issued whether its head exists or not (the last
+            // head's again, zeroed below): a load under a branch would be
+            // waited for at the branch's end, together with the rows.
+            float q[NT][4][8], pe[NT][8];
+            const float *src[NT], *src_pe[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const uint32_t h = min(head0 + head_of(t), a.n_heads - 1);
+                src[t] = a.q + (uint64_t)token * a.q_token_stride + (uint64_t)h * a.q_head_stride + wave * kMlaCols + 8 * grp;
+                src_pe[t] = a.q_pe + (uint64_t)token * a.q_pe_token_stride + (uint64_t)h * a.q_pe_head_stride + wave * kMlaPe + 8 * (grp & 1);
+                if (!FULL) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) pe[t][e] = 0.0f;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) q[t][b][e] = 0.0f;
+                }
+            }
+            if (pl.vec_q) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b) {
+                        if (!FULL && b >= blocks) continue;
+                        const float4 x = *reinterpret_cast<const float4*>(src[t] + 32 * b);
+                        const float4 y = *reinterpret_cast<const float4*>(src[t] + 32 * b + 4);
+                        q[t][b][0] = x.x, q[t][b][1] = x.y, q[t][b][2] = x.z, q[t][b][3] = x.w;
+                        q[t][b][4] = y.x, q[t][b][5] = y.y, q[t][b][6] = y.z, q[t][b][7] = y.w;
+                    }
+                    if (has_pe) {
+                        const float4 x = *reinterpret_cast<const float4*>(src_pe[t]);
+                        const float4 y = *reinterpret_cast<const float4*>(src_pe[t] + 4);
+                        pe[t][0] = x.x, pe[t][1] = x.y, pe[t][2] = x.z, pe[t][3] = x.w;
+                        pe[t][4] = y.x, pe[t][5] = y.y, pe[t][6] = y.z, pe[t][7] = y.w;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b) {
+                        if (!FULL && b >= blocks) continue;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) q[t][b][e] = src[t][32 * b + e];
+                    }
+                    if (has_pe) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) pe[t][e] = src_pe[t][e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) o[c][t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+            // The first tile goes to LDS and the second is asked for before
+            // the queries are waited for.
+            stage();
+            if (count > 1) {
+                load_rows(tile0 + 1);
+                load_ids(tile0 + 2);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const bool there = head0 + head_of(t) < a.n_heads;
+                float top = 0.0f;
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        q[t][b][e] = there ? q[t][b][e] : 0.0f;
+                        top = fmaxf(top, fabsf(q[t][b][e]));
+                    }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    pe[t][e] = there ? pe[t][e] : 0.0f;
+                    top = fmaxf(top, fabsf(pe[t][e]));
+                }
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                if (grp == 0) s.qmax[wave][t * 16 + n16] = top;
+            }
+            lds_barrier();
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const uint32_t r = t * 16 + n16;
+                const float m = fmaxf(fmaxf(s.qmax[0][r], s.qmax[1][r]), fmaxf(s.qmax[2][r], s.qmax[3][r]));
+                // m 2^e in [2^13, 2^14) for m within f32's middle range
+                const int e = m > 0.0f ? min(max(140 - (int)(__float_as_uint(m) >> 23), -115), 115) : 0;
+                const float sc = pow2(e);
+                if (wave == 0 && grp == 0) s.factor[head_of(t)] = a.scale * 1.44269504088896f * pow2(-e);
+                const bool packed = MODE == kPacked && t == 1;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        split2(q[t][b][2 * i] * sc, q[t][b][2 * i + 1] * sc, h[i], l[i]);
+                        if (packed && low_half) h[i] = l[i];
+                    }
+                    qh[t][b] = half8(make_uint4(h[0], h[1], h[2], h[3]));
+                    if (!packed) ql[packed ? 0 : t][b] = half8(make_uint4(l[0], l[1], l[2], l[3]));
+                }
+                // (packed tile: both parts in the columns of the high ones)
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    split2(pe[t][2 * i] * sc, pe[t][2 * i + 1] * sc, h[i], l[i]);
+                    if (grp >= 2) h[i] = l[i];
+                    if (packed && low_half) h[i] = 0;
+                }
+                pe2[t] = half8(make_uint4(h[0], h[1], h[2], h[3]));
+            }
+        }
+
+        // Softmax state: this wave's heads, kPer positions per lane.
+        constexpr uint32_t kPer = MODE == kOne ? 2 : 4, kLanes = kMlaTile / kPer;
+        const uint32_t srow = wave * (64 / kLanes) + lane / kLanes, spos = (lane % kLanes) * kPer;
+        const bool softmax = MODE != kPacked || wave < 3;  // 24 heads: three waves' rows
+        float m_run = -INFINITY, l_run = 0.0f;
+        // Where a lane reads its keys (row n16 of 16 positions, chunk grp of a
+        // block) and values (transposed: rows 4 grp + n16 / 4, 8 bytes of 16
+        // columns); blocks and columns are further bits to flip.
+        const uint32_t k_at = n16 * 256 + ((grp ^ n16) << 4);
+        const uint32_t v_row = 4 * grp + (n16 >> 2);
+        const uint32_t v_at = v_row * 256 + ((((n16 >> 1) & 1) ^ v_row) << 4) + (n16 & 1) * 8;
+
+        for (uint32_t i = 0;;) {
             // ---- S^T partial ----
 #pragma unroll
             for (int pt = 0; pt < 2; ++pt) {
-                v4f sc[HT];
+                v8h k[4];
 #pragma unroll
-                for (int ht = 0; ht < HT; ++ht) sc[ht] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-                const uint32_t p = pt * 16 + n16;
+                for (uint32_t b = 0; b < 4; ++b)
+                    k[b] = half8(*reinterpret_cast<const uint4*>(kv + pt * 4096 + (k_at ^ (b << 6))));
+                const v8h kpe = half8(*reinterpret_cast<const uint4*>(s.pe[wave] + pt * 512 + n16 * 32 + 16 * (grp & 1)));
+                v4f sc[NT];
 #pragma unroll
-                for (uint32_t b = 0; b < 4; ++b) {
-                    if (!FULL && b >= blocks) continue;
-                    const v8h k = half8(*reinterpret_cast<const uint4*>(kv + p * 256 + (((4 * b + grp) ^ n16) << 4)));
-                    if constexpr (Q8) {
+                for (int t = 0; t < NT; ++t) sc[t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (Q8) {
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b) {
+                        if (!FULL && b >= blocks) continue;
                         const v4f d = *reinterpret_cast<const v4f*>(&s.ds[wave][b][pt * 16 + 4 * grp]);
 #pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) {
+                        for (int t = 0; t < NT; ++t) {
                             v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
-                            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[ht][b], x, 0, 0, 0);
-                            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[ht][b], x, 0, 0, 0);
+                            if (!(MODE == kPacked && t == 1)) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b], ql[t % (MODE == kTwo ? 2 : 1)][b], x, 0, 0, 0);
+                            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b], qh[t][b], x, 0, 0, 0);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) sc[ht][e] = fmaf(d[e], x[e], sc[ht][e]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) {
-                            sc[ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[ht][b], sc[ht], 0, 0, 0);
-                            sc[ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[ht][b], sc[ht], 0, 0, 0);
+                            for (int e = 0; e < 4; ++e) sc[t][e] = fmaf(d[e], x[e], sc[t][e]);
                         }
                     }
-                }
-                if (has_pe) {
-                    const v4h k = __builtin_bit_cast(v4h, *reinterpret_cast<const uint2*>(s.pe[wave] + p * 32 + 8 * grp));
-                    if constexpr (Q8) {
+                    if (has_pe) {
                         const v4f d = *reinterpret_cast<const v4f*>(&s.ds[wave][4][pt * 16 + 4 * grp]);
 #pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) {
+                        for (int t = 0; t < NT; ++t) {
                             v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
-                            x = __builtin_amdgcn_mfma_f32_16x16x16f16(k, pel[ht], x, 0, 0, 0);
-                            x = __builtin_amdgcn_mfma_f32_16x16x16f16(k, peh[ht], x, 0, 0, 0);
+                            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kpe, pe2[t], x, 0, 0, 0);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) sc[ht][e] = fmaf(d[e], x[e], sc[ht][e]);
+                            for (int e = 0; e < 4; ++e) sc[t][e] = fmaf(d[e], x[e], sc[t][e]);
                         }
-                    } else {
+                    }
+                } else {
 #pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) {
-                            sc[ht] = __builtin_amdgcn_mfma_f32_16x16x16f16(k, pel[ht], sc[ht], 0, 0, 0);
-                            sc[ht] = __builtin_amdgcn_mfma_f32_16x16x16f16(k, peh[ht], sc[ht], 0, 0, 0);
+                    for (uint32_t b = 0; b < 4; ++b) {
+                        if (!FULL && b >= blocks) continue;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            if (!(MODE == kPacked && t == 1)) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b], ql[t % (MODE == kTwo ? 2 : 1)][b], sc[t], 0, 0, 0);
+                            sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b], qh[t][b], sc[t], 0, 0, 0);
                         }
+                    }
+                    if (has_pe) {
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kpe, pe2[t], sc[t], 0, 0, 0);
                     }
                 }
 #pragma unroll
-                for (int ht = 0; ht < HT; ++ht)
-                    *reinterpret_cast<v4f*>(&s.sp[wave][ht * 16 + n16][pt * 16 + 4 * grp]) = sc[ht];
+                for (int t = 0; t < NT; ++t)
+                    *reinterpret_cast<v4f*>(&s.sp[wave][t * 16 + n16][pt * 16 + 4 * grp]) = sc[t];
             }
             lds_barrier();
 
-            // ---- softmax of this wave's rows ----
-            {
+            // ---- softmax of this wave's heads ----
+            if (softmax) {
                 const float fac = s.factor[srow];
                 float x[kPer], top = -INFINITY;
 #pragma unroll
@@ -520,6 +563,12 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 for (uint32_t w = 1; w < kMlaWaves; ++w)
 #pragma unroll
                     for (uint32_t e = 0; e < kPer; ++e) x[e] += s.sp[w][srow][spos + e];
+                if (MODE == kPacked && wave == 2) {  // heads 16..23: their low parts' products
+#pragma unroll
+                    for (uint32_t w = 0; w < kMlaWaves; ++w)
+#pragma unroll
+                        for (uint32_t e = 0; e < kPer; ++e) x[e] += s.sp[w][(srow + 8) % (16 * NT)][spos + e];
+                }
                 const uint32_t lv = mask >> spos;
 #pragma unroll
                 for (uint32_t e = 0; e < kPer; ++e) {
@@ -548,8 +597,10 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 #pragma unroll
                     for (uint32_t e = 0; e < kPer; ++e) dst[e] = x[e];
                 } else {
+                    // rows: high parts of both tiles, low parts of both; packed: high 16, packed 16, low 16
+                    const bool packed = MODE == kPacked && wave == 2;
                     uint32_t* hi = s.p + srow * 20 + at / 2;
-                    uint32_t* lo = hi + kRows * 20;
+                    uint32_t* lo = hi + (packed ? 8 : 16 * NT) * 20;
 #pragma unroll
                     for (uint32_t e = 0; e < kPer; e += 2) split2(x[e] * kPScale, x[e + 1] * kPScale, hi[e / 2], lo[e / 2]);
                 }
@@ -558,96 +609,104 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 
             // ---- O^T += V^T P^T ----
             {
-                float al[HT];
+                float al[NT];
                 bool same = true;
 #pragma unroll
-                for (int ht = 0; ht < HT; ++ht) {
-                    al[ht] = s.alpha[ht * 16 + n16];
-                    same = same && al[ht] == 1.0f;
+                for (int t = 0; t < NT; ++t) {
+                    al[t] = s.alpha[head_of(t)];
+                    same = same && al[t] == 1.0f;
                 }
                 if (!__all(same)) {
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
 #pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) o[c][ht] *= al[ht];
+                        for (int t = 0; t < NT; ++t) o[c][t] *= al[t];
                 }
                 const auto values = [&](uint32_t c) {  // 16 columns, all 32 positions
-                    v4s t[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t p = 16 * h + 4 * grp + (n16 >> 2);
-                        const uint8_t* src = kv + p * 256 + (((2 * c + ((n16 >> 1) & 1)) ^ (p & 15)) << 4) + (n16 & 1) * 8;
-                        t[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)src);
-                    }
-                    const uint2 x = __builtin_bit_cast(uint2, t[0]), y = __builtin_bit_cast(uint2, t[1]);
+                    const v4s t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + (v_at ^ (c << 5))));
+                    const v4s t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + 4096 + (v_at ^ (c << 5))));
+                    const uint2 x = __builtin_bit_cast(uint2, t0), y = __builtin_bit_cast(uint2, t1);
                     return half8(make_uint4(x.x, x.y, y.x, y.y));
                 };
                 if constexpr (Q8) {
-                    float p[HT][8];
+                    float p[NT][8];
 #pragma unroll
-                    for (int ht = 0; ht < HT; ++ht) {
-                        const float* src = reinterpret_cast<const float*>(s.p) + (ht * 16 + n16) * 36 + grp * 8;
+                    for (int t = 0; t < NT; ++t) {
+                        const float* src = reinterpret_cast<const float*>(s.p) + head_of(t) * 36 + grp * 8;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) p[ht][e] = src[e];
+                        for (int e = 0; e < 8; ++e) p[t][e] = src[e];
                     }
 #pragma unroll
                     for (uint32_t b = 0; b < 4; ++b) {
                         if (!FULL && b >= blocks) continue;
+                        const v8h v[2] = {values(2 * b), values(2 * b + 1)};
                         const v4f d0 = *reinterpret_cast<const v4f*>(&s.dv[wave][b][4 * grp]);
                         const v4f d1 = *reinterpret_cast<const v4f*>(&s.dv[wave][b][16 + 4 * grp]);
-                        v8h ph[HT], plo[HT];
 #pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) {
+                        for (int t = 0; t < NT; ++t) {
+                            const bool packed = MODE == kPacked && t == 1;
                             uint32_t h[4], l[4];
-                            split2(p[ht][0] * d0[0], p[ht][1] * d0[1], h[0], l[0]);
-                            split2(p[ht][2] * d0[2], p[ht][3] * d0[3], h[1], l[1]);
-                            split2(p[ht][4] * d1[0], p[ht][5] * d1[1], h[2], l[2]);
-                            split2(p[ht][6] * d1[2], p[ht][7] * d1[3], h[3], l[3]);
-                            ph[ht] = half8(make_uint4(h[0], h[1], h[2], h[3]));
-                            plo[ht] = half8(make_uint4(l[0], l[1], l[2], l[3]));
-                        }
+                            split2(p[t][0] * d0[0], p[t][1] * d0[1], h[0], l[0]);
+                            split2(p[t][2] * d0[2], p[t][3] * d0[3], h[1], l[1]);
+                            split2(p[t][4] * d1[0], p[t][5] * d1[1], h[2], l[2]);
+                            split2(p[t][6] * d1[2], p[t][7] * d1[3], h[3], l[3]);
+                            if (packed) {
 #pragma unroll
-                        for (uint32_t c = 2 * b; c < 2 * b + 2; ++c) {
-                            const v8h v = values(c);
+                                for (int e = 0; e < 4; ++e) h[e] = low_half ? l[e] : h[e];
+                            }
+                            const v8h ph = half8(make_uint4(h[0], h[1], h[2], h[3]));
+                            const v8h plo = half8(make_uint4(l[0], l[1], l[2], l[3]));
 #pragma unroll
-                            for (int ht = 0; ht < HT; ++ht) {
-                                o[c][ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, plo[ht], o[c][ht], 0, 0, 0);
-                                o[c][ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ht], o[c][ht], 0, 0, 0);
+                            for (uint32_t c = 0; c < 2; ++c) {
+                                if (!packed) o[2 * b + c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], plo, o[2 * b + c][t], 0, 0, 0);
+                                o[2 * b + c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], ph, o[2 * b + c][t], 0, 0, 0);
                             }
                         }
                     }
                 } else {
-                    v8h ph[HT], plo[HT];
+                    v8h ph[NT], plo[MODE == kTwo ? 2 : 1];
 #pragma unroll
-                    for (int ht = 0; ht < HT; ++ht) {
-                        const uint32_t* src = s.p + (ht * 16 + n16) * 20 + grp * 4;
-                        ph[ht] = half8(*reinterpret_cast<const uint4*>(src));
-                        plo[ht] = half8(*reinterpret_cast<const uint4*>(src + kRows * 20));
+                    for (int t = 0; t < NT; ++t) {
+                        const uint32_t* src = s.p + (t * 16 + n16) * 20 + grp * 4;
+                        ph[t] = half8(*reinterpret_cast<const uint4*>(src));
+                        if (!(MODE == kPacked && t == 1)) plo[t % (MODE == kTwo ? 2 : 1)] = half8(*reinterpret_cast<const uint4*>(src + 16 * NT * 20));
                     }
 #pragma unroll
                     for (uint32_t c = 0; c < 8; ++c) {
                         if (!FULL && c >= 2 * blocks) continue;
                         const v8h v = values(c);
 #pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) {
-                            o[c][ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, plo[ht], o[c][ht], 0, 0, 0);
-                            o[c][ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ht], o[c][ht], 0, 0, 0);
+                        for (int t = 0; t < NT; ++t) {
+                            if (!(MODE == kPacked && t == 1)) o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, plo[t % (MODE == kTwo ? 2 : 1)], o[c][t], 0, 0, 0);
+                            o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t], o[c][t], 0, 0, 0);
                         }
                     }
                 }
             }
+            if (++i >= count) break;
+            stage();
+            if (i + 1 < count) {
+                load_rows(tile0 + i + 1);
+                load_ids(tile0 + i + 2);
+            }
         }
 
         // ---- the piece's result ----
-        if (lane % kLanes == 0) s.ml[srow] = make_float2(m_run, l_run);
+        if (softmax && lane % kLanes == 0) s.ml[srow] = make_float2(m_run, l_run);
         lds_barrier();
         const bool first = tile0 == 0, whole = first && count == n_tiles;
         const float back = Q8 ? (e_run == -100 ? 0.0f : pow2(e_run - 14)) : 1.0f / kPScale;
         const uint64_t slot = (uint64_t)wg * 2 + (first ? 1 : 0);
+        if constexpr (MODE == kPacked) {  // both parts' sums
 #pragma unroll
-        for (int ht = 0; ht < HT; ++ht) {
-            const uint32_t r = ht * 16 + n16, h = head0 + r;
-            if (h >= a.n_heads) continue;
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[c][1][e] += __shfl_xor(o[c][1][e], 8, 64);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint32_t r = head_of(t), h = head0 + r;
+            if (h >= a.n_heads || (MODE == kPacked && t == 1 && low_half)) continue;
             const float2 ml = s.ml[r];
             float f2 = back;
             float* dst;
@@ -659,25 +718,28 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                         ml.y == 0.0f ? -INFINITY : 0.69314718055995f * (ml.x + __builtin_amdgcn_logf(ml.y));
             } else {
                 dst = pl.parts + (slot * pl.part_rows + r) * g.rank;
-                if (wave == 0 && grp == 0) pl.part_ml[slot * kRows + r] = ml;
+                if (wave == 0 && grp == 0) pl.part_ml[slot * kHeads + r] = ml;
             }
             dst += wave * kMlaCols + 4 * grp;
-            const bool vec = whole ? pl.vec_out : true;
+            if (!whole || pl.vec_out) {
 #pragma unroll
-            for (uint32_t c = 0; c < 8; ++c) {
-                if (!FULL && c >= 2 * blocks) continue;
-                const v4f v = o[c][ht] * f2;
-                if (vec) {
-                    *reinterpret_cast<v4f*>(dst + 16 * c) = v;
-                } else {
+                for (uint32_t c = 0; c < 8; ++c) {
+                    if (!FULL && c >= 2 * blocks) continue;
+                    *reinterpret_cast<v4f*>(dst + 16 * c) = o[c][t] * f2;
+                }
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dst[16 * c + e] = v[e];
+                for (uint32_t c = 0; c < 8; ++c) {
+                    if (!FULL && c >= 2 * blocks) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dst[16 * c + e] = o[c][t][e] * f2;
                 }
             }
         }
         if (first && !whole) {
             begun.item = token * pl.head_tiles + ht_index;
-            begun.pieces = (uint32_t)((f + n_tiles - 1) / chunk) - wg + 1;
+            const uint64_t last = f + n_tiles - 1;
+            begun.pieces = (last < 0x80000000u ? (uint32_t)last / (uint32_t)chunk : (uint32_t)(last / chunk)) - wg + 1;
         }
         f += count;
         off += count;
@@ -821,13 +883,15 @@ uint32_t mla_groups(int num_cu) { return num_cu * 2 < (int)kMlaMostGroups ? (uin
 uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
 
 struct MlaLayout {
+    int mode;
     uint32_t groups, rows, head_tiles, part_rows;
     uint64_t parts, ml, splits, bytes;
 };
 MlaLayout mla_layout(uint32_t n_heads, uint32_t rank, int num_cu) {
     MlaLayout w;
     w.groups = mla_groups(num_cu);
-    w.rows = n_heads <= 16 ? 16 : 32;
+    w.mode = n_heads <= 16 ? kOne : n_heads <= 24 && rank == kKvMaxRank ? kPacked : kTwo;
+    w.rows = mode_rows(w.mode);
     w.head_tiles = (n_heads + w.rows - 1) / w.rows;
     w.part_rows = n_heads < w.rows ? n_heads : w.rows;
     w.parts = 0;
@@ -838,14 +902,19 @@ MlaLayout mla_layout(uint32_t n_heads, uint32_t rank, int num_cu) {
 }
 
 template <bool Q8>
-void launch_split(const MlaArgs& a, const MlaPlan& p, hipStream_t s) {
-    const bool full = a.geom.rank == 512 && a.geom.width == 576;
-    if (p.rows == 16) {
-        if (full) mla_split_kernel<Q8, 1, true><<<p.groups, kMlaThreads, 0, s>>>(a, p);
-        else mla_split_kernel<Q8, 1, false><<<p.groups, kMlaThreads, 0, s>>>(a, p);
+void launch_split(const MlaArgs& a, const MlaPlan& p, int mode, hipStream_t s) {
+    // Every block and rotary column there is: no test of either in the loops.
+    const bool full = a.geom.rank == kKvMaxRank && a.geom.width == kKvMaxRank + kKvMaxRope;
+    const dim3 grid(p.groups);
+    if (mode == kOne) {
+        if (full) mla_split_kernel<Q8, kOne, true><<<grid, kMlaThreads, 0, s>>>(a, p);
+        else mla_split_kernel<Q8, kOne, false><<<grid, kMlaThreads, 0, s>>>(a, p);
+    } else if (mode == kPacked) {
+        if (full) mla_split_kernel<Q8, kPacked, true><<<grid, kMlaThreads, 0, s>>>(a, p);
+        else mla_split_kernel<Q8, kPacked, false><<<grid, kMlaThreads, 0, s>>>(a, p);
     } else {
-        if (full) mla_split_kernel<Q8, 2, true><<<p.groups, kMlaThreads, 0, s>>>(a, p);
-        else mla_split_kernel<Q8, 2, false><<<p.groups, kMlaThreads, 0, s>>>(a, p);
+        if (full) mla_split_kernel<Q8, kTwo, true><<<grid, kMlaThreads, 0, s>>>(a, p);
+        else mla_split_kernel<Q8, kTwo, false><<<grid, kMlaThreads, 0, s>>>(a, p);
     }
 }
 
@@ -874,8 +943,8 @@ hipError_t launch_mla(const MlaArgs& a, hipStream_t s) {
     p.vec_q = aligned(a.q, a.q_token_stride, a.q_head_stride) &&
               (a.geom.width == a.geom.rank || aligned(a.q_pe, a.q_pe_token_stride, a.q_pe_head_stride));
     p.vec_out = aligned(a.out, a.out_token_stride, a.out_head_stride);
-    if (a.geom.q8) launch_split<true>(a, p, s);
-    else launch_split<false>(a, p, s);
+    if (a.geom.q8) launch_split<true>(a, p, w.mode, s);
+    else launch_split<false>(a, p, w.mode, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     mla_join_kernel<<<a.num_cu, kJoinThreads, 0, s>>>(a, p);
