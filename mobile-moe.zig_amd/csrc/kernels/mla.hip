@@ -113,6 +113,21 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 
 __device__ __forceinline__ v8h half8(const uint4& v) { return __builtin_bit_cast(v8h, v); }
 
+// A value that is the same in all lanes, in scalar registers from here on.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t uniform(uint64_t v) {
+    return (uint64_t)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v);
+}
+
+// A lane-dependent value that the compiler takes as new here: what follows
+// from it is computed again where it is used, not kept in registers over the
+// loop around (registers that run out would go to scratch memory, whose loads
+// wait for every row load in flight).
+__device__ __forceinline__ uint32_t afresh(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // 2^e, e within f32's normal exponents.
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -162,6 +177,8 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         incl += before;
         // (a 64-bit division is some 150 instructions)
         chunk = total < 0x80000000u ? ((uint32_t)total + pl.groups - 1) / pl.groups : (total + pl.groups - 1) / pl.groups;
+        chunk = uniform(chunk);
+        total = uniform(total);
         f = wg * chunk;
         end = f + chunk < total ? f + chunk : total;
         if (f < end && incl - mine <= f && f < incl) {
@@ -189,17 +206,17 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
     const uint32_t blocks = FULL ? 4u : (g.rank / 32 > 4 * wave ? min(g.rank / 32 - 4 * wave, 4u) : 0u);
     const bool has_pe = FULL || kMlaPe * wave < g.width - g.rank;
 
-    uint32_t token = f < end ? s.start_token : 0;
-    uint64_t off = f < end ? s.start_off : 0;
-    uint32_t row = s.start_row, len = s.start_len, of_token = token;
+    uint32_t token = uniform(s.start_token);
+    uint64_t off = uniform(s.start_off);
+    uint32_t row = uniform(s.start_row), len = uniform(s.start_len), of_token = token;
     while (f < end && token < a.n_tokens) {
         if (token != of_token) {
             uint32_t bad;
             len = seen(a, token, row, bad);
             of_token = token;
         }
-        len = __builtin_amdgcn_readfirstlane(len);
-        row = __builtin_amdgcn_readfirstlane(row);
+        len = uniform(len);
+        row = uniform(row);
         const uint32_t n_tiles = tiles_of(len);
         if (n_tiles == 0) {
             ++token;
@@ -226,60 +243,57 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         pre_pe = make_uint4(0, 0, 0, 0);
         pre_d = make_uint2(0, 0);
         auto load_rows = [&](uint32_t tile) {
-            const uint8_t* base[2];
-            const uint8_t* base_d[2];
+            const uint32_t lane = afresh(tid & 63), n16 = lane & 15, grp = lane >> 4;
+            BufRsrc rows[2];
+            const uint8_t *base[2], *base_d[2];
             live = 0;
             const uint32_t p0 = tile * kMlaTile;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int32_t page = __builtin_amdgcn_readfirstlane(id[h]);
+                const int32_t page = (int32_t)uniform((uint32_t)id[h]);
                 const uint32_t p = p0 + 16 * h;
                 const bool want = p < len, ok = want && paged_has(g, page);
                 if (ok) live |= (len - p >= 16 ? 0xFFFFu : (1u << (len - p)) - 1) << (16 * h);
                 else if (want && tid == 0) report(a.status, kBadPage);
-                // A page that is not there is read as page 0 and left out.
+                // 16 rows from p on. A page that is not there is read as page 0
+                // and left out.
                 base[h] = a.pool + paged_row(g, ok ? (uint32_t)page : 0u, p & at_mask);
+                rows[h] = make_rsrc(base[h], 16 * row_bytes);
                 if constexpr (Q8) base_d[h] = a.pool + paged_scales(g, ok ? (uint32_t)page : 0u, p & at_mask);
             }
+            if (FULL || blocks) {
+                // A lane's 16 bytes of the wave's columns (past the columns
+                // there are: the last ones again).
+                const uint32_t at_rows = Q8 ? (lane >> 3) * row_bytes + wave * kMlaCols + 16 * (FULL ? lane & 7 : min(lane & 7, 2 * blocks - 1))
+                                            : grp * row_bytes + wave * (2 * kMlaCols) + 16 * (FULL ? n16 : min(n16, 4 * blocks - 1));
+#pragma unroll
+                for (int j = 0; j < (Q8 ? 4 : 8); ++j) {
+                    if constexpr (Q8) pre[j] = buf_load_b128<kCacheStream>(rows[j >> 1], at_rows, 8 * (j & 1) * row_bytes);
+                    else pre[j] = buf_load_b128<kCacheStream>(rows[j >> 2], at_rows, 4 * (j & 3) * row_bytes);
+                }
+            }
             if constexpr (Q8) {
-                if (FULL || blocks) {
-                    uint32_t c = lane & 7;
-                    if (!FULL) c = min(c, 2 * blocks - 1);
-                    const uint32_t o = (lane >> 3) * row_bytes + wave * kMlaCols + c * 16;
+                // A position per lane, twice over.
+                const uint8_t* d = (lane & 16 ? base_d[1] : base_d[0]) + n16 * (g.width / 32 * 2);
+                if constexpr (FULL) {
+                    pre_d.x = reinterpret_cast<const uint32_t*>(d + wave * 8)[0];
+                    pre_d.y = reinterpret_cast<const uint32_t*>(d + wave * 8)[1];
+                } else if (blocks) {
+                    uint32_t v[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        pre[j] = *reinterpret_cast<const uint4*>(base[j >> 1] + (8 * (j & 1)) * row_bytes + o);
-                    const uint8_t* d = (lane & 16 ? base_d[1] : base_d[0]) + n16 * (g.width / 32 * 2) + wave * 8;
-                    if constexpr (FULL) {
-                        pre_d.x = reinterpret_cast<const uint32_t*>(d)[0];
-                        pre_d.y = reinterpret_cast<const uint32_t*>(d)[1];
-                    } else {
-                        uint32_t v[4];
-#pragma unroll
-                        for (uint32_t b = 0; b < 4; ++b) v[b] = reinterpret_cast<const uint16_t*>(d)[min(b, blocks - 1)];
-                        pre_d = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
-                    }
+                    for (uint32_t b = 0; b < 4; ++b) v[b] = reinterpret_cast<const uint16_t*>(d + wave * 8)[min(b, blocks - 1)];
+                    pre_d = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
                 }
                 if (has_pe) {
-                    const uint8_t* r = (lane & 16 ? base[1] : base[0]) + n16 * row_bytes + g.rank + wave * kMlaPe;
-                    pre_pe = *reinterpret_cast<const uint4*>(r);
-                    const uint8_t* d = (lane & 16 ? base_d[1] : base_d[0]) + n16 * (g.width / 32 * 2) + (g.rank / 32 + wave / 2) * 2;
-                    pre_dpe = *reinterpret_cast<const uint16_t*>(d);
+                    pre_pe = *reinterpret_cast<const uint4*>((lane & 16 ? base[1] : base[0]) + n16 * row_bytes + g.rank + wave * kMlaPe);
+                    pre_dpe = *reinterpret_cast<const uint16_t*>(d + (g.rank / 32 + wave / 2) * 2);
                 }
-            } else {
-                if (FULL || blocks) {
-                    uint32_t c = n16;
-                    if (!FULL) c = min(c, 4 * blocks - 1);
-                    const uint32_t o = grp * row_bytes + wave * (2 * kMlaCols) + c * 16;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        pre[j] = *reinterpret_cast<const uint4*>(base[j >> 2] + (4 * (j & 3)) * row_bytes + o);
-                }
-                if (has_pe)
-                    pre_pe = *reinterpret_cast<const uint4*>((lane & 32 ? base[1] : base[0]) + ((lane >> 1) & 15) * row_bytes +
-                                                             2 * g.rank + wave * (2 * kMlaPe) + (lane & 1) * 16);
+            } else if (has_pe) {
+                pre_pe = *reinterpret_cast<const uint4*>((lane & 32 ? base[1] : base[0]) + ((lane >> 1) & 15) * row_bytes +
+                                                         2 * g.rank + wave * (2 * kMlaPe) + (lane & 1) * 16);
             }
         };
+
         // The wave's slice of the tile in registers -> LDS, in f16. Positions
         // that count for nothing (past the length, on a page that is not
         // there) become zeros: their bytes may be anything.
@@ -287,7 +301,9 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         uint32_t mask = 0;
         v4f o[8][NT];
         int e_run = -100;  // Q8_0: scales so far are below 2^e_run
+        float e_scale = 1.0f;
         auto stage = [&]() {
+            const uint32_t lane = afresh(tid & 63), n16 = lane & 15, grp = lane >> 4;
             mask = live;
             if constexpr (Q8) {
                 if (mask != 0xFFFFFFFFu) {
@@ -319,14 +335,9 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 // f16 scales are below 2^16 (17: infinity).
                 const uint32_t tb = __builtin_amdgcn_readfirstlane(__float_as_uint(top));
                 const int e = tb == 0 ? -100 : min((int)(tb >> 23) - 126, 17);
-                if (e > e_run) {
-                    const float f2 = e_run == -100 ? 1.0f : pow2(e_run - e);
-                    e_run = e;
-#pragma unroll
-                    for (int c = 0; c < 8; ++c)
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) o[c][t] *= f2;
-                }
+                // The sums so far follow in the O phase, with the softmax's factor.
+                e_scale = e > e_run && e_run != -100 ? pow2(e_run - e) : 1.0f;
+                e_run = max(e, e_run);
                 const float sv = pow2(14 - e_run);
                 const uint32_t p = lane & 31;
                 if (lane < 32) {
@@ -365,7 +376,8 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         // (packed tile: each lane has the part of its half)
         v8h qh[NT][4], ql[MODE == kTwo ? 2 : 1][4];
         // The 16 rotary columns fill one product of 32: their keys stand twice,
-        // against the high parts and the low parts.
+        // against the high parts and the low parts. (Products of 16 and of 32
+        // on one accumulator, one right after the other, lost the earlier sum.)
         v8h pe2[NT];
         {
             // Every load is issued whether its head exists or not (the last
@@ -373,6 +385,9 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             // waited for at the branch's end, together with the rows.
             float q[NT][4][8], pe[NT][8];
             const float *src[NT], *src_pe[NT];
+            const uint32_t ln = afresh(lane), n16 = ln & 15, grp = ln >> 4;
+            const bool low_half = n16 >= 8;
+            const auto head_of = [&](int t) { return MODE == kPacked && t == 1 ? 16 + (n16 & 7) : 16 * t + n16; };
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const uint32_t h = min(head0 + head_of(t), a.n_heads - 1);
@@ -420,10 +435,6 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                     }
                 }
             }
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) o[c][t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
             // The first tile goes to LDS and the second is asked for before
             // the queries are waited for.
             stage();
@@ -484,19 +495,26 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             }
         }
 
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[c][t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
         // Softmax state: this wave's heads, kPer positions per lane.
         constexpr uint32_t kPer = MODE == kOne ? 2 : 4, kLanes = kMlaTile / kPer;
-        const uint32_t srow = wave * (64 / kLanes) + lane / kLanes, spos = (lane % kLanes) * kPer;
         const bool softmax = MODE != kPacked || wave < 3;  // 24 heads: three waves' rows
         float m_run = -INFINITY, l_run = 0.0f;
-        // Where a lane reads its keys (row n16 of 16 positions, chunk grp of a
-        // block) and values (transposed: rows 4 grp + n16 / 4, 8 bytes of 16
-        // columns); blocks and columns are further bits to flip.
-        const uint32_t k_at = n16 * 256 + ((grp ^ n16) << 4);
-        const uint32_t v_row = 4 * grp + (n16 >> 2);
-        const uint32_t v_at = v_row * 256 + ((((n16 >> 1) & 1) ^ v_row) << 4) + (n16 & 1) * 8;
 
         for (uint32_t i = 0;;) {
+            const uint32_t ln = afresh(lane), n16 = ln & 15, grp = ln >> 4;
+            const bool low_half = n16 >= 8;
+            const auto head_of = [&](int t) { return MODE == kPacked && t == 1 ? 16 + (n16 & 7) : 16 * t + n16; };
+            // Where a lane reads its keys (row n16 of 16 positions, chunk grp of
+            // a block) and values (transposed: rows 4 grp + n16 / 4, 8 bytes of
+            // 16 columns); blocks and columns are further bits to flip.
+            const uint32_t k_at = n16 * 256 + ((grp ^ n16) << 4);
+            const uint32_t v_row = 4 * grp + (n16 >> 2);
+            const uint32_t v_at = v_row * 256 + ((((n16 >> 1) & 1) ^ v_row) << 4) + (n16 & 1) * 8;
+            const uint32_t srow = wave * (64 / kLanes) + ln / kLanes, spos = (ln % kLanes) * kPer;
             // ---- S^T partial ----
 #pragma unroll
             for (int pt = 0; pt < 2; ++pt) {
@@ -614,6 +632,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     al[t] = s.alpha[head_of(t)];
+                    if constexpr (Q8) al[t] *= e_scale;
                     same = same && al[t] == 1.0f;
                 }
                 if (!__all(same)) {
@@ -692,8 +711,11 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         }
 
         // ---- the piece's result ----
-        if (softmax && lane % kLanes == 0) s.ml[srow] = make_float2(m_run, l_run);
+        if (softmax && lane % kLanes == 0) s.ml[wave * (64 / kLanes) + lane / kLanes] = make_float2(m_run, l_run);
         lds_barrier();
+        const uint32_t ln = afresh(lane), n16 = ln & 15, grp = ln >> 4;
+        const bool low_half = n16 >= 8;
+        const auto head_of = [&](int t) { return MODE == kPacked && t == 1 ? 16 + (n16 & 7) : 16 * t + n16; };
         const bool first = tile0 == 0, whole = first && count == n_tiles;
         const float back = Q8 ? (e_run == -100 ? 0.0f : pow2(e_run - 14)) : 1.0f / kPScale;
         const uint64_t slot = (uint64_t)wg * 2 + (first ? 1 : 0);
