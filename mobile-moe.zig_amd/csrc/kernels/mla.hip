@@ -128,6 +128,31 @@ __device__ __forceinline__ uint32_t afresh(uint32_t v) {
     return v;
 }
 
+// Sums and maxima over groups of 8 or 16 lanes by lane permutes of the vector
+// unit (a shuffle through LDS takes about 0.05 us each). Every lane gets the
+// result; NaN does not enter a maximum.
+template <int CTRL>
+__device__ __forceinline__ float permuted(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
+template <int LANES>
+__device__ __forceinline__ float group_max(float v) {
+    v = fmaxf(v, permuted<kXor1>(v));
+    v = fmaxf(v, permuted<kXor2>(v));
+    v = fmaxf(v, permuted<kHalfMirror>(v));
+    if constexpr (LANES == 16) v = fmaxf(v, permuted<kMirror>(v));
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v) {
+    v += permuted<kXor1>(v);
+    v += permuted<kXor2>(v);
+    v += permuted<kHalfMirror>(v);
+    if constexpr (LANES == 16) v += permuted<kMirror>(v);
+    return v;
+}
+
 // 2^e, e within f32's normal exponents.
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -330,10 +355,9 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 d[3] = f16_scale((uint16_t)(pre_d.y >> 16));
                 d[4] = f16_scale((uint16_t)pre_dpe);
                 float top = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
-#pragma unroll
-                for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-                // f16 scales are below 2^16 (17: infinity).
-                const uint32_t tb = __builtin_amdgcn_readfirstlane(__float_as_uint(top));
+                top = group_max<16>(top);
+                // f16 scales are below 2^16 (17: infinity); as bits they compare like numbers.
+                const uint32_t tb = max(__builtin_amdgcn_readlane(__float_as_uint(top), 0), __builtin_amdgcn_readlane(__float_as_uint(top), 16));
                 const int e = tb == 0 ? -100 : min((int)(tb >> 23) - 126, 17);
                 // The sums so far follow in the O phase, with the softmax's factor.
                 e_scale = e > e_run && e_run != -100 ? pow2(e_run - e) : 1.0f;
@@ -593,8 +617,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                     x[e] = (lv >> e) & 1 ? x[e] * fac : -INFINITY;
                     top = fmaxf(top, x[e]);
                 }
-#pragma unroll
-                for (uint32_t d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+                top = group_max<kLanes>(top);
                 const float m_new = fmaxf(m_run, top), base = m_new == -INFINITY ? 0.0f : m_new;
                 const float al = __builtin_amdgcn_exp2f(m_run - base);
                 float sum = 0.0f;
@@ -603,8 +626,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                     x[e] = __builtin_amdgcn_exp2f(x[e] - base);
                     sum += x[e];
                 }
-#pragma unroll
-                for (uint32_t d = 1; d < kLanes; d <<= 1) sum += __shfl_xor(sum, d, 64);
+                sum = group_sum<kLanes>(sum);
                 l_run = l_run * al + sum;
                 m_run = m_new;
                 if (lane % kLanes == 0) s.alpha[srow] = al;
