@@ -28,8 +28,11 @@
 //
 // Q8_0: codes become f16 integers on their way to LDS. A score is summed block
 // by block, each block's product times the position's block scale. In O the
-// scale is folded into P, block by block, times a power of two that keeps
-// the largest scale seen (running, like the softmax's maximum) within f16.
+// values are scaled: d * code has 19 bits, its f16 rounding and the rest (an
+// FMA away) are both exact, one vector instruction per value for both. (The
+// scale folded into P instead costs three per head tile and value.) Scales of
+// 2^8 and more go in with a power of two less, so that f16 does not overflow;
+// the largest so far is kept like the softmax's maximum.
 //
 // Work is cut evenly, whatever the lengths: the tiles of all tokens and head
 // tiles form one list, of which every workgroup takes an equal run, two
@@ -72,10 +75,10 @@ struct MlaLds {
     uint8_t kv[kMlaWaves][kMlaTile * 256];  // f16 [position][128], 16-byte chunks swizzled by the position
     uint8_t pe[kMlaWaves][kMlaTile * 32];   // f16 [position][16]
     float sp[kMlaWaves][16 * NT][kSpLd];    // score partials, a row per product column
-    // P: f16 in rows of 40 (per tile high parts, low parts; packed as it is), or f32 per head in rows of 36
-    uint32_t p[Q8 ? mode_rows(MODE) * 36 : (MODE == kTwo ? 4 : MODE == kPacked ? 3 : 2) * 16 * 20];
+    // P: f16 in rows of 40 (per tile high parts, low parts; packed as it is)
+    uint32_t p[(MODE == kTwo ? 4 : MODE == kPacked ? 3 : 2) * 16 * 20];
     float ds[Q8 ? kMlaWaves : 1][5][kMlaTile];  // block scales of the keys
-    float dv[Q8 ? kMlaWaves : 1][4][kMlaTile];  // of the values, scaled into range
+    uint16_t dv[Q8 ? kMlaWaves : 1][4][kMlaTile];  // of the values, in f16
     float alpha[16 * NT], factor[16 * NT], qmax[kMlaWaves][16 * NT];
     float2 ml[16 * NT];
     uint64_t scan[kMlaWaves];
@@ -311,7 +314,10 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 }
                 if (has_pe) {
                     pre_pe = *reinterpret_cast<const uint4*>((lane & 16 ? base[1] : base[0]) + n16 * row_bytes + g.rank + wave * kMlaPe);
-                    pre_dpe = *reinterpret_cast<const uint16_t*>(d + (g.rank / 32 + wave / 2) * 2);
+                    // Two blocks' scales in a word, picked from when they are
+                    // used: widening a 16-bit load waits for it right here.
+                    if constexpr (FULL) pre_dpe = *reinterpret_cast<const uint32_t*>(d + 32);
+                    else pre_dpe = *reinterpret_cast<const uint16_t*>(d + (g.rank / 32 + wave / 2) * 2);
                 }
             } else if (has_pe) {
                 pre_pe = *reinterpret_cast<const uint4*>((lane & 32 ? base[1] : base[0]) + ((lane >> 1) & 15) * row_bytes +
@@ -325,7 +331,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         uint8_t* const kv = s.kv[wave];
         uint32_t mask = 0;
         v4f o[8][NT];
-        int e_run = -100;  // Q8_0: scales so far are below 2^e_run
+        int e_run = 0;  // Q8_0: value scales are taken times 2^-e_run
         float e_scale = 1.0f;
         auto stage = [&]() {
             const uint32_t lane = afresh(tid & 63), n16 = lane & 15, grp = lane >> 4;
@@ -353,23 +359,28 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 d[1] = f16_scale((uint16_t)(pre_d.x >> 16));
                 d[2] = f16_scale((uint16_t)(pre_d.y & 0xFFFFu));
                 d[3] = f16_scale((uint16_t)(pre_d.y >> 16));
-                d[4] = f16_scale((uint16_t)pre_dpe);
+                d[4] = f16_scale((uint16_t)(FULL ? pre_dpe >> (wave / 2 * 16) : pre_dpe));
                 float top = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
                 top = group_max<16>(top);
-                // f16 scales are below 2^16 (17: infinity); as bits they compare like numbers.
+                // As bits they compare like numbers; 2^8 and more: 1 to 9 (infinity).
                 const uint32_t tb = max(__builtin_amdgcn_readlane(__float_as_uint(top), 0), __builtin_amdgcn_readlane(__float_as_uint(top), 16));
-                const int e = tb == 0 ? -100 : min((int)(tb >> 23) - 126, 17);
+                const int e = min(max((int)(tb >> 23) - 134, 0), 9);
                 // The sums so far follow in the O phase, with the softmax's factor.
-                e_scale = e > e_run && e_run != -100 ? pow2(e_run - e) : 1.0f;
+                e_scale = e > e_run ? pow2(e_run - e) : 1.0f;
                 e_run = max(e, e_run);
-                const float sv = pow2(14 - e_run);
+                if (e_run) {
+                    const v2h f2 = (v2h)(_Float16)pow2(-e_run);
+                    pre_d.x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, pre_d.x) * f2);
+                    pre_d.y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, pre_d.y) * f2);
+                }
                 const uint32_t p = lane & 31;
                 if (lane < 32) {
 #pragma unroll
-                    for (int b = 0; b < 5; ++b) {
-                        s.ds[wave][b][p] = d[b];
-                        if (b < 4) s.dv[wave][b][p] = d[b] * sv;
-                    }
+                    for (int b = 0; b < 5; ++b) s.ds[wave][b][p] = d[b];
+                    s.dv[wave][0][p] = (uint16_t)(pre_d.x & 0xFFFFu);
+                    s.dv[wave][1][p] = (uint16_t)(pre_d.x >> 16);
+                    s.dv[wave][2][p] = (uint16_t)(pre_d.y & 0xFFFFu);
+                    s.dv[wave][3][p] = (uint16_t)(pre_d.y >> 16);
                     *reinterpret_cast<uint4*>(s.pe[wave] + p * 32) = codes8(pre_pe.x, pre_pe.y);
                     *reinterpret_cast<uint4*>(s.pe[wave] + p * 32 + 16) = codes8(pre_pe.z, pre_pe.w);
                 }
@@ -632,11 +643,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 if (lane % kLanes == 0) s.alpha[srow] = al;
                 // position 16 h + 4 g + e is O^T's operand element 4 h + e of group g
                 const uint32_t at = ((spos >> 2) & 3) * 8 + (spos >> 4) * 4 + (spos & 3);
-                if constexpr (Q8) {
-                    float* dst = reinterpret_cast<float*>(s.p) + srow * 36 + at;
-#pragma unroll
-                    for (uint32_t e = 0; e < kPer; ++e) dst[e] = x[e];
-                } else {
+                {
                     // rows: high parts of both tiles, low parts of both; packed: high 16, packed 16, low 16
                     const bool packed = MODE == kPacked && wave == 2;
                     uint32_t* hi = s.p + srow * 20 + at / 2;
@@ -669,55 +676,33 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                     const uint2 x = __builtin_bit_cast(uint2, t0), y = __builtin_bit_cast(uint2, t1);
                     return half8(make_uint4(x.x, x.y, y.x, y.y));
                 };
-                if constexpr (Q8) {
-                    float p[NT][8];
+                v8h ph[NT], plo[MODE == kTwo ? 2 : 1];
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const float* src = reinterpret_cast<const float*>(s.p) + head_of(t) * 36 + grp * 8;
+                for (int t = 0; t < NT; ++t) {
+                    const uint32_t* src = s.p + (t * 16 + n16) * 20 + grp * 4;
+                    ph[t] = half8(*reinterpret_cast<const uint4*>(src));
+                    if (!(MODE == kPacked && t == 1)) plo[t % (MODE == kTwo ? 2 : 1)] = half8(*reinterpret_cast<const uint4*>(src + 16 * NT * 20));
+                }
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) p[t][e] = src[e];
+                for (uint32_t b = 0; b < 4; ++b) {
+                    if (!FULL && b >= blocks) continue;
+                    v8h d;
+                    if constexpr (Q8) {
+                        const uint2 d0 = *reinterpret_cast<const uint2*>(&s.dv[wave][b][4 * grp]);
+                        const uint2 d1 = *reinterpret_cast<const uint2*>(&s.dv[wave][b][16 + 4 * grp]);
+                        d = half8(make_uint4(d0.x, d0.y, d1.x, d1.y));
                     }
 #pragma unroll
-                    for (uint32_t b = 0; b < 4; ++b) {
-                        if (!FULL && b >= blocks) continue;
-                        const v8h v[2] = {values(2 * b), values(2 * b + 1)};
-                        const v4f d0 = *reinterpret_cast<const v4f*>(&s.dv[wave][b][4 * grp]);
-                        const v4f d1 = *reinterpret_cast<const v4f*>(&s.dv[wave][b][16 + 4 * grp]);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            const bool packed = MODE == kPacked && t == 1;
-                            uint32_t h[4], l[4];
-                            split2(p[t][0] * d0[0], p[t][1] * d0[1], h[0], l[0]);
-                            split2(p[t][2] * d0[2], p[t][3] * d0[3], h[1], l[1]);
-                            split2(p[t][4] * d1[0], p[t][5] * d1[1], h[2], l[2]);
-                            split2(p[t][6] * d1[2], p[t][7] * d1[3], h[3], l[3]);
-                            if (packed) {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) h[e] = low_half ? l[e] : h[e];
-                            }
-                            const v8h ph = half8(make_uint4(h[0], h[1], h[2], h[3]));
-                            const v8h plo = half8(make_uint4(l[0], l[1], l[2], l[3]));
-#pragma unroll
-                            for (uint32_t c = 0; c < 2; ++c) {
-                                if (!packed) o[2 * b + c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], plo, o[2 * b + c][t], 0, 0, 0);
-                                o[2 * b + c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], ph, o[2 * b + c][t], 0, 0, 0);
-                            }
+                    for (uint32_t c = 2 * b; c < 2 * b + 2; ++c) {
+                        v8h v = values(c), rest;
+                        if constexpr (Q8) {
+                            const v8h code = v;
+                            v = code * d;
+                            rest = __builtin_elementwise_fma(code, d, -v);
                         }
-                    }
-                } else {
-                    v8h ph[NT], plo[MODE == kTwo ? 2 : 1];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const uint32_t* src = s.p + (t * 16 + n16) * 20 + grp * 4;
-                        ph[t] = half8(*reinterpret_cast<const uint4*>(src));
-                        if (!(MODE == kPacked && t == 1)) plo[t % (MODE == kTwo ? 2 : 1)] = half8(*reinterpret_cast<const uint4*>(src + 16 * NT * 20));
-                    }
-#pragma unroll
-                    for (uint32_t c = 0; c < 8; ++c) {
-                        if (!FULL && c >= 2 * blocks) continue;
-                        const v8h v = values(c);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
+                            if constexpr (Q8) o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, ph[t], o[c][t], 0, 0, 0);
                             if (!(MODE == kPacked && t == 1)) o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, plo[t % (MODE == kTwo ? 2 : 1)], o[c][t], 0, 0, 0);
                             o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t], o[c][t], 0, 0, 0);
                         }
@@ -739,7 +724,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         const bool low_half = n16 >= 8;
         const auto head_of = [&](int t) { return MODE == kPacked && t == 1 ? 16 + (n16 & 7) : 16 * t + n16; };
         const bool first = tile0 == 0, whole = first && count == n_tiles;
-        const float back = Q8 ? (e_run == -100 ? 0.0f : pow2(e_run - 14)) : 1.0f / kPScale;
+        const float back = Q8 ? pow2(e_run - 15) : 1.0f / kPScale;
         const uint64_t slot = (uint64_t)wg * 2 + (first ? 1 : 0);
         if constexpr (MODE == kPacked) {  // both parts' sums
 #pragma unroll
@@ -813,27 +798,42 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 }
 
 // Joins the pieces of split items, in order: out = sum_k w_k O_k / sum_k w_k l_k
-// with w_k = 2^(m_k - max m). Half-waves of 32 lanes take 128 columns of a
-// head each (16 bytes per lane); for an item of many pieces up to 32
-// half-waves share them and add their sums through LDS.
+// with w_k = 2^(m_k - max m). A team of 32 lanes takes 128 columns of a head
+// (16 bytes per lane); an item of more than 64 pieces goes to teams of 8 lanes
+// and 32 columns, so that it reaches the whole chip. Teams share an item's pieces
+// and add their sums through LDS.
+struct JoinShape {
+    uint32_t lanes;  // of a team
+    uint32_t share;  // teams per head and column part
+    __device__ explicit JoinShape(uint32_t pieces) {
+        lanes = pieces > 64 ? 8 : 32;
+        share = 1;
+        while (share < kJoinThreads / lanes && share * 4 < pieces) share *= 2;
+    }
+    __device__ uint32_t parts(uint32_t rank) const { return (rank + 4 * lanes - 1) / (4 * lanes); }
+    __device__ uint32_t per_job() const { return kJoinThreads / lanes / share; }  // heads x parts
+};
+
 __global__ __launch_bounds__(kJoinThreads) void mla_join_kernel(MlaArgs a, MlaPlan pl) {
-    __shared__ __align__(16) float sums[32][128];
-    // A job's rows times its pieces: at most 32 / (4 share) + 2 rows of 8 share
-    // pieces (parts = 4), 32 / share + 1 rows (parts = 1), or one row of all.
+    __shared__ __align__(16) float sums[kJoinThreads * 4];
+    // A job's heads times the item's pieces: at most 32 / share heads of 4 share
+    // pieces, or 128 / share of them.
     __shared__ float weights[kMlaMostGroups];
-    __shared__ float2 row_ml[33];
+    __shared__ float2 row_ml[32];
     __shared__ uint32_t scan[kJoinThreads / 64];
     __shared__ uint32_t cur[4];
-    const uint32_t tid = threadIdx.x, hw = tid >> 5, l32 = tid & 31, wave = tid >> 6;
-    const uint32_t rank = a.geom.rank, parts = (rank + 127) / 128;
+    const uint32_t tid = threadIdx.x, wave = tid >> 6;
+    const uint32_t rank = a.geom.rank;
     // Thread g knows the item that workgroup g began and did not finish, and
     // which of the call's jobs are that item's.
     MlaSplit sp{0, 0};
     if (tid < pl.groups) sp = reinterpret_cast<const MlaSplit*>(pl.splits)[tid];
-    uint32_t share = 1;  // half-waves per head and 128 columns
-    while (share < 32 && share * 8 < sp.pieces) share *= 2;
-    const uint32_t heads_of = min(pl.rows, a.n_heads - (sp.item % pl.head_tiles) * pl.rows);
-    const uint32_t my_jobs = sp.pieces ? (heads_of * parts * share + 31) / 32 : 0;
+    uint32_t my_jobs = 0;
+    if (sp.pieces) {
+        const JoinShape j(sp.pieces);
+        const uint32_t heads = min(pl.rows, a.n_heads - (sp.item % pl.head_tiles) * pl.rows);
+        my_jobs = (heads * j.parts(rank) + j.per_job() - 1) / j.per_job();
+    }
     uint32_t end = my_jobs;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -857,66 +857,65 @@ __global__ __launch_bounds__(kJoinThreads) void mla_join_kernel(MlaArgs a, MlaPl
             cur[3] = all_job - (end - my_jobs);
         }
         __syncthreads();
-        {
-            const uint32_t g0 = cur[0], item = cur[1], pieces = cur[2], job = cur[3];
-            const uint32_t token = item / pl.head_tiles, head0 = (item % pl.head_tiles) * pl.rows;
-            const uint32_t heads = min(pl.rows, a.n_heads - head0);
-            uint32_t share = 1;
-            while (share < 32 && share * 8 < pieces) share *= 2;
-            const uint32_t per_wg = 32 / share, units = heads * parts;
-            const uint32_t unit = job * per_wg + hw / share, mine = hw % share;
-            const bool on = unit < units;
-            const uint32_t r0 = job * per_wg / parts, r1 = min((job + 1) * per_wg - 1, units - 1) / parts;
-            const uint32_t r = on ? unit / parts : r0, c = (on ? unit % parts : 0) * 128 + l32 * 4;
-            // The weights of this job's rows, a half-wave each.
-            for (uint32_t i = r0 + hw; i <= r1; i += 32) {
-                float top = -INFINITY, l = 0.0f;
-                for (uint32_t q = l32; q < pieces; q += 32)
-                    top = fmaxf(top, pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + i].x);
+        const uint32_t g0 = cur[0], item = cur[1], pieces = cur[2], job = cur[3];
+        const JoinShape j(pieces);
+        const uint32_t token = item / pl.head_tiles, head0 = (item % pl.head_tiles) * pl.rows;
+        const uint32_t heads = min(pl.rows, a.n_heads - head0);
+        const uint32_t parts = j.parts(rank), units = heads * parts, per_job = j.per_job();
+        const uint32_t team = tid / j.lanes, in_team = tid % j.lanes;
+        const uint32_t unit = job * per_job + team / j.share, mine = team % j.share;
+        const bool on = unit < units;
+        const uint32_t r0 = job * per_job / parts, r1 = min((job + 1) * per_job - 1, units - 1) / parts;
+        const uint32_t r = on ? unit / parts : r0, c = (on ? unit % parts : 0) * 4 * j.lanes + in_team * 4;
+        // The weights of this job's heads, 32 lanes each.
+        for (uint32_t i = r0 + tid / 32; i <= r1; i += kJoinThreads / 32) {
+            const uint32_t l32 = tid & 31;
+            float top = -INFINITY, l = 0.0f;
+            for (uint32_t q = l32; q < pieces; q += 32)
+                top = fmaxf(top, pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + i].x);
 #pragma unroll
-                for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-                const float base = top == -INFINITY ? 0.0f : top;
-                for (uint32_t q = l32; q < pieces; q += 32) {
-                    const float2 ml = pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + i];
-                    const float w = __builtin_amdgcn_exp2f(ml.x - base);
-                    weights[(i - r0) * pieces + q] = w;
-                    l += w * ml.y;
-                }
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) l += __shfl_xor(l, d, 64);
-                if (l32 == 0) row_ml[i - r0] = make_float2(top, l);
+            for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+            const float base = top == -INFINITY ? 0.0f : top;
+            for (uint32_t q = l32; q < pieces; q += 32) {
+                const float2 ml = pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + i];
+                const float w = __builtin_amdgcn_exp2f(ml.x - base);
+                weights[(i - r0) * pieces + q] = w;
+                l += w * ml.y;
             }
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) l += __shfl_xor(l, d, 64);
+            if (l32 == 0) row_ml[i - r0] = make_float2(top, l);
+        }
+        __syncthreads();
+        v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (on && c < rank) {
+            const float* src = pl.parts + ((uint64_t)g0 * 2 * pl.part_rows + r) * rank + c;
+            const uint64_t step = 2ull * pl.part_rows * rank, own = (uint64_t)pl.part_rows * rank;
+            const float* w = weights + (r - r0) * pieces;
+#pragma unroll 4
+            for (uint32_t p = mine; p < pieces; p += j.share)
+                acc += *reinterpret_cast<const v4f*>(src + p * step + (p == 0 ? own : 0)) * w[p];
+        }
+        const float top = row_ml[r - r0].x, l = row_ml[r - r0].y;
+        // Halves of a unit's teams, down to one.
+        for (uint32_t n = j.share / 2; n > 0; n /= 2) {
             __syncthreads();
-            v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (on && c < rank) {
-                const float* src = pl.parts + ((uint64_t)g0 * 2 * pl.part_rows + r) * rank + c;
-                const uint64_t step = 2ull * pl.part_rows * rank, own = (uint64_t)pl.part_rows * rank;
-                const float* w = weights + (r - r0) * pieces;
-#pragma unroll 8
-                for (uint32_t p = mine; p < pieces; p += share)
-                    acc += *reinterpret_cast<const v4f*>(src + p * step + (p == 0 ? own : 0)) * w[p];
-            }
-            const float top = row_ml[r - r0].x, l = row_ml[r - r0].y;
-            if (share > 1) {
-                __syncthreads();
-                *reinterpret_cast<v4f*>(&sums[hw][l32 * 4]) = acc;
-                __syncthreads();
-                if (mine == 0)
-                    for (uint32_t i = 1; i < share; ++i) acc += *reinterpret_cast<const v4f*>(&sums[hw + i][l32 * 4]);
-            }
-            if (mine == 0 && on && c < rank) {
-                const v4f v = l == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc / l;
-                float* dst = a.out + (uint64_t)token * a.out_token_stride + (uint64_t)(head0 + r) * a.out_head_stride + c;
-                if (pl.vec_out) {
-                    *reinterpret_cast<v4f*>(dst) = v;
-                } else {
+            if (mine >= n && mine < 2 * n) *reinterpret_cast<v4f*>(&sums[tid * 4]) = acc;
+            __syncthreads();
+            if (mine < n) acc += *reinterpret_cast<const v4f*>(&sums[(tid + n * j.lanes) * 4]);
+        }
+        if (mine == 0 && on && c < rank) {
+            const v4f v = l == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc / l;
+            float* dst = a.out + (uint64_t)token * a.out_token_stride + (uint64_t)(head0 + r) * a.out_head_stride + c;
+            if (pl.vec_out) {
+                *reinterpret_cast<v4f*>(dst) = v;
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dst[e] = v[e];
-                }
-                if (a.lse && c == 0)
-                    a.lse[(uint64_t)token * a.n_heads + head0 + r] =
-                        l == 0.0f ? -INFINITY : 0.69314718055995f * (top + __builtin_amdgcn_logf(l));
+                for (int e = 0; e < 4; ++e) dst[e] = v[e];
             }
+            if (a.lse && c == 0)
+                a.lse[(uint64_t)token * a.n_heads + head0 + r] =
+                    l == 0.0f ? -INFINITY : 0.69314718055995f * (top + __builtin_amdgcn_logf(l));
         }
     }
 }
