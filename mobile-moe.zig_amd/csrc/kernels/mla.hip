@@ -74,7 +74,7 @@ struct MlaLds {
     static constexpr int NT = mode_tiles(MODE);
     uint8_t kv[kMlaWaves][kMlaTile * 256];  // f16 [position][128], 16-byte chunks swizzled by the position
     uint8_t pe[kMlaWaves][kMlaTile * 32];   // f16 [position][16]
-    float sp[kMlaWaves][16 * NT][kSpLd];    // score partials, a row per product column
+    float sp[kMlaWaves][mode_rows(MODE)][kSpLd];  // score partials
     // P: f16 in rows of 40 (per tile high parts, low parts; packed as it is)
     uint32_t p[(MODE == kTwo ? 4 : MODE == kPacked ? 3 : 2) * 16 * 20];
     float ds[Q8 ? kMlaWaves : 1][5][kMlaTile];  // block scales of the keys
@@ -138,7 +138,7 @@ template <int CTRL>
 __device__ __forceinline__ float permuted(float v) {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xF, 0xF, true));
 }
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140, kRotate8 = 0x128;
 template <int LANES>
 __device__ __forceinline__ float group_max(float v) {
     v = fmaxf(v, permuted<kXor1>(v));
@@ -600,8 +600,13 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                         for (int t = 0; t < NT; ++t) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kpe, pe2[t], sc[t], 0, 0, 0);
                     }
                 }
+                if constexpr (MODE == kPacked) {  // high and low parts' products, half a row of lanes apart
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                    for (int e = 0; e < 4; ++e) sc[1][e] += permuted<kRotate8>(sc[1][e]);
+                    if (!low_half) *reinterpret_cast<v4f*>(&s.sp[wave][16 + n16][pt * 16 + 4 * grp]) = sc[1];
+                }
+#pragma unroll
+                for (int t = 0; t < (MODE == kTwo ? 2 : 1); ++t)
                     *reinterpret_cast<v4f*>(&s.sp[wave][t * 16 + n16][pt * 16 + 4 * grp]) = sc[t];
             }
             lds_barrier();
@@ -616,12 +621,6 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 for (uint32_t w = 1; w < kMlaWaves; ++w)
 #pragma unroll
                     for (uint32_t e = 0; e < kPer; ++e) x[e] += s.sp[w][srow][spos + e];
-                if (MODE == kPacked && wave == 2) {  // heads 16..23: their low parts' products
-#pragma unroll
-                    for (uint32_t w = 0; w < kMlaWaves; ++w)
-#pragma unroll
-                        for (uint32_t e = 0; e < kPer; ++e) x[e] += s.sp[w][(srow + 8) % (16 * NT)][spos + e];
-                }
                 const uint32_t lv = mask >> spos;
 #pragma unroll
                 for (uint32_t e = 0; e < kPer; ++e) {
@@ -867,24 +866,30 @@ __global__ __launch_bounds__(kJoinThreads) void mla_join_kernel(MlaArgs a, MlaPl
         const bool on = unit < units;
         const uint32_t r0 = job * per_job / parts, r1 = min((job + 1) * per_job - 1, units - 1) / parts;
         const uint32_t r = on ? unit / parts : r0, c = (on ? unit % parts : 0) * 4 * j.lanes + in_team * 4;
-        // The weights of this job's heads, 32 lanes each.
-        for (uint32_t i = r0 + tid / 32; i <= r1; i += kJoinThreads / 32) {
+        // The weights of this job's heads: every maximum and sum by a thread of
+        // its own, then 32 lanes per head.
+        for (uint32_t i = tid; i < (r1 - r0 + 1) * pieces; i += kJoinThreads) {
+            const uint32_t q = i % pieces, h = r0 + i / pieces;
+            const float2 ml = pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + h];
+            weights[i] = ml.x;
+            sums[i] = ml.y;
+        }
+        __syncthreads();
+        for (uint32_t i = tid / 32; i <= r1 - r0; i += kJoinThreads / 32) {
             const uint32_t l32 = tid & 31;
+            float* w = weights + i * pieces;
             float top = -INFINITY, l = 0.0f;
-            for (uint32_t q = l32; q < pieces; q += 32)
-                top = fmaxf(top, pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + i].x);
+            for (uint32_t q = l32; q < pieces; q += 32) top = fmaxf(top, w[q]);
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
             const float base = top == -INFINITY ? 0.0f : top;
             for (uint32_t q = l32; q < pieces; q += 32) {
-                const float2 ml = pl.part_ml[((uint64_t)(g0 + q) * 2 + (q == 0)) * pl.rows + i];
-                const float w = __builtin_amdgcn_exp2f(ml.x - base);
-                weights[(i - r0) * pieces + q] = w;
-                l += w * ml.y;
+                w[q] = __builtin_amdgcn_exp2f(w[q] - base);
+                l += w[q] * sums[i * pieces + q];
             }
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) l += __shfl_xor(l, d, 64);
-            if (l32 == 0) row_ml[i - r0] = make_float2(top, l);
+            if (l32 == 0) row_ml[i] = make_float2(top, l);
         }
         __syncthreads();
         v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
