@@ -54,7 +54,7 @@ constexpr int kMlaThreads = 256, kMlaWaves = 4;
 constexpr uint32_t kMlaTile = 32;       // positions per tile
 constexpr uint32_t kMlaCols = 128;      // latent columns per wave
 constexpr uint32_t kMlaPe = 16;         // rotary columns per wave
-constexpr uint32_t kSpLd = 36;          // floats between rows of the score partials
+constexpr uint32_t kSpLd = 36;          // floats between rows of the score partials (16-byte rows)
 constexpr float kPScale = 32768.0f;     // P in [0, 1] uses f16's upper range: parts down to 2^-39 survive
 constexpr int kJoinThreads = 1024;
 
@@ -551,76 +551,93 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             const uint32_t v_at = v_row * 256 + ((((n16 >> 1) & 1) ^ v_row) << 4) + (n16 & 1) * 8;
             const uint32_t srow = wave * (64 / kLanes) + ln / kLanes, spos = (ln % kLanes) * kPer;
             // ---- S^T partial ----
+            // The keys of the first 16 positions, then each block's products with
+            // the same block of the other 16 requested behind them: no wait on
+            // LDS but the first. (The scheduling barriers keep that order; left
+            // alone, each read is placed and waited for right before its use.)
+            {
+                const auto key = [&](int pt, uint32_t b) {
+                    return half8(b < 4 ? *reinterpret_cast<const uint4*>(kv + pt * 4096 + (k_at ^ (b << 6)))
+                                       : *reinterpret_cast<const uint4*>(s.pe[wave] + pt * 512 + n16 * 32 + 16 * (grp & 1)));
+                };
+                const auto there = [&](uint32_t b) { return b < 4 ? FULL || b < blocks : has_pe; };
+                v8h k[5];
+                v4f sc[2][NT], x[2][NT], d[2];
 #pragma unroll
-            for (int pt = 0; pt < 2; ++pt) {
-                v8h k[4];
+                for (uint32_t b = 0; b < 5; ++b) k[b] = key(0, b);
+                if constexpr (Q8) d[0] = *reinterpret_cast<const v4f*>(&s.ds[wave][0][4 * grp]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (uint32_t b = 0; b < 4; ++b)
-                    k[b] = half8(*reinterpret_cast<const uint4*>(kv + pt * 4096 + (k_at ^ (b << 6))));
-                const v8h kpe = half8(*reinterpret_cast<const uint4*>(s.pe[wave] + pt * 512 + n16 * 32 + 16 * (grp & 1)));
-                v4f sc[NT];
+                for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) sc[t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (Q8) {
+                    for (int t = 0; t < NT; ++t) sc[pt][t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+                // Step i: block i % 5 (4: the rotary columns) of half i / 5.
 #pragma unroll
-                    for (uint32_t b = 0; b < 4; ++b) {
-                        if (!FULL && b >= blocks) continue;
-                        const v4f d = *reinterpret_cast<const v4f*>(&s.ds[wave][b][pt * 16 + 4 * grp]);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
-                            if (!(MODE == kPacked && t == 1)) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b], ql[t % (MODE == kTwo ? 2 : 1)][b], x, 0, 0, 0);
-                            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b], qh[t][b], x, 0, 0, 0);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) sc[t][e] = fmaf(d[e], x[e], sc[t][e]);
-                        }
-                    }
-                    if (has_pe) {
-                        const v4f d = *reinterpret_cast<const v4f*>(&s.ds[wave][4][pt * 16 + 4 * grp]);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
-                            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kpe, pe2[t], x, 0, 0, 0);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) sc[t][e] = fmaf(d[e], x[e], sc[t][e]);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (uint32_t b = 0; b < 4; ++b) {
-                        if (!FULL && b >= blocks) continue;
+                for (uint32_t i = 0; i <= (Q8 ? 10 : 9); ++i) {
+                    const uint32_t pt = i / 5, b = i % 5;
+                    if (i < 10 && there(b)) {
+                        v4f(&acc)[NT] = Q8 ? x[i & 1] : sc[pt & 1];
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            if (!(MODE == kPacked && t == 1)) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b], ql[t % (MODE == kTwo ? 2 : 1)][b], sc[t], 0, 0, 0);
-                            sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b], qh[t][b], sc[t], 0, 0, 0);
+                            if (Q8) acc[t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+                            if (b < 4 && !(MODE == kPacked && t == 1))
+                                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b], ql[t % (MODE == kTwo ? 2 : 1)][b & 3], acc[t], 0, 0, 0);
                         }
-                    }
-                    if (has_pe) {
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kpe, pe2[t], sc[t], 0, 0, 0);
+                        for (int t = NT - 1; t >= 0; --t)
+                            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b], b < 4 ? qh[t][b & 3] : pe2[t], acc[t], 0, 0, 0);
                     }
-                }
-                if constexpr (MODE == kPacked) {  // high and low parts' products, half a row of lanes apart
+                    if (i < 5) k[b] = key(1, b);
+                    if constexpr (Q8) {
+                        // The block before, while this one's products run.
+                        if (i > 0 && there((i - 1) % 5)) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[1][e] += permuted<kRotate8>(sc[1][e]);
-                    if (!low_half) *reinterpret_cast<v4f*>(&s.sp[wave][16 + n16][pt * 16 + 4 * grp]) = sc[1];
+                            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    sc[(i - 1) / 5][t][e] = fmaf(d[(i - 1) & 1][e], x[(i - 1) & 1][t][e], sc[(i - 1) / 5][t][e]);
+                        }
+                        if (i < 9) d[(i + 1) & 1] = *reinterpret_cast<const v4f*>(&s.ds[wave][(i + 1) % 5][(i + 1) / 5 * 16 + 4 * grp]);
+                    }
+                    if (!Q8 && i < 5) __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
-                for (int t = 0; t < (MODE == kTwo ? 2 : 1); ++t)
-                    *reinterpret_cast<v4f*>(&s.sp[wave][t * 16 + n16][pt * 16 + 4 * grp]) = sc[t];
+                for (int pt = 0; pt < 2; ++pt) {
+                    if constexpr (MODE == kPacked) {  // high and low parts' products, half a row of lanes apart
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sc[pt][1][e] += permuted<kRotate8>(sc[pt][1][e]);
+                    }
+                    *reinterpret_cast<v4f*>(&s.sp[wave][n16][pt * 16 + 4 * grp]) = sc[pt][0];
+                    if (MODE == kTwo || (MODE == kPacked && !low_half))
+                        *reinterpret_cast<v4f*>(&s.sp[wave][16 + n16][pt * 16 + 4 * grp]) = sc[pt][NT - 1];
+                }
             }
             lds_barrier();
 
             // ---- softmax of this wave's heads ----
+            // Half of the values' operands (16 columns, all 32 positions each)
+            // are read behind the scores and arrive meanwhile.
+            typedef float vper __attribute__((ext_vector_type(kPer)));
+            vper part[kMlaWaves];
+            float fac = 0.0f;
             if (softmax) {
-                const float fac = s.factor[srow];
-                float x[kPer], top = -INFINITY;
+                fac = s.factor[srow];
 #pragma unroll
-                for (uint32_t e = 0; e < kPer; ++e) x[e] = s.sp[0][srow][spos + e];
+                for (uint32_t w = 0; w < kMlaWaves; ++w) part[w] = *reinterpret_cast<const vper*>(&s.sp[w][srow][spos]);
+            }
+            v8h val[8];
+            const auto read_values = [&](uint32_t c) {
+                const v4s t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + (v_at ^ (c << 5))));
+                const v4s t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + 4096 + (v_at ^ (c << 5))));
+                const uint2 x = __builtin_bit_cast(uint2, t0), y = __builtin_bit_cast(uint2, t1);
+                val[c] = half8(make_uint4(x.x, x.y, y.x, y.y));
+            };
 #pragma unroll
-                for (uint32_t w = 1; w < kMlaWaves; ++w)
-#pragma unroll
-                    for (uint32_t e = 0; e < kPer; ++e) x[e] += s.sp[w][srow][spos + e];
+            for (uint32_t c = 0; c < 4; ++c) read_values(c);
+            __builtin_amdgcn_sched_barrier(0);
+            if (softmax) {
+                vper x = ((part[0] + part[1]) + part[2]) + part[3];
+                float top = -INFINITY;
                 const uint32_t lv = mask >> spos;
 #pragma unroll
                 for (uint32_t e = 0; e < kPer; ++e) {
@@ -639,16 +656,22 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 sum = group_sum<kLanes>(sum);
                 l_run = l_run * al + sum;
                 m_run = m_new;
-                if (lane % kLanes == 0) s.alpha[srow] = al;
-                // position 16 h + 4 g + e is O^T's operand element 4 h + e of group g
+                if (ln % kLanes == 0) s.alpha[srow] = al;
+                // position 16 h + 4 g + e is O^T's operand element 4 h + e of group g;
+                // rows: high parts of both tiles, low parts of both; packed: high 16, packed 16, low 16
                 const uint32_t at = ((spos >> 2) & 3) * 8 + (spos >> 4) * 4 + (spos & 3);
-                {
-                    // rows: high parts of both tiles, low parts of both; packed: high 16, packed 16, low 16
-                    const bool packed = MODE == kPacked && wave == 2;
-                    uint32_t* hi = s.p + srow * 20 + at / 2;
-                    uint32_t* lo = hi + (packed ? 8 : 16 * NT) * 20;
+                const bool packed = MODE == kPacked && wave == 2;
+                uint32_t* hi = s.p + srow * 20 + at / 2;
+                uint32_t* lo = hi + (packed ? 8 : 16 * NT) * 20;
+                uint32_t h[kPer / 2], l[kPer / 2];
 #pragma unroll
-                    for (uint32_t e = 0; e < kPer; e += 2) split2(x[e] * kPScale, x[e + 1] * kPScale, hi[e / 2], lo[e / 2]);
+                for (uint32_t e = 0; e < kPer; e += 2) split2(x[e] * kPScale, x[e + 1] * kPScale, h[e / 2], l[e / 2]);
+                if constexpr (kPer == 4) {
+                    *reinterpret_cast<uint2*>(hi) = make_uint2(h[0], h[1]);
+                    *reinterpret_cast<uint2*>(lo) = make_uint2(l[0], l[1]);
+                } else {
+                    *hi = h[0];
+                    *lo = l[0];
                 }
             }
             lds_barrier();
@@ -657,9 +680,16 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             {
                 float al[NT];
                 bool same = true;
+                v8h ph[NT], plo[MODE == kTwo ? 2 : 1];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     al[t] = s.alpha[head_of(t)];
+                    const uint32_t* src = s.p + (t * 16 + n16) * 20 + grp * 4;
+                    ph[t] = half8(*reinterpret_cast<const uint4*>(src));
+                    if (!(MODE == kPacked && t == 1)) plo[t % (MODE == kTwo ? 2 : 1)] = half8(*reinterpret_cast<const uint4*>(src + 16 * NT * 20));
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
                     if constexpr (Q8) al[t] *= e_scale;
                     same = same && al[t] == 1.0f;
                 }
@@ -669,43 +699,40 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 #pragma unroll
                         for (int t = 0; t < NT; ++t) o[c][t] *= al[t];
                 }
-                const auto values = [&](uint32_t c) {  // 16 columns, all 32 positions
-                    const v4s t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + (v_at ^ (c << 5))));
-                    const v4s t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + 4096 + (v_at ^ (c << 5))));
-                    const uint2 x = __builtin_bit_cast(uint2, t0), y = __builtin_bit_cast(uint2, t1);
-                    return half8(make_uint4(x.x, x.y, y.x, y.y));
-                };
-                v8h ph[NT], plo[MODE == kTwo ? 2 : 1];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const uint32_t* src = s.p + (t * 16 + n16) * 20 + grp * 4;
-                    ph[t] = half8(*reinterpret_cast<const uint4*>(src));
-                    if (!(MODE == kPacked && t == 1)) plo[t % (MODE == kTwo ? 2 : 1)] = half8(*reinterpret_cast<const uint4*>(src + 16 * NT * 20));
-                }
+                for (uint32_t c = 4; c < 8; ++c) read_values(c);
+                // Two column tiles at a time, so that a product's sum is not
+                // asked for by the next one.
 #pragma unroll
                 for (uint32_t b = 0; b < 4; ++b) {
                     if (!FULL && b >= blocks) continue;
-                    v8h d;
+                    v8h v[2], rest[2];
                     if constexpr (Q8) {
                         const uint2 d0 = *reinterpret_cast<const uint2*>(&s.dv[wave][b][4 * grp]);
                         const uint2 d1 = *reinterpret_cast<const uint2*>(&s.dv[wave][b][16 + 4 * grp]);
-                        d = half8(make_uint4(d0.x, d0.y, d1.x, d1.y));
+                        const v8h d = half8(make_uint4(d0.x, d0.y, d1.x, d1.y));
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            v[c] = val[2 * b + c] * d;
+                            rest[c] = __builtin_elementwise_fma(val[2 * b + c], d, -v[c]);
+                        }
+                    } else {
+                        v[0] = val[2 * b];
+                        v[1] = val[2 * b + 1];
                     }
 #pragma unroll
-                    for (uint32_t c = 2 * b; c < 2 * b + 2; ++c) {
-                        v8h v = values(c), rest;
-                        if constexpr (Q8) {
-                            const v8h code = v;
-                            v = code * d;
-                            rest = __builtin_elementwise_fma(code, d, -v);
-                        }
+                    for (int part = 0; part < 3; ++part)
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            if constexpr (Q8) o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, ph[t], o[c][t], 0, 0, 0);
-                            if (!(MODE == kPacked && t == 1)) o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, plo[t % (MODE == kTwo ? 2 : 1)], o[c][t], 0, 0, 0);
-                            o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t], o[c][t], 0, 0, 0);
-                        }
-                    }
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                v4f& acc = o[2 * b + c][t];
+                                if (part == 0 && !(MODE == kPacked && t == 1))
+                                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], plo[t % (MODE == kTwo ? 2 : 1)], acc, 0, 0, 0);
+                                if (part == 1 && Q8) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest[c], ph[t], acc, 0, 0, 0);
+                                if (part == 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], ph[t], acc, 0, 0, 0);
+                            }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (++i >= count) break;
