@@ -257,12 +257,16 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         const int32_t* table = a.tables + (uint64_t)row * a.table_stride;
 
         // ---- loads of a tile: page numbers one tile before its rows ----
+        // None stands under a branch, past the piece's last tile neither: where
+        // a register is loaded on one way and kept on the other, the ways'
+        // meeting point waits for the load. Rows that are not wanted have an
+        // empty resource (no memory is touched); the few other bytes are read.
         int32_t id[2];
         auto load_ids = [&](uint32_t tile) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint64_t p = (uint64_t)tile * kMlaTile + 16 * h;
-                id[h] = p < len ? table[p >> g.page_shift] : -1;
+                id[h] = table[(p < len ? (uint32_t)p : len - 1) >> g.page_shift];
             }
         };
         uint4 pre[Q8 ? 4 : 8], pre_pe;
@@ -270,7 +274,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         uint32_t pre_dpe = 0, live = 0;
         pre_pe = make_uint4(0, 0, 0, 0);
         pre_d = make_uint2(0, 0);
-        auto load_rows = [&](uint32_t tile) {
+        auto load_rows = [&](uint32_t tile, bool wanted) {
             const uint32_t lane = afresh(tid & 63), n16 = lane & 15, grp = lane >> 4;
             BufRsrc rows[2];
             const uint8_t *base[2], *base_d[2];
@@ -286,7 +290,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 // 16 rows from p on. A page that is not there is read as page 0
                 // and left out.
                 base[h] = a.pool + paged_row(g, ok ? (uint32_t)page : 0u, p & at_mask);
-                rows[h] = make_rsrc(base[h], 16 * row_bytes);
+                rows[h] = make_rsrc(base[h], wanted ? 16 * row_bytes : 0);
                 if constexpr (Q8) base_d[h] = a.pool + paged_scales(g, ok ? (uint32_t)page : 0u, p & at_mask);
             }
             if (FULL || blocks) {
@@ -334,19 +338,9 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         int e_run = 0;  // Q8_0: value scales are taken times 2^-e_run
         float e_scale = 1.0f;
         auto stage = [&]() {
-            const uint32_t lane = afresh(tid & 63), n16 = lane & 15, grp = lane >> 4;
+            const uint32_t lane = afresh(tid & 63);
             mask = live;
             if constexpr (Q8) {
-                if (mask != 0xFFFFFFFFu) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t keep = 0u - ((mask >> (8 * j + (lane >> 3))) & 1u);
-                        pre[j].x &= keep, pre[j].y &= keep, pre[j].z &= keep, pre[j].w &= keep;
-                    }
-                    const uint32_t keep = 0u - ((mask >> (lane & 31)) & 1u);
-                    pre_pe.x &= keep, pre_pe.y &= keep, pre_pe.z &= keep, pre_pe.w &= keep;
-                    pre_d.x &= keep, pre_d.y &= keep, pre_dpe &= keep;
-                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t p = 8 * j + (lane >> 3), c = 2 * (lane & 7);
@@ -354,6 +348,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                     *reinterpret_cast<uint4*>(dst + ((c ^ (p & 15)) << 4)) = codes8(pre[j].x, pre[j].y);
                     *reinterpret_cast<uint4*>(dst + ((c ^ (p & 15) ^ 1) << 4)) = codes8(pre[j].z, pre[j].w);
                 }
+                const uint32_t p = lane & 31;
                 float d[5];
                 d[0] = f16_scale((uint16_t)(pre_d.x & 0xFFFFu));
                 d[1] = f16_scale((uint16_t)(pre_d.x >> 16));
@@ -361,50 +356,57 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 d[3] = f16_scale((uint16_t)(pre_d.y >> 16));
                 d[4] = f16_scale((uint16_t)(FULL ? pre_dpe >> (wave / 2 * 16) : pre_dpe));
                 float top = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
-                top = group_max<16>(top);
+                top = group_max<16>((mask >> p) & 1 ? top : 0.0f);
                 // As bits they compare like numbers; 2^8 and more: 1 to 9 (infinity).
                 const uint32_t tb = max(__builtin_amdgcn_readlane(__float_as_uint(top), 0), __builtin_amdgcn_readlane(__float_as_uint(top), 16));
                 const int e = min(max((int)(tb >> 23) - 134, 0), 9);
                 // The sums so far follow in the O phase, with the softmax's factor.
                 e_scale = e > e_run ? pow2(e_run - e) : 1.0f;
                 e_run = max(e, e_run);
-                if (e_run) {
-                    const v2h f2 = (v2h)(_Float16)pow2(-e_run);
-                    pre_d.x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, pre_d.x) * f2);
-                    pre_d.y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, pre_d.y) * f2);
-                }
-                const uint32_t p = lane & 31;
+                const v2h f2 = (v2h)(_Float16)pow2(-e_run);
+                const uint32_t d01 = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, pre_d.x) * f2);
+                const uint32_t d23 = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, pre_d.y) * f2);
                 if (lane < 32) {
 #pragma unroll
                     for (int b = 0; b < 5; ++b) s.ds[wave][b][p] = d[b];
-                    s.dv[wave][0][p] = (uint16_t)(pre_d.x & 0xFFFFu);
-                    s.dv[wave][1][p] = (uint16_t)(pre_d.x >> 16);
-                    s.dv[wave][2][p] = (uint16_t)(pre_d.y & 0xFFFFu);
-                    s.dv[wave][3][p] = (uint16_t)(pre_d.y >> 16);
+                    s.dv[wave][0][p] = (uint16_t)(d01 & 0xFFFFu);
+                    s.dv[wave][1][p] = (uint16_t)(d01 >> 16);
+                    s.dv[wave][2][p] = (uint16_t)(d23 & 0xFFFFu);
+                    s.dv[wave][3][p] = (uint16_t)(d23 >> 16);
                     *reinterpret_cast<uint4*>(s.pe[wave] + p * 32) = codes8(pre_pe.x, pre_pe.y);
                     *reinterpret_cast<uint4*>(s.pe[wave] + p * 32 + 16) = codes8(pre_pe.z, pre_pe.w);
                 }
             } else {
-                if (mask != 0xFFFFFFFFu) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t keep = 0u - ((mask >> (4 * j + grp)) & 1u);
-                        pre[j].x &= keep, pre[j].y &= keep, pre[j].z &= keep, pre[j].w &= keep;
-                    }
-                    const uint32_t keep = 0u - ((mask >> (lane >> 1)) & 1u);
-                    pre_pe.x &= keep, pre_pe.y &= keep, pre_pe.z &= keep, pre_pe.w &= keep;
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t p = 4 * j + (lane >> 4);
+                    *reinterpret_cast<uint4*>(kv + p * 256 + (((lane & 15) ^ (p & 15)) << 4)) = pre[j];
                 }
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    *reinterpret_cast<uint4*>(kv + j * 1024 + grp * 256 + (((n16 ^ grp) << 4) ^ ((j & 3) << 6))) = pre[j];
                 *reinterpret_cast<uint4*>(s.pe[wave] + lane * 16) = pre_pe;
             }
             // The slice is read back through other types, by this wave alone.
             asm volatile("" ::: "memory");
+            if (mask != 0xFFFFFFFFu) {  // two lanes clear a row
+                const uint32_t p = lane >> 1;
+                if (!((mask >> p) & 1)) {
+                    const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(kv + p * 256 + (lane & 1) * 128 + 16 * j) = zero;
+                    *reinterpret_cast<uint4*>(s.pe[wave] + lane * 16) = zero;
+                    if constexpr (Q8) {
+#pragma unroll
+                        for (int b = 0; b < 5; ++b) {
+                            s.ds[wave][b][p] = 0.0f;
+                            if (b < 4) s.dv[wave][b][p] = 0;
+                        }
+                    }
+                }
+                asm volatile("" ::: "memory");
+            }
         };
 
         load_ids(tile0);
-        load_rows(tile0);
+        load_rows(tile0, true);
         load_ids(tile0 + 1);
 
         // ---- the queries, scaled by a power of two per head, in two parts ----
@@ -473,10 +475,8 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             // The first tile goes to LDS and the second is asked for before
             // the queries are waited for.
             stage();
-            if (count > 1) {
-                load_rows(tile0 + 1);
-                load_ids(tile0 + 2);
-            }
+            load_rows(tile0 + 1, count > 1);
+            load_ids(tile0 + 2);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const bool there = head0 + head_of(t) < a.n_heads;
@@ -619,12 +619,10 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             // are read behind the scores and arrive meanwhile.
             typedef float vper __attribute__((ext_vector_type(kPer)));
             vper part[kMlaWaves];
-            float fac = 0.0f;
-            if (softmax) {
-                fac = s.factor[srow];
+            const uint32_t from = min(srow, kHeads - 1);  // (a wave without heads reads along)
+            const float fac = s.factor[from];
 #pragma unroll
-                for (uint32_t w = 0; w < kMlaWaves; ++w) part[w] = *reinterpret_cast<const vper*>(&s.sp[w][srow][spos]);
-            }
+            for (uint32_t w = 0; w < kMlaWaves; ++w) part[w] = *reinterpret_cast<const vper*>(&s.sp[w][from][spos]);
             v8h val[8];
             const auto read_values = [&](uint32_t c) {
                 const v4s t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + (v_at ^ (c << 5))));
@@ -737,10 +735,8 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             }
             if (++i >= count) break;
             stage();
-            if (i + 1 < count) {
-                load_rows(tile0 + i + 1);
-                load_ids(tile0 + i + 2);
-            }
+            load_rows(tile0 + i + 1, i + 1 < count);
+            load_ids(tile0 + i + 2);
         }
 
         // ---- the piece's result ----
@@ -756,7 +752,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 #pragma unroll
             for (int c = 0; c < 8; ++c)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[c][1][e] += __shfl_xor(o[c][1][e], 8, 64);
+                for (int e = 0; e < 4; ++e) o[c][1][e] += permuted<kRotate8>(o[c][1][e]);
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -777,10 +773,12 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             }
             dst += wave * kMlaCols + 4 * grp;
             if (!whole || pl.vec_out) {
+                // Written through: the next launch reads them on other XCDs, and
+                // lines left in L2 would be flushed at this one's end.
 #pragma unroll
                 for (uint32_t c = 0; c < 8; ++c) {
                     if (!FULL && c >= 2 * blocks) continue;
-                    *reinterpret_cast<v4f*>(dst + 16 * c) = o[c][t] * f2;
+                    __builtin_nontemporal_store(o[c][t] * f2, reinterpret_cast<v4f*>(dst + 16 * c));
                 }
             } else {
 #pragma unroll
@@ -929,12 +927,19 @@ __global__ __launch_bounds__(kJoinThreads) void mla_join_kernel(MlaArgs a, MlaPl
                 acc += *reinterpret_cast<const v4f*>(src + p * step + (p == 0 ? own : 0)) * w[p];
         }
         const float top = row_ml[r - r0].x, l = row_ml[r - r0].y;
-        // Halves of a unit's teams, down to one.
-        for (uint32_t n = j.share / 2; n > 0; n /= 2) {
+        // A unit's teams: those of a wave by shuffles, the waves through LDS.
+        const uint32_t in_wave = min(j.share, 64 / j.lanes);
+        for (uint32_t n = 1; n < in_wave; n *= 2)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], n * j.lanes, 64);
+        if (j.share > in_wave) {
+            const uint32_t waves = j.share / in_wave;
             __syncthreads();
-            if (mine >= n && mine < 2 * n) *reinterpret_cast<v4f*>(&sums[tid * 4]) = acc;
+            if ((tid & 63) < j.lanes) *reinterpret_cast<v4f*>(&sums[(wave * j.lanes + in_team) * 4]) = acc;
             __syncthreads();
-            if (mine < n) acc += *reinterpret_cast<const v4f*>(&sums[(tid + n * j.lanes) * 4]);
+            if (mine == 0) {
+                for (uint32_t n = 1; n < waves; ++n) acc += *reinterpret_cast<const v4f*>(&sums[((wave + n) * j.lanes + in_team) * 4]);
+            }
         }
         if (mine == 0 && on && c < rank) {
             const v4f v = l == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc / l;
@@ -1022,7 +1027,7 @@ hipError_t launch_mla(const MlaArgs& a, hipStream_t s) {
     else launch_split<false>(a, p, w.mode, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    mla_join_kernel<<<a.num_cu, kJoinThreads, 0, s>>>(a, p);
+    mla_join_kernel<<<2 * a.num_cu, kJoinThreads, 0, s>>>(a, p);
     return hipGetLastError();
 }
 
