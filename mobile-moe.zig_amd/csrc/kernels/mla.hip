@@ -159,7 +159,7 @@ __device__ __forceinline__ float group_sum(float v) {
 // 2^e, e within f32's normal exponents.
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-template <bool Q8, int MODE, bool FULL>
+template <bool Q8, int MODE, bool FULL, int POL>
 __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, MlaPlan pl) {
     constexpr int NT = mode_tiles(MODE);       // product tiles of 16 columns
     constexpr uint32_t kHeads = mode_rows(MODE);
@@ -300,8 +300,8 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                                             : grp * row_bytes + wave * (2 * kMlaCols) + 16 * (FULL ? n16 : min(n16, 4 * blocks - 1));
 #pragma unroll
                 for (int j = 0; j < (Q8 ? 4 : 8); ++j) {
-                    if constexpr (Q8) pre[j] = buf_load_b128<kCacheStream>(rows[j >> 1], at_rows, 8 * (j & 1) * row_bytes);
-                    else pre[j] = buf_load_b128<kCacheStream>(rows[j >> 2], at_rows, 4 * (j & 3) * row_bytes);
+                    if constexpr (Q8) pre[j] = buf_load_b128<POL>(rows[j >> 1], at_rows, 8 * (j & 1) * row_bytes);
+                    else pre[j] = buf_load_b128<POL>(rows[j >> 2], at_rows, 4 * (j & 3) * row_bytes);
                 }
             }
             if constexpr (Q8) {
@@ -550,6 +550,9 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             const uint32_t v_row = 4 * grp + (n16 >> 2);
             const uint32_t v_at = v_row * 256 + ((((n16 >> 1) & 1) ^ v_row) << 4) + (n16 & 1) * 8;
             const uint32_t srow = wave * (64 / kLanes) + ln / kLanes, spos = (ln % kLanes) * kPer;
+            // Two workgroups share a CU: the one between its barriers goes first
+            // (1 to 4%).
+            __builtin_amdgcn_s_setprio(1);
             // ---- S^T partial ----
             // The keys of the first 16 positions, then each block's products with
             // the same block of the other 16 requested behind them: no wait on
@@ -675,6 +678,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             lds_barrier();
 
             // ---- O^T += V^T P^T ----
+            __builtin_amdgcn_s_setprio(0);
             {
                 float al[NT];
                 bool same = true;
@@ -981,21 +985,18 @@ MlaLayout mla_layout(uint32_t n_heads, uint32_t rank, int num_cu) {
     return w;
 }
 
-template <bool Q8>
-void launch_split(const MlaArgs& a, const MlaPlan& p, int mode, hipStream_t s) {
+template <bool Q8, int MODE, int POL>
+void launch_mode(const MlaArgs& a, const MlaPlan& p, hipStream_t s) {
     // Every block and rotary column there is: no test of either in the loops.
     const bool full = a.geom.rank == kKvMaxRank && a.geom.width == kKvMaxRank + kKvMaxRope;
-    const dim3 grid(p.groups);
-    if (mode == kOne) {
-        if (full) mla_split_kernel<Q8, kOne, true><<<grid, kMlaThreads, 0, s>>>(a, p);
-        else mla_split_kernel<Q8, kOne, false><<<grid, kMlaThreads, 0, s>>>(a, p);
-    } else if (mode == kPacked) {
-        if (full) mla_split_kernel<Q8, kPacked, true><<<grid, kMlaThreads, 0, s>>>(a, p);
-        else mla_split_kernel<Q8, kPacked, false><<<grid, kMlaThreads, 0, s>>>(a, p);
-    } else {
-        if (full) mla_split_kernel<Q8, kTwo, true><<<grid, kMlaThreads, 0, s>>>(a, p);
-        else mla_split_kernel<Q8, kTwo, false><<<grid, kMlaThreads, 0, s>>>(a, p);
-    }
+    if (full) mla_split_kernel<Q8, MODE, true, POL><<<p.groups, kMlaThreads, 0, s>>>(a, p);
+    else mla_split_kernel<Q8, MODE, false, POL><<<p.groups, kMlaThreads, 0, s>>>(a, p);
+}
+template <bool Q8, int POL>
+void launch_split(const MlaArgs& a, const MlaPlan& p, int mode, hipStream_t s) {
+    if (mode == kOne) launch_mode<Q8, kOne, POL>(a, p, s);
+    else if (mode == kPacked) launch_mode<Q8, kPacked, POL>(a, p, s);
+    else launch_mode<Q8, kTwo, POL>(a, p, s);
 }
 
 }  // namespace
@@ -1023,8 +1024,14 @@ hipError_t launch_mla(const MlaArgs& a, hipStream_t s) {
     p.vec_q = aligned(a.q, a.q_token_stride, a.q_head_stride) &&
               (a.geom.width == a.geom.rank || aligned(a.q_pe, a.q_pe_token_stride, a.q_pe_head_stride));
     p.vec_out = aligned(a.out, a.out_token_stride, a.out_head_stride);
-    if (a.geom.q8) launch_split<true>(a, p, w.mode, s);
-    else launch_split<false>(a, p, w.mode, s);
+    // Rows that several tokens read (more tokens than tables: a prompt's chunk)
+    // stay in the caches, f16 rows read once pass them by: 256 tokens at 4096
+    // positions 171 us against 193, one token at 131072 positions 56 against
+    // 53 and 64 tokens at 4096 positions 81 against 71. Q8_0 rows stay either
+    // way: 241 against 247, 54.5 against 55.7 and 79.3 against 79.5.
+    if (a.geom.q8) launch_split<true, kCacheNormal>(a, p, w.mode, s);
+    else if (a.n_tokens > a.n_tables) launch_split<false, kCacheNormal>(a, p, w.mode, s);
+    else launch_split<false, kCacheStream>(a, p, w.mode, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     mla_join_kernel<<<2 * a.num_cu, kJoinThreads, 0, s>>>(a, p);
