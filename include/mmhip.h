@@ -329,11 +329,12 @@ int mmhip_qmm_dev_noalloc(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat,
  * All of them are asynchronous on mmhip_stream(ctx), allocate nothing and
  * can be captured into a HIP graph. Where a workspace is needed the caller
  * gives it, for as long as the work may run: two calls (or two graphs) that
- * can run at the same time need one each. Arguments are checked before the
- * context is. What only the device can see (slots, page numbers, lengths,
- * positions, tokens) is bounds-checked there and never read or written out
- * of bounds; where it is wrong, the next mmhip_synchronize returns
- * MMHIP_ERR_INVALID and says what was met, once (the last, of several).
+ * can run at the same time need one each. A call takes fewer than 2^24 rows
+ * or tokens. Arguments are checked before the context is. What only the
+ * device can see (slots, page numbers, lengths, positions, tokens) is
+ * bounds-checked there and never read or written out of bounds; where it is
+ * wrong, the next mmhip_synchronize returns MMHIP_ERR_INVALID and says what
+ * was met, once (the last, of several).
  * ====================================================================== */
 
 /* Root-mean-square norm of n_rows rows of cols values, with a residual added

@@ -29,8 +29,9 @@ struct mmhip_rope {
 
 namespace {
 
-// A grid's x dimension, one workgroup per row or token.
-constexpr uint64_t kMostRows = 0x7FFFFFFFull;
+// One workgroup of at most 256 threads per row or token, and fewer than 2^32
+// threads in a launch.
+constexpr uint64_t kMostRows = 0xFFFFFF;
 
 int refuse(int code, const char* what, const char* why) {
     set_error(code, std::string(what) + ": " + why);
@@ -166,7 +167,7 @@ int mmhip_rms_norm_dev(mmhip_ctx* ctx, void* y, uint32_t y_type, uint64_t y_stri
             return refuse(MMHIP_ERR_UNSUPPORTED, what, "y_type must be F32, F16 or Q8_0");
         if (cols == 0 || cols > 0x7FFFFFFFu) return invalid(what, "cols outside [1, 2^31)");
         if (!(eps >= 0.0f)) return invalid(what, "eps must be at least 0");
-        if (n_rows > kMostRows) return invalid(what, "more than 2^31 - 1 rows");
+        if (n_rows > kMostRows) return invalid(what, "2^24 rows or more");
         if (n_rows == 0) return ctx ? MMHIP_OK : invalid(what, "null context");
         if (!y || !x || !weight) return invalid(what, "null pointer");
         if (x_stride < cols || (residual && residual_stride < cols) || (sum && sum_stride < cols) ||
@@ -254,7 +255,7 @@ int mmhip_rope_dev(mmhip_ctx* ctx, const mmhip_rope* rope, float* y, uint64_t y_
         if (!rope) return invalid(what, "null rope");
         if (head_dim < rope->params.dims || first > head_dim - rope->params.dims)
             return invalid(what, "the rotated dims leave the head");
-        if (n_tokens > kMostRows) return invalid(what, "more than 2^31 - 1 tokens");
+        if (n_tokens > kMostRows) return invalid(what, "2^24 tokens or more");
         if (n_tokens == 0 || n_heads == 0) return ctx ? MMHIP_OK : invalid(what, "null context");
         if (!y || !x || !positions) return invalid(what, "null pointer");
         if (n_heads > 1 && (x_head_stride < head_dim || y_head_stride < head_dim))
@@ -299,7 +300,7 @@ int mmhip_kv_store_dev(mmhip_ctx* ctx, const mmhip_kv_cache* cache, const float*
         if (int rc = check_cache(what, cache)) return rc;
         if (rope && rope->params.dims != cache->rope_dims) return invalid(what, "the rope's dims differ from rope_dims");
         if (norm_weight && !(eps >= 0.0f)) return invalid(what, "eps must be at least 0");
-        if (n_tokens > kMostRows) return invalid(what, "more than 2^31 - 1 tokens");
+        if (n_tokens > kMostRows) return invalid(what, "2^24 tokens or more");
         if (n_tokens == 0) return ctx ? MMHIP_OK : invalid(what, "null context");
         if (!kv || !slots || (rope && !positions)) return invalid(what, "null pointer");
         if (n_tokens > 1 && kv_stride < cache->rank + cache->rope_dims) return invalid(what, "kv_stride is below a row");
@@ -338,7 +339,7 @@ int mmhip_mla_attention_dev(mmhip_ctx* ctx, const mmhip_mla_attention* args) {
         if (int rc = check_cache(what, &p.cache)) return rc;
         if (!std::isfinite(p.scale)) return invalid(what, "scale must be finite");
         if (p.n_heads == 0) return invalid(what, "n_heads must be above 0");
-        if ((uint64_t)p.n_tokens * p.n_heads > kMostRows) return invalid(what, "more than 2^31 - 1 tokens times heads");
+        if ((uint64_t)p.n_tokens * p.n_heads > 0x7FFFFFFF) return invalid(what, "more than 2^31 - 1 tokens times heads");
         if (p.n_tables == 0 || p.table_pages == 0 || p.table_stride < p.table_pages)
             return invalid(what, "tables need rows, pages and a stride of at least table_pages");
         if (((uint64_t)p.table_pages * p.cache.page_tokens) > 0xFFFFFFFFull)
@@ -403,7 +404,7 @@ int mmhip_logprobs_dev(mmhip_ctx* ctx, const float* logits, uint64_t stride, uin
         if (vocab == 0 || vocab >= 0x80000000ull) return invalid(what, "vocab outside [1, 2^31)");
         if (top > MMHIP_LOGPROBS_MAX_TOP || top > vocab) return invalid(what, "top is above 32 or above vocab");
         if (n_given >= 0x80000000ull) return invalid(what, "2^31 given tokens or more");
-        if (n_rows > kMostRows) return invalid(what, "more than 2^31 - 1 rows");
+        if (n_rows > kMostRows) return invalid(what, "2^24 rows or more");
         if (n_rows == 0) return ctx ? MMHIP_OK : invalid(what, "null context");
         if (!logits || (n_given && (!tokens || !token_logprobs)) || (top && !top_ids)) return invalid(what, "null pointer");
         if (n_rows > 1 && stride < vocab) return invalid(what, "the stride is below vocab");
