@@ -393,7 +393,7 @@ void mmhip_rope_destroy(mmhip_ctx* ctx, mmhip_rope* rope);
 int mmhip_rope_frequencies(const mmhip_rope_params* params, double* out, double* magnitude);
 /* x [n_tokens][n_heads][head_dim] -> y, dims [first, first + rope.dims) of
  * every head turned by its token's position and the others copied. Strides in
- * floats (head strides at least head_dim). y_dev may be x_dev with the same
+ * floats (head strides at least head_dim); fewer than 2^24 heads. y_dev may be x_dev with the same
  * strides (the other dims are then left alone); otherwise the two must not
  * overlap. */
 int mmhip_rope_dev(mmhip_ctx* ctx, const mmhip_rope* rope, float* y_dev, uint64_t y_token_stride,

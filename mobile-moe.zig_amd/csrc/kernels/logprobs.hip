@@ -1,8 +1,8 @@
 // Log probabilities of the next token over the vocabulary (computeLogits'
 // output, inference.zig:1013-1033) on gfx950: per row the log probabilities of
 // given tokens, the entropy and the `top` largest logits, in one pass over the
-// row. With m the row's maximum, s = sum exp(x - m) and t = sum exp(x - m) (x - m),
-// a token's log probability is (x - m) - ln s and the entropy ln s - t / s.
+// row. With m the row's maximum, s = sum exp(x - m) and t = sum exp(x - m) (x - m), a token's
+// log probability is (x - m) - ln s and the entropy ln s - t / s.
 //
 // Bound: HBM, 4 bytes per logit; for few rows the latency of two launches. A
 // row is cut into pieces, so that few rows reach the whole chip: the first
@@ -20,6 +20,7 @@
 
 #include "device_common.hpp"
 #include "kernels.hpp"
+#include "lanes.hpp"
 
 namespace mmhip {
 
@@ -55,34 +56,40 @@ __device__ __forceinline__ float key_logit(uint64_t k) {
     return b == 0 ? __builtin_nanf("") : __uint_as_float(b & 0x80000000u ? b & 0x7FFFFFFFu : ~b);
 }
 
-// Adds a part (m, s, t) to another. A part without weight at the new maximum
-// adds nothing to t, but a NaN in its sum stays one.
-__device__ __forceinline__ void join(LpSum& a, const LpSum& b) {
-    const float m = fmaxf(a.m, b.m), da = a.m - m, db = b.m - m;
-    const float fa = a.m == m ? 1.0f : expf(da), fb = b.m == m ? 1.0f : expf(db);
-    const float ta = fa == 0.0f ? 0.0f : (a.m == m ? a.t : fa * (a.t + a.s * da));
-    const float tb = fb == 0.0f ? 0.0f : (b.m == m ? b.t : fb * (b.t + b.s * db));
+// The number right above a key's logit (NaN above +infinity).
+__device__ __forceinline__ float above_of(uint64_t k) { return key_logit(k + (1ull << 32)); }
+
+// Sums are taken in base 2: s = sum 2^y and t = sum 2^y y, y = (x - m) log2 e.
+// The product's rounding moves a term by |y| 2^-24 ln 2 of its size at most:
+// a part in 10^6 where y = -24, and what lies further down weighs nothing.
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
+// What a part's weight 2^y, y = (m - M) log2 e, makes of its sums at the larger
+// maximum M. Without weight it adds nothing to t, but a NaN in s stays one.
+__device__ __forceinline__ void rebase(LpSum& a, float m) {
+    if (a.m == m) return;
+    const float y = (a.m - m) * kLog2e, f = __builtin_amdgcn_exp2f(y);
+    a.t = f == 0.0f ? 0.0f : f * (a.t + a.s * y);
+    a.s *= f;
     a.m = m;
-    a.s = a.s * fa + b.s * fb;
-    a.t = ta + tb;
 }
-// Over the workgroup: a wave's lanes, then the waves, in a fixed order (lane
-// 0's). For every thread.
+// Over the workgroup, in a fixed order. For every thread.
 __device__ __forceinline__ LpSum join_all(LpSum v, LpSum* red) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        LpSum o;
-        o.m = __shfl_xor(v.m, off, 64);
-        o.s = __shfl_xor(v.s, off, 64);
-        o.t = __shfl_xor(v.t, off, 64);
-        join(v, o);
-    }
+    rebase(v, group_max<64>(v.m));
+    v.s = group_sum<64>(v.s);
+    v.t = group_sum<64>(v.t);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = red[0];
+    LpSum all{-INFINITY, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 1; w < kLpWaves; ++w) join(v, red[w]);
-    return v;
+    for (int w = 0; w < kLpWaves; ++w) all.m = fmaxf(all.m, red[w].m);
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w) {
+        LpSum o = red[w];
+        rebase(o, all.m);
+        all.s += o.s;
+        all.t += o.t;
+    }
+    return all;
 }
 
 // The `top`-th largest of the lanes' keys (0: none); at least `top` of them
@@ -99,9 +106,24 @@ __device__ __forceinline__ uint64_t wave_kth(uint64_t key, uint32_t top) {
            (uint32_t)__builtin_amdgcn_readlane((uint32_t)key, at);
 }
 
+// Of the lanes' numbers, the `top`-th largest: false where equal ones, NaN or
+// infinite ones leave it undecided which `top` lanes reach it.
+__device__ __forceinline__ bool wave_kth(float m, uint32_t top, float& kth) {
+    uint32_t above = 0;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) above += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), i)) > m;
+    const uint64_t at = __ballot(above == top - 1 && m > -INFINITY);
+    if (__popcll(at) != 1) return false;
+    kth = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), __ffsll((unsigned long long)at) - 1));
+    return true;
+}
+
 // The `top` largest of list[0, n), largest first, into out, 0 behind the last.
-// Between two barriers of the caller's.
-__device__ __forceinline__ void rank_list(const uint64_t* list, uint32_t n, uint64_t* out, uint32_t top) {
+// list has room for kRankStep - 1 keys more. Begins with a barrier.
+constexpr uint32_t kRankStep = 16;
+__device__ __forceinline__ void rank_list(uint64_t* list, uint32_t n, uint64_t* out, uint32_t top) {
+    if (threadIdx.x < kRankStep - 1) list[n + threadIdx.x] = 0;
+    __syncthreads();
     for (uint32_t i = threadIdx.x; i < max(n, top); i += kLpThreads) {
         if (i >= n) {
             out[i] = 0;
@@ -109,15 +131,36 @@ __device__ __forceinline__ void rank_list(const uint64_t* list, uint32_t n, uint
         }
         const uint64_t mine = list[i];
         uint32_t above = 0;
-        for (uint32_t j = 0; j < n; ++j) above += list[j] > mine;
+        for (uint32_t j = 0; j < n; j += kRankStep)
+#pragma unroll
+            for (uint32_t e = 0; e < kRankStep; ++e) above += list[j + e] > mine;
         if (above < top) out[above] = mine;
+    }
+}
+
+// Appends the lanes' keys key(i), i < N, of which want(i) holds to the list.
+template <int N, class Want, class Key>
+__device__ __forceinline__ void keep(Want want, Key key, uint64_t* list, uint32_t* kept) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += (uint32_t)__popcll(__ballot(want(i)));
+    if (n == 0) return;
+    uint32_t at = 0;
+    if ((threadIdx.x & 63) == 0) at = atomicAdd(kept, n);
+    at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint64_t mask = __ballot(want(i));
+        if (mask == 0) continue;
+        if (want(i)) list[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key(i);
+        at += (uint32_t)__popcll(mask);
     }
 }
 
 // The most a chunk keeps: of each wave fewer than `top` lanes that pass the
 // piece's `top`-th, or exactly `top` lanes that reach the wave's; and the
 // piece's own `top`.
-constexpr uint32_t kLpMostKept = kLpWaves * kLpMostTop * kLpPerThread + kLpMostTop;
+constexpr uint32_t kLpMostKept = kLpWaves * kLpMostTop * kLpPerThread + kLpMostTop + kRankStep;
 
 // One workgroup per piece.
 __global__ __launch_bounds__(kLpThreads) void logprobs_split_kernel(LogprobsArgs a, LpPlan p) {
@@ -136,63 +179,65 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_split_kernel(LogprobsArgs
     LpSum sum{-INFINITY, 0.0f, 0.0f, 0.0f};
     uint64_t floor_key = 0;  // the piece's `top`-th so far
     __syncthreads();
+    // Thread t has logits t + 256 i of a chunk, the next one's on their way
+    // while it works on one (nothing is read where there is none).
+    uint32_t pre[kLpPerThread];
+    const auto read = [&](uint32_t c) {
+        const uint32_t first = c * kLpChunk;
+        const BufRsrc r = make_rsrc(x + first, c < c1 ? min(a.vocab - first, kLpChunk) * 4 : 0);
+#pragma unroll
+        for (uint32_t i = 0; i < kLpPerThread; ++i) pre[i] = buf_load_b32<kCacheStream>(r, tid * 4, i * (kLpThreads * 4));
+    };
+    read(c0);
     for (uint32_t c = c0; c < c1; ++c) {
-        // Thread t has logits 4 t .. 4 t + 3 of each quarter of the chunk.
         const uint32_t first = c * kLpChunk, n = min(a.vocab - first, kLpChunk);
-        const BufRsrc r = make_rsrc(x + first, n * 4);
         float v[kLpPerThread];
-        if (n == kLpChunk) {
 #pragma unroll
-            for (uint32_t j = 0; j < kLpPerThread / 4; ++j) {
-                const uint4 q = buf_load_b128<kCacheStream>(r, tid * 16, j * kLpThreads * 16);
-                v[4 * j] = __uint_as_float(q.x);
-                v[4 * j + 1] = __uint_as_float(q.y);
-                v[4 * j + 2] = __uint_as_float(q.z);
-                v[4 * j + 3] = __uint_as_float(q.w);
-            }
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < kLpPerThread; ++i) {
-                const uint32_t at = tid * 4 + (i >> 2) * (kLpThreads * 4) + (i & 3);
-                const uint32_t q = buf_load_b32<kCacheStream>(r, at * 4, 0);
-                v[i] = at < n ? __uint_as_float(q) : -INFINITY;
-            }
-        }
+        for (uint32_t i = 0; i < kLpPerThread; ++i) v[i] = tid + i * kLpThreads < n ? __uint_as_float(pre[i]) : -INFINITY;
+        read(c + 1);
         float m = v[0];
 #pragma unroll
         for (uint32_t i = 1; i < kLpPerThread; ++i) m = fmaxf(m, v[i]);  // leaves NaN out
         {
-            LpSum here{m, 0.0f, 0.0f, 0.0f};
-            const float base = m == -INFINITY || m != m ? 0.0f : m;
+            const float old = sum.m;
+            LpSum here{fmaxf(old, m), 0.0f, 0.0f, 0.0f};
+            const float base = here.m == -INFINITY ? 0.0f : here.m;
 #pragma unroll
             for (uint32_t i = 0; i < kLpPerThread; ++i) {
-                const float d = v[i] - base, e = expf(d);
+                const float y = (v[i] - base) * kLog2e, e = __builtin_amdgcn_exp2f(y);
                 here.s += e;
-                here.t += e == 0.0f ? 0.0f : e * d;
+                here.t += e == 0.0f ? 0.0f : e * y;
             }
-            join(sum, here);
+            rebase(sum, here.m);
+            sum.s += here.s;
+            sum.t += here.t;
         }
         if (top == 0) continue;
-        // Nothing to do where every lane's largest number is below the floor's
-        // (no number: a NaN's, or no floor yet), NaN being below every number.
-        if (__any(!(m < key_logit(floor_key)))) {
-            uint64_t key = 0;
+        // Lanes with a number above the floor's (which may be a NaN's, or none
+        // yet: NaN, which bars nothing). An equal one comes later in the order.
+        const float floor_x = key_logit(floor_key);
+        const uint32_t pass = (uint32_t)__popcll(__ballot(m == m && !(m <= floor_x)));
+        float least_x = above_of(floor_key);
+        bool plain = floor_x == floor_x;
+        if (pass >= top) plain = wave_kth(m, top, least_x);
+        if (plain) {
+            // Compared as numbers. None of the absent: least_x is above -infinity.
+            if (pass)
+                keep<kLpPerThread>([&](int i) { return v[i] >= least_x; },
+                                   [&](int i) { return rank_key(v[i], first + tid + i * kLpThreads); }, list, &kept[c & 1]);
+        } else {
+            // Equal maxima, or NaN among the largest: as keys.
+            uint64_t k[kLpPerThread], key = 0;
 #pragma unroll
             for (uint32_t i = 0; i < kLpPerThread; ++i) {
-                const uint32_t at = tid * 4 + (i >> 2) * (kLpThreads * 4) + (i & 3);
-                if (at < n) key = max(key, rank_key(v[i], first + at));
+                const uint32_t at = tid + i * kLpThreads;
+                k[i] = at < n ? rank_key(v[i], first + at) : 0;
+                key = max(key, k[i]);
             }
             if (key <= floor_key) key = 0;
             uint64_t least = floor_key + 1;
             if ((uint32_t)__popcll(__ballot(key != 0)) >= top) least = wave_kth(key, top);
-            if (key >= least) {
-#pragma unroll
-                for (uint32_t i = 0; i < kLpPerThread; ++i) {
-                    const uint32_t at = tid * 4 + (i >> 2) * (kLpThreads * 4) + (i & 3);
-                    const uint64_t k = rank_key(v[i], first + at);
-                    if (at < n && k >= least) list[atomicAdd(&kept[c & 1], 1u)] = k;
-                }
-            }
+            keep<kLpPerThread>([&](int i) { return k[i] >= least; }, [&](int i) { return k[i]; }, list, &kept[c & 1]);
         }
         __syncthreads();
         uint32_t found = kept[c & 1];
@@ -201,7 +246,6 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_split_kernel(LogprobsArgs
             // The piece's own behind them.
             if (tid < top && best[tid]) list[found + tid] = best[tid];
             found += (uint32_t)__popcll(__ballot((tid & 63) < top && best[tid & 63]));
-            __syncthreads();
             rank_list(list, found, best, top);
         }
         __syncthreads();
@@ -215,7 +259,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_split_kernel(LogprobsArgs
 // One workgroup per row.
 __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobsArgs a, LpPlan p) {
     __shared__ LpSum red[kLpWaves];
-    __shared__ uint64_t list[kLpMostPieces / 64 * kLpMostTop * kLpMostTop];
+    __shared__ uint64_t list[kLpMostPieces / 64 * kLpMostTop * kLpMostTop + kRankStep];
     __shared__ uint64_t best[kLpMostTop];
     __shared__ uint32_t kept;
     const uint64_t row = blockIdx.x;
@@ -226,24 +270,28 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobsArgs 
     if (tid < p.pieces) sum = p.sums[row * p.pieces + tid];
     sum = join_all(sum, red);
     const float log_s = logf(sum.s);
-    if (a.entropy && tid == 0) a.entropy[row] = log_s - sum.t / sum.s;
+    if (a.entropy && tid == 0) a.entropy[row] = log_s - kLn2 * (sum.t / sum.s);
     for (uint64_t i = tid; i < a.n_given; i += kLpThreads) {
         const uint32_t id = a.tokens[row * a.n_given + i];
         if (id >= a.vocab) report(a.status, kBadToken);
         a.token_logprobs[row * a.n_given + i] = id < a.vocab ? (x[id] - sum.m) - log_s : __builtin_nanf("");
     }
     if (top == 0) return;
-    // A lane stands for the pieces lane + 64 i: the `top`-th largest of the
-    // lanes' largest is a floor, where there are as many lanes. Every wave
-    // finds it for itself.
+    // 64 keys, the largest of each piece (of every 64th piece) and where there
+    // are fewer pieces their next ones: the `top`-th largest of these is a
+    // floor. Every wave finds it for itself.
     const uint64_t* keys = p.keys + row * p.pieces * top;
     uint64_t largest = 0;
-    for (uint32_t i = lane; i < p.pieces; i += 64) largest = max(largest, keys[(uint64_t)i * top]);
+    if (p.pieces >= 64) {
+        for (uint32_t i = lane; i < p.pieces; i += 64) largest = max(largest, keys[(uint64_t)i * top]);
+    } else if (lane / p.pieces < top) {
+        largest = keys[lane % p.pieces * top + lane / p.pieces];
+    }
     uint64_t least = 1;
     if ((uint32_t)__popcll(__ballot(largest != 0)) >= top) least = wave_kth(largest, top);
-    for (uint32_t i = tid; i < p.pieces * top; i += kLpThreads) {
-        const uint64_t k = keys[i];
-        if (k >= least) list[atomicAdd(&kept, 1u)] = k;
+    for (uint32_t i = tid; i < (p.pieces * top + 63) / 64 * 64; i += kLpThreads) {
+        const uint64_t k = i < p.pieces * top ? keys[i] : 0;
+        keep<1>([&](int) { return k >= least; }, [&](int) { return k; }, list, &kept);
     }
     __syncthreads();
     rank_list(list, kept, best, top);

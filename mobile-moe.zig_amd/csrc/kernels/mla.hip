@@ -40,6 +40,7 @@
 // sums in the workspace and mla_join_kernel adds them in the list's order.
 #include "device_common.hpp"
 #include "kernels.hpp"
+#include "lanes.hpp"
 
 namespace mmhip {
 
@@ -128,31 +129,6 @@ __device__ __forceinline__ uint64_t uniform(uint64_t v) {
 // wait for every row load in flight).
 __device__ __forceinline__ uint32_t afresh(uint32_t v) {
     asm volatile("" : "+v"(v));
-    return v;
-}
-
-// Sums and maxima over groups of 8 or 16 lanes by lane permutes of the vector
-// unit (a shuffle through LDS takes about 0.05 us each). Every lane gets the
-// result; NaN does not enter a maximum.
-template <int CTRL>
-__device__ __forceinline__ float permuted(float v) {
-    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xF, 0xF, true));
-}
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140, kRotate8 = 0x128;
-template <int LANES>
-__device__ __forceinline__ float group_max(float v) {
-    v = fmaxf(v, permuted<kXor1>(v));
-    v = fmaxf(v, permuted<kXor2>(v));
-    v = fmaxf(v, permuted<kHalfMirror>(v));
-    if constexpr (LANES == 16) v = fmaxf(v, permuted<kMirror>(v));
-    return v;
-}
-template <int LANES>
-__device__ __forceinline__ float group_sum(float v) {
-    v += permuted<kXor1>(v);
-    v += permuted<kXor2>(v);
-    v += permuted<kHalfMirror>(v);
-    if constexpr (LANES == 16) v += permuted<kMirror>(v);
     return v;
 }
 

@@ -11,6 +11,7 @@
 // per value, hidden behind the row's loads.
 #include "device_common.hpp"
 #include "kernels.hpp"
+#include "lanes.hpp"
 #include "q8_ops.hpp"
 
 namespace mmhip {
@@ -45,20 +46,103 @@ __device__ __forceinline__ void store4(float* p, const float (&v)[4], uint32_t c
 
 __device__ __forceinline__ uint32_t half_bits(float v) { return __half_as_ushort(__float2half_rn(v)); }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
-}
-
 // 1 / sqrt(mean + eps), rounded to f32.
 __device__ __forceinline__ float inverse_root(double sum, uint32_t cols, float eps) {
     return (float)(1.0 / sqrt(sum / (double)cols + (double)eps));
 }
 
-// One workgroup per row; thread t has columns 4 (t + 256 i).. of it.
+// Values c .. c + 3 of a row's output.
 template <uint32_t OUT>
+__device__ __forceinline__ void store_normed(const NormArgs& a, uint64_t row, uint32_t c, const float (&v)[4]) {
+    if constexpr (OUT == kOutF32) {
+        store4(static_cast<float*>(a.y) + row * a.y_stride, v, c, a.cols, a.vec);
+    } else if constexpr (OUT == kOutF16) {
+        uint16_t* y = static_cast<uint16_t*>(a.y) + row * a.y_stride + c;
+        if (c + 4 <= a.cols) {
+            const uint2 q = make_uint2(half_bits(v[0]) | half_bits(v[1]) << 16, half_bits(v[2]) | half_bits(v[3]) << 16);
+            __builtin_memcpy(y, &q, 8);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < a.cols) y[e] = (uint16_t)half_bits(v[e]);
+        }
+    } else {
+        // A block's 8 lanes are together.
+        float d;
+        const uint32_t q4 = q8_quad(v, c < a.cols ? min(a.cols - c, 4u) : 0u, d);
+        const uint32_t blocks = (a.cols + 31) / 32, j = (c / 4) & 7;
+        if (c / 32 < blocks) {
+            uint16_t* y = static_cast<uint16_t*>(a.y) + (row * blocks + c / 32) * 17;
+            __builtin_memcpy(y + 1 + 2 * j, &q4, 4);  // 2-byte aligned
+            if (j == 0) y[0] = (uint16_t)f32_to_f16_scale(d);
+        }
+    }
+}
+
+// The workgroup's sum.
+__device__ __forceinline__ double block_sum(double acc, double* part) {
+    acc = group_sum<64>(acc);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    acc = 0.0;
+#pragma unroll
+    for (int i = 0; i < kNormThreads / 64; ++i) acc += part[i];
+    return acc;
+}
+
+// One workgroup per row, which stays in registers: thread t has columns
+// 4 (t + 256 i) .. + 3, i < NV, and reads all of them, the residual and the
+// weight before it uses any.
+template <uint32_t OUT, int NV>
 __global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(NormArgs a) {
+    __shared__ double part[kNormThreads / 64];
+    const uint64_t row = blockIdx.x;
+    // Columns past the row's end, and a residual that is not there, read 0.
+    const BufRsrc x = make_rsrc(a.x + row * a.x_stride, a.cols * 4);
+    const BufRsrc res = make_rsrc(a.residual + row * a.residual_stride, a.residual ? a.cols * 4 : 0);
+    const BufRsrc weight = make_rsrc(a.weight, a.cols * 4);
+    float v[NV][4], r[NV][4], w[NV][4];
+    const auto read = [&](float (&to)[NV][4], BufRsrc from) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (a.vec) {
+                const uint4 q = buf_load_b128(from, threadIdx.x * 16, i * (kNormThreads * 16));
+                to[i][0] = __uint_as_float(q.x);
+                to[i][1] = __uint_as_float(q.y);
+                to[i][2] = __uint_as_float(q.z);
+                to[i][3] = __uint_as_float(q.w);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    to[i][e] = __uint_as_float(buf_load_b32(from, threadIdx.x * 16 + 4 * e + i * (kNormThreads * 16), 0));
+            }
+        }
+    };
+    read(v, x);
+    read(r, res);
+    read(w, weight);
+    double acc = 0.0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (a.residual) v[i][e] = __fadd_rn(v[i][e], r[i][e]);
+            acc = fma((double)v[i][e], (double)v[i][e], acc);
+        }
+        if (a.sum) store4(a.sum + row * a.sum_stride, v[i], (threadIdx.x + i * kNormThreads) * 4, a.cols, a.vec);
+    }
+    const float root = inverse_root(block_sum(acc, part), a.cols, a.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], root), w[i][e]);
+        store_normed<OUT>(a, row, (threadIdx.x + i * kNormThreads) * 4, v[i]);
+    }
+}
+
+// Longer rows are read twice.
+template <uint32_t OUT>
+__global__ __launch_bounds__(kNormThreads) void rms_norm_long_kernel(NormArgs a) {
     __shared__ double part[kNormThreads / 64];
     const uint64_t row = blockIdx.x;
     const float* x = a.x + row * a.x_stride;
@@ -77,13 +161,7 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc = fma((double)v[e], (double)v[e], acc);
     }
-    acc = wave_sum(acc);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
-    __syncthreads();
-    acc = 0.0;
-#pragma unroll
-    for (int i = 0; i < kNormThreads / 64; ++i) acc += part[i];
-    const float r = inverse_root(acc, a.cols, a.eps);
+    const float root = inverse_root(block_sum(acc, part), a.cols, a.eps);
     // Every thread takes every step, so that a Q8_0 block's 8 lanes are together.
     const uint32_t steps = (a.cols + kNormThreads * 4 - 1) / (kNormThreads * 4);
     for (uint32_t i = 0; i < steps; ++i) {
@@ -98,27 +176,17 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(NormArgs a) {
         }
         load4(w, a.weight, c, a.cols, a.vec);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], r), w[e]);
-        if constexpr (OUT == kOutF32) {
-            store4(static_cast<float*>(a.y) + row * a.y_stride, v, c, a.cols, a.vec);
-        } else if constexpr (OUT == kOutF16) {
-            uint16_t* y = static_cast<uint16_t*>(a.y) + row * a.y_stride;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (c + e < a.cols) y[c + e] = (uint16_t)half_bits(v[e]);
-        } else {
-            float d;
-            const uint32_t q4 = q8_quad(v, c < a.cols ? min(a.cols - c, 4u) : 0u, d);
-            const uint32_t blocks = (a.cols + 31) / 32;
-            if (c / 32 < blocks) {
-                uint16_t* y = static_cast<uint16_t*>(a.y) + (row * blocks + c / 32) * 17;
-                const uint32_t j = (c / 4) & 7;
-                y[1 + 2 * j] = (uint16_t)(q4 & 0xFFFFu);
-                y[2 + 2 * j] = (uint16_t)(q4 >> 16);
-                if (j == 0) y[0] = (uint16_t)f32_to_f16_scale(d);
-            }
-        }
+        for (int e = 0; e < 4; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], root), w[e]);
+        store_normed<OUT>(a, row, c, v);
     }
+}
+
+template <uint32_t OUT>
+void launch_norm(const NormArgs& a, unsigned grid, hipStream_t s) {
+    if (a.cols <= 1024) rms_norm_kernel<OUT, 1><<<grid, kNormThreads, 0, s>>>(a);
+    else if (a.cols <= 2048) rms_norm_kernel<OUT, 2><<<grid, kNormThreads, 0, s>>>(a);
+    else if (a.cols <= 4096) rms_norm_kernel<OUT, 4><<<grid, kNormThreads, 0, s>>>(a);
+    else rms_norm_long_kernel<OUT><<<grid, kNormThreads, 0, s>>>(a);
 }
 
 // Cosine and sine of position * frequency, times the magnitude, from the
@@ -141,31 +209,98 @@ __device__ __forceinline__ float rotate(float v, float o, float2 cs, bool second
 
 constexpr int kRopeThreads = 256;
 
-// One workgroup per token: its pairs' cosines once, then all heads. A thread
-// handles a pair (both values), or a value of the other dims.
+// A thread's n-th unit of a token's heads x per_head units, 256 apart, by steps
+// without a division.
+struct RopeUnit {
+    uint32_t h, j;
+    uint32_t step_h, step_j, per_head;
+    __device__ RopeUnit(uint32_t first, uint32_t per)
+        : h(first / per), j(first % per), step_h(kRopeThreads / per), step_j(kRopeThreads % per), per_head(per) {}
+    __device__ void next() {
+        h += step_h;
+        j += step_j;
+        if (j >= per_head) {
+            j -= per_head;
+            ++h;
+        }
+    }
+};
+
+// One workgroup per token. A thread's units are W pairs (both values of each),
+// read before the token's cosines are known; the other dims are copied W at a
+// time in the meantime. W = 4: 16-byte accesses.
+template <int W>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
     __shared__ float2 cs[kRopeMaxPairs];
     const uint64_t t = blockIdx.x;
     const uint32_t pairs = a.dims / 2;
-    if (threadIdx.x < pairs) cs[threadIdx.x] = turn(a.turns[threadIdx.x], a.magnitude, a.positions[t]);
-    __syncthreads();
     const float* x = a.x + t * a.x_token_stride;
     float* y = a.y + t * a.y_token_stride;
-    const uint32_t rest = a.copy ? a.head_dim - a.dims : 0, per_head = pairs + rest;
-    const uint64_t n = (uint64_t)a.n_heads * per_head;
-    for (uint64_t i = threadIdx.x; i < n; i += kRopeThreads) {
-        const uint32_t h = (uint32_t)(i / per_head), j = (uint32_t)(i - (uint64_t)h * per_head);
-        const float* xh = x + h * a.x_head_stride;
-        float* yh = y + h * a.y_head_stride;
-        if (j < pairs) {
-            const uint32_t ia = a.first + (a.half ? j : 2 * j), ib = ia + (a.half ? pairs : 1);
-            const float va = xh[ia], vb = xh[ib];
-            yh[ia] = rotate(va, vb, cs[j], false);
-            yh[ib] = rotate(vb, va, cs[j], true);
+    // Where pair j's values are in a head. Of W = 4 pairs: two runs of 4.
+    const auto place = [&](uint32_t j, uint32_t& ia, uint32_t& ib) {
+        ia = a.first + (a.half ? j : 2 * j);
+        ib = a.half ? ia + pairs : ia + W;
+    };
+    const auto read = [&](float (&v)[W], const float* p) {
+        if constexpr (W == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p);
+            v[0] = q.x;
+            v[1] = q.y;
+            v[2] = q.z;
+            v[3] = q.w;
         } else {
-            const uint32_t k = j - pairs, c = k < a.first ? k : k + a.dims;
-            yh[c] = xh[c];
+            v[0] = *p;
         }
+    };
+    const auto write = [&](float* p, const float (&v)[W]) {
+        if constexpr (W == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        else *p = v[0];
+    };
+    RopeUnit u(threadIdx.x, pairs / W);
+    float va[W], vb[W];
+    uint32_t ia, ib;
+    place(u.j * W, ia, ib);
+    if (u.h < a.n_heads) {
+        read(va, x + u.h * a.x_head_stride + ia);
+        read(vb, x + u.h * a.x_head_stride + ib);
+    }
+    if (threadIdx.x < pairs) cs[threadIdx.x] = turn(a.turns[threadIdx.x], a.magnitude, a.positions[t]);
+    const uint32_t rest = a.copy ? (a.head_dim - a.dims) / W : 0;
+    if (rest) {
+        for (RopeUnit c(threadIdx.x, rest); c.h < a.n_heads; c.next()) {
+            const uint32_t k = c.j * W, i = k < a.first ? k : k + a.dims;
+            float v[W];
+            read(v, x + c.h * a.x_head_stride + i);
+            write(y + c.h * a.y_head_stride + i, v);
+        }
+    }
+    __syncthreads();
+    while (u.h < a.n_heads) {
+        const float2* p = cs + u.j * W;
+        float* to = y + u.h * a.y_head_stride;
+        float ra[W], rb[W];
+        if (W == 1 || a.half) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                ra[e] = rotate(va[e], vb[e], p[e], false);
+                rb[e] = rotate(vb[e], va[e], p[e], true);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e + 1 < W; e += 2) {
+                ra[e] = rotate(va[e], va[e + 1], p[e / 2], false);
+                ra[e + 1] = rotate(va[e + 1], va[e], p[e / 2], true);
+                rb[e] = rotate(vb[e], vb[e + 1], p[(W + e) / 2], false);
+                rb[e + 1] = rotate(vb[e + 1], vb[e], p[(W + e) / 2], true);
+            }
+        }
+        write(to + ia, ra);
+        write(to + ib, rb);
+        u.next();
+        if (u.h >= a.n_heads) break;
+        place(u.j * W, ia, ib);
+        read(va, x + u.h * a.x_head_stride + ia);
+        read(vb, x + u.h * a.x_head_stride + ib);
     }
 }
 
@@ -177,24 +312,27 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(StoreArgs a) {
     __shared__ float2 cs[kKvMaxRope / 2];
     const uint64_t t = blockIdx.x;
     const PagedGeom g = a.geom;
+    const float* x = a.kv + t * a.kv_stride;
+    const uint32_t c = threadIdx.x * 4, pe = g.width - g.rank;
+    const bool live = c < g.width, latent = c < g.rank;
+    // The row, its weight, its slot and its position are read at once.
+    float v[4], w[4];
+    load4(v, x, live ? c : 0, live ? g.width : 0, a.vec);
+    if (a.weight) load4(w, a.weight, latent ? c : 0, latent ? g.rank : 0, a.vec);
     const int32_t slot = a.slots[t];
+    const uint32_t position = a.turns ? a.positions[t] : 0;
     uint32_t page, at;
     if (!paged_slot(g, slot, page, at)) {
         if (slot >= 0 && threadIdx.x == 0) report(a.status, kBadSlot);
         return;
     }
-    const float* x = a.kv + t * a.kv_stride;
-    const uint32_t c = threadIdx.x * 4, pe = g.width - g.rank;
-    const bool live = c < g.width, latent = c < g.rank;
-    float v[4];
-    load4(v, x, live ? c : 0, live ? g.width : 0, a.vec);
-    if (a.turns && threadIdx.x < pe / 2) cs[threadIdx.x] = turn(a.turns[threadIdx.x], a.magnitude, a.positions[t]);
+    if (a.turns && threadIdx.x < pe / 2) cs[threadIdx.x] = turn(a.turns[threadIdx.x], a.magnitude, position);
     double acc = 0.0;
     if (latent && a.weight) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc = fma((double)v[e], (double)v[e], acc);
     }
-    acc = wave_sum(acc);
+    acc = group_sum<64>(acc);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
     __syncthreads();
     if (latent && a.weight) {
@@ -202,8 +340,6 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(StoreArgs a) {
 #pragma unroll
         for (int i = 0; i < kStoreThreads / 64; ++i) acc += part[i];
         const float r = inverse_root(acc, g.rank, a.eps);
-        float w[4];
-        load4(w, a.weight, c, g.rank, a.vec);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], r), w[e]);
     } else if (live && !latent && a.turns) {
@@ -216,10 +352,10 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(StoreArgs a) {
             for (int e = 0; e < 4; ++e) v[e] = rotate(v[e], o[e], cs[(second ? k - half : k) + e], second);
         } else {
             const float2 c0 = cs[k / 2], c1 = cs[k / 2 + 1];
-            const float w[4] = {rotate(v[0], v[1], c0, false), rotate(v[1], v[0], c0, true),
+            const float u[4] = {rotate(v[0], v[1], c0, false), rotate(v[1], v[0], c0, true),
                                 rotate(v[2], v[3], c1, false), rotate(v[3], v[2], c1, true)};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = w[e];
+            for (int e = 0; e < 4; ++e) v[e] = u[e];
         }
     }
     if (g.q8) {
@@ -243,20 +379,24 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 hipError_t launch_rms_norm(const NormArgs& in, uint32_t out, uint64_t n_rows, hipStream_t s) {
     if (n_rows == 0) return hipSuccess;
     NormArgs a = in;
-    a.vec = aligned16(a.x) && a.x_stride % 4 == 0 && aligned16(a.weight) &&
+    a.vec = a.cols % 4 == 0 && aligned16(a.x) && a.x_stride % 4 == 0 && aligned16(a.weight) &&
             (!a.residual || (aligned16(a.residual) && a.residual_stride % 4 == 0)) &&
             (!a.sum || (aligned16(a.sum) && a.sum_stride % 4 == 0)) &&
             (out != kOutF32 || (aligned16(a.y) && a.y_stride % 4 == 0));
     const unsigned grid = (unsigned)n_rows;
-    if (out == kOutF32) rms_norm_kernel<kOutF32><<<grid, kNormThreads, 0, s>>>(a);
-    else if (out == kOutF16) rms_norm_kernel<kOutF16><<<grid, kNormThreads, 0, s>>>(a);
-    else rms_norm_kernel<kOutQ8><<<grid, kNormThreads, 0, s>>>(a);
+    if (out == kOutF32) launch_norm<kOutF32>(a, grid, s);
+    else if (out == kOutF16) launch_norm<kOutF16>(a, grid, s);
+    else launch_norm<kOutQ8>(a, grid, s);
     return hipGetLastError();
 }
 
 hipError_t launch_rope(const RopeArgs& a, uint64_t n_tokens, hipStream_t s) {
     if (n_tokens == 0 || a.n_heads == 0) return hipSuccess;
-    rope_kernel<<<(unsigned)n_tokens, kRopeThreads, 0, s>>>(a);
+    const bool vec = a.dims % 8 == 0 && a.first % 4 == 0 && a.head_dim % 4 == 0 && aligned16(a.x) && aligned16(a.y) &&
+                     a.x_token_stride % 4 == 0 && a.x_head_stride % 4 == 0 && a.y_token_stride % 4 == 0 &&
+                     a.y_head_stride % 4 == 0;
+    if (vec) rope_kernel<4><<<(unsigned)n_tokens, kRopeThreads, 0, s>>>(a);
+    else rope_kernel<1><<<(unsigned)n_tokens, kRopeThreads, 0, s>>>(a);
     return hipGetLastError();
 }
 

@@ -256,6 +256,7 @@ int mmhip_rope_dev(mmhip_ctx* ctx, const mmhip_rope* rope, float* y, uint64_t y_
         if (head_dim < rope->params.dims || first > head_dim - rope->params.dims)
             return invalid(what, "the rotated dims leave the head");
         if (n_tokens > kMostRows) return invalid(what, "2^24 tokens or more");
+        if (n_heads > kMostRows) return invalid(what, "2^24 heads or more");
         if (n_tokens == 0 || n_heads == 0) return ctx ? MMHIP_OK : invalid(what, "null context");
         if (!y || !x || !positions) return invalid(what, "null pointer");
         if (n_heads > 1 && (x_head_stride < head_dim || y_head_stride < head_dim))
