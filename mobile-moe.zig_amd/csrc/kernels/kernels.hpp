@@ -363,7 +363,9 @@ struct NormArgs {
     const float* weight;
     uint32_t cols;
     float eps;
-    bool vec;               // set by the launcher: 16-byte accesses fit
+    // Set by the launcher.
+    double inv_cols;
+    bool vec;               // 16-byte accesses fit
 };
 // out: 0 f32, 1 f16, 2 Q8_0.
 hipError_t launch_rms_norm(const NormArgs& a, uint32_t out, uint64_t n_rows, hipStream_t s);
@@ -393,7 +395,9 @@ struct StoreArgs {
     const uint32_t* positions;
     const int32_t* slots;
     uint32_t* status;
-    bool vec;               // set by the launcher
+    // Set by the launcher.
+    double inv_rank;
+    bool vec;               // 16-byte accesses fit
 };
 hipError_t launch_kv_store(const StoreArgs& a, uint64_t n_tokens, hipStream_t s);
 
