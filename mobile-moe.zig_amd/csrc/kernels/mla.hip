@@ -88,6 +88,10 @@ struct MlaLds {
 };
 
 __device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (uint32_t)(((uint64_t)len + kMlaTile - 1) / kMlaTile); }
+// An item's slots of the list that is cut evenly: its tiles, behind slots that
+// stand for its queries' conversion and its result.
+constexpr uint32_t kItemSlots = 3;
+__device__ __forceinline__ uint32_t slots_of(uint32_t len) { return len ? tiles_of(len) + kItemSlots : 0; }
 
 __device__ __forceinline__ uint32_t seen(const MlaArgs& a, uint32_t t, uint32_t& row, uint32_t& bad) {
     row = a.table_of ? a.table_of[t] : t;
@@ -160,7 +164,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         for (uint64_t t = t0; t < t0 + per && t < a.n_tokens; ++t) {
             uint32_t bad;
             last_len = seen(a, (uint32_t)t, last_row, bad);
-            mine += tiles_of(last_len);
+            mine += slots_of(last_len);
         }
         mine *= pl.head_tiles;
         uint64_t incl = mine;
@@ -192,7 +196,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 uint32_t bad;
                 for (;; ++t) {
                     len = seen(a, t, row, bad);
-                    const uint64_t n = (uint64_t)tiles_of(len) * pl.head_tiles;
+                    const uint64_t n = (uint64_t)slots_of(len) * pl.head_tiles;
                     if (f < at + n || t + 1 >= a.n_tokens) break;
                     at += n;
                 }
@@ -226,9 +230,24 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             ++token;
             continue;
         }
-        const uint32_t ht_index = pl.head_tiles == 1 ? 0u : (uint32_t)(off / n_tiles);
-        const uint32_t tile0 = (uint32_t)(off - (uint64_t)ht_index * n_tiles);
-        const uint32_t count = (uint32_t)(end - f < n_tiles - tile0 ? end - f : n_tiles - tile0);
+        const uint32_t n_slots = n_tiles + kItemSlots;
+        const uint32_t ht_index = pl.head_tiles == 1 ? 0u : (uint32_t)(off / n_slots);
+        const uint32_t slot0 = (uint32_t)(off - (uint64_t)ht_index * n_slots);
+        const uint32_t span = (uint32_t)(end - f < n_slots - slot0 ? end - f : n_slots - slot0);
+        const uint32_t tile0 = max(slot0, kItemSlots) - kItemSlots;
+        const uint32_t count = max(slot0 + span, kItemSlots) - kItemSlots - tile0;
+        const auto advance = [&] {
+            f += span;
+            off += span;
+            if (off == (uint64_t)n_slots * pl.head_tiles) {
+                off = 0;
+                ++token;
+            }
+        };
+        if (count == 0) {
+            advance();
+            continue;
+        }
         const uint32_t head0 = ht_index * kHeads;
         const int32_t* table = a.tables + (uint64_t)row * a.table_stride;
 
@@ -771,15 +790,10 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         }
         if (first && !whole) {
             begun.item = token * pl.head_tiles + ht_index;
-            const uint64_t last = f + n_tiles - 1;
+            const uint64_t last = f + (n_slots - slot0) - 1;
             begun.pieces = (last < 0x80000000u ? (uint32_t)last / (uint32_t)chunk : (uint32_t)(last / chunk)) - wg + 1;
         }
-        f += count;
-        off += count;
-        if (off == (uint64_t)n_tiles * pl.head_tiles) {
-            off = 0;
-            ++token;
-        }
+        advance();
         lds_barrier();
     }
     if (tid == 0) splits[wg] = begun;
