@@ -816,28 +816,27 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 }
 
 // Joins the pieces of split items, in order: out = sum_k w_k O_k / sum_k w_k l_k
-// with w_k = 2^(m_k - max m). A team of 32 lanes takes 128 columns of a head
-// (16 bytes per lane); an item of more than 64 pieces goes to teams of 8 lanes
-// and 32 columns, so that it reaches the whole chip. Teams share an item's pieces
-// and add their sums through LDS.
+// with w_k = 2^(m_k - max m). A team of 8 lanes takes 32 columns of a head (16
+// bytes per lane), so that one item reaches the whole chip (teams of 32 lanes:
+// one token at 131072 positions in Q8_0 58 us instead of 56, the others alike).
+// Teams share an item's pieces, up to four each, and add their sums through LDS.
+constexpr uint32_t kTeam = 8, kJoinTeams = kJoinThreads / kTeam;
 struct JoinShape {
-    uint32_t lanes;  // of a team
     uint32_t share;  // teams per head and column part
     __device__ explicit JoinShape(uint32_t pieces) {
-        lanes = pieces > 64 ? 8 : 32;
         share = 1;
-        while (share < kJoinThreads / lanes && share * 4 < pieces) share *= 2;
+        while (share < kJoinTeams && share * 4 < pieces) share *= 2;
     }
-    __device__ uint32_t parts(uint32_t rank) const { return (rank + 4 * lanes - 1) / (4 * lanes); }
-    __device__ uint32_t per_job() const { return kJoinThreads / lanes / share; }  // heads x parts
+    __device__ static uint32_t parts(uint32_t rank) { return rank / (4 * kTeam); }
+    __device__ uint32_t per_job() const { return kJoinTeams / share; }  // heads x parts
 };
 
 // (64 registers, so that two workgroups fit a CU: with 66 the join of 512 pieces
 // took 17 us instead of 13)
 __global__ __launch_bounds__(kJoinThreads, 8) void mla_join_kernel(MlaArgs a, MlaPlan pl) {
     __shared__ __align__(16) float sums[kJoinThreads * 4];
-    // A job's heads times the item's pieces: at most 32 / share heads of 4 share
-    // pieces, or 128 / share of them.
+    // A job's heads times the item's pieces: at most 128 / share heads of 4 share
+    // pieces, or one of kMlaMostGroups.
     __shared__ float weights[kMlaMostGroups];
     __shared__ float2 row_ml[32];
     __shared__ uint32_t scan[kJoinThreads / 64];
@@ -882,14 +881,14 @@ __global__ __launch_bounds__(kJoinThreads, 8) void mla_join_kernel(MlaArgs a, Ml
         const uint32_t token = item / pl.head_tiles, head0 = (item % pl.head_tiles) * pl.rows;
         const uint32_t heads = min(pl.rows, a.n_heads - head0);
         const uint32_t parts = j.parts(rank), units = heads * parts, per_job = j.per_job();
-        const uint32_t team = tid / j.lanes, in_team = tid % j.lanes;
+        const uint32_t team = tid / kTeam, in_team = tid % kTeam;
         const uint32_t unit = job * per_job + team / j.share, mine = team % j.share;
         const bool on = unit < units;
         const uint32_t r0 = job * per_job / parts, r1 = min((job + 1) * per_job - 1, units - 1) / parts;
-        const uint32_t r = on ? unit / parts : r0, c = (on ? unit % parts : 0) * 4 * j.lanes + in_team * 4;
+        const uint32_t r = on ? unit / parts : r0, c = ((on ? unit % parts : 0) * kTeam + in_team) * 4;
         // A thread's first four pieces are read while the weights are found (the
-        // last piece, or columns, again where there are fewer).
-        const float* src = pl.parts + ((uint64_t)g0 * 2 * pl.part_rows + r) * rank + min(c, rank - 4);
+        // last piece again where there are fewer).
+        const float* src = pl.parts + ((uint64_t)g0 * 2 * pl.part_rows + r) * rank + c;
         const uint64_t step = 2ull * pl.part_rows * rank, own = (uint64_t)pl.part_rows * rank;
         v4f early[4];
 #pragma unroll
@@ -924,7 +923,7 @@ __global__ __launch_bounds__(kJoinThreads, 8) void mla_join_kernel(MlaArgs a, Ml
         }
         __syncthreads();
         v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (on && c < rank) {
+        if (on) {
             const float* w = weights + (r - r0) * pieces;
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k)
@@ -934,20 +933,20 @@ __global__ __launch_bounds__(kJoinThreads, 8) void mla_join_kernel(MlaArgs a, Ml
         }
         const float top = row_ml[r - r0].x, l = row_ml[r - r0].y;
         // A unit's teams: those of a wave by shuffles, the waves through LDS.
-        const uint32_t in_wave = min(j.share, 64 / j.lanes);
+        const uint32_t in_wave = min(j.share, 64 / kTeam);
         for (uint32_t n = 1; n < in_wave; n *= 2)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], n * j.lanes, 64);
+            for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], n * kTeam, 64);
         if (j.share > in_wave) {
             const uint32_t waves = j.share / in_wave;
             __syncthreads();
-            if ((tid & 63) < j.lanes) *reinterpret_cast<v4f*>(&sums[(wave * j.lanes + in_team) * 4]) = acc;
+            if ((tid & 63) < kTeam) *reinterpret_cast<v4f*>(&sums[(wave * kTeam + in_team) * 4]) = acc;
             __syncthreads();
             if (mine == 0) {
-                for (uint32_t n = 1; n < waves; ++n) acc += *reinterpret_cast<const v4f*>(&sums[((wave + n) * j.lanes + in_team) * 4]);
+                for (uint32_t n = 1; n < waves; ++n) acc += *reinterpret_cast<const v4f*>(&sums[((wave + n) * kTeam + in_team) * 4]);
             }
         }
-        if (mine == 0 && on && c < rank) {
+        if (mine == 0 && on) {
             const v4f v = l == 0.0f ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc / l;
             float* dst = a.out + (uint64_t)token * a.out_token_stride + (uint64_t)(head0 + r) * a.out_head_stride + c;
             if (pl.vec_out) {
