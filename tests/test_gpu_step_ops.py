@@ -95,6 +95,12 @@ def test_norm(ctx, n, cols, residual):
         assert np.array_equal(q[r].reshape(-1), ctx.quantize_q8_0(y[r])), r
 
 
+@pytest.mark.parametrize("n,cols", [(3, 1024), (2, 1028), (3, 4096), (2, 4095), (2, 4100), (1, 20000)])
+def test_norm_widths(ctx, n, cols):
+    """Either side of the widths at which a row is held differently."""
+    test_norm(ctx, n, cols, True)
+
+
 def test_norm_in_place(ctx):
     """y on x, y on the residual, the sum on x: each gives what separate buffers give."""
     rng = np.random.default_rng(3)
@@ -180,6 +186,39 @@ def test_rope(ctx, layout, kw, tokens, heads, head_dim, first):
             ctx.rope_dev(rope, dx, dx, dp, tokens, heads, head_dim, first)  # in place: the same bits
             ctx.synchronize()
             same_bits(f32(dx, x.size).reshape(x.shape), y.copy())
+        finally:
+            rope.free()
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dims,heads,head_dim,first", [(64, 20, 192, 128), (64, 130, 72, 4), (8, 700, 8, 0), (256, 9, 260, 4),
+                                                       (128, 3, 1024, 512)])
+def test_rope_aligned(ctx, layout, dims, heads, head_dim, first):
+    """Buffers of 16-byte aligned rows and heads, copied and in place, with more pairs than a workgroup has threads: the
+    bits of buffers that are one float off."""
+    rng = np.random.default_rng(heads)
+    tokens = 3
+    x = rng.standard_normal((tokens, heads, head_dim)).astype(np.float32)
+    pos = np.array([0, 77, 131071], np.uint32)
+    rope = mm.Rope(ctx, dims=dims, base=1e5, layout=layout)
+    with Buffers(ctx) as d:
+        try:
+            dp, dx, dy = d.put(pos), d.put(x), d.new(x.size * 4)
+            ctx.rope_dev(rope, dy, dx, dp, tokens, heads, head_dim, first)
+            ctx.synchronize()
+            y = f32(dy, x.size).reshape(x.shape)
+            same_bits(np.delete(y, np.r_[first:first + dims], -1), np.delete(x, np.r_[first:first + dims], -1))
+            part = slice(first, first + dims)
+            want = ref.rope64(x[..., part], pos, layout, ref.frequencies64(dims, 1e5))
+            assert (np.abs(y[..., part] - want) <= (4 * U + 1e-9) * 2 * np.abs(x).max()).all()
+            odd, off = d.put(np.concatenate([np.zeros(1, np.float32), x.ravel()])), d.new(x.size * 4 + 4)
+            ctx.rope_dev(rope, At(off, 4), At(odd, 4), dp, tokens, heads, head_dim, first)
+            ctx.rope_dev(rope, dx, dx, dp, tokens, heads, head_dim, first)
+            ctx.synchronize()
+            same_bits(f32(off, x.size + 1)[1:].reshape(x.shape).copy(), y)
+            same_bits(f32(dx, x.size).reshape(x.shape), y)
+            with pytest.raises(mm.MmhipError, match="heads"):
+                ctx.rope_dev(rope, dy, dx, dp, 1, 1 << 24, head_dim, first)
         finally:
             rope.free()
 
@@ -634,6 +673,53 @@ def test_logprobs_without_probabilities(ctx):
         assert np.isnan(got[0][r]).all() and np.isnan(got[1][r]) and np.isnan(got[3][r]).all(), r
     assert np.array_equal(got[2], ref.top_ids(x, 8))
     check_logprobs(x[5:], tokens[5:], 8, tuple(g[5:] for g in got))
+
+
+@pytest.mark.parametrize("n,v", [(1100, 12300), (300, 20000), (1, (1 << 22) + 5)])
+@pytest.mark.parametrize("top", [1, 32])
+def test_logprobs_long_pieces(ctx, n, v, top):
+    """Rows whose pieces take several steps, the largest found so far going from one to the next: rising, falling and
+    equal logits, the largest in the last step, masks, NaN late in a row."""
+    rng = np.random.default_rng(n + top)
+    x = (rng.standard_normal((n, v)) * 3).astype(np.float32)
+    for r in range(n):
+        kind = r % 11
+        if kind == 1:
+            x[r].sort()
+        elif kind == 2:
+            x[r] = np.sort(x[r])[::-1]
+        elif kind == 3:
+            x[r] = 2.5
+        elif kind == 4:
+            x[r] = np.rint(x[r] / 4)
+        elif kind == 5:
+            x[r, :-20] = -np.inf
+        elif kind == 6:
+            x[r, -7:] = np.nan
+        elif kind == 7:
+            x[r, 40:] = np.finfo(np.float32).min
+        elif kind == 8:
+            x[r, :-3] = np.nan
+        elif kind == 9:
+            x[r, v // 2] = np.inf
+        elif kind == 10:
+            x[r] = np.where(np.arange(v) < v - 33, -np.inf, -0.0)
+    tokens = rng.integers(0, v, (n, 2))
+    check_logprobs(x, tokens, top, run_logprobs(ctx, x, tokens, top))
+
+
+def test_logprobs_refuses_a_small_workspace(ctx):
+    need = ctx.logprobs_workspace(3, 5000, 7)
+    assert need > 0
+    with Buffers(ctx) as d:
+        x, out = d.put(np.zeros((3, 5000), np.float32)), d.new(3 * 7 * 4)
+        work = d.new(need + 16)
+        for w in (At(work, 0, need - 1), At(work, 8, need)):
+            with pytest.raises(mm.MmhipError, match="workspace"):
+                ctx.logprobs_dev(x, 3, 5000, top=7, top_ids=out, workspace=w)
+        ctx.logprobs_dev(x, 3, 5000, top=7, top_ids=out, workspace=At(work, 16, need))
+        ctx.synchronize()
+        assert np.array_equal(out.to_numpy(np.uint32, 21).reshape(3, 7), np.tile(np.arange(7), (3, 1)))
 
 
 def test_logprobs_outputs_left_out(ctx):

@@ -185,6 +185,13 @@ def test_logprobs():
         assert "null context" not in mm.load_library().mmhip_last_error().decode(), bad
 
 
+def test_most_rows():
+    """Calls of 2^24 rows or tokens are refused, of one less not."""
+    for call in (norm, store, logprobs):
+        refused(call(n=1 << 24), mm.ERR_INVALID, "2^24")
+        refused(call(n=(1 << 24) - 1), mm.ERR_INVALID, "null context")
+
+
 def test_workspaces_without_a_context():
     lib = mm.load_library()
     assert lib.mmhip_mla_attention_workspace(None, 1, 1, 512) == 0
