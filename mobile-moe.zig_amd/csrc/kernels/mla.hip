@@ -185,7 +185,12 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         incl += before;
         // (a 64-bit division is some 150 instructions)
         chunk = total < 0x80000000u ? ((uint32_t)total + pl.groups - 1) / pl.groups : (total + pl.groups - 1) / pl.groups;
-        chunk = uniform(chunk);
+        // Up to three slots, one workgroup per CU is enough: fewer pieces to join.
+        // (One token at 12288 positions 21.7 us instead of 27.2, at 24576 25.3
+        // instead of 30.0, four at 4096 22.2 instead of 24.0; with four slots
+        // eight at 4096 take 31.0 instead of 30.2.)
+        const uint64_t least = total <= pl.groups / 2 ? 1 : total <= pl.groups ? 2 : 3;
+        chunk = uniform(chunk < least ? least : chunk);
         total = uniform(total);
         f = wg * chunk;
         end = f + chunk < total ? f + chunk : total;
