@@ -4,13 +4,21 @@
 // that the token's page table names. One pass over the rows with the running
 // maximum and sum of the softmax; all heads of a token share the read rows.
 //
-// Bound: HBM. A row of 512 + 64 values is 1152 B in f16 (612 B in Q8_0) and
-// costs 2 x 20 x 1088 operations. The matrix work is more than that: the f32
-// operand of each product enters as two f16 parts (22 bits; the cached values
-// are exact in f16), and heads come in tiles of 16. From 17 to 24 heads the
-// second tile holds up to 8 heads' high parts in its first half and their low
-// parts in the other, one product in place of two (kPacked): a quarter of the
-// matrix work and of the queries' registers less at 20 heads.
+// A row of 512 + 64 values is 1152 B in f16 (612 B in Q8_0) and costs 2 x 20 x
+// 1088 operations. The matrix work is more than that: the f32 operand of each
+// product enters as two f16 parts (22 bits; the cached values are exact in
+// f16), and heads come in tiles of 16. From 17 to 24 heads the second tile holds
+// up to 8 heads' high parts in its first half and their low parts in the other,
+// one product in place of two (kPacked; at 20 heads against two full tiles: 64
+// ragged contexts in Q8_0 56 us against 59, a chunk of 256 tokens 161 against
+// 168, f16 contexts alike).
+//
+// What bounds it: with long contexts in f16, HBM (131072 positions of one token
+// 39 us, 3.9 TB/s, and 13 for the join of its pieces; 64 times 4096 75 us, 4.0
+// TB/s). Otherwise a wave's chain through a tile, about 5000 cycles with two
+// workgroups on a CU: 64 ragged contexts up to 16384 in Q8_0 56 us, 256 tokens
+// over the same 4096 positions in f16 161 us (matrix cores busy 30% of the
+// time, LDS 41%). One short context: two launches, 16 us.
 //
 // A workgroup is four waves and takes tiles of 32 positions. Wave w owns the
 // latent columns 128 w .. 128 w + 127 and 16 of the rotary ones, both as keys
@@ -36,7 +44,7 @@
 //
 // Work is cut evenly, whatever the lengths: the tiles of all tokens and head
 // tiles form one list, of which every workgroup takes an equal run, two
-// workgroups per CU. A run may end inside a token; such pieces leave their
+// workgroups per CU (one: 64 ragged contexts in Q8_0 69 us instead of 57). A run may end inside a token; such pieces leave their
 // sums in the workspace and mla_join_kernel adds them in the list's order.
 #include "device_common.hpp"
 #include "kernels.hpp"
@@ -89,7 +97,9 @@ struct MlaLds {
 
 __device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (uint32_t)(((uint64_t)len + kMlaTile - 1) / kMlaTile); }
 // An item's slots of the list that is cut evenly: its tiles, behind slots that
-// stand for its queries' conversion and its result.
+// stand for its queries' conversion and its result. (64 ragged contexts 57 us
+// instead of 71; 64 times 4096, whose pieces ended with the sequences before, 76
+// instead of 71.)
 constexpr uint32_t kItemSlots = 3;
 __device__ __forceinline__ uint32_t slots_of(uint32_t len) { return len ? tiles_of(len) + kItemSlots : 0; }
 
