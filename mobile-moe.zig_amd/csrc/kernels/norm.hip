@@ -372,8 +372,12 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(StoreArgs a) {
         }
     }
     if (g.q8) {
+        // (A block without values would send its wave through the exact
+        // divisions: lanes past the row have ones.)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = live ? v[e] : 1.0f;
         float d;
-        const uint32_t q4 = q8_quad(v, live ? 4u : 0u, d);
+        const uint32_t q4 = q8_quad(v, 4u, d);
         if (live) {
             *reinterpret_cast<uint32_t*>(a.pool + paged_row(g, page, at) + c) = q4;
             if ((threadIdx.x & 7) == 0)
