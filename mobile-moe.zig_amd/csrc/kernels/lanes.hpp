@@ -46,4 +46,26 @@ __device__ __forceinline__ T group_sum(T v) {
     return v;
 }
 
+// The sum over lanes 0 .. this one, of all 64 lanes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {  // 0 where no lane moves to
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)v, CTRL, ROWS, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), CTRL, ROWS, 0xF, true);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+    v += moved<0x111, 0xF>(v);  // within rows of 16: from 1, 2, 4, 8 lanes below
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<0x142, 0xA>(v);  // a row's last lane to the row above: rows 1 and 3
+    v += moved<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
+    return v;
+}
+// A lane's value, the same for all.
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, uint32_t lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, lane);
+}
+
 }  // namespace mmhip

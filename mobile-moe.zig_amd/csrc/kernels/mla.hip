@@ -165,8 +165,35 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
     const auto head_of = [&](int t) { return MODE == kPacked && t == 1 ? 16 + (n16 & 7) : 16 * t + n16; };
 
     // ---- this workgroup's run of the list ----
-    uint64_t f, end, total, chunk;
-    {
+    uint64_t f, end, total, off;
+    uint64_t chunk;
+    uint32_t token, row, len;
+    const auto cut = [&] {
+        // (a 64-bit division is some 150 instructions)
+        chunk = total < 0x80000000u ? ((uint32_t)total + pl.groups - 1) / pl.groups : (total + pl.groups - 1) / pl.groups;
+        // Up to three slots, one workgroup per CU is enough: fewer pieces to join.
+        // (One token at 12288 positions 21.7 us instead of 27.2, at 24576 25.3
+        // instead of 30.0, four at 4096 22.2 instead of 24.0; with four slots
+        // eight at 4096 take 31.0 instead of 30.2.)
+        const uint64_t least = total <= pl.groups / 2 ? 1 : total <= pl.groups ? 2 : 3;
+        if (chunk < least) chunk = least;
+        f = wg * chunk;
+        end = f + chunk < total ? f + chunk : total;
+    };
+    if (a.n_tokens <= 64) {
+        // Every wave finds it for itself.
+        uint32_t bad, my_row = 0, my_len = 0;
+        if (lane < a.n_tokens) my_len = seen(a, lane, my_row, bad);
+        const uint64_t mine = (uint64_t)slots_of(my_len) * pl.head_tiles, incl = wave_scan(mine);
+        total = lane_value(incl, 63);
+        cut();
+        const uint64_t here = __ballot(incl - mine <= f && f < incl);
+        token = here ? __builtin_ctzll(here) : a.n_tokens;
+        const uint32_t at = here ? token : 0;
+        row = __builtin_amdgcn_readlane(my_row, at);
+        len = __builtin_amdgcn_readlane(my_len, at);
+        off = f - lane_value(incl - mine, at);
+    } else {
         const uint32_t per = (a.n_tokens + kMlaThreads - 1) / kMlaThreads;
         const uint64_t t0 = (uint64_t)tid * per;
         uint64_t mine = 0;
@@ -177,12 +204,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             mine += slots_of(last_len);
         }
         mine *= pl.head_tiles;
-        uint64_t incl = mine;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint64_t o = __shfl_up((unsigned long long)incl, off, 64);
-            if ((int)lane >= off) incl += o;
-        }
+        uint64_t incl = wave_scan(mine);
         if (lane == 63) s.scan[wave] = incl;
         __syncthreads();
         total = 0;
@@ -193,17 +215,8 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             total += s.scan[w];
         }
         incl += before;
-        // (a 64-bit division is some 150 instructions)
-        chunk = total < 0x80000000u ? ((uint32_t)total + pl.groups - 1) / pl.groups : (total + pl.groups - 1) / pl.groups;
-        // Up to three slots, one workgroup per CU is enough: fewer pieces to join.
-        // (One token at 12288 positions 21.7 us instead of 27.2, at 24576 25.3
-        // instead of 30.0, four at 4096 22.2 instead of 24.0; with four slots
-        // eight at 4096 take 31.0 instead of 30.2.)
-        const uint64_t least = total <= pl.groups / 2 ? 1 : total <= pl.groups ? 2 : 3;
-        chunk = uniform(chunk < least ? least : chunk);
         total = uniform(total);
-        f = wg * chunk;
-        end = f + chunk < total ? f + chunk : total;
+        cut();
         if (f < end && incl - mine <= f && f < incl) {
             uint64_t at = incl - mine;
             uint32_t t = (uint32_t)t0, row = last_row, len = last_len;
@@ -222,6 +235,10 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             s.start_off = f - at;
         }
         __syncthreads();
+        token = uniform(s.start_token);
+        row = uniform(s.start_row);
+        len = uniform(s.start_len);
+        off = uniform(s.start_off);
     }
     MlaSplit begun{0, 0};
 
@@ -229,9 +246,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
     const uint32_t blocks = FULL ? 4u : (g.rank / 32 > 4 * wave ? min(g.rank / 32 - 4 * wave, 4u) : 0u);
     const bool has_pe = FULL || kMlaPe * wave < g.width - g.rank;
 
-    uint32_t token = uniform(s.start_token);
-    uint64_t off = uniform(s.start_off);
-    uint32_t row = uniform(s.start_row), len = uniform(s.start_len), of_token = token;
+    uint32_t of_token = token;
     while (f < end && token < a.n_tokens) {
         if (token != of_token) {
             uint32_t bad;
