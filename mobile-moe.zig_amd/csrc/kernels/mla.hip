@@ -783,40 +783,41 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[c][1][e] += permuted<kRotate8>(o[c][1][e]);
         }
+        // Through the wave's slice of LDS, so that a store writes two heads'
+        // whole runs of 512 bytes and not 64 bytes of 16 heads each.
+        float* const dst = (whole ? a.out + (uint64_t)token * a.out_token_stride + (uint64_t)head0 * a.out_head_stride
+                                  : pl.parts + slot * pl.part_rows * g.rank) + wave * kMlaCols + 4 * (ln & 31);
+        const uint64_t head_step = whole ? a.out_head_stride : g.rank;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const uint32_t r = head_of(t), h = head0 + r;
-            if (h >= a.n_heads || (MODE == kPacked && t == 1 && low_half)) continue;
             const float2 ml = s.ml[r];
-            float f2 = back;
-            float* dst;
-            if (whole) {
-                f2 = ml.y == 0.0f ? 0.0f : back / ml.y;
-                dst = a.out + (uint64_t)token * a.out_token_stride + (uint64_t)h * a.out_head_stride;
-                if (a.lse && wave == 0 && grp == 0)
+            const float f2 = !whole ? back : ml.y == 0.0f ? 0.0f : back / ml.y;
+            if (wave == 0 && grp == 0 && h < a.n_heads && !(MODE == kPacked && t == 1 && low_half)) {
+                if (!whole) pl.part_ml[slot * kHeads + r] = ml;
+                else if (a.lse)
                     a.lse[(uint64_t)token * a.n_heads + h] =
                         ml.y == 0.0f ? -INFINITY : 0.69314718055995f * (ml.x + __builtin_amdgcn_logf(ml.y));
-            } else {
-                dst = pl.parts + (slot * pl.part_rows + r) * g.rank;
-                if (wave == 0 && grp == 0) pl.part_ml[slot * kHeads + r] = ml;
             }
-            dst += wave * kMlaCols + 4 * grp;
-            if (!whole || pl.vec_out) {
-                // Written through: the next launch reads them on other XCDs, and
-                // lines left in L2 would be flushed at this one's end.
 #pragma unroll
-                for (uint32_t c = 0; c < 8; ++c) {
-                    if (!FULL && c >= 2 * blocks) continue;
-                    __builtin_nontemporal_store(o[c][t] * f2, reinterpret_cast<v4f*>(dst + 16 * c));
-                }
-            } else {
+            for (uint32_t c = 0; c < 8; ++c) *reinterpret_cast<v4f*>(kv + n16 * 512 + (((4 * c + grp) ^ n16) << 4)) = o[c][t] * f2;
+            asm volatile("" ::: "memory");
 #pragma unroll
-                for (uint32_t c = 0; c < 8; ++c) {
-                    if (!FULL && c >= 2 * blocks) continue;
+            for (uint32_t j = 0; j < (MODE == kPacked && t == 1 ? 4 : 8); ++j) {
+                const uint32_t n = 2 * j + (ln >> 5);
+                const v4f v = *reinterpret_cast<const v4f*>(kv + n * 512 + (((ln & 31) ^ n) << 4));
+                if (head0 + 16 * t + n >= a.n_heads || (!FULL && (ln & 31) >= 8 * blocks)) continue;
+                float* to = dst + (16 * t + n) * head_step;
+                if (!whole || pl.vec_out) {
+                    // Written through: the next launch reads them on other XCDs,
+                    // and lines left in L2 would be flushed at this one's end.
+                    __builtin_nontemporal_store(v, reinterpret_cast<v4f*>(to));
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dst[16 * c + e] = o[c][t][e] * f2;
+                    for (int e = 0; e < 4; ++e) to[e] = v[e];
                 }
             }
+            asm volatile("" ::: "memory");
         }
         if (first && !whole) {
             begun.item = token * pl.head_tiles + ht_index;
