@@ -884,12 +884,7 @@ __global__ __launch_bounds__(kJoinThreads, 8) void mla_join_kernel(MlaArgs a, Ml
         const uint32_t heads = min(pl.rows, a.n_heads - (sp.item % pl.head_tiles) * pl.rows);
         my_jobs = (heads * j.parts(rank) + j.per_job() - 1) / j.per_job();
     }
-    uint32_t end = my_jobs;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t o = __shfl_up(end, off, 64);
-        if ((int)(tid & 63) >= off) end += o;
-    }
+    uint32_t end = (uint32_t)wave_scan(my_jobs);
     if ((tid & 63) == 63) scan[wave] = end;
     __syncthreads();
     uint32_t total = 0;
@@ -967,7 +962,7 @@ __global__ __launch_bounds__(kJoinThreads, 8) void mla_join_kernel(MlaArgs a, Ml
         const uint32_t in_wave = min(j.share, 64 / kTeam);
         for (uint32_t n = 1; n < in_wave; n *= 2)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], n * kTeam, 64);
+            for (int e = 0; e < 4; ++e) acc[e] += n == 1 ? permuted<kRotate8>(acc[e]) : __shfl_xor(acc[e], n * kTeam, 64);
         if (j.share > in_wave) {
             const uint32_t waves = j.share / in_wave;
             __syncthreads();

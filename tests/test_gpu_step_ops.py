@@ -444,6 +444,23 @@ def test_attention_shared_table(ctx, ggml_type, tokens, length):
 
 
 @pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
+@pytest.mark.parametrize("heads", [7, 20, 33])
+def test_attention_unaligned_rows(ctx, ggml_type, heads):
+    """Queries and outputs whose rows are not 16-byte aligned, of whole and of split tokens: the bits of aligned ones."""
+    rng = np.random.default_rng(heads)
+    pt, lens = 16, np.array([3, 1700, 0, 40, 16])
+    n_pages = 200
+    pool = Pool(rng, ggml_type, 512, 64, pt, n_pages)
+    tables = tables_for(rng, lens, pt, n_pages)
+    q, q_pe = queries(rng, len(lens), heads, 512, 64)
+    a = run_attention(ctx, pool, q, q_pe, tables, lens, 0.07)
+    b = run_attention(ctx, pool, q, q_pe, tables, lens, 0.07, pad=1)
+    same_bits(a[0], b[0])
+    same_bits(a[1], b[1])
+    check_attention(*a, *ref.attention64(q, q_pe, pool.values, tables, np.arange(len(lens)), lens, pt, 0.07, 512))
+
+
+@pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
 def test_attention_many_ragged_tokens(ctx, ggml_type):
     """More tokens than the chip has workgroups, most of them short, empty ones between, a few long."""
     rng = np.random.default_rng(31)
