@@ -729,26 +729,31 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 #pragma unroll
                 for (uint32_t c = 4; c < 8; ++c) read_values(c);
                 // Two column tiles at a time, so that a product's sum is not
-                // asked for by the next one.
-#pragma unroll
-                for (uint32_t b = 0; b < 4; ++b) {
-                    if (!FULL && b >= blocks) continue;
-                    v8h v[2], rest[2];
+                // asked for by the next one. (Q8_0: the next two tiles' values
+                // are scaled between this one's products.)
+                v8h v[2], rest[2];
+                const auto scale = [&](uint32_t b, v8h (&to)[2], v8h (&left)[2]) {
                     if constexpr (Q8) {
                         const uint2 d0 = *reinterpret_cast<const uint2*>(&s.dv[wave][b][4 * grp]);
                         const uint2 d1 = *reinterpret_cast<const uint2*>(&s.dv[wave][b][16 + 4 * grp]);
                         const v8h d = half8(make_uint4(d0.x, d0.y, d1.x, d1.y));
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            v[c] = val[2 * b + c] * d;
-                            rest[c] = __builtin_elementwise_fma(val[2 * b + c], d, -v[c]);
+                            to[c] = val[2 * b + c] * d;
+                            left[c] = __builtin_elementwise_fma(val[2 * b + c], d, -to[c]);
                         }
                     } else {
-                        v[0] = val[2 * b];
-                        v[1] = val[2 * b + 1];
+                        to[0] = val[2 * b];
+                        to[1] = val[2 * b + 1];
                     }
+                };
+                scale(0, v, rest);
 #pragma unroll
-                    for (int part = 0; part < 3; ++part)
+                for (uint32_t b = 0; b < 4; ++b) {
+                    if (!FULL && b >= blocks) continue;
+                    v8h nv[2], nrest[2];
+#pragma unroll
+                    for (int part = 0; part < 3; ++part) {
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -759,7 +764,13 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                                 if (part == 1 && Q8) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest[c], ph[t], acc, 0, 0, 0);
                                 if (part == 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], ph[t], acc, 0, 0, 0);
                             }
+                        if (part == 0 && b < 3) scale(b + 1, nv, nrest);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
+                    if (b < 3) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) v[c] = nv[c], rest[c] = nrest[c];
+                    }
                 }
             }
             if (++i >= count) break;
