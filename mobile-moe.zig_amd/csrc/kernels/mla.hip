@@ -290,13 +290,14 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         auto load_ids = [&](uint32_t tile) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint64_t p = (uint64_t)tile * kMlaTile + 16 * h;
-                id[h] = table[(p < len ? (uint32_t)p : len - 1) >> g.page_shift];
+                const uint32_t p = min(tile, n_tiles - 1) * kMlaTile | 16 * h;
+                id[h] = table[min(p, len - 1) >> g.page_shift];
             }
         };
         uint4 pre[Q8 ? 4 : 8], pre_pe;
         uint2 pre_d;
         uint32_t pre_dpe = 0, live = 0;
+        bool lost = false;  // a page that the pool does not have
         pre_pe = make_uint4(0, 0, 0, 0);
         pre_d = make_uint2(0, 0);
         auto load_rows = [&](uint32_t tile, bool wanted) {
@@ -310,8 +311,8 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 const int32_t page = (int32_t)uniform((uint32_t)id[h]);
                 const uint32_t p = p0 + 16 * h;
                 const bool want = p < len, ok = want && paged_has(g, page);
-                if (ok) live |= (len - p >= 16 ? 0xFFFFu : (1u << (len - p)) - 1) << (16 * h);
-                else if (want && tid == 0) report(a.status, kBadPage);
+                live |= ok ? 0xFFFFu >> (16 - min(len - p, 16u)) << (16 * h) : 0;
+                lost |= want && !ok;
                 // 16 rows from p on. A page that is not there is read as page 0
                 // and left out.
                 base[h] = a.pool + paged_row(g, ok ? (uint32_t)page : 0u, p & at_mask);
@@ -367,11 +368,11 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             mask = live;
             if constexpr (Q8) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t p = 8 * j + (lane >> 3), c = 2 * (lane & 7);
-                    uint8_t* dst = kv + p * 256;
-                    *reinterpret_cast<uint4*>(dst + ((c ^ (p & 15)) << 4)) = codes8(pre[j].x, pre[j].y);
-                    *reinterpret_cast<uint4*>(dst + ((c ^ (p & 15) ^ 1) << 4)) = codes8(pre[j].z, pre[j].w);
+                for (uint32_t j = 0; j < 4; ++j) {  // row 8 j + lane / 8
+                    uint8_t* dst = kv + 2048 * j;
+                    const uint32_t at = (lane >> 3) * 256 + (((lane >> 3) ^ 2 * (lane & 7)) << 4) ^ (j & 1) << 7;
+                    *reinterpret_cast<uint4*>(dst + at) = codes8(pre[j].x, pre[j].y);
+                    *reinterpret_cast<uint4*>(dst + (at ^ 16)) = codes8(pre[j].z, pre[j].w);
                 }
                 const uint32_t p = lane & 31;
                 float d[5];
@@ -403,9 +404,9 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t p = 4 * j + (lane >> 4);
-                    *reinterpret_cast<uint4*>(kv + p * 256 + (((lane & 15) ^ (p & 15)) << 4)) = pre[j];
+                for (uint32_t j = 0; j < 8; ++j) {  // row 4 j + lane / 16
+                    const uint32_t at = (lane >> 4) * 256 + (((lane >> 4) ^ (lane & 15)) << 4) ^ (j & 3) << 6;
+                    *reinterpret_cast<uint4*>(kv + 1024 * j + at) = pre[j];
                 }
                 *reinterpret_cast<uint4*>(s.pe[wave] + lane * 16) = pre_pe;
             }
@@ -780,6 +781,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         }
 
         // ---- the piece's result ----
+        if (lost && tid == 0) report(a.status, kBadPage);
         if (softmax && lane % kLanes == 0) s.ml[wave * (64 / kLanes) + lane / kLanes] = make_float2(m_run, l_run);
         lds_barrier();
         const uint32_t ln = afresh(lane), n16 = ln & 15, grp = ln >> 4;
