@@ -16,8 +16,8 @@
 // What bounds it: with long contexts in f16, HBM (131072 positions of one token
 // 38 us, 4.0 TB/s, and 13 for the join of its pieces; 64 times 4096 73 us, 4.1
 // TB/s). Otherwise a wave's chain through a tile, about 5000 cycles with two
-// workgroups on a CU: 64 ragged contexts up to 16384 in Q8_0 56 us, 256 tokens
-// over the same 4096 positions in f16 161 us (matrix cores busy 30% of the
+// workgroups on a CU: 64 ragged contexts up to 16384 in Q8_0 54 us, 256 tokens
+// over the same 4096 positions in f16 158 us (matrix cores busy 30% of the
 // time, LDS 41%). One short context: two launches, 16 us.
 //
 // A workgroup is four waves and takes tiles of 32 positions. Wave w owns the

@@ -9,10 +9,10 @@
 // shared the sum, and the cache writer stores the bits that norm and codec
 // would give one after the other. The f64 sum costs a conversion and an FMA
 // per value, hidden behind the row's loads. 4099 rows of 2048 with a residual,
-// its sum and Q8_0 out: 18.8 us, 5.8 TB/s; one row 1.8 us.
+// its sum and Q8_0 out: 18.5 us, 5.9 TB/s; one row 1.8 us.
 //
 // Rotary positions: 4096 tokens of 20 heads of 192 values, 64 of them turned:
-// 21.7 us, 5.8 TB/s; one token 2.3 us. The angles' 64-bit arithmetic is a
+// 19.2 us, 6.6 TB/s; one token 2.3 us. The angles' 64-bit arithmetic is a
 // wave's work per token and runs while the other values are copied.
 //
 // Cache writer: 4096 positions to Q8_0 8 us, 1.5 TB/s: a workgroup's chain of
@@ -423,7 +423,8 @@ hipError_t launch_rope(const RopeArgs& a, uint64_t n_tokens, hipStream_t s) {
     const bool vec = a.dims % 8 == 0 && a.first % 4 == 0 && a.head_dim % 4 == 0 && aligned16(a.x) && aligned16(a.y) &&
                      a.x_token_stride % 4 == 0 && a.x_head_stride % 4 == 0 && a.y_token_stride % 4 == 0 &&
                      a.y_head_stride % 4 == 0;
-    // (4096 tokens of 20 heads of 192: 21.4 us; pair by pair 30.5)
+    // (4096 tokens of 20 heads of 192 with ordinary stores:
+    // 21.4 us; pair by pair 30.5)
     if (vec) rope_kernel<4><<<(unsigned)n_tokens, kRopeThreads, 0, s>>>(a);
     else rope_kernel<1><<<(unsigned)n_tokens, kRopeThreads, 0, s>>>(a);
     return hipGetLastError();
