@@ -38,9 +38,10 @@
 // by block, each block's product times the position's block scale. In O the
 // values are scaled: d * code has 19 bits, its f16 rounding and the rest (an
 // FMA away) are both exact, one vector instruction per value for both. (The
-// scale folded into P instead costs three per head tile and value.) Scales of
-// 2^8 and more go in with a power of two less, so that f16 does not overflow;
-// the largest so far is kept like the softmax's maximum.
+// scale folded into P instead costs three per head tile and value.) From scales
+// of 2^9 on d * code can pass f16's range. Such blocks count as 0 in these
+// products and are taken in a second round, only by tiles that have any, with
+// 2^-9 d, which is as exact; so no scale costs another block or position any bits.
 //
 // Work is cut evenly, whatever the lengths: the tiles of all tokens and head
 // tiles form one list, of which every workgroup takes an equal run, two
@@ -87,7 +88,8 @@ struct MlaLds {
     // P: f16 in rows of 40 (per tile high parts, low parts; packed as it is)
     uint32_t p[(MODE == kTwo ? 4 : MODE == kPacked ? 3 : 2) * 16 * 20];
     float ds[Q8 ? kMlaWaves : 1][5][kMlaTile];  // block scales of the keys
-    uint16_t dv[Q8 ? kMlaWaves : 1][4][kMlaTile];  // of the values, in f16
+    uint16_t dv[Q8 ? kMlaWaves : 1][4][kMlaTile];  // of the values, in f16: those below 2^9,
+    uint16_t db[Q8 ? kMlaWaves : 1][4][kMlaTile];  // and the others times 2^-9
     float alpha[16 * NT], factor[16 * NT], qmax[kMlaWaves][16 * NT];
     float2 ml[16 * NT];
     uint64_t scan[kMlaWaves];
@@ -361,8 +363,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         uint8_t* const kv = s.kv[wave];
         uint32_t mask = 0;
         v4f o[8][NT];
-        int e_run = 0;  // Q8_0: value scales are taken times 2^-e_run
-        float e_scale = 1.0f;
+        uint32_t big = 0;  // Q8_0: positions with block scales of 2^9 and more, NaN among them
         auto stage = [&]() {
             const uint32_t lane = afresh(tid & 63);
             mask = live;
@@ -381,17 +382,24 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 d[2] = f16_scale((uint16_t)(pre_d.y & 0xFFFFu));
                 d[3] = f16_scale((uint16_t)(pre_d.y >> 16));
                 d[4] = f16_scale((uint16_t)(FULL ? pre_dpe >> (wave / 2 * 16) : pre_dpe));
-                float top = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
-                top = group_max<16>((mask >> p) & 1 ? top : 0.0f);
-                // As bits they compare like numbers; 2^8 and more: 1 to 9 (infinity).
-                const uint32_t tb = max(__builtin_amdgcn_readlane(__float_as_uint(top), 0), __builtin_amdgcn_readlane(__float_as_uint(top), 16));
-                const int e = min(max((int)(tb >> 23) - 134, 0), 9);
-                // The sums so far follow in the O phase, with the softmax's factor.
-                e_scale = e > e_run ? pow2(e_run - e) : 1.0f;
-                e_run = max(e, e_run);
-                const v2h f2 = (v2h)(_Float16)pow2(-e_run);
-                const uint32_t d01 = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, pre_d.x) * f2);
-                const uint32_t d23 = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, pre_d.y) * f2);
+                // (the two highest bits of the exponent)
+                uint32_t d01 = pre_d.x, d23 = pre_d.y;
+                const uint32_t b01 = d01 & d01 << 1 & 0x40004000u, b23 = d23 & d23 << 1 & 0x40004000u;
+                big = uniform((uint32_t)__ballot(b01 | b23) & mask);
+                if (big) {
+                    const uint32_t m01 = (b01 >> 14) * 0xFFFFu, m23 = (b23 >> 14) * 0xFFFFu;
+                    const v2h f = {(_Float16)0x1p-9f, (_Float16)0x1p-9f};
+                    const uint32_t s01 = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, d01 & m01) * f);
+                    const uint32_t s23 = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, d23 & m23) * f);
+                    d01 &= ~m01;
+                    d23 &= ~m23;
+                    if (lane < 32) {
+                        s.db[wave][0][p] = (uint16_t)(s01 & 0xFFFFu);
+                        s.db[wave][1][p] = (uint16_t)(s01 >> 16);
+                        s.db[wave][2][p] = (uint16_t)(s23 & 0xFFFFu);
+                        s.db[wave][3][p] = (uint16_t)(s23 >> 16);
+                    }
+                }
                 if (lane < 32) {
 #pragma unroll
                     for (int b = 0; b < 5; ++b) s.ds[wave][b][p] = d[b];
@@ -423,7 +431,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 #pragma unroll
                         for (int b = 0; b < 5; ++b) {
                             s.ds[wave][b][p] = 0.0f;
-                            if (b < 4) s.dv[wave][b][p] = 0;
+                            if (b < 4) s.dv[wave][b][p] = s.db[wave][b][p] = 0;
                         }
                     }
                 }
@@ -573,8 +581,11 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             // a block) and values (transposed: rows 4 grp + n16 / 4, 8 bytes of
             // 16 columns); blocks and columns are further bits to flip.
             const uint32_t k_at = n16 * 256 + ((grp ^ n16) << 4);
-            const uint32_t v_row = 4 * grp + (n16 >> 2);
-            const uint32_t v_at = v_row * 256 + ((((n16 >> 1) & 1) ^ v_row) << 4) + (n16 & 1) * 8;
+            const auto value_place = [](uint32_t ln) {
+                const uint32_t n16 = ln & 15, row = 4 * (ln >> 4) + (n16 >> 2);
+                return row * 256 + ((((n16 >> 1) & 1) ^ row) << 4) + (n16 & 1) * 8;
+            };
+            const uint32_t v_at = value_place(ln);
             const uint32_t srow = wave * (64 / kLanes) + ln / kLanes, spos = (ln % kLanes) * kPer;
             // Two workgroups share a CU: the one between its barriers goes first
             // (1 to 4%).
@@ -653,12 +664,13 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 #pragma unroll
             for (uint32_t w = 0; w < kMlaWaves; ++w) part[w] = *reinterpret_cast<const vper*>(&s.sp[w][from][spos]);
             v8h val[8];
-            const auto read_values = [&](uint32_t c) {
-                const v4s t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + (v_at ^ (c << 5))));
-                const v4s t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + 4096 + (v_at ^ (c << 5))));
+            const auto values = [&](uint32_t c, uint32_t at) {
+                const v4s t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + (at ^ (c << 5))));
+                const v4s t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(kv + 4096 + (at ^ (c << 5))));
                 const uint2 x = __builtin_bit_cast(uint2, t0), y = __builtin_bit_cast(uint2, t1);
-                val[c] = half8(make_uint4(x.x, x.y, y.x, y.y));
+                return half8(make_uint4(x.x, x.y, y.x, y.y));
             };
+            const auto read_values = [&](uint32_t c) { val[c] = values(c, v_at); };
 #pragma unroll
             for (uint32_t c = 0; c < 4; ++c) read_values(c);
             __builtin_amdgcn_sched_barrier(0);
@@ -718,7 +730,6 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    if constexpr (Q8) al[t] *= e_scale;
                     same = same && al[t] == 1.0f;
                 }
                 if (!__all(same)) {
@@ -773,6 +784,30 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                         for (int c = 0; c < 2; ++c) v[c] = nv[c], rest[c] = nrest[c];
                     }
                 }
+                // The blocks of large scales, into sums 2^-9 as large. (Places are
+                // formed anew: kept from above they would cost the general kernels
+                // 8 more spilled registers and a tenth of their speed.)
+                if (Q8 && big) {
+                    const uint32_t ln = afresh(lane), at = value_place(ln), d_at = 4 * (ln >> 4);
+#pragma unroll
+                    for (uint32_t c = 0; c < 8; ++c) {
+                        const uint2 d0 = *reinterpret_cast<const uint2*>(&s.db[wave][c / 2][d_at]);
+                        const uint2 d1 = *reinterpret_cast<const uint2*>(&s.db[wave][c / 2][16 + d_at]);
+                        const v8h d = half8(make_uint4(d0.x, d0.y, d1.x, d1.y));
+                        const v8h code = values(c, at), high = code * d, left = __builtin_elementwise_fma(code, d, -high);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            v4f& acc = o[c][t];
+                            acc *= 0x1p-9f;
+                            if (!(MODE == kPacked && t == 1))
+                                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, plo[t % (MODE == kTwo ? 2 : 1)], acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(left, ph[t], acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, ph[t], acc, 0, 0, 0);
+                            acc *= 0x1p9f;
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
             }
             if (++i >= count) break;
             stage();
@@ -788,7 +823,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
         const bool low_half = n16 >= 8;
         const auto head_of = [&](int t) { return MODE == kPacked && t == 1 ? 16 + (n16 & 7) : 16 * t + n16; };
         const bool first = tile0 == 0, whole = first && count == n_tiles;
-        const float back = Q8 ? pow2(e_run - 15) : 1.0f / kPScale;
+        const float back = 1.0f / kPScale;
         const uint64_t slot = (uint64_t)wg * 2 + (first ? 1 : 0);
         if constexpr (MODE == kPacked) {  // both parts' sums
 #pragma unroll
