@@ -451,7 +451,10 @@ int mmhip_kv_store_dev(mmhip_ctx* ctx, const mmhip_kv_cache* cache, const float*
  * tables do not have counts as length 0; each is reported (above).
  * Scores, softmax statistics and sums are f32; queries and probabilities enter
  * the matrix cores as two f16 parts each (22 bits), cached values exactly.
- * Queries beyond 1e30 in size or not finite give NaN. The work is split
+ * Queries beyond 1e30 in size or not finite give NaN. Infinite cached values
+ * follow the formula: a score of -infinity drops its position like a mask (a
+ * latent one still leaves NaN in its own column, 0 times infinity), one of
+ * +infinity or NaN gives NaN. The work is split
  * over the positions and joined, in an order that depends on the call's
  * shape and lengths alone, so a call repeated gives the same bits. */
 typedef struct {

@@ -158,13 +158,8 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
     __shared__ __align__(256) MlaLds<Q8, MODE> s;
     const PagedGeom g = a.geom;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t n16 = lane & 15, grp = lane >> 4;
     const uint32_t wg = blockIdx.x;
     MlaSplit* const splits = reinterpret_cast<MlaSplit*>(pl.splits);
-    // The head (of the head tile) behind column n16 of product tile t; in a
-    // packed tile column 8 + k has head k's low parts.
-    const bool low_half = n16 >= 8;
-    const auto head_of = [&](int t) { return MODE == kPacked && t == 1 ? 16 + (n16 & 7) : 16 * t + n16; };
 
     // ---- this workgroup's run of the list ----
     uint64_t f, end, total, off;
@@ -456,6 +451,8 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             // waited for at the branch's end, together with the rows.
             float q[NT][4][8], pe[NT][8];
             const float *src[NT], *src_pe[NT];
+            // The head (of the head tile) behind column n16 of product tile t; in
+            // a packed tile column 8 + k has head k's low parts.
             const uint32_t ln = afresh(lane), n16 = ln & 15, grp = ln >> 4;
             const bool low_half = n16 >= 8;
             const auto head_of = [&](int t) { return MODE == kPacked && t == 1 ? 16 + (n16 & 7) : 16 * t + n16; };
@@ -676,41 +673,78 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             __builtin_amdgcn_sched_barrier(0);
             if (softmax) {
                 vper x = ((part[0] + part[1]) + part[2]) + part[3];
-                float top = -INFINITY;
                 const uint32_t lv = mask >> spos;
 #pragma unroll
-                for (uint32_t e = 0; e < kPer; ++e) {
-                    x[e] = (lv >> e) & 1 ? x[e] * fac : -INFINITY;
-                    top = fmaxf(top, x[e]);
-                }
-                top = group_max<kLanes>(top);
-                const float m_new = fmaxf(m_run, top), base = m_new == -INFINITY ? 0.0f : m_new;
-                const float al = __builtin_amdgcn_exp2f(m_run - base);
-                float sum = 0.0f;
+                for (uint32_t e = 0; e < kPer; ++e) x[e] = (lv >> e) & 1 ? x[e] * fac : -INFINITY;
+                const float m_was = m_run, l_was = l_run;
+                const auto weigh = [&](vper x) {
+                    float top = x[0];
 #pragma unroll
-                for (uint32_t e = 0; e < kPer; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(x[e] - base);
-                    sum += x[e];
-                }
-                sum = group_sum<kLanes>(sum);
-                l_run = l_run * al + sum;
-                m_run = m_new;
-                if (ln % kLanes == 0) s.alpha[srow] = al;
-                // position 16 h + 4 g + e is O^T's operand element 4 h + e of group g;
-                // rows: high parts of both tiles, low parts of both; packed: high 16, packed 16, low 16
-                const uint32_t at = ((spos >> 2) & 3) * 8 + (spos >> 4) * 4 + (spos & 3);
-                const bool packed = MODE == kPacked && wave == 2;
-                uint32_t* hi = s.p + srow * 20 + at / 2;
-                uint32_t* lo = hi + (packed ? 8 : 16 * NT) * 20;
-                uint32_t h[kPer / 2], l[kPer / 2];
+                    for (uint32_t e = 1; e < kPer; ++e) top = fmaxf(top, x[e]);
+                    top = group_max<kLanes>(top);
+                    const float m_new = fmaxf(m_was, top), base = m_new == -INFINITY ? 0.0f : m_new;
+                    const float al = __builtin_amdgcn_exp2f(m_was - base);
+                    float sum = 0.0f;
 #pragma unroll
-                for (uint32_t e = 0; e < kPer; e += 2) split2(x[e] * kPScale, x[e + 1] * kPScale, h[e / 2], l[e / 2]);
-                if constexpr (kPer == 4) {
-                    *reinterpret_cast<uint2*>(hi) = make_uint2(h[0], h[1]);
-                    *reinterpret_cast<uint2*>(lo) = make_uint2(l[0], l[1]);
-                } else {
-                    *hi = h[0];
-                    *lo = l[0];
+                    for (uint32_t e = 0; e < kPer; ++e) {
+                        x[e] = __builtin_amdgcn_exp2f(x[e] - base);
+                        sum += x[e];
+                    }
+                    sum = group_sum<kLanes>(sum);
+                    l_run = l_was * al + sum;
+                    m_run = m_new;
+                    if (ln % kLanes == 0) s.alpha[srow] = al;
+                    // position 16 h + 4 g + e is O^T's operand element 4 h + e of group g;
+                    // rows: high parts of both tiles, low parts of both; packed: high 16, packed 16, low 16
+                    const uint32_t at = ((spos >> 2) & 3) * 8 + (spos >> 4) * 4 + (spos & 3);
+                    const bool packed = MODE == kPacked && wave == 2;
+                    uint32_t* hi = s.p + srow * 20 + at / 2;
+                    uint32_t* lo = hi + (packed ? 8 : 16 * NT) * 20;
+                    uint32_t h[kPer / 2], l[kPer / 2];
+#pragma unroll
+                    for (uint32_t e = 0; e < kPer; e += 2) split2(x[e] * kPScale, x[e + 1] * kPScale, h[e / 2], l[e / 2]);
+                    if constexpr (kPer == 4) {
+                        *reinterpret_cast<uint2*>(hi) = make_uint2(h[0], h[1]);
+                        *reinterpret_cast<uint2*>(lo) = make_uint2(l[0], l[1]);
+                    } else {
+                        *hi = h[0];
+                        *lo = l[0];
+                    }
+                    return sum;
+                };
+                const float sum = weigh(x);
+                // NaN: an infinite cached value met a part of the query that is 0
+                // or of the other sign, where the formula has an infinity, or the
+                // formula has NaN too. Such scores again, from the slices of all
+                // waves; the terms that are not finite decide. (A query that is not
+                // finite gives NaN.)
+                if (__any(sum != sum) && sum != sum) {  // (alike for a head's lanes)
+                    const uint32_t h = min(head0 + from, a.n_heads - 1), t = afresh(token);
+                    const float* q = a.q + (uint64_t)t * a.q_token_stride + (uint64_t)h * a.q_head_stride;
+                    const float* q_pe = a.q_pe + (uint64_t)t * a.q_pe_token_stride + (uint64_t)h * a.q_pe_head_stride;
+#pragma unroll 1
+                    for (uint32_t p = spos; p < spos + kPer; ++p) {
+                        float score = (((s.sp[0][from][p] + s.sp[1][from][p]) + s.sp[2][from][p]) + s.sp[3][from][p]) * fac;
+                        if (score != score) {
+                            score = 0.0f;
+#pragma unroll 1
+                            for (uint32_t c = 0; c < g.width; ++c) {
+                                const bool pe = c >= g.rank;
+                                const uint32_t i = pe ? c - g.rank : c, w = pe ? i / kMlaPe : i / kMlaCols;
+                                const uint32_t j = pe ? i % kMlaPe : i % kMlaCols;
+                                const uint8_t* at = pe ? s.pe[w] + p * 32 + 2 * j : s.kv[w] + p * 256 + (((j >> 3) ^ (p & 15)) << 4) + 2 * (j & 7);
+                                float k = (float)*reinterpret_cast<const _Float16*>(at);
+                                if constexpr (Q8) k *= s.ds[w][pe ? 4 : j / 32][p];
+                                const float x = pe ? q_pe[i] : q[i];
+                                score += (fabsf(k) < INFINITY ? 0.0f : x * k) + (x - x);
+                            }
+                            score *= a.scale;
+                        }
+                        s.sp[0][from][p] = score;
+                    }
+#pragma unroll
+                    for (uint32_t e = 0; e < kPer; ++e) x[e] = (lv >> e) & 1 ? s.sp[0][from][spos + e] : -INFINITY;
+                    (void)weigh(x);
                 }
             }
             lds_barrier();

@@ -73,3 +73,82 @@ def test_attention_block_scales(ctx, heads, rank, pe, length, where):
     err = np.linalg.norm((out[1] - want[1]).reshape(heads, nb, 32), axis=-1)
     assert (err <= 1e-5 * np.linalg.norm(want[1].reshape(heads, nb, 32), axis=-1)).all()
     assert (np.abs(lse - want_lse) <= 1e-5 * np.maximum(1, np.abs(want_lse))).all()
+
+
+# ---- infinities -----------------------------------------------------------
+
+def infinite_row(pool, page, at, col, sign):
+    """A value of the row (a whole block of it in Q8_0, all of one sign) becomes infinite."""
+    if pool.type == mm.F16:
+        pool.bytes.view(np.float16).reshape(pool.n_pages, pool.page_tokens, -1)[page, at, col] = sign * np.inf
+        return [col]
+    codes, scales = parts(pool)
+    b = col // 32
+    codes[page, at, 32 * b:32 * b + 32] = sign * 5
+    scales[page, at, b] = np.inf
+    return list(range(32 * b, 32 * b + 32))
+
+
+@pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
+@pytest.mark.parametrize("heads", [5, 16, 17, 20, 24, 33])
+@pytest.mark.parametrize("rank,pe,length", [(512, 64, 50), (512, 64, 2000), (96, 32, 50)])
+def test_attention_infinite_rotary_values(ctx, ggml_type, heads, rank, pe, length):
+    """A score of -infinity only drops its position, one of +infinity gives NaN, whatever the query's bits: the values of
+    every other head are those of the formula."""
+    rng = np.random.default_rng(heads + rank)
+    pt, n_pages = 16, (length + 15) // 16
+    pool = Pool(rng, ggml_type, rank, pe, pt, n_pages)
+    q, q_pe = queries(rng, 2, heads, rank, pe)
+    q_pe[:, ::2] = np.where(q_pe[:, ::2] < 0, -0.5, 0.5)  # bits that fit f16: nothing is left for a second part
+    for at, col in ((3, rank + pe - 3), (17, rank + 1), (length - 1, rank + pe - 20)):
+        cols = [c - rank for c in infinite_row(pool, at // pt, at % pt, col, -1)]
+        q_pe[..., cols] = np.abs(q_pe[..., cols])
+    revalue(pool)
+    up = np.zeros(heads, bool)
+    up[[1, heads - 1]] = True
+    q_pe[1, up] *= -1  # the second token's heads 1 and last: +infinity (some rows also -infinity)
+    lens, ids, tables = np.array([length, length]), np.zeros(2, np.int64), np.arange(n_pages)[None]
+    with np.errstate(invalid="ignore"):
+        want, want_lse = ref.attention64(q, q_pe, pool.values, tables, ids, lens, pt, 0.07, rank)
+    out, lse = run_attention(ctx, pool, q, q_pe, tables, lens, 0.07, table_of=ids)
+    assert np.isnan(want[1, up]).all() and np.isfinite(want[0]).all() and np.isfinite(want[1, ~up]).all()
+    assert np.isnan(out[1, up]).all() and np.isnan(lse[1, up]).all()
+    check_attention(out[0], lse[0], want[0], want_lse[0])
+    check_attention(out[1, ~up], lse[1, ~up], want[1, ~up], want_lse[1, ~up])
+
+
+@pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
+@pytest.mark.parametrize("heads", [5, 20, 33])
+def test_attention_infinite_latent_values(ctx, ggml_type, heads):
+    """An infinite latent value whose score is -infinity: NaN in its own columns (0 times infinity), the formula's values
+    in all others."""
+    rng = np.random.default_rng(heads)
+    pool = Pool(rng, ggml_type, 512, 64, 16, 4)
+    q, q_pe = queries(rng, 1, heads, 512, 64)
+    cols = infinite_row(pool, 2, 5, 300, 1)
+    revalue(pool)
+    q[..., cols] = -np.abs(q[..., cols])
+    q[:, ::2, cols] = -0.25
+    lens, tables = np.array([64]), np.arange(4)[None]
+    with np.errstate(invalid="ignore"):
+        want, want_lse = ref.attention64(q, q_pe, pool.values, tables, [0], lens, 16, 0.07, 512)
+    out, lse = run_attention(ctx, pool, q, q_pe, tables, lens, 0.07)
+    assert np.isnan(out[..., cols]).all()
+    keep = np.setdiff1d(np.arange(512), cols)
+    check_attention(out[..., keep], lse, want[..., keep], want_lse)
+
+
+@pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
+def test_attention_without_a_finite_score(ctx, ggml_type):
+    """Every score -infinity: like nothing seen, out 0 and lse -infinity; the other heads as always."""
+    rng = np.random.default_rng(3)
+    pool = Pool(rng, ggml_type, 512, 64, 16, 2)
+    q, q_pe = queries(rng, 1, 20, 512, 64)
+    for at in range(20):
+        cols = [c - 512 for c in infinite_row(pool, at // 16, at % 16, 515, 1)]
+    q_pe[..., cols] = -np.abs(q_pe[..., cols])
+    q_pe[:, 7:9, cols] *= -1
+    out, lse = run_attention(ctx, pool, q, q_pe, np.array([[0, 1]]), np.array([20]), 0.07)
+    rest = np.r_[0:7, 9:20]
+    assert (out[0, rest] == 0).all() and (lse[0, rest] == -np.inf).all()
+    assert np.isnan(out[0, 7:9]).all() and np.isnan(lse[0, 7:9]).all()
