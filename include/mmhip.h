@@ -450,7 +450,9 @@ int mmhip_kv_store_dev(mmhip_ctx* ctx, const mmhip_kv_cache* cache, const float*
  * pool does not have is left out like a masked one, and a row number that the
  * tables do not have counts as length 0; each is reported (above).
  * Scores, softmax statistics and sums are f32; queries and probabilities enter
- * the matrix cores as two f16 parts each (22 bits), cached values exactly.
+ * the matrix cores as two f16 parts each that hold all of their 24 bits (down to
+ * 2^-38 of a head's largest query and 2^-40 of a probability), cached values
+ * exactly.
  * Queries beyond 1e30 in size or not finite give NaN. Infinite cached values
  * follow the formula: a score of -infinity drops its position like a mask (a
  * latent one still leaves NaN in its own column, 0 times infinity), one of

@@ -6,7 +6,7 @@
 //
 // A row of 512 + 64 values is 1152 B in f16 (612 B in Q8_0) and costs 2 x 20 x
 // 1088 operations. The matrix work is more than that: the f32 operand of each
-// product enters as two f16 parts (22 bits; the cached values are exact in
+// product enters as two f16 parts (all 24 bits; the cached values are exact in
 // f16), and heads come in tiles of 16. From 17 to 24 heads the second tile holds
 // up to 8 heads' high parts in its first half and their low parts in the other,
 // one product in place of two (kPacked; at 20 heads against two full tiles: 64
@@ -38,6 +38,7 @@
 // by block, each block's product times the position's block scale. In O the
 // values are scaled: d * code has 19 bits, its f16 rounding and the rest (an
 // FMA away) are both exact, one vector instruction per value for both. (The
+// rest times P's lower part, 2^-24 of the product at most, is left out. The
 // scale folded into P instead costs three per head tile and value.) From scales
 // of 2^9 on d * code can pass f16's range. Such blocks count as 0 in these
 // products and are taken in a second round, only by tiles that have any, with
@@ -57,6 +58,7 @@ namespace {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
@@ -122,11 +124,12 @@ __device__ __forceinline__ uint4 codes8(uint32_t a, uint32_t b) {
     return make_uint4(codes2(x, 0x04010400u), codes2(x, 0x04030402u), codes2(y, 0x04010400u), codes2(y, 0x04030402u));
 }
 
-// Two values as f16 parts: hi + lo is the value to 22 bits (hi truncated, lo
-// the rest).
+// Two values as f16 parts, both rounded to nearest: what hi leaves is at most
+// half a step of 11 bits, with a sign, on the grid of 24, so lo holds it and
+// hi + lo is the value, down to f16's smallest step (2^-24; half of one is lost).
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    const auto l = __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]);
+    const v2h h = __builtin_convertvector((v2f){a, b}, v2h);
+    const v2h l = __builtin_convertvector((v2f){a - (float)h[0], b - (float)h[1]}, v2h);
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, l);
 }
@@ -677,20 +680,21 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
 #pragma unroll
                 for (uint32_t e = 0; e < kPer; ++e) x[e] = (lv >> e) & 1 ? x[e] * fac : -INFINITY;
                 const float m_was = m_run, l_was = l_run;
-                const auto weigh = [&](vper x) {
+                float sum;
+                const auto weigh = [&](vper x) {  // (gives the lane's own sum)
                     float top = x[0];
 #pragma unroll
                     for (uint32_t e = 1; e < kPer; ++e) top = fmaxf(top, x[e]);
                     top = group_max<kLanes>(top);
                     const float m_new = fmaxf(m_was, top), base = m_new == -INFINITY ? 0.0f : m_new;
                     const float al = __builtin_amdgcn_exp2f(m_was - base);
-                    float sum = 0.0f;
+                    float own = 0.0f;
 #pragma unroll
                     for (uint32_t e = 0; e < kPer; ++e) {
                         x[e] = __builtin_amdgcn_exp2f(x[e] - base);
-                        sum += x[e];
+                        own += x[e];
                     }
-                    sum = group_sum<kLanes>(sum);
+                    sum = group_sum<kLanes>(own);
                     l_run = l_was * al + sum;
                     m_run = m_new;
                     if (ln % kLanes == 0) s.alpha[srow] = al;
@@ -710,15 +714,15 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                         *hi = h[0];
                         *lo = l[0];
                     }
-                    return sum;
+                    return own;
                 };
-                const float sum = weigh(x);
+                const float own = weigh(x);
                 // NaN: an infinite cached value met a part of the query that is 0
                 // or of the other sign, where the formula has an infinity, or the
                 // formula has NaN too. Such scores again, from the slices of all
                 // waves; the terms that are not finite decide. (A query that is not
                 // finite gives NaN.)
-                if (__any(sum != sum) && sum != sum) {  // (alike for a head's lanes)
+                if (__any(own != own) && sum != sum) {  // (alike for a head's lanes)
                     const uint32_t h = min(head0 + from, a.n_heads - 1), t = afresh(token);
                     const float* q = a.q + (uint64_t)t * a.q_token_stride + (uint64_t)h * a.q_head_stride;
                     const float* q_pe = a.q_pe + (uint64_t)t * a.q_pe_token_stride + (uint64_t)h * a.q_pe_head_stride;

@@ -33,6 +33,52 @@ def revalue(pool):
                 .reshape(codes.shape)
 
 
+# ---- operands of 24 bits --------------------------------------------------
+
+@pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
+@pytest.mark.parametrize("heads", [5, 20, 33])
+def test_attention_uses_every_bit_of_a_query(ctx, ggml_type, heads):
+    """A query of 2 - 2^-23 against -2: the score is -2^-23 times the cached value, all of it the query's last bit. (Its
+    terms are below 2^17 and are added with three roundings of at most half a step, 2^-8 each.)"""
+    rng = np.random.default_rng(1)
+    pool = Pool(rng, ggml_type, 512, 64, 16, 1)
+    c = 65504.0 if ggml_type == mm.F16 else 127 * 512.0
+    if ggml_type == mm.F16:
+        pool.bytes.view(np.float16)[...] = 0
+        pool.bytes.view(np.float16).reshape(16, 576)[0, [40, 41]] = c
+    else:
+        codes, scales = parts(pool)
+        codes[...], scales[...] = 0, 512.0
+        codes[0, 0, [40, 41]] = 127
+    q, q_pe = np.zeros((1, heads, 512), np.float32), np.zeros((1, heads, 64), np.float32)
+    q[..., 40], q[..., 41] = np.float32(2 - 2.0 ** -23), -2.0
+    lse = run_attention(ctx, pool, q, q_pe, np.zeros((1, 1)), np.array([1]), 1.0)[1]
+    assert (np.abs(lse + c * 2.0 ** -23) <= 3 * 2.0 ** -8).all(), lse
+
+
+@pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
+@pytest.mark.parametrize("heads", [5, 20, 33])
+@pytest.mark.parametrize("length", [32, 900])
+def test_attention_probabilities_add_up_to_one(ctx, ggml_type, heads, length):
+    """Where every cached value is 1.25, so is the output, up to roundings to nearest (running sums, the division): as
+    much as forty whole ones on a value's way, without a side. The mean over N values then has a deviation of at most
+    sqrt(40 / 3 / N) u; 4 of these for N = 4000 are 0.23 u, and 0.4 u is allowed. Probabilities cut to 22 bits are 1.25 u
+    too small."""
+    rng = np.random.default_rng(heads + length)
+    pt, n_pages, n = 16, (length + 15) // 16, (4000 + heads - 1) // heads
+    pool = Pool(rng, ggml_type, 512, 64, pt, n_pages)
+    if ggml_type == mm.F16:
+        pool.bytes.view(np.float16).reshape(n_pages, pt, 576)[..., :512] = 1.25
+    else:
+        codes, scales = parts(pool)
+        codes[..., :512], scales[..., :16] = 80, 2.0 ** -6
+    q, q_pe = np.zeros((n, heads, 512), np.float32), rng.standard_normal((n, heads, 64)).astype(np.float32)
+    out, _ = run_attention(ctx, pool, q, q_pe, np.arange(n_pages)[None], np.full(n, length), 0.1, table_of=np.zeros(n, np.int64))
+    assert (np.abs(out - 1.25) <= 1e-5 * 1.25).all()
+    mean = (out.astype(np.float64) / 1.25 - 1).mean()
+    assert abs(mean) <= 0.4 * U, mean / U
+
+
 # ---- block scales of all sizes --------------------------------------------
 
 @pytest.mark.parametrize("heads", [5, 20, 33])
