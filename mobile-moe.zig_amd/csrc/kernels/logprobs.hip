@@ -63,14 +63,17 @@ __device__ __forceinline__ float key_logit(uint64_t k) {
 __device__ __forceinline__ float above_of(uint64_t k) { return key_logit(k + (1ull << 32)); }
 
 // Sums are taken in base 2: s = sum 2^y and t = sum 2^y y, y = (x - m) log2 e.
-// The product's rounding moves a term by |y| 2^-24 ln 2 of its size at most:
-// a part in 10^6 where y = -24, and what lies further down weighs nothing.
-constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
+// The product's rounding moves a term by |y| 2^-24 ln 2 of its size at most, up
+// or down: a part in 10^6 where y = -24, and what lies further down weighs
+// nothing. log2 e enters in two parts: rounded to f32 it is 1.3e-8 too small,
+// which would move all terms to one side.
+constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596300e-8f;
+__device__ __forceinline__ float in_base2(float d) { return fmaf(d, kLog2e, d * kLog2eRest); }
 // What a part's weight 2^y, y = (m - M) log2 e, makes of its sums at the larger
 // maximum M. Without weight it adds nothing to t, but a NaN in s stays one.
 __device__ __forceinline__ void rebase(LpSum& a, float m) {
     if (a.m == m) return;
-    const float y = (a.m - m) * kLog2e, f = __builtin_amdgcn_exp2f(y);
+    const float y = in_base2(a.m - m), f = __builtin_amdgcn_exp2f(y);
     a.t = f == 0.0f ? 0.0f : f * (a.t + a.s * y);
     a.s *= f;
     a.m = m;
@@ -207,9 +210,10 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_split_kernel(LogprobsArgs
             const float base = here.m == -INFINITY ? 0.0f : here.m;
 #pragma unroll
             for (uint32_t i = 0; i < kLpPerThread; ++i) {
-                const float y = (v[i] - base) * kLog2e, e = __builtin_amdgcn_exp2f(y);
+                // (below y = -256 e is 0; a NaN stays one in e)
+                const float y = in_base2(v[i] - base), e = __builtin_amdgcn_exp2f(y);
                 here.s += e;
-                here.t += e == 0.0f ? 0.0f : e * y;
+                here.t = fmaf(e, fmaxf(y, -256.0f), here.t);
             }
             rebase(sum, here.m);
             sum.s += here.s;
@@ -272,12 +276,15 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobsArgs 
     LpSum sum{-INFINITY, 0.0f, 0.0f, 0.0f};
     if (tid < p.pieces) sum = p.sums[row * p.pieces + tid];
     sum = join_all(sum, red);
-    const float log_s = logf(sum.s);
-    if (a.entropy && tid == 0) a.entropy[row] = log_s - kLn2 * (sum.t / sum.s);
+    // The logarithm and what follows in 64 bits, rounded once: logf is up to two
+    // units too small and hardly ever too large (half a unit on average).
+    const double log_s = log((double)sum.s);
+    const auto log_prob = [&](float x) { return (float)(((double)x - (double)sum.m) - log_s); };
+    if (a.entropy && tid == 0) a.entropy[row] = (float)(log_s - M_LN2 * ((double)sum.t / (double)sum.s));
     for (uint64_t i = tid; i < a.n_given; i += kLpThreads) {
         const uint32_t id = a.tokens[row * a.n_given + i];
         if (id >= a.vocab) report(a.status, kBadToken);
-        a.token_logprobs[row * a.n_given + i] = id < a.vocab ? (x[id] - sum.m) - log_s : __builtin_nanf("");
+        a.token_logprobs[row * a.n_given + i] = id < a.vocab ? log_prob(x[id]) : __builtin_nanf("");
     }
     if (top == 0) return;
     // 64 keys, the largest of each piece (of every 64th piece) and where there
@@ -301,7 +308,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobsArgs 
     __syncthreads();
     if (tid < top) {
         a.top_ids[row * top + tid] = key_id(best[tid]);
-        if (a.top_logprobs) a.top_logprobs[row * top + tid] = (key_logit(best[tid]) - sum.m) - log_s;
+        if (a.top_logprobs) a.top_logprobs[row * top + tid] = log_prob(key_logit(best[tid]));
     }
 }
 

@@ -198,3 +198,20 @@ def test_attention_without_a_finite_score(ctx, ggml_type):
     rest = np.r_[0:7, 9:20]
     assert (out[0, rest] == 0).all() and (lse[0, rest] == -np.inf).all()
     assert np.isnan(out[0, 7:9]).all() and np.isnan(lse[0, 7:9]).all()
+
+
+# ---- log probabilities ----------------------------------------------------
+
+def test_logprobs_have_no_side(ctx):
+    """One large logit and 32767 about 10.4 below it, which together weigh as much: log probabilities near -0.7, whose
+    own rounding is at most u / 2, to either side. Over 512 rows the mean's deviation is below 0.05 u, that of the sums,
+    some ten roundings, below 0.1 u; 0.5 u is allowed. An exponent off by 1.3e-8 of its size (log2 e rounded to f32) puts
+    all of them 1.1 u too low, a logarithm that is cut off 0.5 u too high."""
+    rng = np.random.default_rng(10)
+    n, v = 512, 32768
+    x = (-10.4 + rng.uniform(-0.5, 0.5, (n, v)) + rng.uniform(-0.2, 0.2, (n, 1))).astype(np.float32)
+    x[:, 5] = 0.0
+    got = run_logprobs(ctx, x, np.full((n, 1), 5), 0)
+    lp, h = ref.logprobs64(x)
+    assert (np.abs(got[0][:, 0] - lp[:, 5]) <= 6e-6).all()
+    assert abs((got[0][:, 0] - lp[:, 5]).mean()) <= 0.5 * U, (got[0][:, 0] - lp[:, 5]).mean() / U
