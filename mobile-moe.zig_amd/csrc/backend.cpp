@@ -7,6 +7,7 @@
 #include <string>
 
 #include "../../include/mmhip.h"
+#include "status.hpp"
 
 namespace mmhip {
 
@@ -27,18 +28,16 @@ int hip_fail(hipError_t e, const char* what) {
 }
 
 int check_device_status(mmhip_ctx* ctx, const char* what) {
-    const uint32_t st = ctx->status ? __atomic_load_n(ctx->status, __ATOMIC_ACQUIRE) : 0u;
+    const uint32_t st = ctx->status ? take_status(ctx->status) : 0u;
     if (st == 0) return MMHIP_OK;
-    __atomic_store_n(ctx->status, 0u, __ATOMIC_RELEASE);
     set_error(MMHIP_ERR_HIP, std::string(what) + ": decode MoE launch: a grid-wide wait timed out (code " +
                                  std::to_string(st) + "); its output is invalid");
     return MMHIP_ERR_HIP;
 }
 
 int check_step_status(mmhip_ctx* ctx, const char* what) {
-    const uint32_t st = ctx->status ? __atomic_load_n(ctx->status + 1, __ATOMIC_ACQUIRE) : 0u;
+    const uint32_t st = ctx->status ? take_status(ctx->status + 1) : 0u;
     if (st == 0) return MMHIP_OK;
-    __atomic_store_n(ctx->status + 1, 0u, __ATOMIC_RELEASE);
     static const char* const met[] = {"",
                                       "kv_store: a slot that the pool does not have (its token was not stored)",
                                       "mla_attention: a table row that does not exist (its token saw nothing)",
