@@ -240,6 +240,15 @@ def _ptr(a: np.ndarray) -> int:
     return a.ctypes.data
 
 
+def _optional(b) -> Optional[int]:
+    """The address of an optional buffer, None where it is left out. A freed one is not left out."""
+    if b is None:
+        return None
+    if b.ptr is None:
+        raise MmhipError("an optional argument", ERR_INVALID, "the buffer was freed")
+    return b.ptr
+
+
 class DeviceArray:
     """Device buffer owned through the library's allocator."""
 
@@ -471,9 +480,9 @@ class Context:
                      residual_stride: Optional[int] = None, sum_out=None, sum_stride: Optional[int] = None):
         """mmhip_rms_norm_dev: y = norm(x + residual) * weight, sum_out = x + residual. Strides default to cols."""
         check(self.lib.mmhip_rms_norm_dev(
-            self.handle, y.ptr, y_type, cols if y_stride is None else y_stride, None if sum_out is None else sum_out.ptr,
+            self.handle, y.ptr, y_type, cols if y_stride is None else y_stride, _optional(sum_out),
             cols if sum_stride is None else sum_stride, x.ptr, cols if x_stride is None else x_stride,
-            None if residual is None else residual.ptr, cols if residual_stride is None else residual_stride,
+            _optional(residual), cols if residual_stride is None else residual_stride,
             weight.ptr, n_rows, cols, eps), "mmhip_rms_norm_dev")
 
     def rope_dev(self, rope: "Rope", y, x, positions, n_tokens: int, n_heads: int, head_dim: int, first: int = 0,
@@ -490,9 +499,9 @@ class Context:
                      kv_offset: int = 0):
         """mmhip_kv_store_dev: KVCache.put for n_tokens positions, norm and rope included."""
         check(self.lib.mmhip_kv_store_dev(
-            self.handle, ctypes.byref(cache.desc), kv.ptr + kv_offset, cache.width if kv_stride is None else kv_stride,
-            None if norm_weight is None else norm_weight.ptr, eps, None if rope is None else rope.handle,
-            None if positions is None else positions.ptr, slots.ptr, n_tokens), "mmhip_kv_store_dev")
+            self.handle, ctypes.byref(cache.checked()), kv.ptr + kv_offset,
+            cache.width if kv_stride is None else kv_stride, _optional(norm_weight), eps,
+            None if rope is None else rope.checked(), _optional(positions), slots.ptr, n_tokens), "mmhip_kv_store_dev")
 
     def mla_attention_workspace(self, n_tokens: int, n_heads: int, rank: int) -> int:
         return self.lib.mmhip_mla_attention_workspace(self.handle, n_tokens, n_heads, rank)
@@ -504,18 +513,18 @@ class Context:
         """The mmhip_mla_attention that mla_attention_dev takes (built once, reusable; it keeps the buffers alive).
         Strides are (token, head) in floats, by default those of contiguous [n_tokens][n_heads][row]; offsets are in
         bytes."""
-        d = cache.desc
+        d = cache.checked()
         a = MlaAttention()
         a.cache = d
         a.q_dev, a.out_dev = q.ptr + q_offset, out.ptr + out_offset
-        a.q_pe_dev = None if q_pe is None else q_pe.ptr + q_pe_offset
-        a.lse_dev = None if lse is None else lse.ptr
+        a.q_pe_dev = None if q_pe is None else _optional(q_pe) + q_pe_offset
+        a.lse_dev = _optional(lse)
         a.q_token_stride, a.q_head_stride = q_strides or (n_heads * d.rank, d.rank)
         a.q_pe_token_stride, a.q_pe_head_stride = q_pe_strides or (n_heads * d.rope_dims, d.rope_dims)
         a.out_token_stride, a.out_head_stride = out_strides or (n_heads * d.rank, d.rank)
         a.tables_dev, a.table_stride = tables.ptr, table_pages if table_stride is None else table_stride
         a.n_tables, a.table_pages = n_tables, table_pages
-        a.table_of_dev = None if table_of is None else table_of.ptr
+        a.table_of_dev = _optional(table_of)
         a.lens_dev, a.n_tokens, a.n_heads, a.scale = lens.ptr, n_tokens, n_heads, scale
         a.workspace_dev, a.workspace_bytes = workspace.ptr, workspace.nbytes
         a._keep = (cache, q, q_pe, out, lse, tables, table_of, lens, workspace)
@@ -532,7 +541,7 @@ class Context:
                      n_given: int = 0, token_logprobs=None, entropy=None, top: int = 0, top_ids=None,
                      top_logprobs=None, workspace=None):
         """mmhip_logprobs_dev: log probabilities of the given tokens, entropy and the largest alternatives."""
-        p = [None if b is None else b.ptr for b in (tokens, token_logprobs, entropy, top_ids, top_logprobs, workspace)]
+        p = [_optional(b) for b in (tokens, token_logprobs, entropy, top_ids, top_logprobs, workspace)]
         check(self.lib.mmhip_logprobs_dev(self.handle, logits.ptr, vocab if stride is None else stride, n_rows, vocab,
                                           p[0], n_given, p[1], p[2], top, p[3], p[4], p[5],
                                           0 if workspace is None else workspace.nbytes), "mmhip_logprobs_dev")
@@ -566,6 +575,12 @@ class Rope:
         check(ctx.lib.mmhip_rope_create(ctx.handle, ctypes.byref(self.params), ctypes.byref(h)), "mmhip_rope_create")
         self.handle = h.value
 
+    def checked(self) -> int:
+        """The handle; a freed plan is refused (a null one would stand for no rotation)."""
+        if not self.handle:
+            raise MmhipError("rope", ERR_INVALID, "the rotary plan was freed")
+        return self.handle
+
     def free(self):
         if self.handle:
             self.ctx.lib.mmhip_rope_destroy(self.ctx.handle, self.handle)
@@ -579,6 +594,12 @@ class KvCache:
         self.pool = pool
         self.desc = KvCacheDesc(pool.ptr, ggml_type, rank, rope_dims, page_tokens, n_pages)
         self.width = rank + rope_dims
+
+    def checked(self) -> KvCacheDesc:
+        """The description; a freed pool is refused."""
+        if self.pool.ptr is None:
+            raise MmhipError("kv cache", ERR_INVALID, "the pool was freed")
+        return self.desc
 
     @staticmethod
     def page_bytes(ggml_type: int, rank: int, rope_dims: int, page_tokens: int) -> int:
