@@ -342,8 +342,9 @@ int mmhip_qmm_dev_noalloc(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat,
  *     s = x + residual                      (s = x where residual_dev is NULL)
  *     y = (s * r) * weight,  r = 1 / sqrt(mean(s^2) + eps)
  * s and the two products are f32 operations; the sum of squares and r are
- * computed in 64 bits and r is rounded to f32 once, so a row's result does not
- * depend on how its sum was split. sum_dev (NULL: not wanted) receives s, the
+ * computed in 64 bits and r is rounded to f32 once. The sum's order depends on
+ * cols alone, so a row's bits depend on its values, not on the other rows,
+ * strides, alignment or y_type. sum_dev (NULL: not wanted) receives s, the
  * next residual. y_type: MMHIP_TYPE_F32, MMHIP_TYPE_F16 (rounded to nearest
  * even), or MMHIP_TYPE_Q8_0 (ceil(cols / 32) blocks of 34 bytes per row, the
  * rows back to back, each block as mmhip_quantize_q8_0 gives it; y_dev 2-byte
@@ -453,10 +454,11 @@ int mmhip_kv_store_dev(mmhip_ctx* ctx, const mmhip_kv_cache* cache, const float*
  * the matrix cores as two f16 parts each that hold all of their 24 bits (down to
  * 2^-38 of a head's largest query and 2^-40 of a probability), cached values
  * exactly.
- * Queries beyond 1e30 in size or not finite give NaN. Infinite cached values
- * follow the formula: a score of -infinity drops its position like a mask (a
- * latent one still leaves NaN in its own column, 0 times infinity), one of
- * +infinity or NaN gives NaN. The work is split
+ * Finite queries may have any size; one that is not finite gives NaN.
+ * Infinite cached values, and scores beyond f32's range, follow the formula: a
+ * score of -infinity drops its position like a mask (a latent value still leaves
+ * NaN in its own column, 0 times infinity), one of +infinity or NaN gives NaN.
+ * Outputs and workspace overlap neither the inputs nor each other. The work is split
  * over the positions and joined, in an order that depends on the call's
  * shape and lengths alone, so a call repeated gives the same bits. */
 typedef struct {
@@ -494,7 +496,8 @@ int mmhip_mla_attention_dev(mmhip_ctx* ctx, const mmhip_mla_attention* args);
  * reported (above). n_given may be 0 (tokens and their outputs unused), and
  * so may top (ids and log probabilities unused; top_logprobs_dev may be NULL
  * too); entropy_dev may be NULL. top <= MMHIP_LOGPROBS_MAX_TOP, top <= vocab,
- * 1 <= vocab < 2^31, n_given < 2^31. Outputs are contiguous. */
+ * 1 <= vocab < 2^31, n_given < 2^31. Outputs are contiguous; they and the
+ * workspace overlap neither the inputs nor each other. */
 #define MMHIP_LOGPROBS_MAX_TOP 32u
 uint64_t mmhip_logprobs_workspace(mmhip_ctx* ctx, uint64_t n_rows, uint64_t vocab, uint32_t top);
 int mmhip_logprobs_dev(mmhip_ctx* ctx, const float* logits_dev, uint64_t stride, uint64_t n_rows, uint64_t vocab,

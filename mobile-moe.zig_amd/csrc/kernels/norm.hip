@@ -5,9 +5,10 @@
 //
 // Norm: a row's sum of squares and the inverse root are in f64 and the root is
 // rounded to f32 once; every other operation is one f32 operation per value,
-// never contracted. So a value depends on its row alone, not on how threads
-// shared the sum, and the cache writer stores the bits that norm and codec
-// would give one after the other. The f64 sum costs a conversion and an FMA
+// never contracted. The sum's order depends on the width alone, and the cache
+// writer keeps it (both give thread t columns 4t .. 4t + 3, and rows end within
+// the first two waves), so it stores the bits that norm and codec would give one
+// after the other. The f64 sum costs a conversion and an FMA
 // per value, hidden behind the row's loads. 4099 rows of 2048 with a residual,
 // its sum and Q8_0 out: 18.5 us, 5.9 TB/s; one row 1.8 us.
 //

@@ -200,6 +200,23 @@ def test_attention_without_a_finite_score(ctx, ggml_type):
     assert np.isnan(out[0, 7:9]).all() and np.isnan(lse[0, 7:9]).all()
 
 
+# ---- sizes of queries -----------------------------------------------------
+
+@pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
+@pytest.mark.parametrize("size", [1e-30, 1e32, 1e36])
+def test_attention_query_sizes(ctx, ggml_type, size):
+    """Finite queries of any size, as long as the scores stay in f32's range."""
+    rng = np.random.default_rng(2)
+    pool = Pool(rng, ggml_type, 512, 64, 16, 8)
+    q, q_pe = (np.clip(a, -4, 4) for a in queries(rng, 2, 20, 512, 64))
+    q, q_pe = (a * np.float32(size) for a in (q, q_pe))
+    scale = float(np.float32(0.07 / size))
+    lens, tables = np.array([128, 77]), np.arange(8)[None]
+    ids = np.zeros(2, np.int64)
+    want = ref.attention64(q, q_pe, pool.values, tables, ids, lens, 16, scale, 512)
+    check_attention(*run_attention(ctx, pool, q, q_pe, tables, lens, scale, table_of=ids), *want)
+
+
 # ---- log probabilities ----------------------------------------------------
 
 def test_logprobs_have_no_side(ctx):
