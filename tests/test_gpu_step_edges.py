@@ -217,6 +217,45 @@ def test_attention_query_sizes(ctx, ggml_type, size):
     check_attention(*run_attention(ctx, pool, q, q_pe, tables, lens, scale, table_of=ids), *want)
 
 
+# ---- every kernel ---------------------------------------------------------
+
+@pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
+@pytest.mark.parametrize("heads", [17, 24, 33, 70])
+@pytest.mark.parametrize("rank,pe,pt", [(512, 0, 16), (512, 32, 32), (480, 64, 16), (256, 32, 64), (96, 0, 16), (32, 64, 16)])
+def test_attention_sizes_and_heads(ctx, ggml_type, heads, rank, pe, pt):
+    """Two product tiles, a packed one, several head tiles, each at ranks and rotary parts that leave waves partly or
+    wholly without columns; a table per token, and one table of all (which f16 rows are read otherwise for)."""
+    rng = np.random.default_rng(heads + rank + pe)
+    lens = np.array([77, 0, 300, 1, 160])
+    n_pages = int(((lens + pt - 1) // pt).sum()) + 1
+    pool = Pool(rng, ggml_type, rank, pe, pt, n_pages)
+    q, q_pe = queries(rng, 5, heads, rank, pe)
+    scale = (rank + pe) ** -0.5 * 1.5
+    tables = tables_for(rng, lens, pt, n_pages, more=0)
+    want = ref.attention64(q, q_pe, pool.values, tables, np.arange(5), lens, pt, scale, rank)
+    check_attention(*run_attention(ctx, pool, q, q_pe, tables, lens, scale, pad=3), *want)
+    tables, rows = tables[2:3], np.zeros(5, np.int64)
+    want = ref.attention64(q, q_pe, pool.values, tables, rows, lens, pt, scale, rank)
+    check_attention(*run_attention(ctx, pool, q, q_pe, tables, lens, scale, table_of=rows), *want)
+
+
+@pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
+@pytest.mark.parametrize("heads,rank,pe", [(20, 512, 64), (40, 512, 64), (20, 512, 32), (40, 96, 32)])
+@pytest.mark.parametrize("n", [65, 300])
+def test_attention_many_tokens_and_heads(ctx, ggml_type, heads, rank, pe, n):
+    """More tokens than a wave has lanes (and than a workgroup has threads), with a packed tile and with two head tiles."""
+    rng = np.random.default_rng(n + heads)
+    pt, n_pages = 16, 300
+    lens = np.where(rng.random(n) < 0.2, 0, np.exp(rng.uniform(0, np.log(150), n)).astype(np.int64))
+    lens[::41] = 700
+    pool = Pool(rng, ggml_type, rank, pe, pt, n_pages)
+    tables = rng.integers(0, n_pages, (20, 44)).astype(np.int32)
+    rows = rng.integers(0, 20, n)
+    q, q_pe = queries(rng, n, heads, rank, pe)
+    want = ref.attention64(q, q_pe, pool.values, tables, rows, lens, pt, 0.08, rank)
+    check_attention(*run_attention(ctx, pool, q, q_pe, tables, lens, 0.08, table_of=rows), *want)
+
+
 # ---- log probabilities ----------------------------------------------------
 
 def test_logprobs_have_no_side(ctx):
@@ -232,3 +271,27 @@ def test_logprobs_have_no_side(ctx):
     lp, h = ref.logprobs64(x)
     assert (np.abs(got[0][:, 0] - lp[:, 5]) <= 6e-6).all()
     assert abs((got[0][:, 0] - lp[:, 5]).mean()) <= 0.5 * U, (got[0][:, 0] - lp[:, 5]).mean() / U
+
+
+# ---- two contexts ---------------------------------------------------------
+
+def test_two_contexts_as_each_alone(mm, ctx):
+    """Each context's step from its own run, finished before the other begins: the bits of both queued together."""
+    from test_gpu_step_ops import Step
+    with mm.Context(0) as other, Buffers(ctx) as d, Buffers(other) as e:
+        pair = [Step(ctx, d, np.random.default_rng(5), mm.F16, [3000, 17, 900, 1300] * 8),
+                Step(other, e, np.random.default_rng(6), mm.Q8_0, [2500, 64, 1, 800] * 8)]
+        alone = []
+        for i, s in enumerate(pair):
+            s.fill(np.random.default_rng(40 + i))
+            s.run()
+            alone.append(s.results())
+        for i, s in enumerate(pair):
+            s.fill(np.random.default_rng(40 + i))
+        for s in pair:
+            s.run()
+        for s, want in zip(pair, alone):
+            got = s.results()
+            for k in got:
+                same_bits(got[k], want[k])
+            s.rope.free()
