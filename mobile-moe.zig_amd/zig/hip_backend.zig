@@ -370,6 +370,12 @@ pub const HipBackend = struct {
         try check(mmhip_rms_norm_dev(self.ctx, @ptrCast(y_dev), 0, cols, sum_dev, cols, x_dev, cols, residual_dev, cols, weight_dev, n_rows, cols, eps));
     }
 
+    /// The same for rows any stride apart (in elements), to f32, f16 or Q8_0
+    /// blocks (y_type 0, 1, 8).
+    pub fn rmsNormRowsDev(self: *Self, y_dev: *anyopaque, y_type: u32, y_stride: u64, sum_dev: ?[*]f32, sum_stride: u64, x_dev: [*]const f32, x_stride: u64, residual_dev: ?[*]const f32, residual_stride: u64, weight_dev: [*]const f32, n_rows: u64, cols: u32, eps: f32) !void {
+        try check(mmhip_rms_norm_dev(self.ctx, y_dev, y_type, y_stride, sum_dev, sum_stride, x_dev, x_stride, residual_dev, residual_stride, weight_dev, n_rows, cols, eps));
+    }
+
     /// RoPECache's role (math.zig:197-240): frequencies kept on the device.
     pub fn createRope(self: *Self, params: RopeParams) !*RopeHandle {
         var h: ?*RopeHandle = null;
@@ -386,6 +392,23 @@ pub const HipBackend = struct {
     pub fn ropeDev(self: *Self, rope: *const RopeHandle, x_dev: [*]f32, positions_dev: [*]const u32, n_tokens: u64, n_heads: u32, head_dim: u32, first: u32) !void {
         const row: u64 = @as(u64, n_heads) * head_dim;
         try check(mmhip_rope_dev(self.ctx, rope, x_dev, row, head_dim, x_dev, row, head_dim, positions_dev, n_tokens, n_heads, head_dim, first));
+    }
+
+    /// The same from one buffer to another, heads and tokens any strides apart
+    /// (in floats).
+    pub fn ropeRowsDev(self: *Self, rope: *const RopeHandle, y_dev: [*]f32, y_token_stride: u64, y_head_stride: u64, x_dev: [*]const f32, x_token_stride: u64, x_head_stride: u64, positions_dev: [*]const u32, n_tokens: u64, n_heads: u32, head_dim: u32, first: u32) !void {
+        try check(mmhip_rope_dev(self.ctx, rope, y_dev, y_token_stride, y_head_stride, x_dev, x_token_stride, x_head_stride, positions_dev, n_tokens, n_heads, head_dim, first));
+    }
+
+    /// Radians per position of each of dims / 2 pairs, and the magnitude; host
+    /// only.
+    pub fn ropeFrequencies(params: *const RopeParams, out: [*]f64, magnitude: *f64) !void {
+        try check(mmhip_rope_frequencies(params, out, magnitude));
+    }
+
+    /// Bytes of one page; 0 if such a cache is not supported.
+    pub fn kvPageBytes(cache: *const LatentCache) u64 {
+        return mmhip_kv_page_bytes(cache);
     }
 
     /// KVCache.put (kv_cache.zig:279-362) for n_tokens positions: kv_a's rows
@@ -408,6 +431,11 @@ pub const HipBackend = struct {
     /// the entropy, for contiguous rows of device logits.
     pub fn logprobsDev(self: *Self, logits_dev: [*]const f32, n_rows: u64, vocab: u64, tokens_dev: ?[*]const u32, n_given: u64, token_logprobs_dev: ?[*]f32, entropy_dev: ?[*]f32, top: u32, top_ids_dev: ?[*]u32, top_logprobs_dev: ?[*]f32, workspace_dev: ?*anyopaque, workspace_bytes: u64) !void {
         try check(mmhip_logprobs_dev(self.ctx, logits_dev, vocab, n_rows, vocab, tokens_dev, n_given, token_logprobs_dev, entropy_dev, top, top_ids_dev, top_logprobs_dev, workspace_dev, workspace_bytes));
+    }
+
+    /// The same for rows of logits any stride apart (in floats).
+    pub fn logprobsRowsDev(self: *Self, logits_dev: [*]const f32, stride: u64, n_rows: u64, vocab: u64, tokens_dev: ?[*]const u32, n_given: u64, token_logprobs_dev: ?[*]f32, entropy_dev: ?[*]f32, top: u32, top_ids_dev: ?[*]u32, top_logprobs_dev: ?[*]f32, workspace_dev: ?*anyopaque, workspace_bytes: u64) !void {
+        try check(mmhip_logprobs_dev(self.ctx, logits_dev, stride, n_rows, vocab, tokens_dev, n_given, token_logprobs_dev, entropy_dev, top, top_ids_dev, top_logprobs_dev, workspace_dev, workspace_bytes));
     }
 
     pub fn logprobsWorkspace(self: *Self, n_rows: u64, vocab: u64, top: u32) u64 {
