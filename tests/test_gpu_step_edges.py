@@ -8,7 +8,7 @@ import pytest
 
 import mmhip as mm
 import step_reference as ref
-from step_reference import Buffers, Pool, U
+from step_reference import Buffers, Graph, Pool, U
 from test_gpu_step_ops import check_attention, f32, queries, run_attention, run_logprobs, same_bits, tables_for
 
 pytestmark = pytest.mark.gpu
@@ -295,3 +295,71 @@ def test_two_contexts_as_each_alone(mm, ctx):
             for k in got:
                 same_bits(got[k], want[k])
             s.rope.free()
+
+
+# ---- a captured batch of fixed size ---------------------------------------
+
+@pytest.mark.parametrize("ggml_type", [mm.F16, mm.Q8_0])
+@pytest.mark.parametrize("n", [5, 70])
+def test_captured_batch_with_other_sequences(ctx, ggml_type, n):
+    """A captured cache write and attention, replayed with other slots, tables, lengths, positions and padding, the
+    program's own calls between the replays: the bits of the calls made one by one, and the formula's values."""
+    rng = np.random.default_rng(n)
+    pt, pages_each, heads = 16, 40, 20
+    n_pages = n * pages_each
+    pool = Pool(rng, ggml_type, 512, 64, pt, n_pages)
+    rope = mm.Rope(ctx, dims=64, base=1e6)
+    with Buffers(ctx) as d:
+        sides = []
+        for _ in range(2):
+            b = dict(pool=d.put(pool.bytes), kv=d.new(n * 576 * 4), slots=d.new(n * 4), pos=d.new(n * 4), lens=d.new(n * 4),
+                     tables=d.new(n * pages_each * 4), q=d.new(n * heads * 512 * 4), q_pe=d.new(n * heads * 64 * 4),
+                     out=d.new(n * heads * 512 * 4), lse=d.new(n * heads * 4),
+                     work=d.new(ctx.mla_attention_workspace(n, heads, 512)))
+            cache = mm.KvCache(b["pool"], ggml_type, rank=512, rope_dims=64, page_tokens=pt, n_pages=n_pages)
+            args = ctx.mla_attention_args(cache, q=b["q"], q_pe=b["q_pe"], out=b["out"], lse=b["lse"], lens=b["lens"],
+                                          tables=b["tables"], n_tables=n, table_pages=pages_each, n_tokens=n,
+                                          n_heads=heads, scale=0.07, workspace=b["work"])
+            sides.append((b, cache, args))
+
+        def fill(b, seed):
+            g = np.random.default_rng(seed)
+            lens = np.where(g.random(n) < 0.3, 0, np.exp(g.uniform(0, np.log(pages_each * pt), n))).astype(np.uint32)
+            tables = g.permutation(n_pages).reshape(n, pages_each).astype(np.int32)
+            last = np.maximum(lens.astype(np.int64) - 1, 0)
+            slots = np.where(lens > 0, tables[np.arange(n), last // pt] * pt + last % pt, -1).astype(np.int32)
+            x = dict(kv=g.standard_normal((n, 576)), q=g.standard_normal((n, heads, 512)), q_pe=g.standard_normal((n, heads, 64)))
+            x = {k: v.astype(np.float32) for k, v in x.items()}
+            x.update(slots=slots, pos=last.astype(np.uint32), lens=lens, tables=tables)
+            for k, v in x.items():
+                mm.check(ctx.lib.mmhip_memcpy_h2d(ctx.handle, b[k].ptr, v.ctypes.data, v.nbytes), "h2d")
+            return x
+
+        def run(side):
+            b, cache, args = side
+            ctx.kv_store_dev(cache, b["kv"], b["slots"], n, rope=rope, positions=b["pos"])
+            ctx.mla_attention_dev(args)
+
+        fill(sides[0][0], 0)
+        fill(sides[1][0], 0)
+        for side in sides:
+            run(side)  # the kernels are loaded outside the capture
+        ctx.synchronize()
+        g = Graph(ctx, lambda: run(sides[0]))
+        try:
+            for seed in (1, 2, 3):
+                x = [fill(b, seed) for b, _, _ in sides][0]
+                g.replay()
+                run(sides[1])
+                ctx.synchronize()
+                got = [[b["out"].to_numpy(np.float32, n * heads * 512), b["lse"].to_numpy(np.float32, n * heads),
+                        b["pool"].to_numpy(np.uint8, pool.bytes.size)] for b, _, _ in sides]
+                for a, c in zip(*got):
+                    same_bits(a, c)
+                pool.bytes = got[0][2].reshape(pool.bytes.shape).copy()
+                revalue(pool)
+                want = ref.attention64(x["q"], x["q_pe"], pool.values, x["tables"], np.arange(n), x["lens"], pt, 0.07, 512)
+                check_attention(got[0][0].reshape(n, heads, 512), got[0][1].reshape(n, heads), *want)
+        finally:
+            g.free()
+            rope.free()
