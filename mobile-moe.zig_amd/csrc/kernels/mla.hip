@@ -675,16 +675,16 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
             for (uint32_t c = 0; c < 4; ++c) read_values(c);
             __builtin_amdgcn_sched_barrier(0);
             if (softmax) {
-                vper x = ((part[0] + part[1]) + part[2]) + part[3];
                 const uint32_t lv = mask >> spos;
-#pragma unroll
-                for (uint32_t e = 0; e < kPer; ++e) x[e] = (lv >> e) & 1 ? x[e] * fac : -INFINITY;
                 const float m_was = m_run, l_was = l_run;
-                float sum;
-                const auto weigh = [&](vper x) {  // (gives the lane's own sum)
-                    float top = x[0];
+                // Scores to probabilities; the lane's own sum.
+                const auto weigh = [&](vper x) {
+                    float top = -INFINITY;
 #pragma unroll
-                    for (uint32_t e = 1; e < kPer; ++e) top = fmaxf(top, x[e]);
+                    for (uint32_t e = 0; e < kPer; ++e) {
+                        x[e] = (lv >> e) & 1 ? x[e] : -INFINITY;
+                        top = fmaxf(top, x[e]);
+                    }
                     top = group_max<kLanes>(top);
                     const float m_new = fmaxf(m_was, top), base = m_new == -INFINITY ? 0.0f : m_new;
                     const float al = __builtin_amdgcn_exp2f(m_was - base);
@@ -694,8 +694,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                         x[e] = __builtin_amdgcn_exp2f(x[e] - base);
                         own += x[e];
                     }
-                    sum = group_sum<kLanes>(own);
-                    l_run = l_was * al + sum;
+                    l_run = l_was * al + group_sum<kLanes>(own);
                     m_run = m_new;
                     if (ln % kLanes == 0) s.alpha[srow] = al;
                     // position 16 h + 4 g + e is O^T's operand element 4 h + e of group g;
@@ -716,39 +715,39 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                     }
                     return own;
                 };
-                const float own = weigh(x);
+                const float own = weigh((((part[0] + part[1]) + part[2]) + part[3]) * fac);
                 // NaN: an infinite cached value met a part of the query that is 0
                 // or of the other sign, where the formula has an infinity, or the
                 // formula has NaN too. Such scores again, from the slices of all
                 // waves; the terms that are not finite decide. (A query that is not
                 // finite gives NaN.)
-                if (__any(own != own) && sum != sum) {  // (alike for a head's lanes)
-                    const uint32_t h = min(head0 + from, a.n_heads - 1), t = afresh(token);
-                    const float* q = a.q + (uint64_t)t * a.q_token_stride + (uint64_t)h * a.q_head_stride;
-                    const float* q_pe = a.q_pe + (uint64_t)t * a.q_pe_token_stride + (uint64_t)h * a.q_pe_head_stride;
+                if (__builtin_expect(__any(own != own), 0)) {
+                    if (__builtin_expect(group_max<kLanes>(own != own ? 1.0f : 0.0f) > 0.0f, 0)) {  // alike for a head's lanes
+                        const uint32_t h = min(head0 + from, a.n_heads - 1), t = afresh(token);
+                        const float* q = a.q + (uint64_t)t * a.q_token_stride + (uint64_t)h * a.q_head_stride;
+                        const float* q_pe = a.q_pe + (uint64_t)t * a.q_pe_token_stride + (uint64_t)h * a.q_pe_head_stride;
 #pragma unroll 1
-                    for (uint32_t p = spos; p < spos + kPer; ++p) {
-                        float score = (((s.sp[0][from][p] + s.sp[1][from][p]) + s.sp[2][from][p]) + s.sp[3][from][p]) * fac;
-                        if (score != score) {
-                            score = 0.0f;
+                        for (uint32_t p = spos; p < spos + kPer; ++p) {
+                            float score = (((s.sp[0][from][p] + s.sp[1][from][p]) + s.sp[2][from][p]) + s.sp[3][from][p]) * fac;
+                            if (score != score) {
+                                score = 0.0f;
 #pragma unroll 1
-                            for (uint32_t c = 0; c < g.width; ++c) {
-                                const bool pe = c >= g.rank;
-                                const uint32_t i = pe ? c - g.rank : c, w = pe ? i / kMlaPe : i / kMlaCols;
-                                const uint32_t j = pe ? i % kMlaPe : i % kMlaCols;
-                                const uint8_t* at = pe ? s.pe[w] + p * 32 + 2 * j : s.kv[w] + p * 256 + (((j >> 3) ^ (p & 15)) << 4) + 2 * (j & 7);
-                                float k = (float)*reinterpret_cast<const _Float16*>(at);
-                                if constexpr (Q8) k *= s.ds[w][pe ? 4 : j / 32][p];
-                                const float x = pe ? q_pe[i] : q[i];
-                                score += (fabsf(k) < INFINITY ? 0.0f : x * k) + (x - x);
+                                for (uint32_t c = 0; c < g.width; ++c) {
+                                    const bool pe = c >= g.rank;
+                                    const uint32_t i = pe ? c - g.rank : c, w = pe ? i / kMlaPe : i / kMlaCols;
+                                    const uint32_t j = pe ? i % kMlaPe : i % kMlaCols;
+                                    const uint8_t* at = pe ? s.pe[w] + p * 32 + 2 * j : s.kv[w] + p * 256 + (((j >> 3) ^ (p & 15)) << 4) + 2 * (j & 7);
+                                    float k = (float)*reinterpret_cast<const _Float16*>(at);
+                                    if constexpr (Q8) k *= s.ds[w][pe ? 4 : j / 32][p];
+                                    const float x = pe ? q_pe[i] : q[i];
+                                    score += (fabsf(k) < INFINITY ? 0.0f : x * k) + (x - x);
+                                }
+                                score *= a.scale;
                             }
-                            score *= a.scale;
+                            s.sp[0][from][p] = score;
                         }
-                        s.sp[0][from][p] = score;
+                        (void)weigh(*reinterpret_cast<const vper*>(&s.sp[0][from][spos]));
                     }
-#pragma unroll
-                    for (uint32_t e = 0; e < kPer; ++e) x[e] = (lv >> e) & 1 ? s.sp[0][from][spos + e] : -INFINITY;
-                    (void)weigh(x);
                 }
             }
             lds_barrier();
@@ -825,7 +824,7 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 // The blocks of large scales, into sums 2^-9 as large. (Places are
                 // formed anew: kept from above they would cost the general kernels
                 // 8 more spilled registers and a tenth of their speed.)
-                if (Q8 && big) {
+                if (Q8 && __builtin_expect(big != 0, 0)) {
                     const uint32_t ln = afresh(lane), at = value_place(ln), d_at = 4 * (ln >> 4);
 #pragma unroll
                     for (uint32_t c = 0; c < 8; ++c) {
