@@ -9,8 +9,8 @@
 // launch leaves every piece's (m, s, t) and its `top` largest logits in the
 // workspace, the second joins a row's pieces. Sums are taken in a fixed order:
 // nothing but the row and the number of rows decides an output. One row of
-// 154880, top 20: 7.5 us and 4.9; 64 rows, top 5: 16.2 and 4.5 (11 and 3.9
-// without the largest, 3.5 TB/s).
+// 154880, top 20: 7.4 us and 5.3; 64 rows, top 5: 16.5 and 4.6 (a call 21, without
+// the largest 12.5).
 //
 // The largest logits are keys of 64 bits (rank_key) that no two logits share,
 // so their order is total and the order in which candidates are found does not

@@ -16,9 +16,10 @@
 // What bounds it: with long contexts in f16, HBM (131072 positions of one token
 // 38 us, 4.0 TB/s, and 13 for the join of its pieces; 64 times 4096 73 us, 4.1
 // TB/s). Otherwise a wave's chain through a tile, about 5000 cycles with two
-// workgroups on a CU: 64 ragged contexts up to 16384 in Q8_0 54 us, 256 tokens
-// over the same 4096 positions in f16 158 us (matrix cores busy 30% of the
-// time, LDS 41%). One short context: two launches, 16 us.
+// workgroups on a CU: 64 ragged contexts up to 16384 in Q8_0 43 to 55 us by their
+// lengths, 256 tokens over the same 4096 positions in f16 162 us, in Q8_0 223
+// (f16: matrix cores busy 31% of the time, LDS 42%). One short context: two
+// launches, 16 us.
 //
 // A workgroup is four waves and takes tiles of 32 positions. Wave w owns the
 // latent columns 128 w .. 128 w + 127 and 16 of the rotary ones, both as keys
@@ -46,8 +47,9 @@
 //
 // Work is cut evenly, whatever the lengths: the tiles of all tokens and head
 // tiles form one list, of which every workgroup takes an equal run, two
-// workgroups per CU (one: 64 ragged contexts in Q8_0 69 us instead of 57). A run may end inside a token; such pieces leave their
-// sums in the workspace and mla_join_kernel adds them in the list's order.
+// workgroups per CU (one: 64 ragged contexts in Q8_0 69 us instead of 57). A run
+// may end inside a token; such pieces leave their sums in the workspace and
+// mla_join_kernel adds them in the list's order.
 #include "device_common.hpp"
 #include "kernels.hpp"
 #include "lanes.hpp"
@@ -102,8 +104,9 @@ struct MlaLds {
 __device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (uint32_t)(((uint64_t)len + kMlaTile - 1) / kMlaTile); }
 // An item's slots of the list that is cut evenly: its tiles, behind slots that
 // stand for its queries' conversion and its result. (64 ragged contexts 57 us
-// instead of 71; 64 times 4096, whose pieces ended with the sequences before, 76
-// instead of 71.)
+// instead of 71. Equal lengths lose: 64 times 4096, whose pieces ended with the
+// sequences before, 76 instead of 71, and one token at 131072 positions has runs
+// of 9 tiles where 8 would do.)
 constexpr uint32_t kItemSlots = 3;
 __device__ __forceinline__ uint32_t slots_of(uint32_t len) { return len ? tiles_of(len) + kItemSlots : 0; }
 

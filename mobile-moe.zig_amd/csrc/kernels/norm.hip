@@ -16,8 +16,9 @@
 // 19.2 us, 6.6 TB/s; one token 2.3 us. The angles' 64-bit arithmetic is a
 // wave's work per token and runs while the other values are copied.
 //
-// Cache writer: 4096 positions to Q8_0 8 us, 1.5 TB/s: a workgroup's chain of
-// slot, row, angles, sum and root is longer than its bytes; 64 positions 3 us.
+// Cache writer: 4096 positions to Q8_0 7.2 us a call, 1.7 TB/s: a workgroup's
+// chain of slot, row, angles, sum and root is longer than its bytes; 64 positions
+// 3 us.
 #include "device_common.hpp"
 #include "kernels.hpp"
 #include "lanes.hpp"
@@ -45,8 +46,11 @@ __device__ __forceinline__ void load4(float (&v)[4], const float* p, uint32_t c,
 }
 // Stores past the caches: lines left in L2 are written back at the launch's end
 // (norm of 4099 rows 21.9 -> 18.5 us, rotary positions of 4096 tokens 27.1 ->
-// 19.2 us, whole calls; loads past them as well: 21.7 and 23.7). A wave's stores
-// fill whole lines.
+// 19.2 us, whole calls; loads past them as well: 21.7 and 23.7). A reader right
+// behind takes back what it saves: norm to f32 and the product of its rows with
+// 1344 Q8_0 columns, ordinary stores against these, 256 rows 15.8 / 16.1 us, 2048
+// rows 77.5 / 76.6, 4099 rows 142.9 / 143.3; rotation and a norm of the whole
+// rows, 4096 tokens, 48.1 / 48.9. A wave's stores fill whole lines.
 __device__ __forceinline__ void stream4(float* p, float a, float b, float c, float d) {
     typedef float f4 __attribute__((ext_vector_type(4)));
     __builtin_nontemporal_store((f4){a, b, c, d}, reinterpret_cast<f4*>(p));
@@ -424,8 +428,8 @@ hipError_t launch_rope(const RopeArgs& a, uint64_t n_tokens, hipStream_t s) {
     const bool vec = a.dims % 8 == 0 && a.first % 4 == 0 && a.head_dim % 4 == 0 && aligned16(a.x) && aligned16(a.y) &&
                      a.x_token_stride % 4 == 0 && a.x_head_stride % 4 == 0 && a.y_token_stride % 4 == 0 &&
                      a.y_head_stride % 4 == 0;
-    // (4096 tokens of 20 heads of 192 with ordinary stores:
-    // 21.4 us; pair by pair 30.5)
+    // (The kernel alone, 4096 tokens of 20 heads of 192, with ordinary stores:
+    // 21.4 us; pair by pair 30.5.)
     if (vec) rope_kernel<4><<<(unsigned)n_tokens, kRopeThreads, 0, s>>>(a);
     else rope_kernel<1><<<(unsigned)n_tokens, kRopeThreads, 0, s>>>(a);
     return hipGetLastError();
