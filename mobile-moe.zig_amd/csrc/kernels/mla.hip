@@ -721,33 +721,37 @@ __global__ __launch_bounds__(kMlaThreads, 2) void mla_split_kernel(MlaArgs a, Ml
                 const float own = weigh((((part[0] + part[1]) + part[2]) + part[3]) * fac);
                 // NaN: an infinite cached value met a part of the query that is 0
                 // or of the other sign, where the formula has an infinity, or the
-                // formula has NaN too. Such scores again, from the slices of all
-                // waves; the terms that are not finite decide. (A query that is not
-                // finite gives NaN.)
+                // formula has NaN too. Such scores again, a head's lanes sharing the
+                // columns of all waves' slices; the terms that are not finite
+                // decide. (A query that is not finite gives NaN.)
                 if (__builtin_expect(__any(own != own), 0)) {
                     if (__builtin_expect(group_max<kLanes>(own != own ? 1.0f : 0.0f) > 0.0f, 0)) {  // alike for a head's lanes
-                        const uint32_t h = min(head0 + from, a.n_heads - 1), t = afresh(token);
+                        const uint32_t h = min(head0 + from, a.n_heads - 1), t = afresh(token), c0 = ln % kLanes;
                         const float* q = a.q + (uint64_t)t * a.q_token_stride + (uint64_t)h * a.q_head_stride;
                         const float* q_pe = a.q_pe + (uint64_t)t * a.q_pe_token_stride + (uint64_t)h * a.q_pe_head_stride;
+                        const auto query = [&](uint32_t c) { return c < g.rank ? q[c] : q_pe[c - g.rank]; };
+                        float none = 0.0f;
+#pragma unroll 4
+                        for (uint32_t c = c0; c < g.width; c += kLanes) none += query(c) - query(c);
+                        none = group_sum<kLanes>(none);
 #pragma unroll 1
-                        for (uint32_t p = spos; p < spos + kPer; ++p) {
+                        for (uint32_t p = 0; p < kMlaTile; ++p) {
                             float score = (((s.sp[0][from][p] + s.sp[1][from][p]) + s.sp[2][from][p]) + s.sp[3][from][p]) * fac;
-                            if (score != score) {
+                            if (score != score && none == 0.0f) {
                                 score = 0.0f;
 #pragma unroll 1
-                                for (uint32_t c = 0; c < g.width; ++c) {
+                                for (uint32_t c = c0; c < g.width; c += kLanes) {
                                     const bool pe = c >= g.rank;
                                     const uint32_t i = pe ? c - g.rank : c, w = pe ? i / kMlaPe : i / kMlaCols;
                                     const uint32_t j = pe ? i % kMlaPe : i % kMlaCols;
                                     const uint8_t* at = pe ? s.pe[w] + p * 32 + 2 * j : s.kv[w] + p * 256 + (((j >> 3) ^ (p & 15)) << 4) + 2 * (j & 7);
                                     float k = (float)*reinterpret_cast<const _Float16*>(at);
                                     if constexpr (Q8) k *= s.ds[w][pe ? 4 : j / 32][p];
-                                    const float x = pe ? q_pe[i] : q[i];
-                                    score += (fabsf(k) < INFINITY ? 0.0f : x * k) + (x - x);
+                                    if (!(fabsf(k) < INFINITY)) score += query(c) * k;
                                 }
-                                score *= a.scale;
+                                score = group_sum<kLanes>(score) * a.scale;
                             }
-                            s.sp[0][from][p] = score;
+                            if (c0 == 0) s.sp[0][from][p] = score;
                         }
                         (void)weigh(*reinterpret_cast<const vper*>(&s.sp[0][from][spos]));
                     }
