@@ -387,6 +387,9 @@ typedef struct {
     float magnitude;
 } mmhip_rope_params;
 typedef struct mmhip_rope mmhip_rope;
+/* Every context of ctx's device can use the plan. It waits for ctx's stream
+ * before it goes; work of other contexts and captured graphs that use it must
+ * have ended by then. */
 int mmhip_rope_create(mmhip_ctx* ctx, const mmhip_rope_params* params, mmhip_rope** out_rope);
 void mmhip_rope_destroy(mmhip_ctx* ctx, mmhip_rope* rope);
 /* The frequency of each pair in radians per position (dims / 2 values) and the
