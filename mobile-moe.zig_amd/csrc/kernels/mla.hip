@@ -17,7 +17,7 @@
 // 38 us, 4.0 TB/s, and 13 for the join of its pieces; 64 times 4096 73 us, 4.1
 // TB/s). Otherwise a wave's chain through a tile, about 5000 cycles with two
 // workgroups on a CU: 64 ragged contexts up to 16384 in Q8_0 43 to 55 us by their
-// lengths, 256 tokens over the same 4096 positions in f16 162 us, in Q8_0 223
+// lengths, 256 tokens over the same 4096 positions in f16 162 to 168 us, in Q8_0 223
 // (f16: matrix cores busy 31% of the time, LDS 42%). One short context: two
 // launches, 16 us.
 //
