@@ -18,7 +18,12 @@
  * Tensor types use GgmlType ids (src/gguf.zig:21-56). Quantised weights are
  * passed as raw GGUF bytes: Q8_0 blocks {f16 d; i8 qs[32]} (34 B,
  * src/dequant.zig:372-377) and IQ2_XXS superblocks {f16 d; u16 qs[32]}
- * (66 B, src/dequant.zig:305-311), row-major, rows of ceil(cols/bs) blocks.
+ * (66 B, src/dequant.zig:305-311), row-major, rows of ceil(cols/bs) blocks;
+ * and 4-bit blocks of 32 weights {f16 d; u8 qs[16]} (18 B), the code of weight
+ * j < 16 in the lower half of qs[j], that of weight 16 + j in the upper half:
+ * Q4_0, (code - 8) * d, and IQ4_NL, d times entry `code` of -127 -104 -83 -65
+ * -49 -35 -22 -10 1 13 25 38 53 69 89 113. Rows of 4-bit weights hold whole
+ * blocks and fewer than 2^23 columns. MoE layers take Q8_0 and IQ2_XXS.
  * Uploading converts them once into the device tile layout the kernels read;
  * the bytes per block stay the same.
  *
@@ -49,8 +54,10 @@ extern "C" {
 /* ---- GgmlType ids (src/gguf.zig:21-56) ---- */
 #define MMHIP_TYPE_F32 0u
 #define MMHIP_TYPE_F16 1u
+#define MMHIP_TYPE_Q4_0 2u
 #define MMHIP_TYPE_Q8_0 8u
 #define MMHIP_TYPE_IQ2_XXS 16u
+#define MMHIP_TYPE_IQ4_NL 20u
 
 typedef struct mmhip_ctx mmhip_ctx;
 typedef struct mmhip_weight mmhip_weight;
@@ -80,8 +87,8 @@ void mmhip_destroy(mmhip_ctx* ctx);
  * (mmhip_moe_ffn_dev): MMHIP_ERR_HIP with the reason, once, and the status
  * is cleared. A caller that synchronises the raw stream from mmhip_stream()
  * instead never sees that error. Then it reports, as MMHIP_ERR_INVALID and
- * once, what a call of the operators between the products (below) met in
- * device data. */
+ * once, what a call of the operators between the products and at a step's
+ * ends (below) met in device data. */
 int mmhip_synchronize(mmhip_ctx* ctx);
 /* The context's hipStream_t, as an opaque pointer. */
 void* mmhip_stream(mmhip_ctx* ctx);
@@ -92,7 +99,8 @@ int mmhip_num_cu(mmhip_ctx* ctx);
  * stream around every launch of the hot kernels; mmhip_profile_read sums
  * them per kernel family ("gemv_q", "gemv_float", "qmm", "quantize",
  * "moe_router", "moe_route", "moe_quantize", "moe_gateup", "moe_down", "moe_decode",
- * "moe_combine", "rms_norm", "rope", "kv_store", "attention", "logprobs"). This fills the role
+ * "moe_combine", "rms_norm", "rope", "kv_store", "attention", "logprobs", "embed",
+ * "kv_plan", "sample"). This fills the role
  * of the per-op GPU timings the reference leaves empty
  * (op_perf_db.zig:88-97). Enabling resets the accumulators. */
 int mmhip_profile_enable(mmhip_ctx* ctx, int enable);
@@ -203,7 +211,7 @@ int mmhip_moe_layer_create_gguf(mmhip_ctx* ctx, const mmhip_gguf* g, uint32_t la
  *   dequant.dequantize (src/dequant.zig:632-659)
  * and OpenCLBackend.matMulQ8_0 (src/opencl_backend.zig:412-453). The weight
  * is uploaded on first use and kept resident, keyed by (ptr, type, shape).
- * Supported types: F32, F16, Q8_0, IQ2_XXS.
+ * Supported types: F32, F16, Q8_0, Q4_0, IQ4_NL, IQ2_XXS.
  * ====================================================================== */
 
 int mmhip_mat_vec_mul(mmhip_ctx* ctx, float* out_host, const void* ptr_host,
@@ -270,7 +278,7 @@ int mmhip_gemv_batched_dev(mmhip_ctx* ctx, const mmhip_weight* w,
                            float* y_dev, uint64_t y_stride);
 /* Several mmhip_gemv_batched_dev calls in ONE launch: each group is a range
  * of matrices of its own weight (weights may differ in shape, not in type;
- * Q8_0 or IQ2_XXS), with its own inputs and outputs (strides in floats, 0
+ * quantised ones), with its own inputs and outputs (strides in floats, 0
  * shares one input vector). No counterpart in the reference: it issues the
  * matVecMulUnified calls of a layer's experts (expertFFN,
  * inference.zig:1171-1185), e.g. the routed experts' gate/up [1536 x 2048]
@@ -507,6 +515,132 @@ int mmhip_logprobs_dev(mmhip_ctx* ctx, const float* logits_dev, uint64_t stride,
                        const uint32_t* tokens_dev, uint64_t n_given, float* token_logprobs_dev, float* entropy_dev,
                        uint32_t top, uint32_t* top_ids_dev, float* top_logprobs_dev, void* workspace_dev,
                        uint64_t workspace_bytes);
+
+/* ======================================================================
+ * The two ends of a decode step: a token's row of the embedding table, the
+ * pages, slots and positions of the step's tokens, and the next tokens drawn
+ * from the logits. They take the place of embedToken (src/inference.zig:388),
+ * of the block bookkeeping of KVCache and BatchScheduler
+ * (src/kv_cache.zig:24-141, src/batch_queue.zig:75-232) and of sampleGreedy
+ * (src/inference.zig:376-386) with a temperature and filters, so that a step's
+ * tokens lead to the next step's on the device. Asynchrony, graphs, workspaces
+ * and reports are those of the operators between the products (above). A token
+ * or row number of MMHIP_NO_TOKEN is not there: its outputs are left as they
+ * are.
+ * ====================================================================== */
+#define MMHIP_NO_TOKEN 0xFFFFFFFFu
+
+/* y[t] = scale * row tokens[t] of a table of `rows` rows of cols values, in
+ * device memory as raw GGUF bytes (F32, F16, Q8_0, Q4_0, IQ4_NL, IQ2_XXS; rows of
+ * tensorBytes(cols) bytes back to back; 2-byte aligned, F32 4-byte). A value is
+ * the exact f32 that mmhip_dequantize gives, times scale, rounded once. With an
+ * F32 table it gathers rows, e.g. the last hidden row of each request
+ * (mmhip_kv_plan's last_dev). A token outside the table gives NaN and is
+ * reported. y_stride in floats, at least cols. Buffers must not overlap. */
+int mmhip_embed_dev(mmhip_ctx* ctx, float* y_dev, uint64_t y_stride, const void* table_dev, uint32_t type, uint64_t rows,
+                    uint32_t cols, const uint32_t* tokens_dev, uint64_t n_tokens, float scale);
+
+/* Plans a step of n_requests requests over a paged cache (mmhip_kv_cache).
+ * Request r owns row r of the page tables and has lens[r] positions cached;
+ * new[r] tokens are to be added (0: it is idle). free_dev is a stack of the
+ * numbers of free pages, the first free_count of n_pages entries.
+ *  1. Where release[r] is not 0 (release_dev NULL: nowhere) the request that
+ *     had row r is over: its pages, but for the first shared[r] (which other
+ *     tables name too; shared_dev NULL: none), go onto the stack, requests and
+ *     pages in order, and the row begins anew with no positions.
+ *  2. A request gets its tokens where its table has the pages for all of its
+ *     positions, where the tokens asked for by it and all before it are at
+ *     most max_tokens, and where it needs no new page or the new pages needed by
+ *     it and all before it are at most those on the stack. granted[r] is 1
+ *     there and 0 elsewhere; a request that gets none keeps its positions.
+ *  3. New pages are taken from the top of the stack, requests and positions in
+ *     order, and written to the tables. next_lens[r] and next_free_count are the
+ *     values for the next step.
+ *  4. The step's tokens stand request by request: request r's are [firsts[r],
+ *     firsts[r + 1]), token t at positions[t] of table_of[t], to be written to
+ *     slots[t] and to see seen[t] = positions[t] + 1 positions: what
+ *     mmhip_rope_dev, mmhip_kv_store_dev and mmhip_mla_attention_dev take.
+ *     last[r] is its last token (MMHIP_NO_TOKEN: it has none; last_dev may be
+ *     NULL). Behind the last token, up to max_tokens, stand slot -1 and zeros.
+ * next_lens_dev may be lens_dev and next_free_count_dev may be free_count_dev, so
+ * that a captured step goes on from itself; no other buffers overlap. Shared
+ * pages have to be full. A length or a request beyond its table and tokens
+ * beyond max_tokens are reported; so is a page number on the stack or in a table
+ * that the pool does not have (its positions get slot -1) and a stack that
+ * would hold more than n_pages pages (it is cut there). Too few free pages are no
+ * fault: granted says so. n_requests below 2^24, max_tokens below 2^31;
+ * page_tokens, n_pages as in mmhip_kv_cache, table_pages as in mmhip_mla_attention. */
+typedef struct {
+    uint32_t n_requests;
+    uint32_t page_tokens, n_pages;
+    uint32_t table_pages;
+    const uint32_t* lens_dev;      /* [n_requests] */
+    const uint32_t* new_dev;       /* [n_requests] */
+    const uint32_t* release_dev;   /* [n_requests] or NULL */
+    const uint32_t* shared_dev;    /* [n_requests] or NULL */
+    uint32_t* next_lens_dev;       /* [n_requests] */
+    int32_t* tables_dev;           /* [n_requests][table_stride], table_pages of each used */
+    uint64_t table_stride;
+    int32_t* free_dev;             /* [n_pages] */
+    const uint32_t* free_count_dev;
+    uint32_t* next_free_count_dev;
+    uint32_t max_tokens;
+    uint32_t* positions_dev;       /* [max_tokens], as the next three */
+    int32_t* slots_dev;
+    uint32_t* table_of_dev;
+    uint32_t* seen_dev;
+    uint32_t* firsts_dev;          /* [n_requests + 1] */
+    uint32_t* granted_dev;         /* [n_requests] */
+    uint32_t* last_dev;            /* [n_requests] or NULL */
+    void* workspace_dev;           /* 16-byte aligned */
+    uint64_t workspace_bytes;      /* at least mmhip_kv_plan_workspace */
+} mmhip_kv_plan;
+uint64_t mmhip_kv_plan_workspace(mmhip_ctx* ctx, uint32_t n_requests);
+int mmhip_kv_plan_dev(mmhip_ctx* ctx, const mmhip_kv_plan* args);
+
+/* Draws a token from each of n_rows rows of logits. Output r reads row r, or row
+ * rows[r] of n_logits where rows_dev is given. With m the largest logit, T =
+ * temperature[r] and w_v = exp((x_v - m) / T), the tokens stand in order of their
+ * logits, largest first, equal ones by the lower id, and of them are kept
+ *   the first top_k[r] (0: all of them),
+ *   of these the fewest whose weights reach top_p[r] of their sum (1 or more:
+ *     all; always at least one),
+ *   and of these those with w_v >= min_p[r].
+ * The token drawn is the lowest kept id at which the running sum of the kept
+ * weights, in the order of ids, exceeds uniform[r] times their sum; probs[r] is
+ * its weight over that sum, kept[r] the number of tokens kept. T = 0 takes the
+ * first token of the order (probability 1, one kept). Where NULL: temperature 1,
+ * top_k 0, top_p 1, min_p 0; probs_dev, kept_dev: not wanted.
+ * Weights are computed in 64 bits and summed as whole multiples of 2^-44 of the
+ * largest (from 2^18 tokens on of 2^(b - 62), 2^b >= vocab), in integers: the
+ * result does not depend on the order of the sums, and a call repeated gives the
+ * same bits. NaN and -infinity (masked logits) are never drawn; among +infinities
+ * all weigh the same and finite logits nothing. A row without a logit above
+ * -infinity, settings out of range (T outside [0, f32's largest], top_p < 0,
+ * min_p or uniform outside [0, 1] and [0, 1), a NaN) and a row number that the
+ * logits do not have give MMHIP_NO_TOKEN, NaN and 0, and are reported. stride in
+ * floats, at least vocab. Outputs and workspace overlap neither the inputs nor
+ * each other. */
+#define MMHIP_SAMPLE_MAX_VOCAB (1u << 24)
+typedef struct {
+    const float* logits_dev;       /* [n_rows or n_logits][stride] */
+    uint64_t stride;
+    uint64_t n_rows, vocab;
+    const uint32_t* rows_dev;      /* [n_rows] or NULL */
+    uint64_t n_logits;             /* rows of logits_dev; unused where rows_dev is NULL */
+    const float* temperature_dev;  /* [n_rows] or NULL, as the next three */
+    const uint32_t* top_k_dev;
+    const float* top_p_dev;
+    const float* min_p_dev;
+    const float* uniform_dev;      /* [n_rows] */
+    uint32_t* tokens_dev;          /* [n_rows] */
+    float* probs_dev;              /* [n_rows] or NULL */
+    uint32_t* kept_dev;            /* [n_rows] or NULL */
+    void* workspace_dev;           /* 16-byte aligned */
+    uint64_t workspace_bytes;      /* at least mmhip_sample_workspace */
+} mmhip_sample;
+uint64_t mmhip_sample_workspace(mmhip_ctx* ctx, uint64_t n_rows, uint64_t vocab);
+int mmhip_sample_dev(mmhip_ctx* ctx, const mmhip_sample* args);
 
 /* ======================================================================
  * MoE FFN layer: replaces moeFFN (src/inference.zig:886-1010) with

@@ -486,7 +486,7 @@ int mmhip_gemv_grouped_dev(mmhip_ctx* ctx, const mmhip_gemv_group* groups, uint3
             return MMHIP_ERR_INVALID;
         }
         if (gr.w->type == kF32 || gr.w->type == kF16) {
-            set_error(MMHIP_ERR_UNSUPPORTED, "gemv_grouped_dev: quantised weights only (Q8_0, IQ2_XXS)");
+            set_error(MMHIP_ERR_UNSUPPORTED, "gemv_grouped_dev: quantised weights only (Q8_0, Q4_0, IQ4_NL, IQ2_XXS)");
             return MMHIP_ERR_UNSUPPORTED;
         }
         if (gr.first + gr.n_mats > gr.w->count || gr.first + gr.n_mats < gr.first) {

@@ -2,6 +2,7 @@
 // and the device-pointer GEMV / QMM drivers used by every entry point.
 #include "backend.hpp"
 
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
 #include <string>
@@ -43,7 +44,15 @@ int check_step_status(mmhip_ctx* ctx, const char* what) {
                                       "mla_attention: a table row that does not exist (its token saw nothing)",
                                       "mla_attention: a length beyond its table's pages (cut there)",
                                       "mla_attention: a page that the pool does not have (left out)",
-                                      "logprobs: a token outside the vocabulary (NaN)"};
+                                      "logprobs: a token outside the vocabulary (NaN)",
+                                      "embed: a token outside the table (NaN)",
+                                      "kv_plan: a length beyond a table's pages (its request got nothing)",
+                                      "kv_plan: more tokens than max_tokens (the requests behind them got nothing)",
+                                      "kv_plan: a page that the pool does not have (its positions got no slot)",
+                                      "kv_plan: more free pages than the pool has (cut there)",
+                                      "sample: a row that the logits do not have (no token)",
+                                      "sample: a setting or random number out of range (no token)",
+                                      "sample: a row without a token to draw (no token)"};
     set_error(MMHIP_ERR_INVALID, std::string(what) + ": an earlier call met " +
                                      (st < sizeof(met) / sizeof(met[0]) ? met[st] : "an unknown fault"));
     return MMHIP_ERR_INVALID;
@@ -52,7 +61,7 @@ int check_step_status(mmhip_ctx* ctx, const char* what) {
 uint64_t block_size(uint32_t type) {
     switch (type) {
         case kF32: case kF16: return 1;
-        case kQ8_0: return 32;
+        case kQ8_0: case kQ4_0: case kIq4Nl: return 32;
         case kIq2Xxs: return 256;
         default: return 0;
     }
@@ -63,6 +72,7 @@ uint64_t block_bytes(uint32_t type) {
         case kF32: return 4;
         case kF16: return 2;
         case kQ8_0: return 34;
+        case kQ4_0: case kIq4Nl: return 18;
         case kIq2Xxs: return 66;
         default: return 0;
     }
@@ -159,12 +169,20 @@ int weight_create_segments(mmhip_ctx* ctx, const WeightSegment* segs, size_t n_s
     }
     if (block_size(type) == 0) {
         set_error(MMHIP_ERR_UNSUPPORTED, "weight: GgmlType " + std::to_string(type) +
-                                             " is not on this backend's path (F32, F16, Q8_0, IQ2_XXS)");
+                                             " is not on this backend's path (F32, F16, Q8_0, Q4_0, IQ4_NL, IQ2_XXS)");
         return MMHIP_ERR_UNSUPPORTED;
     }
     if (type == kIq2Xxs && cols % 256 != 0) {
         set_error(MMHIP_ERR_INVALID, "weight: IQ2_XXS rows must hold whole 256-element superblocks");
         return MMHIP_ERR_INVALID;
+    }
+    if (type_4bit(type) && cols % 32 != 0) {
+        set_error(MMHIP_ERR_INVALID, "weight: rows of 4-bit weights must hold whole blocks of 32");
+        return MMHIP_ERR_INVALID;
+    }
+    if (type_4bit(type) && cols >= kQ4MostCols) {
+        set_error(MMHIP_ERR_UNSUPPORTED, "weight: rows of 4-bit weights must stay below 2^23 columns");
+        return MMHIP_ERR_UNSUPPORTED;
     }
     const uint64_t row_bytes = ((cols + block_size(type) - 1) / block_size(type)) * block_bytes(type);
     const uint64_t mat_bytes = row_bytes * rows;
@@ -219,6 +237,14 @@ int weight_create_segments(mmhip_ctx* ctx, const WeightSegment* segs, size_t n_s
     // Scales are stored per row ([tile][row][unit]) so that one vector load
     // fetches a row's scales for several units.
     g.d_row = ((g.units * ((type == kIq2Xxs) ? 1 : 2) + 7) / 8) * 8;
+    if (type_4bit(type)) {
+        g.fmt = type == kQ4_0 ? kFmtQ4 : kFmtIq4;
+        g.unit_cols = 128;
+        g.units = (cols + 127) / 128;
+        g.cols_pad = g.units * g.unit_cols;
+        g.rec_stride = g.tiles * g.units * 64;
+        g.d_row = (g.units + 3) / 4 * 16;
+    }
     g.d_stride = g.tiles * 16 * g.d_row;
     // Every kernel reads one matrix through a buffer resource with 32-bit
     // offsets, 2^31 being its out-of-range sentinel.
@@ -343,7 +369,7 @@ int qmm_device(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat, const float*
                               (uint32_t)w->cols, ctx->num_cu, ctx->stream);
         return e == hipSuccess ? MMHIP_OK : hip_fail(e, "qmm: launch");
     }
-    if (qmm_path(ctx, w, batch) == QmmPath::kTwoLaunch) {
+    if (!type_4bit(w->type) && qmm_path(ctx, w, batch) == QmmPath::kTwoLaunch) {
         e = qscratch->ensure(quant_act_bytes(batch, w->geom.cols_pad));
         if (e != hipSuccess) return hip_fail(e, "qmm: scratch");
     }
@@ -374,7 +400,22 @@ int qmm_quantised(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat, const flo
                   int out_layout, void* qbuf, bool timed) {
     const TileGeom& g = w->geom;
     const uint64_t ld = out_layout == 0 ? w->rows : batch;
-    hipError_t e;
+    hipError_t e = hipSuccess;
+    if (fmt_4bit(g.fmt)) {
+        // One launch reading the f32 activations (qbuf unused): up to four
+        // vectors as the decode kernel takes them, more on the bf16 matrix cores.
+        const uint64_t y_slot = out_layout == 0 ? ld : 1, y_row = out_layout == 0 ? 1 : ld;
+        TimedLaunch tl(timed ? ctx : nullptr, "qmm");
+        if (batch <= 4 && out_layout == 0) {
+            e = launch_gemv_q4_vecs(gemv_args(w, mat, 1, x, w->cols, y, ld), (uint32_t)batch, g.fmt, ctx->num_cu, ctx->stream);
+            return e == hipSuccess ? MMHIP_OK : hip_fail(e, "qmm: launch");
+        }
+        const uint64_t most = gemm_q4_most(g);
+        for (uint64_t b = 0; b < batch && e == hipSuccess; b += most)
+            e = launch_gemm_q4(w->recs, w->dvals, g, mat, x + b * w->cols, w->cols, (uint32_t)std::min(most, batch - b),
+                               y + b * y_slot, y_slot, y_row, ctx->num_cu, ctx->stream);
+        return e == hipSuccess ? MMHIP_OK : hip_fail(e, "qmm: launch");
+    }
     const QmmPath path = qmm_path(ctx, w, batch);
     if (path == QmmPath::kTile) {
         // One launch reading the f32 activations (qbuf unused).

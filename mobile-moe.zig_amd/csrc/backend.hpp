@@ -17,7 +17,8 @@
 
 namespace mmhip {
 
-enum GgmlType : uint32_t { kF32 = 0, kF16 = 1, kQ8_0 = 8, kIq2Xxs = 16 };
+enum GgmlType : uint32_t { kF32 = 0, kF16 = 1, kQ4_0 = 2, kQ8_0 = 8, kIq2Xxs = 16, kIq4Nl = 20 };
+constexpr bool type_4bit(uint32_t type) { return type == kQ4_0 || type == kIq4Nl; }
 
 // GgmlType.blockSize / blockBytes / tensorBytes (src/gguf.zig:59-117) for the
 // types this backend accepts; 0 for the others.

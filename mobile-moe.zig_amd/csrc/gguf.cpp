@@ -128,12 +128,19 @@ Value read_value(Cursor& c, uint32_t type) {
     return v;
 }
 
-uint64_t block_elems(uint32_t t) { return t == MMHIP_TYPE_Q8_0 ? 32 : t == MMHIP_TYPE_IQ2_XXS ? 256 : 1; }
+uint64_t block_elems(uint32_t t) {
+    switch (t) {
+        case MMHIP_TYPE_Q8_0: case MMHIP_TYPE_Q4_0: case MMHIP_TYPE_IQ4_NL: return 32;
+        case MMHIP_TYPE_IQ2_XXS: return 256;
+        default: return 1;
+    }
+}
 uint64_t block_bytes(uint32_t t) {
     switch (t) {
         case MMHIP_TYPE_F32: return 4;
         case MMHIP_TYPE_F16: return 2;
         case MMHIP_TYPE_Q8_0: return 34;
+        case MMHIP_TYPE_Q4_0: case MMHIP_TYPE_IQ4_NL: return 18;
         case MMHIP_TYPE_IQ2_XXS: return 66;
         default: return 0;
     }

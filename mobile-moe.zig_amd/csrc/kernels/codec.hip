@@ -2,13 +2,14 @@
 // one-time repack into the tile layout, and activation quantisation.
 #include "device_common.hpp"
 #include "kernels.hpp"
+#include "q4_ops.hpp"
 #include "q8_ops.hpp"
 
 namespace mmhip {
 
 namespace {
 
-constexpr uint32_t kTypeF32 = 0, kTypeF16 = 1, kTypeQ8_0 = 8, kTypeIq2 = 16;
+constexpr uint32_t kTypeF32 = 0, kTypeF16 = 1, kTypeQ4_0 = 2, kTypeQ8_0 = 8, kTypeIq2 = 16, kTypeIq4Nl = 20;
 
 // Raw GGUF bytes are only 2-byte aligned (34 / 66-byte blocks): read u16s.
 __device__ __forceinline__ uint32_t ld16(const uint8_t* p) {
@@ -68,6 +69,63 @@ __global__ void dequant_iq2_kernel(const uint8_t* __restrict__ raw, uint64_t n, 
 __global__ void dequant_f16_kernel(const uint16_t* __restrict__ raw, uint64_t n, float* __restrict__ out) {
     uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i < n) out[i] = f16_bits_to_f32(raw[i]);
+}
+
+// Q4_0 and IQ4_NL blocks {f16 d; u8 qs[16]}: code j of a block is the lower
+// half of byte j, code 16 + j its upper half. One thread per four bytes of codes:
+// values 4 j .. and 16 + 4 j .., two 16-byte stores.
+template <bool NL>
+__global__ __launch_bounds__(256) void dequant_4bit_kernel(const uint8_t* __restrict__ raw, uint64_t n, bool vec,
+                                                           float* __restrict__ out) {
+    const uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t blk = t >> 2, base = blk * 32 + 4 * (t & 3);
+    if (base >= n) return;
+    const uint8_t* b = raw + blk * 18;
+    const float d = f16_bits_to_f32(ld16(b));
+    const uint32_t c = ld32u(b + 2 + 4 * (t & 3));
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = d * (float)q4_code<NL>((c >> (8 * e + 4 * h)) & 15u);
+        float* dst = out + base + 16 * h;
+        if (vec && base + 16 * h + 4 <= n) {
+            typedef float v4f_ __attribute__((ext_vector_type(4)));
+            __builtin_nontemporal_store(v4f_{v[0], v[1], v[2], v[3]}, reinterpret_cast<v4f_*>(dst));
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                if (base + 16 * h + e < n) dst[e] = v[e];
+        }
+    }
+}
+
+// Raw 4-bit blocks -> tile records and scales (q4_ops.hpp). One thread per
+// (matrix, row tile, unit, lane).
+template <bool NL>
+__global__ void repack_4bit_kernel(const uint8_t* __restrict__ raw, uint64_t rows, uint64_t nb, uint64_t nu, uint64_t tiles,
+                                   uint64_t total, uint64_t d_row, uint4* __restrict__ recs, uint16_t* __restrict__ dvals) {
+    const uint64_t gid = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (gid >= total) return;
+    const uint32_t lane = (uint32_t)(gid & 63), n = lane & 15, g = lane >> 4;
+    const uint64_t unit = gid >> 6, u = unit % nu, tm = unit / nu, t = tm % tiles, mat = tm / tiles, row = t * 16 + n;
+    const uint8_t* const src = raw + (mat * rows + row) * nb * 18;
+    uint32_t w[4] = {0, 0, 0, 0}, dbits = 0;
+    if (row < rows) {
+#pragma unroll
+        for (uint32_t b = 0; b < 4; ++b) {
+            const uint64_t blk = 4 * u + b;
+            if (blk >= nb) continue;
+            // Columns 8 g .. 8 g + 7: eight bytes' lower (g < 2) or upper halves.
+            const uint8_t* q = src + blk * 18 + 2 + 8 * (g & 1);
+            const uint32_t s = g < 2 ? 0 : 4;
+            const uint32_t lo = (ld32u(q) >> s) & 0x0F0F0F0Fu, hi = (ld32u(q + 4) >> s) & 0x0F0F0F0Fu;
+            w[b] = (lo | hi << 4) ^ (NL ? 0u : 0x88888888u);
+        }
+        if (4 * u + g < nb) dbits = ld16(src + (4 * u + g) * 18);
+    }
+    recs[gid] = make_uint4(w[0], w[1], w[2], w[3]);
+    dvals[tm * 16 * d_row + (u >> 2) * 256 + lane * 4 + (u & 3)] = (uint16_t)dbits;
 }
 
 // Raw IQ2_XXS -> tile records (layout in device_common.hpp). One thread per
@@ -412,6 +470,14 @@ hipError_t launch_dequant(const void* raw, uint32_t type, uint64_t n, float* out
             dequant_iq2_kernel<<<(unsigned)((quads + bs - 1) / bs), bs, 0, s>>>((const uint8_t*)raw, n, vec, out);
             break;
         }
+        case kTypeQ4_0:
+        case kTypeIq4Nl: {
+            const bool vec = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+            const unsigned grid = (unsigned)(((n + 31) / 32 * 4 + 255) / 256);
+            if (type == kTypeQ4_0) dequant_4bit_kernel<false><<<grid, 256, 0, s>>>((const uint8_t*)raw, n, vec, out);
+            else dequant_4bit_kernel<true><<<grid, 256, 0, s>>>((const uint8_t*)raw, n, vec, out);
+            break;
+        }
         default:
             return hipErrorInvalidValue;
     }
@@ -426,6 +492,14 @@ hipError_t launch_repack(const void* raw, const TileGeom& g, uint4* recs, uint16
     if (g.fmt == kFmtIq2) {
         repack_iq2_kernel<<<grid, bs, 0, s>>>((const uint8_t*)raw, g.rows, g.units, g.tiles, total, g.d_row, recs,
                                               dvals);
+    } else if (fmt_4bit(g.fmt)) {
+        const uint64_t nb = g.cols / 32;
+        if (g.fmt == kFmtQ4)
+            repack_4bit_kernel<false><<<grid, bs, 0, s>>>((const uint8_t*)raw, g.rows, nb, g.units, g.tiles, total, g.d_row,
+                                                          recs, dvals);
+        else
+            repack_4bit_kernel<true><<<grid, bs, 0, s>>>((const uint8_t*)raw, g.rows, nb, g.units, g.tiles, total, g.d_row,
+                                                         recs, dvals);
     } else {
         uint64_t nb = (g.cols + 31) / 32;
         repack_q8_kernel<<<grid, bs, 0, s>>>((const uint8_t*)raw, g.rows, nb, g.units, g.tiles, total, g.d_row, recs,

@@ -6,7 +6,7 @@
 // disappears), and its waves then stream equal shares of the range's 1 KiB
 // record units, one 128-bit load per lane, steps ahead of the compute. Every
 // weight byte is read exactly once. IQ2_XXS weights have their own kernel
-// (gemv_iq2.hip); launch_gemv_q forwards them there.
+// (gemv_iq2.hip), as do 4-bit ones (gemv_q4.hip); launch_gemv_q forwards them there.
 //
 // f32 / f16 weights (the router, matVecMulUnified's f32 branch): one
 // workgroup per output row, summing in the reference's order
@@ -525,6 +525,7 @@ hipError_t launch_gemv_q(const GemvArgs& a, uint32_t fmt, int num_cu, hipStream_
 hipError_t launch_gemv_segments(const GemvArgs* segs_in, uint32_t n_segs, uint32_t fmt, int num_cu, hipStream_t s) {
     if (n_segs == 0 || n_segs > kGemvMaxSegs) return hipErrorInvalidValue;
     if (fmt == kFmtIq2) return launch_gemv_iq2(segs_in, n_segs, num_cu, s);
+    if (fmt_4bit(fmt)) return launch_gemv_q4(segs_in, n_segs, fmt, num_cu > 0 ? num_cu : 256, s);
     GemvArgs segs[kGemvMaxSegs];
     uint32_t n = 0;
     for (uint32_t i = 0; i < n_segs; ++i)

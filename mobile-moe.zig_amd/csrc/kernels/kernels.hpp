@@ -10,7 +10,8 @@
 
 namespace mmhip {
 
-enum TileFormat : uint32_t { kFmtQ8 = 0, kFmtIq2 = 1 };
+enum TileFormat : uint32_t { kFmtQ8 = 0, kFmtIq2 = 1, kFmtQ4 = 2, kFmtIq4 = 3 };
+constexpr bool fmt_4bit(uint32_t fmt) { return fmt == kFmtQ4 || fmt == kFmtIq4; }
 
 // Geometry of a stacked weight in the tile layout (device_common.hpp).
 struct TileGeom {
@@ -18,10 +19,10 @@ struct TileGeom {
     uint64_t rows, cols, count;
     uint64_t tiles;        // ceil(rows / 16)
     uint64_t units;        // record units per row tile
-    uint64_t unit_cols;    // 256 (IQ2_XXS) or 64 (Q8_0)
+    uint64_t unit_cols;    // 256 (IQ2_XXS), 64 (Q8_0) or 128 (4 bits)
     uint64_t cols_pad;     // units * unit_cols
     uint64_t rec_stride;   // uint4 records per matrix = tiles * units * 64
-    uint64_t d_row;        // u16 scales per row, padded: roundup(units * (1 | 2), 8)
+    uint64_t d_row;        // u16 scales per row, padded: roundup(units * (1 | 2), 8); 4 bits: roundup(units, 4) * 4
     uint64_t d_stride;     // u16 scales per matrix = tiles * 16 * d_row
 };
 
@@ -187,6 +188,19 @@ hipError_t launch_gemv_segments(const GemvArgs* segs, uint32_t n_segs, uint32_t 
 // forward IQ2_XXS here.
 hipError_t launch_gemv_iq2(const GemvArgs* segs, uint32_t n_segs, int num_cu, hipStream_t s);
 
+// 4-bit weights (q4_ops.hpp): launch_gemv_segments forwards them here; no
+// problem lists, no silu_mul.
+hipError_t launch_gemv_q4(const GemvArgs* segs, uint32_t n_segs, uint32_t fmt, int num_cu, hipStream_t s);
+// n_vec vectors (x_stride, y_stride apart) times matrix first_mat.
+hipError_t launch_gemv_q4_vecs(const GemvArgs& a, uint32_t n_vec, uint32_t fmt, int num_cu, hipStream_t s);
+// Many vectors times one matrix: y[j * y_slot + r * y_row] = x[j] . W[r]. At
+// most gemm_q4_most(g) vectors a launch; rows below kQ4MostCols columns.
+constexpr uint64_t kQ4MostCols = 1u << 23;
+uint64_t gemm_q4_most(const TileGeom& g);
+hipError_t launch_gemm_q4(const uint4* recs, const uint16_t* dvals, const TileGeom& g, uint64_t mat, const float* x,
+                          uint64_t x_stride, uint32_t batch, float* y, uint64_t y_slot, uint64_t y_row, int num_cu,
+                          hipStream_t s);
+
 // Decode (one token) down projection of the computed experts and the
 // combine, IQ2_XXS experts with the shared expert merged (or none): problem
 // p of probs[0, *n_active) is {matrix, activation slot, output slot, 0};
@@ -344,7 +358,11 @@ constexpr uint32_t kRopeMaxPairs = 128, kKvMaxRank = 512, kKvMaxRope = 64, kLogp
 
 // What device code met in device data (a host-visible word, 0: nothing), for
 // the next synchronisation to report.
-enum StepStatus : uint32_t { kBadSlot = 1, kBadTableRow, kBadLength, kBadPage, kBadToken };
+enum StepStatus : uint32_t {
+    kBadSlot = 1, kBadTableRow, kBadLength, kBadPage, kBadToken,
+    kBadEmbedToken, kBadPlanLength, kBadPlanTokens, kBadPlanPage, kBadPlanFree, kBadSampleRow, kBadSampleSetting, kNoSampleToken
+};
+constexpr uint32_t kNoToken = 0xFFFFFFFFu;  // a token or row that is not there
 #if defined(__HIPCC__)
 __device__ __forceinline__ void report(uint32_t* status, uint32_t code) {
     __hip_atomic_store(status, code, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
@@ -449,5 +467,69 @@ struct LogprobsArgs {
 };
 uint64_t logprobs_workspace_bytes(uint64_t n_rows, uint64_t vocab, uint32_t top);
 hipError_t launch_logprobs(const LogprobsArgs& a, uint64_t n_rows, hipStream_t s);
+
+// ---- The two ends of a step (embed.hip, kv_plan.hip, sampling.hip) ----
+
+struct EmbedArgs {
+    float* y;
+    uint64_t y_stride;
+    const uint8_t* table;
+    uint64_t row_bytes;
+    uint64_t rows;
+    uint32_t cols;
+    const uint32_t* tokens;
+    float scale;
+    uint32_t* status;
+    // Set by the launcher.
+    bool vec;               // 16-byte stores fit
+};
+hipError_t launch_embed(const EmbedArgs& a, uint32_t ggml_type, uint64_t n_tokens, hipStream_t s);
+
+// A request's part of a plan, between its launches.
+struct PlanRow {
+    uint32_t start;         // positions before the step's tokens
+    uint32_t pages;         // free pages that the requests before it take
+    uint32_t back, back_from, back_at;  // pages given back: table entries [back_from, + back) to free[back_at ..)
+};
+struct PlanArgs {
+    uint32_t n_requests, page_shift, n_pages, table_pages, max_tokens;
+    const uint32_t *lens, *added, *release, *shared;  // release, shared or null
+    uint32_t* next_lens;
+    int32_t* tables;
+    uint64_t table_stride;
+    int32_t* free;
+    const uint32_t* free_count;
+    uint32_t* next_free_count;
+    uint32_t* positions;
+    int32_t* slots;
+    uint32_t *table_of, *seen, *firsts, *granted, *last;  // last or null
+    uint32_t* status;
+    // Set by the launcher, in the workspace.
+    uint32_t* top;          // free pages before any is taken
+    PlanRow* work;          // [n_requests]
+};
+uint64_t plan_workspace_bytes(uint32_t n_requests);
+hipError_t launch_kv_plan(const PlanArgs& a, void* work, hipStream_t s);
+
+struct SampleArgs {
+    const float* logits;
+    uint64_t stride;
+    uint64_t n_logits;
+    uint32_t vocab;
+    const uint32_t* rows;   // or null
+    const float* temperature;  // or null, as the next three
+    const uint32_t* top_k;
+    const float *top_p, *min_p;
+    const float* uniform;
+    uint32_t* tokens;
+    float* probs;           // or null
+    uint32_t* kept;         // or null
+    void* work;
+    uint32_t* status;
+    // Set by the launcher.
+    int shift;              // weights are whole multiples of 2^-shift
+};
+uint64_t sample_workspace_bytes(uint64_t n_rows, uint64_t vocab);
+hipError_t launch_sample(const SampleArgs& a, uint64_t n_rows, hipStream_t s);
 
 }  // namespace mmhip

@@ -1,6 +1,7 @@
 // extern "C" surface of the operators between a decode step's products: norm,
 // rotary positions, the paged latent cache and its attention, log
-// probabilities (declared in include/mmhip.h). Host side: argument checks,
+// probabilities; and of those at a step's two ends: embedding rows, the page
+// plan, sampling (declared in include/mmhip.h). Host side: argument checks,
 // the rotary plan's frequencies, launches. Arguments are checked before the
 // context, so that every refusal can be met without a device.
 #include <cmath>
@@ -17,6 +18,8 @@ static_assert(MMHIP_ROPE_MAX_DIMS == 2 * mmhip::kRopeMaxPairs, "rope limit in th
 static_assert(MMHIP_KV_MAX_RANK == mmhip::kKvMaxRank && MMHIP_KV_MAX_ROPE == mmhip::kKvMaxRope,
               "cache limits in the header and the library differ");
 static_assert(MMHIP_LOGPROBS_MAX_TOP == mmhip::kLogprobsMaxTop, "top limit in the header and the library differ");
+
+static_assert(MMHIP_NO_TOKEN == mmhip::kNoToken, "the absent token in the header and the library differ");
 
 using namespace mmhip;
 
@@ -430,6 +433,143 @@ int mmhip_logprobs_dev(mmhip_ctx* ctx, const float* logits, uint64_t stride, uin
         a.work = workspace;
         a.status = ctx->step_status_dev();
         return launch(ctx, what, [&] { return launch_logprobs(a, n_rows, ctx->stream); });
+    });
+}
+
+int mmhip_embed_dev(mmhip_ctx* ctx, float* y, uint64_t y_stride, const void* table, uint32_t type, uint64_t rows,
+                    uint32_t cols, const uint32_t* tokens, uint64_t n_tokens, float scale) {
+    return guarded([&]() -> int {
+        const char* what = "embed";
+        if (block_size(type) == 0) return refuse(MMHIP_ERR_UNSUPPORTED, what, "the table's type is not on this path");
+        if (rows == 0 || rows > 0xFFFFFFFFull) return invalid(what, "rows outside [1, 2^32)");
+        if (cols == 0 || cols > 0x7FFFFFFFu) return invalid(what, "cols outside [1, 2^31)");
+        if ((type == kIq2Xxs || type_4bit(type)) && cols % block_size(type))
+            return invalid(what, "cols must hold whole blocks of the table's type");
+        if (n_tokens > kMostRows) return invalid(what, "2^24 tokens or more");
+        // One workgroup of 256 threads per 1024 values, and fewer than 2^32 threads.
+        if (n_tokens * (((uint64_t)cols + 1023) / 1024) > kMostRows) return invalid(what, "2^24 pieces of 1024 values or more");
+        if (n_tokens == 0) return ctx ? MMHIP_OK : invalid(what, "null context");
+        if (!y || !table || !tokens) return invalid(what, "null pointer");
+        if (n_tokens > 1 && y_stride < cols) return invalid(what, "y_stride is below cols");
+        if (misaligned(y, 4) || misaligned(tokens, 4) || misaligned(table, type == kF32 ? 4 : 2))
+            return invalid(what, "misaligned pointer");
+        EmbedArgs a{};
+        a.y = y;
+        a.y_stride = y_stride;
+        a.table = static_cast<const uint8_t*>(table);
+        a.row_bytes = tensor_bytes(type, cols);
+        a.rows = rows;
+        a.cols = cols;
+        a.tokens = tokens;
+        a.scale = scale;
+        return launch(ctx, what, [&] {
+            a.status = ctx->step_status_dev();
+            return launch_embed(a, type, n_tokens, ctx->stream);
+        });
+    });
+}
+
+uint64_t mmhip_kv_plan_workspace(mmhip_ctx* ctx, uint32_t n_requests) {
+    if (!ctx) return 0;
+    return plan_workspace_bytes(n_requests);
+}
+
+int mmhip_kv_plan_dev(mmhip_ctx* ctx, const mmhip_kv_plan* args) {
+    return guarded([&]() -> int {
+        const char* what = "kv_plan";
+        if (!args) return invalid(what, "null arguments");
+        const mmhip_kv_plan& p = *args;
+        if (p.page_tokens < 16 || p.page_tokens > 1024 || (p.page_tokens & (p.page_tokens - 1)))
+            return invalid(what, "page_tokens must be a power of two, 16..1024");
+        if (p.n_pages == 0 || (uint64_t)p.n_pages * p.page_tokens >= 0x80000000ull)
+            return invalid(what, "n_pages * page_tokens must be in [1, 2^31)");
+        if (p.n_requests > kMostRows) return invalid(what, "2^24 requests or more");
+        if (p.table_pages == 0 || (p.n_requests > 1 && p.table_stride < p.table_pages))
+            return invalid(what, "tables need pages and a stride of at least table_pages");
+        if ((uint64_t)p.table_pages * p.page_tokens > 0xFFFFFFFFull) return invalid(what, "a table names 2^32 positions or more");
+        if (p.max_tokens > 0x7FFFFFFFu) return invalid(what, "2^31 tokens or more");
+        if (!p.free_dev || !p.free_count_dev || !p.next_free_count_dev || !p.firsts_dev) return invalid(what, "null pointer");
+        if (p.n_requests && (!p.lens_dev || !p.new_dev || !p.next_lens_dev || !p.tables_dev || !p.granted_dev))
+            return invalid(what, "null pointer");
+        if (p.max_tokens && (!p.positions_dev || !p.slots_dev || !p.table_of_dev || !p.seen_dev)) return invalid(what, "null pointer");
+        if (p.shared_dev && !p.release_dev) return invalid(what, "shared_dev without release_dev");
+        const void* all[] = {p.lens_dev, p.new_dev, p.release_dev, p.shared_dev, p.next_lens_dev, p.tables_dev, p.free_dev,
+                             p.free_count_dev, p.next_free_count_dev, p.positions_dev, p.slots_dev, p.table_of_dev, p.seen_dev,
+                             p.firsts_dev, p.granted_dev, p.last_dev};
+        for (const void* b : all)
+            if (misaligned(b, 4)) return invalid(what, "misaligned pointer");
+        if (!ctx) return invalid(what, "null context");
+        if (p.workspace_bytes < plan_workspace_bytes(p.n_requests) || !p.workspace_dev || misaligned(p.workspace_dev, 16))
+            return invalid(what, "the workspace is too small, null or not 16-byte aligned");
+        PlanArgs a{};
+        a.n_requests = p.n_requests;
+        while ((1u << a.page_shift) < p.page_tokens) ++a.page_shift;
+        a.n_pages = p.n_pages;
+        a.table_pages = p.table_pages;
+        a.max_tokens = p.max_tokens;
+        a.lens = p.lens_dev;
+        a.added = p.new_dev;
+        a.release = p.release_dev;
+        a.shared = p.shared_dev;
+        a.next_lens = p.next_lens_dev;
+        a.tables = p.tables_dev;
+        a.table_stride = p.table_stride;
+        a.free = p.free_dev;
+        a.free_count = p.free_count_dev;
+        a.next_free_count = p.next_free_count_dev;
+        a.positions = p.positions_dev;
+        a.slots = p.slots_dev;
+        a.table_of = p.table_of_dev;
+        a.seen = p.seen_dev;
+        a.firsts = p.firsts_dev;
+        a.granted = p.granted_dev;
+        a.last = p.last_dev;
+        a.status = ctx->step_status_dev();
+        return launch(ctx, what, [&] { return launch_kv_plan(a, p.workspace_dev, ctx->stream); });
+    });
+}
+
+uint64_t mmhip_sample_workspace(mmhip_ctx* ctx, uint64_t n_rows, uint64_t vocab) {
+    if (!ctx) return 0;
+    return sample_workspace_bytes(n_rows, vocab);
+}
+
+int mmhip_sample_dev(mmhip_ctx* ctx, const mmhip_sample* args) {
+    return guarded([&]() -> int {
+        const char* what = "sample";
+        if (!args) return invalid(what, "null arguments");
+        const mmhip_sample& p = *args;
+        if (p.vocab == 0 || p.vocab > MMHIP_SAMPLE_MAX_VOCAB) return invalid(what, "vocab outside [1, 2^24]");
+        if (p.n_rows > kMostRows) return invalid(what, "2^24 rows or more");
+        if (p.rows_dev && (p.n_logits == 0 || p.n_logits >= MMHIP_NO_TOKEN)) return invalid(what, "n_logits outside [1, 2^32 - 1)");
+        if (p.n_rows == 0) return ctx ? MMHIP_OK : invalid(what, "null context");
+        if (!p.logits_dev || !p.uniform_dev || !p.tokens_dev) return invalid(what, "null pointer");
+        if ((p.rows_dev ? p.n_logits : p.n_rows) > 1 && p.stride < p.vocab) return invalid(what, "the stride is below vocab");
+        const void* all[] = {p.logits_dev, p.rows_dev, p.temperature_dev, p.top_k_dev, p.top_p_dev,
+                             p.min_p_dev, p.uniform_dev, p.tokens_dev, p.probs_dev, p.kept_dev};
+        for (const void* b : all)
+            if (misaligned(b, 4)) return invalid(what, "misaligned pointer");
+        if (!ctx) return invalid(what, "null context");
+        const uint64_t need = sample_workspace_bytes(p.n_rows, p.vocab);
+        if (p.workspace_bytes < need || (need && (!p.workspace_dev || misaligned(p.workspace_dev, 16))))
+            return invalid(what, "the workspace is too small, null or not 16-byte aligned");
+        SampleArgs a{};
+        a.logits = p.logits_dev;
+        a.stride = p.stride;
+        a.n_logits = p.n_logits;
+        a.vocab = (uint32_t)p.vocab;
+        a.rows = p.rows_dev;
+        a.temperature = p.temperature_dev;
+        a.top_k = p.top_k_dev;
+        a.top_p = p.top_p_dev;
+        a.min_p = p.min_p_dev;
+        a.uniform = p.uniform_dev;
+        a.tokens = p.tokens_dev;
+        a.probs = p.probs_dev;
+        a.kept = p.kept_dev;
+        a.work = p.workspace_dev;
+        a.status = ctx->step_status_dev();
+        return launch(ctx, what, [&] { return launch_sample(a, p.n_rows, ctx->stream); });
     });
 }
 

@@ -7,6 +7,8 @@ missing or unloadable libmmhip raises instead of degrading to anything else.
 Block formats (src/dequant.zig:305-311, 372-377 in the reference):
   Q8_0     34 B  = f16 d, int8 qs[32]
   IQ2_XXS  66 B  = f16 d, u16 qs[32]  (256 weights)
+  Q4_0     18 B  = f16 d, u8 qs[16]  (32 weights: lower halves, then upper halves)
+  IQ4_NL   18 B  = the same, the codes by a table
 """
 from __future__ import annotations
 
@@ -22,9 +24,10 @@ PKG_DIR = os.path.dirname(_HERE)
 # sanitizer build, lib/libmmhip_san.so).
 LIB_PATH = os.environ.get("MMHIP_LIBRARY") or os.path.join(PKG_DIR, "lib", "libmmhip.so")
 
-F32, F16, Q8_0, IQ2_XXS = 0, 1, 8, 16
-BLOCK_SIZE = {F32: 1, F16: 1, Q8_0: 32, IQ2_XXS: 256}
-BLOCK_BYTES = {F32: 4, F16: 2, Q8_0: 34, IQ2_XXS: 66}
+F32, F16, Q4_0, Q8_0, IQ2_XXS, IQ4_NL = 0, 1, 2, 8, 16, 20
+BLOCK_SIZE = {F32: 1, F16: 1, Q4_0: 32, Q8_0: 32, IQ2_XXS: 256, IQ4_NL: 32}
+BLOCK_BYTES = {F32: 4, F16: 2, Q4_0: 18, Q8_0: 34, IQ2_XXS: 66, IQ4_NL: 18}
+NO_TOKEN = 0xFFFFFFFF  # a token or row that is not there
 
 OK, ERR_UNAVAILABLE, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP, ERR_NOMEM = 0, -1, -2, -3, -4, -5
 
@@ -105,6 +108,25 @@ class MlaAttention(ctypes.Structure):
                 ("workspace_bytes", _u64)]
 
 
+class KvPlan(ctypes.Structure):
+    _fields_ = [("n_requests", _u32), ("page_tokens", _u32), ("n_pages", _u32), ("table_pages", _u32),
+                ("lens_dev", _c_void_p), ("new_dev", _c_void_p), ("release_dev", _c_void_p), ("shared_dev", _c_void_p),
+                ("next_lens_dev", _c_void_p), ("tables_dev", _c_void_p), ("table_stride", _u64),
+                ("free_dev", _c_void_p), ("free_count_dev", _c_void_p), ("next_free_count_dev", _c_void_p),
+                ("max_tokens", _u32), ("positions_dev", _c_void_p), ("slots_dev", _c_void_p),
+                ("table_of_dev", _c_void_p), ("seen_dev", _c_void_p), ("firsts_dev", _c_void_p),
+                ("granted_dev", _c_void_p), ("last_dev", _c_void_p), ("workspace_dev", _c_void_p),
+                ("workspace_bytes", _u64)]
+
+
+class Sample(ctypes.Structure):
+    _fields_ = [("logits_dev", _c_void_p), ("stride", _u64), ("n_rows", _u64), ("vocab", _u64),
+                ("rows_dev", _c_void_p), ("n_logits", _u64), ("temperature_dev", _c_void_p),
+                ("top_k_dev", _c_void_p), ("top_p_dev", _c_void_p), ("min_p_dev", _c_void_p),
+                ("uniform_dev", _c_void_p), ("tokens_dev", _c_void_p), ("probs_dev", _c_void_p),
+                ("kept_dev", _c_void_p), ("workspace_dev", _c_void_p), ("workspace_bytes", _u64)]
+
+
 _SIGS = {
     "mmhip_last_error": (ctypes.c_char_p, []),
     "mmhip_is_available": (ctypes.c_int, []),
@@ -160,6 +182,12 @@ _SIGS = {
     "mmhip_logprobs_workspace": (_u64, [_c_void_p, _u64, _u64, _u32]),
     "mmhip_logprobs_dev": (ctypes.c_int, [_c_void_p, _c_void_p, _u64, _u64, _u64, _c_void_p, _u64, _c_void_p,
                                           _c_void_p, _u32, _c_void_p, _c_void_p, _c_void_p, _u64]),
+    "mmhip_embed_dev": (ctypes.c_int, [_c_void_p, _c_void_p, _u64, _c_void_p, _u32, _u64, _u32, _c_void_p, _u64,
+                                       ctypes.c_float]),
+    "mmhip_kv_plan_workspace": (_u64, [_c_void_p, _u32]),
+    "mmhip_kv_plan_dev": (ctypes.c_int, [_c_void_p, ctypes.POINTER(KvPlan)]),
+    "mmhip_sample_workspace": (_u64, [_c_void_p, _u64, _u64]),
+    "mmhip_sample_dev": (ctypes.c_int, [_c_void_p, ctypes.POINTER(Sample)]),
     "mmhip_moe_layer_create": (ctypes.c_int, [_c_void_p, ctypes.POINTER(MoeWeights), ctypes.POINTER(_c_void_p)]),
     "mmhip_moe_layer_destroy": (None, [_c_void_p, _c_void_p]),
     "mmhip_moe_ffn": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _u32,
@@ -546,6 +574,50 @@ class Context:
                                           p[0], n_given, p[1], p[2], top, p[3], p[4], p[5],
                                           0 if workspace is None else workspace.nbytes), "mmhip_logprobs_dev")
 
+    # -- the two ends of a decode step --
+    def embed_dev(self, y, table, ggml_type: int, rows: int, cols: int, tokens, n_tokens: int, scale: float = 1.0,
+                  y_stride: Optional[int] = None, y_offset: int = 0):
+        """mmhip_embed_dev: y[t] = scale * row tokens[t] of a table of raw blocks (embedToken, inference.zig:388)."""
+        check(self.lib.mmhip_embed_dev(self.handle, y.ptr + y_offset, cols if y_stride is None else y_stride, table.ptr,
+                                       ggml_type, rows, cols, tokens.ptr, n_tokens, scale), "mmhip_embed_dev")
+
+    def kv_plan_workspace(self, n_requests: int) -> int:
+        return self.lib.mmhip_kv_plan_workspace(self.handle, n_requests)
+
+    def kv_plan_args(self, *, n_requests: int, lens, new, next_lens, tables, table_pages: int, page_tokens: int,
+                     n_pages: int, free, free_count, next_free_count, max_tokens: int, positions, slots, table_of, seen,
+                     firsts, granted, workspace, release=None, shared=None, last=None,
+                     table_stride: Optional[int] = None) -> KvPlan:
+        """The mmhip_kv_plan that kv_plan_dev takes (built once, reusable; it keeps the buffers alive)."""
+        a = KvPlan(n_requests, page_tokens, n_pages, table_pages, lens.ptr, new.ptr, _optional(release),
+                   _optional(shared), next_lens.ptr, tables.ptr, table_pages if table_stride is None else table_stride,
+                   free.ptr, free_count.ptr, next_free_count.ptr, max_tokens, positions.ptr, slots.ptr, table_of.ptr,
+                   seen.ptr, firsts.ptr, granted.ptr, _optional(last), workspace.ptr, workspace.nbytes)
+        a._keep = (lens, new, release, shared, next_lens, tables, free, free_count, next_free_count, positions, slots,
+                   table_of, seen, firsts, granted, last, workspace)
+        return a
+
+    def kv_plan_dev(self, args: KvPlan):
+        """mmhip_kv_plan_dev: pages, slots and positions of a step's tokens from the requests' lengths."""
+        check(self.lib.mmhip_kv_plan_dev(self.handle, ctypes.byref(args)), "mmhip_kv_plan_dev")
+
+    def sample_workspace(self, n_rows: int, vocab: int) -> int:
+        return self.lib.mmhip_sample_workspace(self.handle, n_rows, vocab)
+
+    def sample_args(self, *, logits, n_rows: int, vocab: int, uniform, tokens, workspace=None, stride: Optional[int] = None,
+                    rows=None, n_logits: int = 0, temperature=None, top_k=None, top_p=None, min_p=None, probs=None,
+                    kept=None) -> Sample:
+        """The mmhip_sample that sample_dev takes (built once, reusable; it keeps the buffers alive)."""
+        a = Sample(logits.ptr, vocab if stride is None else stride, n_rows, vocab, _optional(rows), n_logits,
+                   _optional(temperature), _optional(top_k), _optional(top_p), _optional(min_p), uniform.ptr, tokens.ptr,
+                   _optional(probs), _optional(kept), _optional(workspace), 0 if workspace is None else workspace.nbytes)
+        a._keep = (logits, uniform, tokens, workspace, rows, temperature, top_k, top_p, min_p, probs, kept)
+        return a
+
+    def sample_dev(self, args: Sample):
+        """mmhip_sample_dev: a token of each row by temperature, top-k, top-p, min-p and a given random number."""
+        check(self.lib.mmhip_sample_dev(self.handle, ctypes.byref(args)), "mmhip_sample_dev")
+
 
 ROPE_LAYOUT = dict(interleaved=0, half=1)
 ROPE_SCALING = dict(none=0, linear=1, yarn=2)
@@ -930,11 +1002,23 @@ def make_iq2_xxs(rng: np.random.Generator, rows: int, cols: int, count: int = 1,
     return sb.reshape(-1)
 
 
+def make_4bit(rng: np.random.Generator, rows: int, cols: int, count: int = 1, d_sigma: float = 0.005) -> np.ndarray:
+    """Q4_0 or IQ4_NL blocks: random codes, d = f16(|N(0, d_sigma)|)."""
+    assert cols % 32 == 0
+    n = count * rows * (cols // 32)
+    blk = np.empty((n, 18), dtype=np.uint8)
+    blk[:, 0:2] = f16_bits(np.abs(rng.normal(0.0, d_sigma, n))).view(np.uint8).reshape(n, 2)
+    blk[:, 2:] = rng.integers(0, 256, (n, 16), dtype=np.uint8)
+    return blk.reshape(-1)
+
+
 def make_weight(rng: np.random.Generator, ggml_type: int, rows: int, cols: int, count: int = 1) -> np.ndarray:
     if ggml_type == Q8_0:
         return make_q8_0(rng, rows, cols, count)
     if ggml_type == IQ2_XXS:
         return make_iq2_xxs(rng, rows, cols, count)
+    if ggml_type in (Q4_0, IQ4_NL):
+        return make_4bit(rng, rows, cols, count, 0.005 if ggml_type == Q4_0 else 0.0006)
     if ggml_type == F32:
         return rng.normal(0.0, 0.02, count * rows * cols).astype(np.float32).view(np.uint8)
     if ggml_type == F16:

@@ -161,6 +161,57 @@ pub const mmhip_mla_attention = extern struct {
 };
 pub const MlaAttention = mmhip_mla_attention;
 
+pub const mmhip_kv_plan = extern struct {
+    n_requests: u32,
+    page_tokens: u32,
+    n_pages: u32,
+    table_pages: u32,
+    lens_dev: ?[*]const u32,
+    new_dev: ?[*]const u32,
+    release_dev: ?[*]const u32 = null,
+    shared_dev: ?[*]const u32 = null,
+    next_lens_dev: ?[*]u32,
+    tables_dev: ?[*]i32,
+    table_stride: u64,
+    free_dev: ?[*]i32,
+    free_count_dev: ?*const u32,
+    next_free_count_dev: ?*u32,
+    max_tokens: u32,
+    positions_dev: ?[*]u32,
+    slots_dev: ?[*]i32,
+    table_of_dev: ?[*]u32,
+    seen_dev: ?[*]u32,
+    firsts_dev: ?[*]u32,
+    granted_dev: ?[*]u32,
+    last_dev: ?[*]u32 = null,
+    workspace_dev: ?*anyopaque,
+    workspace_bytes: u64,
+};
+pub const KvPlan = mmhip_kv_plan;
+
+pub const mmhip_sample = extern struct {
+    logits_dev: ?[*]const f32,
+    stride: u64,
+    n_rows: u64,
+    vocab: u64,
+    rows_dev: ?[*]const u32 = null,
+    n_logits: u64 = 0,
+    temperature_dev: ?[*]const f32 = null,
+    top_k_dev: ?[*]const u32 = null,
+    top_p_dev: ?[*]const f32 = null,
+    min_p_dev: ?[*]const f32 = null,
+    uniform_dev: ?[*]const f32,
+    tokens_dev: ?[*]u32,
+    probs_dev: ?[*]f32 = null,
+    kept_dev: ?[*]u32 = null,
+    workspace_dev: ?*anyopaque,
+    workspace_bytes: u64,
+};
+pub const Sample = mmhip_sample;
+
+/// A token or row number that is not there (MMHIP_NO_TOKEN).
+pub const no_token: u32 = 0xFFFFFFFF;
+
 pub const max_moe_tokens: u32 = 256;
 
 extern fn mmhip_last_error() [*:0]const u8;
@@ -223,6 +274,11 @@ extern fn mmhip_mla_attention_workspace(ctx: *Ctx, n_tokens: u32, n_heads: u32, 
 extern fn mmhip_mla_attention_dev(ctx: *Ctx, args: *const mmhip_mla_attention) c_int;
 extern fn mmhip_logprobs_workspace(ctx: *Ctx, n_rows: u64, vocab: u64, top: u32) u64;
 extern fn mmhip_logprobs_dev(ctx: *Ctx, logits_dev: ?[*]const f32, stride: u64, n_rows: u64, vocab: u64, tokens_dev: ?[*]const u32, n_given: u64, token_logprobs_dev: ?[*]f32, entropy_dev: ?[*]f32, top: u32, top_ids_dev: ?[*]u32, top_logprobs_dev: ?[*]f32, workspace_dev: ?*anyopaque, workspace_bytes: u64) c_int;
+extern fn mmhip_embed_dev(ctx: *Ctx, y_dev: ?[*]f32, y_stride: u64, table_dev: ?*const anyopaque, type_: u32, rows: u64, cols: u32, tokens_dev: ?[*]const u32, n_tokens: u64, scale: f32) c_int;
+extern fn mmhip_kv_plan_workspace(ctx: *Ctx, n_requests: u32) u64;
+extern fn mmhip_kv_plan_dev(ctx: *Ctx, args: *const mmhip_kv_plan) c_int;
+extern fn mmhip_sample_workspace(ctx: *Ctx, n_rows: u64, vocab: u64) u64;
+extern fn mmhip_sample_dev(ctx: *Ctx, args: *const mmhip_sample) c_int;
 extern fn mmhip_moe_layer_create(ctx: *Ctx, wts: *const MoeWeights, out_layer: *?*MoeLayerHandle) c_int;
 extern fn mmhip_moe_layer_destroy(ctx: *Ctx, layer: ?*MoeLayerHandle) void;
 extern fn mmhip_moe_ffn(ctx: *Ctx, layer: *MoeLayerHandle, hidden_host: [*]const f32, out_host: [*]f32, n_tokens: u32, rp: ?*const RouteParams, route_ids_host: ?[*]u32, route_weights_host: ?[*]f32) c_int;
@@ -286,7 +342,7 @@ pub const HipBackend = struct {
     }
 
     /// matVecMulUnified (inference.zig:1200-1228) on the device: out = W . x
-    /// for Q8_0 / IQ2_XXS / F32 / F16 weights given as mmap'd GGUF bytes.
+    /// for Q8_0 / Q4_0 / IQ4_NL / IQ2_XXS / F32 / F16 weights given as mmap'd GGUF bytes.
     /// The weight is uploaded on first use and stays resident, keyed by its
     /// host address (getOrUploadMatBuffer's role).
     pub fn matVecMulUnified(self: *Self, out: []f32, ptr: [*]const u8, type_: gguf.GgmlType, x: []const f32, out_dim: usize, in_dim: usize) !void {
@@ -440,6 +496,31 @@ pub const HipBackend = struct {
 
     pub fn logprobsWorkspace(self: *Self, n_rows: u64, vocab: u64, top: u32) u64 {
         return mmhip_logprobs_workspace(self.ctx, n_rows, vocab, top);
+    }
+
+    /// embedToken (inference.zig:388) for n_tokens tokens: rows of a table of raw
+    /// GGUF bytes in device memory, times scale; y_dev rows y_stride floats apart.
+    pub fn embedDev(self: *Self, y_dev: [*]f32, y_stride: u64, table_dev: *const anyopaque, type_: u32, rows: u64, cols: u32, tokens_dev: [*]const u32, n_tokens: u64, scale: f32) !void {
+        try check(mmhip_embed_dev(self.ctx, y_dev, y_stride, table_dev, type_, rows, cols, tokens_dev, n_tokens, scale));
+    }
+
+    /// Pages, slots and positions of a step's tokens from the requests' lengths.
+    pub fn kvPlanDev(self: *Self, args: *const KvPlan) !void {
+        try check(mmhip_kv_plan_dev(self.ctx, args));
+    }
+
+    pub fn kvPlanWorkspace(self: *Self, n_requests: u32) u64 {
+        return mmhip_kv_plan_workspace(self.ctx, n_requests);
+    }
+
+    /// sampleGreedy's place (inference.zig:376-386) with temperature, top-k,
+    /// top-p, min-p and given random numbers, a token for each row of logits.
+    pub fn sampleDev(self: *Self, args: *const Sample) !void {
+        try check(mmhip_sample_dev(self.ctx, args));
+    }
+
+    pub fn sampleWorkspace(self: *Self, n_rows: u64, vocab: u64) u64 {
+        return mmhip_sample_workspace(self.ctx, n_rows, vocab);
     }
 
     /// Drops the resident copy of a weight (e.g. before unmapping the file).
