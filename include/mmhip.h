@@ -618,8 +618,8 @@ int mmhip_kv_plan_dev(mmhip_ctx* ctx, const mmhip_kv_plan* args);
  * all weigh the same and finite logits nothing. A row without a logit above
  * -infinity, settings out of range (T outside [0, f32's largest], top_p < 0,
  * min_p or uniform outside [0, 1] and [0, 1), a NaN) and a row number that the
- * logits do not have give MMHIP_NO_TOKEN, NaN and 0, and are reported. stride in
- * floats, at least vocab. Outputs and workspace overlap neither the inputs nor
+ * logits do not have give MMHIP_NO_TOKEN, NaN and 0, and are reported. Fewer than
+ * 2^22 rows; stride in floats, at least vocab. Outputs and workspace overlap neither the inputs nor
  * each other. */
 #define MMHIP_SAMPLE_MAX_VOCAB (1u << 24)
 typedef struct {

@@ -11,6 +11,8 @@
 // A comparison of sums must not depend on how they were taken, so weights are
 // computed in 64 bits (weight()) and summed as whole multiples of 2^-shift
 // (44 for up to 2^18 tokens): integer sums have no order.
+#include <algorithm>
+
 #include "device_common.hpp"
 #include "kernels.hpp"
 #include "lanes.hpp"
@@ -19,8 +21,14 @@ namespace mmhip {
 
 namespace {
 
-constexpr uint32_t kSmThreads = 1024, kSmWaves = kSmThreads / 64;
-constexpr uint32_t kSmDigit = 11, kSmBins = 1u << kSmDigit;
+// Threads of the launches over pieces, and of those over rows.
+constexpr uint32_t kSmPiece = 256, kSmThreads = 1024, kSmWaves = kSmThreads / 64;
+constexpr uint32_t kSmChunk = 1024;      // logits that a wave takes at a time
+constexpr uint32_t kSmBins = 1024;       // of the row's histogram
+constexpr uint32_t kSmMostPieces = 1024;
+constexpr uint32_t kSmWorkgroups = 2048; // pieces of a call that are enough
+constexpr uint32_t kSmPerThread = 8;     // tokens beside the cut that a thread of the last launch takes
+constexpr uint32_t kSmList = kSmPerThread * kSmThreads;
 
 // A logit's place in the order: larger is earlier, equal ones by the lower id.
 // NaN and -infinity, which are never drawn, are below kLeastKey.
@@ -64,54 +72,369 @@ __device__ __forceinline__ uint64_t whole_weight(double z, int shift) {
     return __double_as_longlong(weight(z, shift) + 0x1p52) & 0xFFFFFFFFFFFFFull;
 }
 
+template <uint32_t WAVES>
 __device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t* red) {
     __syncthreads();
     v = wave_scan(v);
     if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t all = 0;
-    for (uint32_t w = 0; w < kSmWaves; ++w) all += red[w];
+    for (uint32_t w = 0; w < WAVES; ++w) all += red[w];
     return all;
 }
-__device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* red) {
+// Over threads 0 .. this one.
+template <uint32_t WAVES>
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* red, uint64_t& all) {
     __syncthreads();
+    v = wave_scan(v);
+    if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    uint64_t before = 0;
+    all = 0;
+    for (uint32_t w = 0; w < WAVES; ++w) {
+        if (w < threadIdx.x >> 6) before += red[w];
+        all += red[w];
+    }
+    return before + v;
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
 #pragma unroll
     for (int off = 32; off; off >>= 1) v = max(v, (uint64_t)__shfl_xor((unsigned long long)v, off, 64));
+    return v;
+}
+template <uint32_t WAVES>
+__device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* red) {
+    __syncthreads();
+    v = wave_max(v);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t all = 0;
-    for (uint32_t w = 0; w < kSmWaves; ++w) all = max(all, red[w]);
+    for (uint32_t w = 0; w < WAVES; ++w) all = max(all, red[w]);
     return all;
 }
 
+// What a row asks for.
+enum SmMode : uint32_t { kSmAbsent, kSmNoRow, kSmBadSetting, kSmEmpty, kSmFirst, kSmAll, kSmCut };
 struct RowSettings {
-    float m;
+    SmMode mode;
+    const float* x;
+    uint64_t best;  // the first token's key
+    float m, bin_c;
     double inv_t, least_z;
+    float p, u;
+    uint32_t k;     // 0: no cut by number
+    bool by_mass;   // a cut by probability
     int shift;
 };
 
+struct SmRow {
+    uint32_t listed;           // tokens in bins beside a cut (at most kSmList are in the list)
+    uint32_t k_bin, k_rank;    // the cut by number: the bin, and which of its tokens is the last
+    uint32_t p_lo, p_hi;       // the cut by probability: the bins that it may be in
+    uint64_t k_mass, p_mass;   // of the tokens in bins before k_bin, before p_lo
+};
+struct SmPlan {
+    uint32_t chunks, pieces, list;
+    uint64_t* best;            // [rows][pieces]
+    float* lowest;             // [rows][pieces]
+    unsigned long long* mass;  // [rows][kSmBins]
+    uint32_t* count;           // [rows][kSmBins]
+    uint64_t* chunk_mass;      // [rows][chunks]: kept for certain
+    uint32_t* chunk_count;     // [rows][chunks]
+    uint64_t* keys;            // [rows][list]
+    SmRow* rows;
+};
+constexpr uint32_t kNoBin = 0xFFFFFFFFu;
+
+// A row's settings, from those of its pieces' largest and lowest logits. For the
+// whole workgroup.
+template <uint32_t WAVES>
+__device__ __forceinline__ RowSettings row_settings(const SampleArgs& a, const SmPlan& p, uint32_t out, uint64_t* red) {
+    RowSettings s{};
+    uint32_t row = out;
+    if (a.rows) row = a.rows[out];
+    const float t = a.temperature ? a.temperature[out] : 1.0f, least = a.min_p ? a.min_p[out] : 0.0f;
+    s.p = a.top_p ? a.top_p[out] : 1.0f;
+    s.u = a.uniform[out];
+    s.k = a.top_k ? a.top_k[out] : 0;
+    uint64_t best = 0;
+    float low = INFINITY;
+    for (uint32_t i = threadIdx.x; i < p.pieces; i += WAVES * 64) {
+        best = max(best, p.best[(uint64_t)out * p.pieces + i]);
+        low = fminf(low, p.lowest[(uint64_t)out * p.pieces + i]);
+    }
+    s.best = block_max<WAVES>(best, red);
+    low = -key_value(block_max<WAVES>(order_bits(-low), red) << 32);
+    if (a.rows && row == kNoToken) s.mode = kSmAbsent;
+    else if (a.rows && row >= a.n_logits) s.mode = kSmNoRow;
+    else if (!(t >= 0.0f && t <= 3.4028235e38f && s.p >= 0.0f && least >= 0.0f && least <= 1.0f && s.u >= 0.0f && s.u < 1.0f))
+        s.mode = kSmBadSetting;
+    else if (s.best < kLeastKey) s.mode = kSmEmpty;
+    else if (t == 0.0f || s.k == 1) s.mode = kSmFirst;
+    else {
+        if (s.k >= a.vocab) s.k = 0;
+        s.by_mass = s.p < 1.0f;
+        s.mode = s.k || s.by_mass ? kSmCut : kSmAll;
+    }
+    if (s.mode < kSmFirst) return s;
+    s.x = a.logits + row * a.stride;
+    s.m = key_value(s.best);
+    s.inv_t = 1.0 / (double)t;
+    s.least_z = log((double)least);
+    s.shift = a.shift;
+    // Bins of 1/32 of the temperature next to the largest logit, twice as wide
+    // from four temperatures below it on, and so on; narrower ones where the
+    // row's logits are closer together than that.
+    s.bin_c = fminf(fmaxf(0.25f / t, 7.0f / (s.m - low)), 1e30f);
+    return s;
+}
+// The bin of a logit: never smaller for a smaller logit.
+__device__ __forceinline__ uint32_t bin_of(float x, const RowSettings& s) {
+    const float d = s.m - x;
+    const float y = x == s.m ? 1.0f : fminf(fmaf(d, s.bin_c, 1.0f), 255.9f);
+    return min((__float_as_uint(y) - 0x3F800000u) >> 16, kSmBins - 1);
+}
+__device__ __forceinline__ uint64_t mass_target(float p, uint64_t sum) {
+    return max((uint64_t)ceil((double)p * (double)sum), (uint64_t)1);
+}
+
+// A wave's chunk: logit i * 64 + lane, NaN where there is none.
+__device__ __forceinline__ void load_chunk(const float* x, uint32_t vocab, uint32_t chunk, float (&v)[kSmChunk / 64]) {
+    const uint32_t first = chunk * kSmChunk, n = min(vocab - first, kSmChunk), lane = threadIdx.x & 63;
+    const BufRsrc r = make_rsrc(x + first, n * 4);
+#pragma unroll
+    for (uint32_t i = 0; i < kSmChunk / 64; ++i) v[i] = __uint_as_float(buf_load_b32(r, lane * 4, i * 256));
+#pragma unroll
+    for (uint32_t i = 0; i < kSmChunk / 64; ++i)
+        if (i * 64 + lane >= n) v[i] = __builtin_nanf("");
+}
+
+// The largest and lowest logits of a piece, and the row's memory cleared.
+__global__ __launch_bounds__(kSmPiece) void sample_best_kernel(SampleArgs a, SmPlan p) {
+    __shared__ uint64_t red[2][kSmPiece / 64];
+    const uint32_t out = blockIdx.x / p.pieces, piece = blockIdx.x - out * p.pieces;
+    const uint32_t c0 = (uint32_t)((uint64_t)piece * p.chunks / p.pieces), c1 = (uint32_t)((uint64_t)(piece + 1) * p.chunks / p.pieces);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (uint32_t i = piece * kSmPiece + threadIdx.x; i < kSmBins; i += p.pieces * kSmPiece) {
+        p.mass[(uint64_t)out * kSmBins + i] = 0;
+        p.count[(uint64_t)out * kSmBins + i] = 0;
+    }
+    if (piece == 0 && threadIdx.x == 0) p.rows[out].listed = 0;
+    uint32_t row = out;
+    if (a.rows) row = a.rows[out];
+    uint32_t bits = 0, id = 0;
+    float low = INFINITY;
+    if (!a.rows || row < a.n_logits) {
+        const float* x = a.logits + row * a.stride;
+        for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
+            float v[kSmChunk / 64];
+            load_chunk(x, a.vocab, c, v);
+#pragma unroll
+            for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
+                const uint32_t b = order_bits(v[i]);
+                if (b > bits) bits = b, id = c * kSmChunk + i * 64 + lane;
+                if (v[i] > -INFINITY) low = fminf(low, v[i]);
+            }
+        }
+    }
+    const uint64_t best = wave_max((uint64_t)bits << 32 | (0xFFFFFFFFu - id)), lowest = wave_max((uint64_t)order_bits(-low));
+    if (lane == 0) red[0][wave] = best, red[1][wave] = lowest;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint64_t b = 0, l = 0;
+        for (uint32_t w = 0; w < kSmPiece / 64; ++w) b = max(b, red[0][w]), l = max(l, red[1][w]);
+        p.best[blockIdx.x] = b;
+        p.lowest[blockIdx.x] = -key_value(l << 32);
+    }
+}
+
+// How many tokens, and how much of the weights, each bin of the row holds. Rows
+// without a cut: what each chunk keeps.
+__global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmPlan p) {
+    __shared__ uint64_t red[kSmPiece / 64];
+    __shared__ unsigned long long mass[kSmBins];
+    __shared__ uint32_t count[kSmBins];
+    const uint32_t out = blockIdx.x / p.pieces, piece = blockIdx.x - out * p.pieces;
+    const uint32_t c0 = (uint32_t)((uint64_t)piece * p.chunks / p.pieces), c1 = (uint32_t)((uint64_t)(piece + 1) * p.chunks / p.pieces);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const RowSettings s = row_settings<kSmPiece / 64>(a, p, out, red);
+    if (s.mode < kSmAll) return;
+    if (s.mode == kSmAll) {
+        for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
+            float v[kSmChunk / 64];
+            load_chunk(s.x, a.vocab, c, v);
+            uint64_t sum = 0;
+            uint32_t n = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
+                const double z = scaled(v[i], s.m, s.inv_t);
+                if (v[i] > -INFINITY && z >= s.least_z) {
+                    sum += whole_weight(z, s.shift);
+                    n += 1;
+                }
+            }
+            sum = wave_scan(sum);
+            n = (uint32_t)wave_scan(n);
+            if (lane == 63) {
+                p.chunk_mass[(uint64_t)out * p.chunks + c] = sum;
+                p.chunk_count[(uint64_t)out * p.chunks + c] = n;
+            }
+        }
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < kSmBins; i += kSmPiece) mass[i] = 0, count[i] = 0;
+    __syncthreads();
+    for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
+        float v[kSmChunk / 64];
+        load_chunk(s.x, a.vocab, c, v);
+#pragma unroll
+        for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
+            if (!(v[i] > -INFINITY)) continue;
+            const uint32_t b = bin_of(v[i], s);
+            if (s.k) atomicAdd(&count[b], 1u);
+            if (s.by_mass) atomicAdd(&mass[b], (unsigned long long)whole_weight(scaled(v[i], s.m, s.inv_t), s.shift));
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < kSmBins; i += kSmPiece) {
+        if (count[i]) atomicAdd(&p.count[(uint64_t)out * kSmBins + i], count[i]);
+        if (mass[i]) atomicAdd(&p.mass[(uint64_t)out * kSmBins + i], mass[i]);
+    }
+}
+
+// The bins that the cuts are in: their tokens go into the row's list, and what
+// each chunk has in the bins before all of them is kept for certain.
+__global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmPlan p) {
+    constexpr uint32_t kWaves = kSmPiece / 64, kPer = kSmBins / kSmPiece;
+    __shared__ uint64_t red[kWaves];
+    __shared__ SmRow row;
+    __shared__ uint64_t k_here;
+    const uint32_t out = blockIdx.x / p.pieces, piece = blockIdx.x - out * p.pieces;
+    const uint32_t c0 = (uint32_t)((uint64_t)piece * p.chunks / p.pieces), c1 = (uint32_t)((uint64_t)(piece + 1) * p.chunks / p.pieces);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = threadIdx.x;
+    const RowSettings s = row_settings<kWaves>(a, p, out, red);
+    if (s.mode != kSmCut) return;
+    if (tid == 0) {
+        row = SmRow{0, kNoBin, 0, kNoBin, kNoBin, 0, 0};
+        k_here = 0;
+    }
+    uint64_t m[kPer], all_mass = 0, sum = 0;
+    uint32_t n[kPer];
+    uint64_t num = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) {
+        m[i] = p.mass[(uint64_t)out * kSmBins + tid * kPer + i];
+        n[i] = p.count[(uint64_t)out * kSmBins + tid * kPer + i];
+        sum += m[i];
+        num += n[i];
+    }
+    const uint64_t mass_to = block_scan<kWaves>(sum, red, all_mass) - sum;
+    uint64_t all_num;
+    const uint64_t num_to = block_scan<kWaves>(num, red, all_num) - num;
+    __syncthreads();
+    if (s.k && s.k < all_num) {
+        uint64_t at = num_to, w = mass_to;
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) {
+            if (at < s.k && s.k <= at + n[i]) {
+                row.k_bin = tid * kPer + i;
+                row.k_rank = (uint32_t)(s.k - at);
+                row.k_mass = w;
+                k_here = m[i];
+            }
+            at += n[i];
+            w += m[i];
+        }
+    }
+    __syncthreads();
+    if (s.by_mass) {
+        // The sum that the cut is a part of, at least and at most.
+        const bool by_k = row.k_bin != kNoBin;
+        const uint64_t lo = mass_target(s.p, by_k ? row.k_mass : all_mass), hi = mass_target(s.p, by_k ? row.k_mass + k_here : all_mass);
+        uint64_t w = mass_to;
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) {
+            if (w < lo && lo <= w + m[i]) {
+                row.p_lo = tid * kPer + i;
+                row.p_mass = w;
+            }
+            if (w < hi && hi <= w + m[i]) row.p_hi = tid * kPer + i;
+            w += m[i];
+        }
+        __syncthreads();
+    }
+    const SmRow r = row;
+    if (piece == 0 && tid == 0) {
+        SmRow* to = &p.rows[out];
+        to->k_bin = r.k_bin;
+        to->k_rank = r.k_rank;
+        to->p_lo = r.p_lo;
+        to->p_hi = r.p_hi;
+        to->k_mass = r.k_mass;
+        to->p_mass = r.p_mass;
+    }
+    const uint32_t sure = min(r.k_bin, r.p_lo);
+    for (uint32_t c = c0 + wave; c < c1; c += kWaves) {
+        float v[kSmChunk / 64];
+        load_chunk(s.x, a.vocab, c, v);
+        uint64_t mine = 0;
+        uint32_t kept = 0, to_list = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
+            if (!(v[i] > -INFINITY)) continue;
+            const uint32_t b = bin_of(v[i], s);
+            if (b < sure) {
+                const double z = scaled(v[i], s.m, s.inv_t);
+                if (z >= s.least_z) {
+                    mine += whole_weight(z, s.shift);
+                    kept += 1;
+                }
+            } else if (b == r.k_bin || (b >= r.p_lo && b <= r.p_hi)) {
+                to_list |= 1u << i;
+            }
+        }
+        mine = wave_scan(mine);
+        kept = (uint32_t)wave_scan(kept);
+        if (lane == 63) {
+            p.chunk_mass[(uint64_t)out * p.chunks + c] = mine;
+            p.chunk_count[(uint64_t)out * p.chunks + c] = kept;
+        }
+        const uint32_t here = (uint32_t)__popc(to_list);
+        if (__ballot(here != 0) == 0) continue;
+        const uint32_t to = (uint32_t)wave_scan(here);
+        uint32_t at = 0;
+        if (lane == 63) at = atomicAdd(&p.rows[out].listed, to);
+        at = (uint32_t)__shfl((int)at, 63, 64) + to - here;
+#pragma unroll
+        for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
+            if (!(to_list >> i & 1u)) continue;
+            if (at < p.list) p.keys[(uint64_t)out * p.list + at] = order_key(v[i], c * kSmChunk + i * 64 + lane);
+            ++at;
+        }
+    }
+}
+
+// The key at which the running total of keys >= floor of the row, largest first,
+// reaches `target`: of tokens (MASS false) or of weights. 64-bit keys in digits of
+// ten bits, each by a histogram of the row's keys with the digits before it: for
+// rows with more tokens in one bin than the list holds.
 struct Bins {
     unsigned long long mass[kSmBins];
     uint32_t count[kSmBins];
-    uint32_t found;
+    uint32_t found, found_n;
     uint64_t above;
 };
-
-// The key at which the running total of keys >= floor in descending order first
-// reaches `target`: of tokens (MASS false) or of weights. 64-bit keys in six digits
-// of 11 bits, each by a histogram of the row's keys with the digits before it.
 template <bool MASS>
-__device__ uint64_t find_cut(const float* x, uint32_t vocab, const RowSettings& s, uint64_t floor, uint64_t target, Bins& b) {
+__device__ uint64_t find_cut(const RowSettings& s, uint32_t vocab, uint64_t floor, uint64_t target, Bins& b) {
     uint64_t prefix = 0, before = 0;
-    for (int level = 0; level < 6; ++level) {
-        const int low = level == 5 ? 0 : 53 - 11 * level, bits = level == 5 ? 9 : 11;
+    for (int low = 54, bits = 10;; bits = low < 10 ? 4 : 10, low -= bits) {
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < kSmBins; i += kSmThreads) b.mass[i] = 0, b.count[i] = 0;
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < vocab; i += kSmThreads) {
-            const float v = x[i];
+            const float v = s.x[i];
             const uint64_t k = order_key(v, i);
-            if (k < floor || (level && (k >> (low + bits)) != prefix)) continue;
+            if (k < floor || (low < 54 && (k >> (low + bits)) != prefix)) continue;
             const uint32_t at = (uint32_t)(k >> low) & ((1u << bits) - 1);
             atomicAdd(&b.count[at], 1u);
             if (MASS) atomicAdd(&b.mass[at], (unsigned long long)whole_weight(scaled(v, s.m, s.inv_t), s.shift));
@@ -134,105 +457,254 @@ __device__ uint64_t find_cut(const float* x, uint32_t vocab, const RowSettings& 
         __syncthreads();
         prefix = prefix << bits | b.found;
         before = b.above;
+        if (low == 0) return prefix;
     }
-    return prefix;
 }
 
-__global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SampleArgs a) {
+// The same among the keys that a workgroup's threads hold (those of `in`), by
+// their distance from the largest of them: 1024 bins over the distances that are
+// left, until one is left or distances are told apart to the last bit. Ends with
+// what is above the key in *above.
+template <bool MASS>
+__device__ uint64_t find_listed(const uint64_t (&key)[kSmPerThread], const uint64_t (&w)[kSmPerThread], uint32_t in, uint64_t target,
+                                Bins& b, uint64_t* red, uint64_t& above) {
+    uint64_t top = 0, low = ~0ull;
+#pragma unroll
+    for (uint32_t i = 0; i < kSmPerThread; ++i)
+        if (in >> i & 1u) top = max(top, key[i]), low = min(low, key[i]);
+    top = block_max<kSmWaves>(top, red);
+    low = ~block_max<kSmWaves>(~low, red);
+    above = 0;
+    // Each turn leaves at most a 1024th of the span: seven for 64 bits.
+    for (int turn = 0; turn < 7; ++turn) {
+        const uint64_t span = top - low;
+        const uint32_t sh = span < kSmBins ? 0 : 54 - (uint32_t)__clzll((long long)span);
+        __syncthreads();
+        b.mass[threadIdx.x] = 0;
+        b.count[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kSmPerThread; ++i)
+            if (in >> i & 1u) {
+                const uint32_t at = (uint32_t)((top - key[i]) >> sh);
+                atomicAdd(&b.count[at], 1u);
+                if (MASS) atomicAdd(&b.mass[at], (unsigned long long)w[i]);
+            }
+        __syncthreads();
+        const uint64_t here = MASS ? b.mass[threadIdx.x] : b.count[threadIdx.x];
+        uint64_t all;
+        const uint64_t to = above + block_scan<kSmWaves>(here, red, all);
+        if (to - here < target && target <= to) {
+            b.found = threadIdx.x;
+            b.found_n = b.count[threadIdx.x];
+            b.above = to - here;
+        }
+        __syncthreads();
+        const uint32_t at = b.found;
+        above = b.above;
+        if (sh == 0) return top - at;
+        uint64_t one = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kSmPerThread; ++i) {
+            if ((in >> i & 1u) && (uint32_t)((top - key[i]) >> sh) != at) in &= ~(1u << i);
+            if (in >> i & 1u) one = key[i];
+        }
+        if (b.found_n == 1) return block_max<kSmWaves>(one, red);
+        const uint64_t end = top - ((uint64_t)at << sh), last = end - (((uint64_t)1 << sh) - 1);
+        low = max(low, last);  // (of two different integer types max would go through doubles)
+        top = end;
+    }
+    return top;
+}
+
+// One workgroup per row: the cut among the listed tokens, the chunk in which the
+// running sum passes u times all, and the token in it.
+__global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, SmPlan p) {
     __shared__ uint64_t red[kSmWaves];
     __shared__ Bins bins;
+    __shared__ uint32_t found;
+    __shared__ uint64_t found_before;
     const uint32_t out = blockIdx.x, tid = threadIdx.x;
-    uint32_t row = out;
-    if (a.rows) {
-        row = a.rows[out];
-        if (row == kNoToken) return;
-        if (row >= a.n_logits) {
-            if (tid == 0) {
-                report(a.status, kBadSampleRow);
-                a.tokens[out] = kNoToken;
-                if (a.probs) a.probs[out] = __builtin_nanf("");
-                if (a.kept) a.kept[out] = 0;
-            }
-            return;
-        }
-    }
-    const float* x = a.logits + row * a.stride;
-    const float t = a.temperature ? a.temperature[out] : 1.0f, p = a.top_p ? a.top_p[out] : 1.0f;
-    const float min_p = a.min_p ? a.min_p[out] : 0.0f, u = a.uniform[out];
-    uint32_t k = a.top_k ? a.top_k[out] : 0;
-    const bool ok = t >= 0.0f && t <= 3.4028235e38f && p >= 0.0f && min_p >= 0.0f && min_p <= 1.0f && u >= 0.0f && u < 1.0f;
-    uint64_t best = 0;
-    for (uint32_t i = tid; i < a.vocab; i += kSmThreads) best = max(best, order_key(x[i], i));
-    best = block_max(best, red);
-    if (!ok || best < kLeastKey) {
+    const RowSettings s = row_settings<kSmWaves>(a, p, out, red);
+    if (s.mode == kSmAbsent) return;
+    if (s.mode < kSmAll) {
         if (tid == 0) {
-            report(a.status, ok ? kNoSampleToken : kBadSampleSetting);
-            a.tokens[out] = kNoToken;
-            if (a.probs) a.probs[out] = __builtin_nanf("");
-            if (a.kept) a.kept[out] = 0;
+            const bool first = s.mode == kSmFirst;
+            if (!first) report(a.status, s.mode == kSmNoRow ? kBadSampleRow : s.mode == kSmBadSetting ? kBadSampleSetting : kNoSampleToken);
+            a.tokens[out] = first ? 0xFFFFFFFFu - (uint32_t)s.best : kNoToken;
+            if (a.probs) a.probs[out] = first ? 1.0f : __builtin_nanf("");
+            if (a.kept) a.kept[out] = first;
         }
         return;
     }
-    if (t == 0.0f || k == 1) {
-        if (tid == 0) {
-            a.tokens[out] = 0xFFFFFFFFu - (uint32_t)best;
-            if (a.probs) a.probs[out] = 1.0f;
-            if (a.kept) a.kept[out] = 1;
-        }
-        return;
-    }
-    const RowSettings s{key_value(best), 1.0 / (double)t, log((double)min_p), a.shift};
     uint64_t cut = kLeastKey;
-    if (k != 0 && k < a.vocab) cut = max(cut, find_cut<false>(x, a.vocab, s, cut, k, bins));
-    if (p < 1.0f) {
-        uint64_t sum = 0;
-        for (uint32_t i = tid; i < a.vocab; i += kSmThreads) {
-            const float v = x[i];
-            if (order_key(v, i) >= cut) sum += whole_weight(scaled(v, s.m, s.inv_t), s.shift);
-        }
-        sum = block_sum(sum, red);
-        cut = max(cut, find_cut<true>(x, a.vocab, s, cut, (uint64_t)ceil((double)p * (double)sum), bins));
-    }
-    const auto weight_of = [&](uint32_t i, uint64_t& kept) -> uint64_t {
-        const float v = x[i];
-        if (order_key(v, i) < cut) return 0;
-        const double z = scaled(v, s.m, s.inv_t);
-        if (!(z >= s.least_z)) return 0;
-        ++kept;
-        return whole_weight(z, s.shift);
-    };
-    uint64_t sum = 0, kept = 0;
-    for (uint32_t i = tid; i < a.vocab; i += kSmThreads) sum += weight_of(i, kept);
-    sum = block_sum(sum, red);
-    kept = block_sum(kept, red);
-    // The first id whose running sum is above u times all of it.
-    const uint64_t target = (uint64_t)((double)u * (double)sum);
-    uint64_t before = 0, none = 0;
-    for (uint32_t i0 = 0; i0 < a.vocab; i0 += kSmThreads) {
-        const uint32_t i = i0 + tid;
-        const uint64_t w = i < a.vocab ? weight_of(i, none) : 0;
-        const uint64_t all = block_sum(w, red);
-        if (before + all > target) {
-            const uint64_t in = wave_scan(w);
-            uint64_t here = before + in;
-            for (uint32_t v = 0; v < tid >> 6; ++v) here += red[v];
-            if (w && here > target && here - w <= target) {
-                a.tokens[out] = i;
-                if (a.probs) a.probs[out] = (float)(weight(scaled(x[i], s.m, s.inv_t), s.shift) / (double)sum);
-                if (a.kept) a.kept[out] = (uint32_t)kept;
+    uint64_t key[kSmPerThread], w[kSmPerThread];
+    uint32_t in = 0, in_k = 0, in_p = 0;
+    bool from_chunks = true;  // what the chunks keep for certain is in the workspace
+    if (s.mode == kSmCut) {
+        const SmRow r = p.rows[out];
+        if (r.listed <= p.list) {
+#pragma unroll
+            for (uint32_t i = 0; i < kSmPerThread; ++i) {
+                const uint32_t at = i * kSmThreads + tid;
+                key[i] = w[i] = 0;
+                if (at >= r.listed) continue;
+                key[i] = p.keys[(uint64_t)out * p.list + at];
+                const float v = key_value(key[i]);
+                const uint32_t b = bin_of(v, s);
+                w[i] = whole_weight(scaled(v, s.m, s.inv_t), s.shift);
+                in |= 1u << i;
+                in_k |= (uint32_t)(b == r.k_bin) << i;
+                in_p |= (uint32_t)(b >= r.p_lo && b <= r.p_hi) << i;
             }
-            return;
+            uint64_t above, sum = 0;
+            if (r.k_bin != kNoBin) {
+                cut = find_listed<false>(key, w, in_k, r.k_rank, bins, red, above);
+                if (s.by_mass) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kSmPerThread; ++i)
+                        if ((in_k >> i & 1u) && key[i] >= cut) sum += w[i];
+                    sum = r.k_mass + block_sum<kSmWaves>(sum, red);
+                }
+            } else if (s.by_mass) {
+                for (uint32_t i = tid; i < kSmBins; i += kSmThreads) sum += p.mass[(uint64_t)out * kSmBins + i];
+                sum = block_sum<kSmWaves>(sum, red);
+            }
+            if (s.by_mass) {
+#pragma unroll
+                for (uint32_t i = 0; i < kSmPerThread; ++i)
+                    if ((in_p >> i & 1u) && key[i] < cut) in_p &= ~(1u << i);
+                cut = max(cut, find_listed<true>(key, w, in_p, mass_target(s.p, sum) - r.p_mass, bins, red, above));
+            }
+        } else {
+            from_chunks = false;
+            in = 0;
+            if (s.k) cut = max(cut, find_cut<false>(s, a.vocab, cut, s.k, bins));
+            if (s.by_mass) {
+                uint64_t sum = 0;
+                for (uint32_t i = tid; i < a.vocab; i += kSmThreads) {
+                    const float v = s.x[i];
+                    if (order_key(v, i) >= cut) sum += whole_weight(scaled(v, s.m, s.inv_t), s.shift);
+                }
+                sum = block_sum<kSmWaves>(sum, red);
+                cut = max(cut, find_cut<true>(s, a.vocab, cut, mass_target(s.p, sum), bins));
+            }
         }
-        before += all;
     }
+    const auto weight_of = [&](uint32_t i) -> uint64_t {
+        if (i >= a.vocab) return 0;
+        const float v = s.x[i];
+        const double z = scaled(v, s.m, s.inv_t);
+        return order_key(v, i) >= cut && z >= s.least_z ? whole_weight(z, s.shift) : 0;
+    };
+    // Kept weights by group of chunks, a thread for each group.
+    const uint32_t per = (p.chunks + kSmThreads - 1) / kSmThreads;
+    uint64_t mine = 0, kept = 0;
+    if (!from_chunks) {
+        // (as the launches over pieces leave them where the list suffices)
+        for (uint32_t c = tid >> 6; c < p.chunks; c += kSmWaves) {
+            uint64_t sum = 0;
+            uint32_t n = 0;
+            for (uint32_t i = c * kSmChunk + (tid & 63); i < min((c + 1) * kSmChunk, a.vocab); i += 64) {
+                const float v = s.x[i];
+                const double z = scaled(v, s.m, s.inv_t);
+                if (order_key(v, i) >= cut && z >= s.least_z) sum += whole_weight(z, s.shift), ++n;
+            }
+            sum = wave_scan(sum);
+            n = (uint32_t)wave_scan(n);
+            if ((tid & 63) == 63) {
+                p.chunk_mass[(uint64_t)out * p.chunks + c] = sum;
+                p.chunk_count[(uint64_t)out * p.chunks + c] = n;
+            }
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    bins.mass[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kSmPerThread; ++i) {
+        if (!(in >> i & 1u)) continue;
+        if (key[i] < cut || !(scaled(key_value(key[i]), s.m, s.inv_t) >= s.least_z)) {
+            in &= ~(1u << i);
+            continue;
+        }
+        ++kept;
+        atomicAdd(&bins.mass[(0xFFFFFFFFu - (uint32_t)key[i]) / kSmChunk / per], (unsigned long long)w[i]);
+    }
+    for (uint32_t c = tid * per; c < min((tid + 1) * per, p.chunks); ++c) {
+        mine += p.chunk_mass[(uint64_t)out * p.chunks + c];
+        kept += p.chunk_count[(uint64_t)out * p.chunks + c];
+    }
+    __syncthreads();
+    mine += bins.mass[tid];
+    uint64_t sum;
+    const uint64_t to = block_scan<kSmWaves>(mine, red, sum);
+    const uint64_t target = (uint64_t)((double)s.u * (double)sum);
+    if (mine && to > target && to - mine <= target) found = tid, found_before = to - mine;
+    kept = block_sum<kSmWaves>(kept, red);
+    // The chunk of the group.
+    const uint32_t group = found;
+    uint64_t before = found_before;
+    uint32_t chunk = group * per;
+    if (per > 1) {
+        __syncthreads();
+        bins.mass[tid] = tid < per && chunk + tid < p.chunks ? p.chunk_mass[(uint64_t)out * p.chunks + chunk + tid] : 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kSmPerThread; ++i) {
+            const uint32_t c = (0xFFFFFFFFu - (uint32_t)key[i]) / kSmChunk;
+            if ((in >> i & 1u) && c / per == group) atomicAdd(&bins.mass[c - chunk], (unsigned long long)w[i]);
+        }
+        __syncthreads();
+        for (uint32_t c = 0; c + 1 < per && before + bins.mass[c] <= target; ++c) {
+            before += bins.mass[c];
+            ++chunk;
+        }
+    }
+    const uint32_t id = chunk * kSmChunk + tid;
+    const uint64_t here = weight_of(id);
+    uint64_t all;
+    const uint64_t now = before + block_scan<kSmWaves>(here, red, all);
+    if (here && now > target && now - here <= target) {
+        a.tokens[out] = id;
+        if (a.probs) a.probs[out] = (float)(weight(scaled(s.x[id], s.m, s.inv_t), s.shift) / (double)sum);
+        if (a.kept) a.kept[out] = (uint32_t)kept;
+    }
+}
+
+SmPlan sm_plan(uint64_t n_rows, uint64_t vocab) {
+    SmPlan p{};
+    p.chunks = (uint32_t)((vocab + kSmChunk - 1) / kSmChunk);
+    const uint64_t want = (kSmWorkgroups + n_rows - 1) / n_rows, most = (p.chunks + 3) / 4;
+    p.pieces = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(want, kSmMostPieces), most);
+    p.list = (uint32_t)std::min<uint64_t>(kSmList, vocab);
+    return p;
+}
+uint64_t sm_layout(SmPlan& p, uint64_t n_rows, uint8_t* base) {
+    uint64_t at = 0;
+    const auto take = [&](uint64_t bytes) {
+        uint8_t* here = base + at;
+        at += (bytes + 15) / 16 * 16;
+        return here;
+    };
+    p.best = reinterpret_cast<uint64_t*>(take(n_rows * p.pieces * 8));
+    p.lowest = reinterpret_cast<float*>(take(n_rows * p.pieces * 4));
+    p.mass = reinterpret_cast<unsigned long long*>(take(n_rows * kSmBins * 8));
+    p.count = reinterpret_cast<uint32_t*>(take(n_rows * kSmBins * 4));
+    p.chunk_mass = reinterpret_cast<uint64_t*>(take(n_rows * p.chunks * 8));
+    p.chunk_count = reinterpret_cast<uint32_t*>(take(n_rows * p.chunks * 4));
+    p.keys = reinterpret_cast<uint64_t*>(take(n_rows * p.list * 8));
+    p.rows = reinterpret_cast<SmRow*>(take(n_rows * sizeof(SmRow)));
+    return at;
 }
 
 }  // namespace
 
 uint64_t sample_workspace_bytes(uint64_t n_rows, uint64_t vocab) {
-    (void)n_rows;
-    (void)vocab;
-    return 0;
+    if (n_rows == 0 || vocab == 0) return 0;
+    SmPlan p = sm_plan(n_rows, vocab);
+    return sm_layout(p, n_rows, nullptr);
 }
 
 hipError_t launch_sample(const SampleArgs& a_in, uint64_t n_rows, hipStream_t s) {
@@ -241,7 +713,17 @@ hipError_t launch_sample(const SampleArgs& a_in, uint64_t n_rows, hipStream_t s)
     uint32_t bits = 0;
     while ((1ull << bits) < a.vocab) ++bits;
     a.shift = bits <= 18 ? 44 : 62 - bits;
-    sample_row_kernel<<<(unsigned)n_rows, kSmThreads, 0, s>>>(a);
+    SmPlan p = sm_plan(n_rows, a.vocab);
+    sm_layout(p, n_rows, static_cast<uint8_t*>(a.work));
+    const unsigned grid = (unsigned)(n_rows * p.pieces);
+    sample_best_kernel<<<grid, kSmPiece, 0, s>>>(a, p);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    sample_bins_kernel<<<grid, kSmPiece, 0, s>>>(a, p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    sample_list_kernel<<<grid, kSmPiece, 0, s>>>(a, p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    sample_draw_kernel<<<(unsigned)n_rows, kSmThreads, 0, s>>>(a, p);
     return hipGetLastError();
 }
 

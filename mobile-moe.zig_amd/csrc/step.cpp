@@ -540,7 +540,7 @@ int mmhip_sample_dev(mmhip_ctx* ctx, const mmhip_sample* args) {
         if (!args) return invalid(what, "null arguments");
         const mmhip_sample& p = *args;
         if (p.vocab == 0 || p.vocab > MMHIP_SAMPLE_MAX_VOCAB) return invalid(what, "vocab outside [1, 2^24]");
-        if (p.n_rows > kMostRows) return invalid(what, "2^24 rows or more");
+        if (p.n_rows >= 1u << 22) return invalid(what, "2^22 rows or more");
         if (p.rows_dev && (p.n_logits == 0 || p.n_logits >= MMHIP_NO_TOKEN)) return invalid(what, "n_logits outside [1, 2^32 - 1)");
         if (p.n_rows == 0) return ctx ? MMHIP_OK : invalid(what, "null context");
         if (!p.logits_dev || !p.uniform_dev || !p.tokens_dev) return invalid(what, "null pointer");

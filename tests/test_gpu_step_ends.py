@@ -454,6 +454,28 @@ def test_chosen_rows(ctx, vocab):
     check_sample([g[keep] for g in got], x, u[keep], t=0.9, p=0.9, rows=rows[keep])
 
 
+@pytest.mark.parametrize("n,vocab", [(1, 3_000_000), (3, 1_100_000), (700, 2500)])
+@pytest.mark.parametrize("settings", [dict(t=0.7), dict(t=0.8, k=100), dict(p=0.9), dict(t=0.2, k=40, p=0.99, least=1e-4)], ids=str)
+def test_wide_and_many_rows(ctx, n, vocab, settings):
+    """Several chunks to a thread of the last launch; pieces of one chunk and of many."""
+    rng = np.random.default_rng(n)
+    x, u = logits_like(rng, n, vocab), rng.random(n).astype(np.float32)
+    check_sample(run_sample(ctx, x, u, **settings), x, u, **settings)
+
+
+@pytest.mark.parametrize("spread", [0.0, 1e-6, 0.03, 30.0])
+@pytest.mark.parametrize("settings", [dict(k=7), dict(k=20000), dict(p=0.5), dict(t=2.0, k=30000, p=0.7, least=0.4)], ids=str)
+def test_cuts_among_many_tokens(ctx, spread, settings):
+    """Logits so close or so far apart that a bin of the histogram holds more tokens than the list, or nearly none; with
+    one at the type's lowest value, as masks leave it."""
+    rng = np.random.default_rng(8)
+    x = (spread * rng.standard_normal((3, 40000))).astype(np.float32)
+    x[1, 77] = np.finfo(np.float32).min
+    x[2, 500:] = np.round(x[2, 500:], 2)
+    u = rng.random(3).astype(np.float32)
+    check_sample(run_sample(ctx, x, u, **settings), x, u, **settings)
+
+
 def test_frequencies_of_drawn_tokens(ctx):
     """Even steps of u over a row: each token is drawn as often as its probability says, to one draw."""
     rng = np.random.default_rng(4)

@@ -84,7 +84,7 @@ def test_sample():
     for ok in (dict(), dict(n_rows=0), dict(n_rows=1, stride=0), dict(rows_dev=P, n_logits=1, stride=0), dict(vocab=1 << 24, stride=1 << 24),
                dict(temperature_dev=P, top_k_dev=P, top_p_dev=P, min_p_dev=P, probs_dev=P, kept_dev=P)):
         refused(sample(**ok), mm.ERR_INVALID, "sample: null context")
-    for bad in (dict(vocab=0), dict(vocab=(1 << 24) + 1, stride=1 << 25), dict(n_rows=2 ** 24), dict(stride=99), dict(logits_dev=None), dict(uniform_dev=None),
+    for bad in (dict(vocab=0), dict(vocab=(1 << 24) + 1, stride=1 << 25), dict(n_rows=2 ** 22), dict(stride=99), dict(logits_dev=None), dict(uniform_dev=None),
                 dict(tokens_dev=None), dict(rows_dev=P), dict(rows_dev=P, n_logits=2, stride=99), dict(rows_dev=P, n_logits=0xFFFFFFFF),
                 dict(logits_dev=P + 2), dict(tokens_dev=P + 1), dict(probs_dev=P + 3), dict(top_k_dev=P + 2)):
         refused(sample(**bad), mm.ERR_INVALID, "sample")
