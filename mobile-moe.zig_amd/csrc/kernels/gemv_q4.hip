@@ -24,11 +24,13 @@ namespace mmhip {
 namespace {
 
 constexpr uint32_t kQ4Ups = 4;        // units per step
-constexpr uint32_t kQ4MostTiles = 64; // tiles per workgroup (LDS row sums)
 
 // Columns whose digits are in LDS at once, in units.
 template <int TOK>
-constexpr uint32_t q4_chunk() { return TOK == 1 ? 64 : 16; }
+constexpr uint32_t q4_chunk() { return TOK == 1 ? 64 : 24; }
+// Tiles per workgroup (LDS row sums; all of its LDS stays below 64 KiB).
+template <int TOK>
+constexpr uint32_t q4_tiles() { return TOK == 1 ? 64 : 40; }
 // LDS digits of a unit, by the lane (row m of A, column group g) that reads them.
 // One vector: A has the four digits of block b in rows 4 b .. 4 b + 3, so a lane
 // reads 8 bytes of the one block it has a row of. Four vectors: rows 4 t .. 4 t + 3
@@ -101,7 +103,7 @@ struct Q4Set {
 // TOK 1: grid row y is a problem, a matrix and a vector of its own. TOK 4: grid
 // row y is a group of up to four vectors, all with the first matrix.
 template <int FMT, int TOK, int WG, int DEPTH, int NSEG>
-__global__ __launch_bounds__(WG, 1024 / WG) void gemv_q4_kernel(Q4Set<NSEG> set) {
+__global__ __launch_bounds__(WG, WG == 256 ? 2 : 4) void gemv_q4_kernel(Q4Set<NSEG> set) {
     constexpr uint32_t kWaves = WG / 64, kRing = DEPTH + 1;
     constexpr uint32_t kChunk = q4_chunk<TOK>(), kOut = TOK == 1 ? 16 : 64;
     const GemvArgs& a = set.seg[NSEG > 1 ? blockIdx.z : 0].a;
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(WG, 1024 / WG) void gemv_q4_kernel(Q4Set<NSEG> set)
     const uint32_t n_vec = TOK == 1 ? 1 : min(set.seg[0].n_vec - blockIdx.y * TOK, (uint32_t)TOK);
     const uint32_t t_begin = blockIdx.x * a.tiles_per_wg;
     if (t_begin >= a.tiles || (TOK == 1 && blockIdx.y >= a.n_probs)) return;  // whole workgroup
-    __shared__ float row_sum[kQ4MostTiles * kOut];
+    __shared__ float row_sum[q4_tiles<TOK>() * kOut];
     __shared__ float edge[2][kWaves * kOut];
     extern __shared__ __align__(16) uint8_t smem[];
     const uint32_t chunk = min(a.units, kChunk);
@@ -158,24 +160,46 @@ __global__ __launch_bounds__(WG, 1024 / WG) void gemv_q4_kernel(Q4Set<NSEG> set)
             if (++nxt_s == S) nxt_s = 0, ++nxt_t;
         }
     };
-    const auto fill = [&](uint32_t u0, uint32_t units) {
-        // 8 lanes a block, four columns each; columns past the end are zeros.
+    // The vectors' digits: 8 lanes a block, four columns each (columns past the
+    // end are zeros), a pass of the workgroup over WG / 8 blocks. Vectors that are
+    // not there leave rows of A that only results that are not there come from.
+    const auto x_load = [&](uint32_t u0, uint32_t i, uint32_t tok) {
+        const BufRsrc r = make_rsrc(x + (tok < n_vec ? tok * a.x_stride : 0), tok < n_vec ? a.cols * 4 : 0);
+        return buf_load_b128(r, (u0 * kQ4UnitCols + i * 4) * 4, 0);
+    };
+    const auto x_store = [&](const uint4& q, uint32_t i, uint32_t units, uint32_t tok) {
+        if (i >= units * 32 || tok >= n_vec) return;
+        const float v[4] = {__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z), __uint_as_float(q.w)};
+        store_digits<TOK>(v, tok, i >> 3, i & 7, aq, xs);
+    };
+    const auto fill = [&](uint32_t u0, uint32_t units, uint32_t i0) {
+        for (uint32_t i = i0 + threadIdx.x; i < units * 32; i += WG) {
+            uint4 q[TOK];
 #pragma unroll
-        for (uint32_t tok = 0; tok < TOK; ++tok) {
-            const bool live = TOK == 1 || tok < n_vec;
-            const BufRsrc r = make_rsrc(x + (live ? tok * a.x_stride : 0), live ? a.cols * 4 : 0);
-            for (uint32_t i = threadIdx.x; i < units * 32; i += WG) {
-                float v[4];
+            for (uint32_t tok = 0; tok < TOK; ++tok) q[tok] = x_load(u0, i, tok);
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) v[e] = __uint_as_float(buf_load_b32(r, (u0 * kQ4UnitCols + i * 4 + e) * 4, 0));
-                store_digits<TOK>(v, tok, i >> 3, i & 7, aq, xs);
-            }
+            for (uint32_t tok = 0; tok < TOK; ++tok) x_store(q[tok], i, units, tok);
         }
     };
 
-    start(chunk);
-    for (uint32_t i = threadIdx.x; i < n_tiles * kOut; i += WG) row_sum[i] = 0.0f;
-    fill(0, chunk);
+    {
+        // The first passes' vectors are asked for before any weight: a CU returns
+        // loads in the order of their issue, and the barrier orders the waves'.
+        constexpr uint32_t kPre = TOK == 1 ? 1024 / WG : 1;
+        uint4 pre[kPre][TOK];
+#pragma unroll
+        for (uint32_t q = 0; q < kPre; ++q)
+#pragma unroll
+            for (uint32_t tok = 0; tok < TOK; ++tok) pre[q][tok] = x_load(0, q * WG + threadIdx.x, tok);
+        __builtin_amdgcn_s_barrier();
+        start(chunk);
+        for (uint32_t i = threadIdx.x; i < n_tiles * kOut; i += WG) row_sum[i] = 0.0f;
+#pragma unroll
+        for (uint32_t q = 0; q < kPre; ++q)
+#pragma unroll
+            for (uint32_t tok = 0; tok < TOK; ++tok) x_store(pre[q][tok], q * WG + threadIdx.x, chunk, tok);
+        fill(0, chunk, kPre * WG);
+    }
     float acc = 0.0f;
     bool whole = cur_s == 0;  // the current tile's part began at its first step
     const auto compute = [&](uint32_t j, const uint4 (&r)[kQ4Ups], const uint2& d) {
@@ -183,10 +207,9 @@ __global__ __launch_bounds__(WG, 1024 / WG) void gemv_q4_kernel(Q4Set<NSEG> set)
 #pragma unroll
         for (uint32_t i = 0; i < kQ4Ups; ++i) {
             const uint32_t u = cur_s * kQ4Ups + i;  // of the chunk
-            const uint32_t ul = min(u, n_units - 1);  // a step's absent units count nothing
+            const uint32_t ul = min(u, n_units - 1);  // (a step's absent units have scales of 0)
             const uint8_t* p = aq + ul * q4_unit_bytes<TOK>() + a_lane;
             const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-            const bool in = u < n_units;
             const float dw = f16_scale((uint16_t)(scale4[i >> 1] >> (16 * (i & 1)))) * q4_unscale<FMT>();
             if constexpr (TOK == 1) {
                 // Block b's digits are in rows 4 b ..: four products into one
@@ -198,8 +221,7 @@ __global__ __launch_bounds__(WG, 1024 / WG) void gemv_q4_kernel(Q4Set<NSEG> set)
                     const long av = (long)(((uint64_t)(h.y & mine[b]) << 32) | (h.x & mine[b]));
                     dv = __builtin_amdgcn_mfma_i32_16x16x32_i8(av, q4_bop<FMT>(w[b]), dv, 0, 0, 0);
                 }
-                const float c = in ? xs[ul * 4 + g] : 0.0f;
-                acc = fmaf(digits_value(dv[0] * 256 + dv[1], dv[2] * 256 + dv[3]) * dw, c, acc);
+                acc = fmaf(digits_value(dv[0] * 256 + dv[1], dv[2] * 256 + dv[3]) * dw, xs[ul * 4 + g], acc);
             } else {
                 const uint4 h0 = *reinterpret_cast<const uint4*>(p), h1 = *reinterpret_cast<const uint4*>(p + 1024);
                 const long av[4] = {(long)(((uint64_t)h0.y << 32) | h0.x), (long)(((uint64_t)h0.w << 32) | h0.z),
@@ -213,8 +235,7 @@ __global__ __launch_bounds__(WG, 1024 / WG) void gemv_q4_kernel(Q4Set<NSEG> set)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const v4i dv = mfma_i8(av[b], q4_bop<FMT>(w[b]));
-                    const float c = in ? xb[b] : 0.0f;
-                    acc = fmaf(digits_value(dv[0] * 256 + dv[1], dv[2] * 256 + dv[3]) * db4[b], c, acc);
+                    acc = fmaf(digits_value(dv[0] * 256 + dv[1], dv[2] * 256 + dv[3]) * db4[b], xb[b], acc);
                 }
             }
         }
@@ -274,7 +295,7 @@ __global__ __launch_bounds__(WG, 1024 / WG) void gemv_q4_kernel(Q4Set<NSEG> set)
         const uint32_t units = min(chunk, a.units - kb);
         start(units);
         whole = cur_s == 0;
-        fill(kb, units);
+        fill(kb, units, 0);
     }
 }
 
@@ -284,14 +305,14 @@ size_t q4_lds(uint32_t units) {
     return (size_t)chunk * (q4_unit_bytes<TOK>() + 16 * TOK);
 }
 
-template <int TOK, int N>
+template <int TOK, int WG, int DEPTH, int N>
 hipError_t launch_set(const Q4Args* segs, uint32_t n, uint32_t fmt, uint32_t grid_x, uint32_t grid_y, size_t lds, hipStream_t s) {
     Q4Set<N> set{};
     for (uint32_t i = 0; i < (uint32_t)N; ++i) set.seg[i] = segs[i < n ? i : 0];
-    const void* fn = fmt == kFmtQ4 ? reinterpret_cast<const void*>(&gemv_q4_kernel<kFmtQ4, TOK, 256, 2, N>)
-                                   : reinterpret_cast<const void*>(&gemv_q4_kernel<kFmtIq4, TOK, 256, 2, N>);
+    const void* fn = fmt == kFmtQ4 ? reinterpret_cast<const void*>(&gemv_q4_kernel<kFmtQ4, TOK, WG, DEPTH, N>)
+                                   : reinterpret_cast<const void*>(&gemv_q4_kernel<kFmtIq4, TOK, WG, DEPTH, N>);
     void* args[] = {&set};
-    return hipLaunchKernel(fn, dim3(grid_x, grid_y, n), dim3(256), args, lds, s);
+    return hipLaunchKernel(fn, dim3(grid_x, grid_y, n), dim3(WG), args, lds, s);
 }
 
 }  // namespace
@@ -309,21 +330,27 @@ hipError_t launch_gemv_q4(const GemvArgs* segs_in, uint32_t n_segs, uint32_t fmt
     if (n == 0) return hipSuccess;
     // About the same number of units for every workgroup, one workgroup per CU.
     const uint64_t per_wg = (units + num_cu - 1) / num_cu;
-    uint32_t grid_x = 1, grid_y = 1;
+    uint32_t grid_x = 1, grid_y = 1, steps = 0;
     size_t lds = 0;
     for (uint32_t i = 0; i < n; ++i) {
         GemvArgs& a = segs[i].a;
         const uint64_t t = (per_wg + a.units - 1) / a.units;
-        a.tiles_per_wg = (uint32_t)(t > kQ4MostTiles ? kQ4MostTiles : t);
+        a.tiles_per_wg = (uint32_t)(t > q4_tiles<1>() ? q4_tiles<1>() : t);
         if (a.tiles_per_wg > a.tiles) a.tiles_per_wg = a.tiles;
+        const uint32_t chunk = a.units < q4_chunk<1>() ? a.units : q4_chunk<1>();
+        if (a.tiles_per_wg * ((chunk + kQ4Ups - 1) / kQ4Ups) > steps) steps = a.tiles_per_wg * ((chunk + kQ4Ups - 1) / kQ4Ups);
         const uint32_t gx = (a.tiles + a.tiles_per_wg - 1) / a.tiles_per_wg;
         if (gx > grid_x) grid_x = gx;
         if (a.n_probs > grid_y) grid_y = a.n_probs;
         if (q4_lds<1>(a.units) > lds) lds = q4_lds<1>(a.units);
     }
     if (grid_y > 65535) return hipErrorInvalidValue;
-    if (n == 1) return launch_set<1, 1>(segs, 1, fmt, grid_x, grid_y, lds, s);
-    return launch_set<1, kGemvMaxSegs>(segs, n, fmt, grid_x, grid_y, lds, s);
+    // Eight waves a workgroup (64 matrices of [1536 x 2048] 21.9 us, four waves 27.4;
+    // [154880 x 2048] 29.4 and 30.8), but four where that is a step for each ([768 x
+    // 2048] 4.13 us against 4.51, [3840 x 768] 3.85 against 4.19).
+    if (n == 1 && steps <= 4) return launch_set<1, 256, 2, 1>(segs, 1, fmt, grid_x, grid_y, lds, s);
+    if (n == 1) return launch_set<1, 512, 1, 1>(segs, 1, fmt, grid_x, grid_y, lds, s);
+    return launch_set<1, 512, 1, kGemvMaxSegs>(segs, n, fmt, grid_x, grid_y, lds, s);
 }
 
 hipError_t launch_gemv_q4_vecs(const GemvArgs& a_in, uint32_t n_vec, uint32_t fmt, int num_cu, hipStream_t s) {
@@ -331,9 +358,9 @@ hipError_t launch_gemv_q4_vecs(const GemvArgs& a_in, uint32_t n_vec, uint32_t fm
     Q4Args seg{a_in, n_vec};
     GemvArgs& a = seg.a;
     const uint64_t t = (a.tiles + num_cu - 1) / num_cu;
-    a.tiles_per_wg = (uint32_t)(t > kQ4MostTiles ? kQ4MostTiles : t);
+    a.tiles_per_wg = (uint32_t)(t > q4_tiles<4>() ? q4_tiles<4>() : t);
     a.n_probs = 1;
-    return launch_set<4, 1>(&seg, 1, fmt, (a.tiles + a.tiles_per_wg - 1) / a.tiles_per_wg, (n_vec + 3) / 4, q4_lds<4>(a.units), s);
+    return launch_set<4, 512, 1, 1>(&seg, 1, fmt, (a.tiles + a.tiles_per_wg - 1) / a.tiles_per_wg, (n_vec + 3) / 4, q4_lds<4>(a.units), s);
 }
 
 }  // namespace mmhip
