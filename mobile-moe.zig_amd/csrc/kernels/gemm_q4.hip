@@ -1,10 +1,27 @@
-// 4-bit weights (q4_ops.hpp) times many f32 vectors on gfx950's bf16 matrix
+// 4-bit weights (q4_ops.hpp) times many f32 vectors on gfx950's f16 matrix
 // cores: prompts.
 //
-// The integer weights are exact in bf16 and an f32 value is the sum of three
-// bf16 numbers, so a 32-column block of 16 weight rows times 16 vectors is
-// three v_mfma_f32_16x16x32_bf16 (the smallest parts first) and one multiply-add
-// per output with the block's scale: the sums of f32 products, no coarser.
+// The integer weights are exact in f16. A vector's value, times a power of two
+// that keeps the vector's largest below 2^15, is the sum of two f16 numbers: the
+// nearest one, and the nearest to what that leaves, off by 2^-23 of the value at
+// most (where that is more, by 2^-28 of the largest of its first 64 or by 2^-39
+// of the vector's largest). A 32-column block of 16
+// weight rows times 16 vectors is two v_mfma_f32_16x16x32_f16 (the smaller parts
+// first) and one multiply-add per output with the block's scale.
+//
+// Bound: vector instructions (per value of x two conversions, per eight weights
+// 11 or 21 operations, per output and block one multiply-add) beside the matrix
+// cores. A workgroup's waves share the x tile in LDS: each converts its part of
+// the next 64 columns while the matrix cores work on the last ones, and a wave
+// unpacks weights of its own rows straight from their records. Waves may also
+// split the columns (KS groups), their sums added at the end.
+//
+// Measured: [10240 x 2048] times 256 vectors 34.8 us (309 Tflop/s of products; the
+// two matrix instructions per product alone would take 17 us), [3840 x 768] times
+// 77 vectors 7.7 us; with bf16 parts (three instructions per product, four
+// conversions) 74 and 10.9 us.
+#include <type_traits>
+
 #include "device_common.hpp"
 #include "gemm_tile_ops.hpp"
 #include "kernels.hpp"
@@ -13,6 +30,9 @@
 namespace mmhip {
 
 namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 struct GemmQ4Args {
     const uint4* recs;
@@ -23,172 +43,343 @@ struct GemmQ4Args {
     uint32_t batch, cols, tiles, units, rows, d_row;
     uint32_t rec_bytes, d_bytes;
     uint32_t groups, items;  // tile groups, groups of vectors
+    uint32_t wg_tiles;       // weight tiles of a workgroup: at most NJ for each of its RS waves
 };
 
-// Four f32 values as three times four bf16: what each rounding leaves goes into
-// the next part, 24 bits of significand together. Times 2^-12 (kActScale), so
-// that a block's products stay finite for every finite x.
-__device__ __forceinline__ void split3(const uint4& q, uint2 (&part)[3]) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    uint32_t out[3][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        f32x2 v = {__uint_as_float(w[2 * i]) * kActScale, __uint_as_float(w[2 * i + 1]) * kActScale};
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-            out[p][i] = h;
-            v = f32x2{v[0] - __uint_as_float(h << 16), v[1] - __uint_as_float(h & 0xFFFF0000u)};
-        }
-    }
-#pragma unroll
-    for (int p = 0; p < 3; ++p) part[p] = make_uint2(out[p][0], out[p][1]);
+// Eight weights as f16, in the order of columns 0 2, 4 6, 1 3, 5 7: 0x6400 | u is
+// 1024 + u.
+__device__ __forceinline__ uint32_t f16_less(uint32_t h, float by) {
+    const f16x2 b = {(_Float16)by, (_Float16)by};
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, h) - b);
 }
-
 template <int FMT>
-__device__ __forceinline__ bf16x8 q4_bop_bf16(uint32_t d) {
-    uint32_t w0, w1;
-    q4_words<FMT>(d, w0, w1);
-    return q8_bop(w0, w1);
+__device__ __forceinline__ f16x8 q4_bop_f16(uint32_t d) {
+    uint32_t h[4];
+    if constexpr (FMT == kFmtQ4) {
+        // (the stored codes have their top bit flipped)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = f16_less(((d >> (4 * k)) & 0x000F000Fu) ^ 0x64086408u, 1032.0f);
+    } else {
+        uint32_t w[2];
+        q4_words<FMT>(d, w[0], w[1]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            h[k] = f16_less(__builtin_amdgcn_perm(0x64646464u, w[k & 1] ^ 0x80808080u, k < 2 ? 0x04020400u : 0x04030401u), 1152.0f);
+    }
+    return __builtin_bit_cast(f16x8, make_uint4(h[0], h[1], h[2], h[3]));
 }
 
-// Waves of a workgroup split the columns: wave v takes the v-th share of the
-// units and the shares are added at the end. MT: 16 vectors each, NJ: 16 weight
-// rows each.
-template <int FMT, int MT, int NJ, int KS>
-__global__ __launch_bounds__(KS * 64, 2) void gemm_q4_kernel(GemmQ4Args a) {
-    constexpr uint32_t kSlot = MT * NJ * 4 * 64;                  // floats of a wave's sums
-    constexpr uint32_t kX = MT * 3 * kPlaneBytes;                 // a wave's 64 columns of x
-    constexpr uint32_t kRed = KS * kSlot * 4, kMain = KS * kX;
+// A half step's x tile in LDS: 64 columns of MT * 16 vectors, per 16 vectors and
+// part eight runs (block, column group), each the 16 vectors' eight columns in
+// the weights' order. Vectors' places are changed four by four, in an order of
+// its own for each column group: a wave's 16-byte reads meet no bank twice, its
+// 4-byte writes (eight runs, four vectors) none more than twice.
+constexpr uint32_t kQ4Run = 256, kQ4Part = 8 * kQ4Run;
+__device__ __forceinline__ uint32_t run_place(uint32_t vec, uint32_t group) {
+    return (vec & 15) ^ ((0x2130u >> (4 * group) & 3u) << 2);  // 0 3 1 2 fours for groups 0 1 2 3
+}
+
+// A vector's power of two: its largest |x| becomes at least 2^at and less than
+// twice that. Below 2^-95 as 2^-95.
+__device__ __forceinline__ float fit(float most, uint32_t at) {
+    const uint32_t e = min(max(__float_as_uint(most) >> 23, 32u), 254u);
+    return __uint_as_float((254 + at - e) << 23);
+}
+constexpr float kQ4Fits = 32768.0f;
+__device__ __forceinline__ float row_max(float m) {  // over 16 lanes
+    m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0xB1, 0xF, 0xF, false)));
+    m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x4E, 0xF, 0xF, false)));
+    m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x141, 0xF, 0xF, false)));
+    return fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x140, 0xF, 0xF, false)));
+}
+// max(m, |a|, |b|), NaN left out (fmaxf would quiet each operand first).
+__device__ __forceinline__ void max_abs2(float& m, uint32_t a, uint32_t b) {
+    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(a), "v"(b));
+}
+
+// MT: 16 vectors each; NJ: 16 weight rows each of a wave; RS waves share an x
+// tile, KS groups of them the columns.
+//
+// A vector's power of two comes from its first 64 columns, with room for values
+// 2048 times as large; where one is larger still, which shows at the end, the
+// workgroup goes over its columns a second time with what it knows then. So the
+// loop has no case for it.
+template <int FMT, int MT, int NJ, int RS, int KS>
+__global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_kernel(GemmQ4Args a) {
+    constexpr int kQuads = MT * 4 / RS;                              // of x, a thread and half step
+    static_assert(kQuads >= 1 && MT * 4 % RS == 0, "a wave stages whole rows of four vectors");
+    constexpr uint32_t kBuf = MT * 2 * kQ4Part;
+    constexpr uint32_t kSlot = MT * NJ * 4 * 64;                     // floats of a wave's sums
+    constexpr uint32_t kRed = KS > 1 ? RS * KS * kSlot * 4 : 0, kMain = KS * 2 * kBuf;
+    constexpr int kAhead = 2;
     __shared__ __align__(16) uint8_t lds[kRed > kMain ? kRed : kMain];
-    const uint32_t item = blockIdx.x % a.items, tg = blockIdx.x / a.items;
+    __shared__ float undo[KS][MT * 16];
+    __shared__ uint32_t again;
+    // Tile group tg runs on XCD tg % 8, its groups of vectors one after the other:
+    // each XCD's L2 holds an eighth of the matrix, read once.
+    const uint32_t r8 = blockIdx.x >> 3, item = r8 % a.items, tg = r8 / a.items * 8 + (blockIdx.x & 7);
+    if (tg >= a.groups) return;  // whole workgroup
     const uint32_t first = item * (MT * 16), count = min(a.batch - first, MT * 16u);
     const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t rw = wave % RS, kg = wave / RS;
     const BufRsrc rec_r = make_rsrc(a.recs, a.rec_bytes), d_r = make_rsrc(a.dvals, a.d_bytes);
     const BufRsrc x_r = make_rsrc(a.x + first * a.x_stride, (uint32_t)(((count - 1) * a.x_stride + a.cols) * 4));
-    uint8_t* const xs = lds + wave * kX;
+    uint8_t* const xs = lds + kg * 2 * kBuf;
+    // Its tiles, as evenly over the waves as they go.
+    const uint32_t each = a.wg_tiles / RS, more = a.wg_tiles % RS;
+    const uint32_t tile0 = tg * a.wg_tiles + rw * each + min(rw, more), n_tiles = each + (rw < more);
+    if (threadIdx.x == 0) again = 0;
+
+    // Units of this group; all groups take as many turns.
+    const uint32_t u0 = a.units * kg / KS, u1 = a.units * (kg + 1) / KS, turns = (a.units + KS - 1) / KS;
+    // This lane stages four columns of vectors r0 + 4 RS i.
+    const uint32_t r0 = 4 * rw + g;
+    uint32_t x_voff[kQuads];
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+        const uint32_t r = r0 + 4 * RS * i;
+        x_voff[i] = r < count ? (uint32_t)(r * a.x_stride + 4 * n) * 4 : kBufOob;
+    }
+    const uint32_t upper = n >= 8 ? kBufOob : 0;  // of a half step: out of range where columns end in its middle
+    uint8_t* const dst = xs + (n >> 1) * kQ4Run + (n & 1) * 4 + (r0 >> 4) * (2 * kQ4Part);
+    uint32_t place[4];  // of vectors r0 + 4 RS i: the same for all where RS is 4 or 8
+#pragma unroll
+    for (int i = 0; i < 4; ++i) place[i] = run_place(r0 + 4 * RS * i, (n >> 1) & 3) * 16;
 
     f32x4 acc[MT][NJ];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    const uint32_t u0 = a.units * wave / KS, u1 = a.units * (wave + 1) / KS;
-    uint4 xv[2][MT * 4], wv[NJ];
-    uint32_t dv[NJ];
+    float pow2[kQuads], most[kQuads];
+    // Loads in flight: of x a unit ahead (each half when the last one's is in
+    // LDS), of the weights kAhead.
+    uint4 xv[2][kQuads], wv[kAhead][NJ];
+    uint32_t dv[kAhead][NJ];
     const auto load_x = [&](uint32_t u, int h) {
-        const uint32_t col = u * kQ4UnitCols + 64 * h + 4 * n;
+        const uint32_t col = u * kQ4UnitCols + 64 * h;
+        const uint32_t part = u < u1 && col + 32 == a.cols ? upper : 0;
+        const uint32_t soff = u < u1 && col < a.cols ? col * 4 : kBufOob;
 #pragma unroll
-        for (int i = 0; i < MT * 4; ++i) {
-            const uint32_t r = 4 * i + g;
-            xv[h][i] = buf_load_b128(x_r, u < u1 && r < count && col < a.cols ? (uint32_t)(r * a.x_stride + col) * 4 : kBufOob, 0);
+        for (int i = 0; i < kQuads; ++i) xv[h][i] = buf_load_b128(x_r, x_voff[i] | part, soff);
+    };
+    const auto load_w = [&](auto nj, uint32_t u, uint4 (&wq)[NJ], uint32_t (&dq)[NJ]) {
+#pragma unroll
+        for (int j = 0; j < nj(); ++j) {
+            const uint32_t t = tile0 + j;
+            const bool ok = u < u1 && t < a.tiles && j < (int)n_tiles;
+            wq[j] = buf_load_b128(rec_r, lane * 16, ok ? (t * a.units + u) * 1024 : kBufOob);
+            dq[j] = buf_load_b16(d_r, lane * 8, ok ? t * a.d_row * 32 + (u >> 2) * kQ4StepScaleBytes + (u & 3) * 2 : kBufOob);
         }
     };
-    const auto load_w = [&](uint32_t u) {
+    // Half h's loaded values into its buffer.
+    const auto stage = [&](int h) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const uint32_t t = tg * NJ + j;
-            const bool ok = u < u1 && t < a.tiles;
-            wv[j] = buf_load_b128(rec_r, lane * 16, ok ? (t * a.units + u) * 1024 : kBufOob);
-            dv[j] = buf_load_b16(d_r, lane * 8, ok ? t * a.d_row * 32 + (u >> 2) * kQ4StepScaleBytes + (u & 3) * 2 : kBufOob);
+        for (int i = 0; i < kQuads; ++i) {
+            const float s = pow2[i];
+            max_abs2(most[i], xv[h][i].x, xv[h][i].y);
+            max_abs2(most[i], xv[h][i].z, xv[h][i].w);
+            const float v[4] = {__uint_as_float(xv[h][i].x), __uint_as_float(xv[h][i].y), __uint_as_float(xv[h][i].z),
+                                __uint_as_float(xv[h][i].w)};
+            _Float16 hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                hi[e] = (_Float16)(v[e] * s);
+                lo[e] = (_Float16)fmaf(v[e], s, -(float)hi[e]);
+            }
+            uint8_t* p = dst + place[RS >= 4 ? 0 : i & 3] + h * kBuf + (4 * RS * i >> 4) * (2 * kQ4Part);
+            *reinterpret_cast<f16x2*>(p) = f16x2{hi[0], hi[2]};
+            *reinterpret_cast<f16x2*>(p + 8) = f16x2{hi[1], hi[3]};
+            *reinterpret_cast<f16x2*>(p + kQ4Part) = f16x2{lo[0], lo[2]};
+            *reinterpret_cast<f16x2*>(p + kQ4Part + 8) = f16x2{lo[1], lo[3]};
         }
     };
-    load_w(u0);
-    load_x(u0, 0);
-    load_x(u0, 1);
-    for (uint32_t u = u0; u < u1; ++u) {
-        uint4 w[NJ];
-        float c[NJ][4];
+    const auto products = [&](auto nj, int h, const uint4 (&w)[NJ], const float (&c)[NJ][4]) {
+        const uint8_t* src = xs + h * kBuf + g * kQ4Run + run_place(n, g) * 16;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            w[j] = wv[j];
-            broadcast_rows4(f16_scale((uint16_t)dv[j]) * (q4_unscale<FMT>() * kActUnscale), c[j]);
-        }
-        load_w(u + 1);
+        for (int b = 0; b < 2; ++b) {
+            f16x8 hi[MT], lo[MT];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            {
-                uint8_t* dst = xs + (n >> 1) * kRunBytes + g * 16 + (n & 1) * 8;
+            for (int m = 0; m < MT; ++m) {
+                const uint8_t* p = src + m * (2 * kQ4Part) + b * 4 * kQ4Run;
+                hi[m] = __builtin_bit_cast(f16x8, *reinterpret_cast<const uint4*>(p));
+                lo[m] = __builtin_bit_cast(f16x8, *reinterpret_cast<const uint4*>(p + kQ4Part));
+            }
 #pragma unroll
-                for (int i = 0; i < MT * 4; ++i) {
-                    uint2 part[3];
-                    split3(xv[h][i], part);
+            for (int j = 0; j < nj(); ++j) {
+                const f16x8 wb = q4_bop_f16<FMT>(h == 0 ? (b == 0 ? w[j].x : w[j].y) : (b == 0 ? w[j].z : w[j].w));
 #pragma unroll
-                    for (int p = 0; p < 3; ++p)
-                        *reinterpret_cast<uint2*>(dst + (i >> 2) * (3 * kPlaneBytes) + p * kPlaneBytes + (i & 3) * 64) = part[p];
+                for (int m = 0; m < MT; ++m) {
+                    f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
+                    p = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[m], wb, p, 0, 0, 0);
+                    p = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[m], wb, p, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[m][j][e] = fmaf(p[e], c[j][2 * h + b], acc[m][j][e]);
                 }
             }
-            load_x(u + 1, h);
-            wave_lds_order();
-            const uint8_t* src = xs + g * kRunBytes + n * 16;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                bf16x8 part[MT][3];
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int p = 0; p < 3; ++p)
-                        part[m][p] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(
-                            src + (m * 3 + p) * kPlaneBytes + b * 4 * kRunBytes));
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const uint32_t d = h == 0 ? (b == 0 ? w[j].x : w[j].y) : (b == 0 ? w[j].z : w[j].w);
-                    const bf16x8 wb = q4_bop_bf16<FMT>(d);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
-                        p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(part[m][2], wb, p, 0, 0, 0);
-                        p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(part[m][1], wb, p, 0, 0, 0);
-                        p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(part[m][0], wb, p, 0, 0, 0);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[m][j][e] = fmaf(p[e], c[j][2 * h + b], acc[m][j][e]);
-                    }
-                }
-            }
-            wave_lds_order();
         }
+    };
+
+    // All columns, for a wave with so many tiles. As many barriers whatever it has.
+    const auto sweep = [&](auto nj, bool begin) {
+        load_x(u0, 0);
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) load_w(nj, u0 + q, wv[q], dv[q]);
+        load_x(u0, 1);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (begin) {
+#pragma unroll
+            for (int i = 0; i < kQuads; ++i) {
+                most[i] = 0.0f;
+                max_abs2(most[i], xv[0][i].x, xv[0][i].y);
+                max_abs2(most[i], xv[0][i].z, xv[0][i].w);
+                pow2[i] = fit(row_max(most[i]), 3);
+            }
+        }
+        stage(0);
+        load_x(u0 + 1, 0);
+        lds_barrier();
+        for (uint32_t k = 0; k < turns; k += kAhead) {
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q) {
+                if (k + q >= turns) break;  // for the whole workgroup
+                const uint32_t u = u0 + k + q;
+                float c[NJ][4];
+#pragma unroll
+                for (int j = 0; j < nj(); ++j) broadcast_rows4(f16_scale((uint16_t)dv[q][j]), c[j]);
+                stage(1);
+                load_x(u + 1, 1);
+                products(nj, 0, wv[q], c);
+                lds_barrier();
+                stage(0);
+                load_x(u + 2, 0);
+                products(nj, 1, wv[q], c);
+                load_w(nj, u + kAhead, wv[q], dv[q]);
+                lds_barrier();
+            }
+        }
+    };
+    for (int pass = 0; pass < 2; ++pass) {
+        if (NJ > 1 && n_tiles < NJ) sweep(std::integral_constant<int, (NJ > 1 ? NJ - 1 : 1)>(), pass == 0);
+        else sweep(std::integral_constant<int, NJ>(), pass == 0);
+        // Did all of them fit?
+        bool far = false;
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+            const float m = row_max(most[i]);
+            far |= m * pow2[i] >= kQ4Fits;
+            if (pass == 0 && m * pow2[i] >= kQ4Fits) pow2[i] = fit(m, 14);
+        }
+        if (pass == 0 && __any(far) && lane == 0) again = 1;
+        lds_barrier();
+        if (!again) break;
     }
 
-    lds_barrier();  // the sums take the memory over
-    float* const red = reinterpret_cast<float*>(lds);
+    // The vectors' powers of two, undone.
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i)
+        if (n == 0) undo[kg][r0 + 4 * RS * i] = 1.0f / pow2[i];
+    lds_barrier();
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int e = 0; e < 4; ++e) {
+            const float f = undo[kg][m * 16 + 4 * g + e];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) red[wave * kSlot + ((m * NJ + j) * 4 + r) * 64 + lane] = acc[m][j][r];
-    lds_barrier();
-    for (uint32_t e = wave; e < MT * NJ; e += KS) {
-        const uint32_t m = e / NJ, j = e % NJ, row = (tg * NJ + j) * 16 + n;
+            for (int j = 0; j < NJ; ++j) acc[m][j][e] *= f;
+        }
+    const auto put = [&](uint32_t m, uint32_t j, uint32_t e, float v) {
+        const uint32_t t = m * 16 + 4 * g + e, row = (tile0 + j) * 16 + n;
+        if (j < n_tiles && t < count && row < a.rows) a.y[(uint64_t)(first + t) * a.y_slot + (uint64_t)row * a.y_row] = v;
+    };
+    if constexpr (KS == 1) {
 #pragma unroll
-        for (uint32_t r = 0; r < 4; ++r) {
-            float v = 0.0f;
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int k = 0; k < KS; ++k) v += red[k * kSlot + (e * 4 + r) * 64 + lane];
-            const uint32_t t = m * 16 + 4 * g + r;
-            if (t < count && row < a.rows) a.y[(uint64_t)(first + t) * a.y_slot + (uint64_t)row * a.y_row] = v;
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) put(m, j, e, acc[m][j][e]);
+    } else {
+        float* const red = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) red[wave * kSlot + ((m * NJ + j) * 4 + e) * 64 + lane] = acc[m][j][e];
+        lds_barrier();
+        for (uint32_t q = kg; q < MT * NJ; q += KS) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                float v = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) v += red[(k * RS + rw) * kSlot + (q * 4 + e) * 64 + lane];
+                put(q / NJ, q % NJ, e, v);
+            }
         }
     }
+}
+
+// A launch's tile: 16 mt vectors by `tiles` weight tiles (at most nj for each of
+// rs waves), ks groups of columns.
+struct Shape {
+    int mt, nj, rs, ks;
+    uint32_t tiles;
+};
+template <int FMT>
+const void* fn_of(const Shape& t) {
+    if (t.mt == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 4, 2, 8, 1>);
+    if (t.mt == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 2, 8, 1>);
+    if (t.ks == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 4, 4>);
+    if (t.ks == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 2>);
+    return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 1>);
+}
+
+// By the number of 16 x 16 tiles of the result. Few: sixteen waves a workgroup in
+// four groups of columns, up to a workgroup per CU; then larger tiles and fewer
+// groups; many: as many vectors to a weight as there are. Measured, us, with
+// {1,1,4,4} / {1,2,4,2} / {1,2,4,1} / {2,2,8,1} / {4,2,8,1}: [2048 x 2560] times 16
+// (128 tiles) 9.8 / 14.4 / 19.9 / 29.0 / 38, times 128 (1024) 10.7 / 15.2 / 21.6 /
+// 30.2 / 39, times 256 (2048) 19.0 / 15.4 / 21.7 / 30.3 / 39; [10240 x 2048] times 256
+// (10240) 74.7 / 42.9 / 41.1 / 39.7 / 33.9; [154880 x 2048] times 16 (9680) 89 / 55 /
+// 51 / 66 / 125, times 32 (19360) 154 / 92 / 86 / 74 / 127.
+//
+// The largest tile takes as many weight tiles as cost least: rounds of one
+// workgroup per CU, times the tiles of a SIMD's two waves ([10240 x 2048] times 256
+// with 10 tiles, one round of 256 workgroups, 33.9 us, with 16 tiles 42.4, with 8
+// 55.0).
+Shape shape_of(uint32_t tiles, uint32_t batch, uint32_t cus) {
+    const uint64_t results = (uint64_t)tiles * ((batch + 15) / 16);
+    if (results <= 4ull * cus) return Shape{1, 1, 4, 4, 4};
+    if (results <= 16ull * cus) return Shape{1, 2, 4, 2, 8};
+    if (batch <= 16) return Shape{1, 2, 4, 1, 8};
+    if (batch <= 32) return Shape{2, 2, 8, 1, 16};
+    uint32_t best = 16;
+    uint64_t least = ~0ull;
+    for (uint32_t t = 16; t >= 8; --t) {
+        const uint64_t groups = (uint64_t)((tiles + t - 1) / t) * ((batch + 63) / 64);
+        const uint64_t cost = (groups + cus - 1) / cus * ((t + 3) / 4);
+        if (cost < least) {
+            least = cost;
+            best = t;
+        }
+    }
+    return Shape{4, 2, 8, 1, best};
 }
 
 }  // namespace
 
-// Vectors of one launch: x is read through 32-bit offsets from a group's first
-// row, and a launch has fewer than 2^32 threads.
+// Vectors of one launch: fewer than 2^32 threads.
 uint64_t gemm_q4_most(const TileGeom& g) {
-    const uint64_t groups = (g.tiles + 3) / 4;
-    const uint64_t items = ((1ull << 23) - 1) / groups;
+    const uint64_t items = ((1ull << 21) - 1) / (g.tiles + 8);
     return items ? items * 16 : 16;
 }
 
 hipError_t launch_gemm_q4(const uint4* recs, const uint16_t* dvals, const TileGeom& g, uint64_t mat, const float* x,
                           uint64_t x_stride, uint32_t batch, float* y, uint64_t y_slot, uint64_t y_row, int num_cu,
                           hipStream_t s) {
-    (void)num_cu;
     if (batch == 0) return hipSuccess;
-    if (x_stride >= 1ull << 25 || batch > gemm_q4_most(g)) return hipErrorInvalidValue;
+    if (x_stride >= kQ4MostCols || batch > gemm_q4_most(g)) return hipErrorInvalidValue;
     GemmQ4Args a{};
     a.recs = recs + mat * g.rec_stride;
     a.dvals = dvals + mat * g.d_stride;
@@ -205,12 +396,13 @@ hipError_t launch_gemm_q4(const uint4* recs, const uint16_t* dvals, const TileGe
     a.units = (uint32_t)g.units;
     a.rows = (uint32_t)g.rows;
     a.d_row = (uint32_t)g.d_row;
-    a.groups = (a.tiles + 3) / 4;
-    a.items = (batch + 15) / 16;
-    const unsigned blocks = a.groups * a.items;
-    if (g.fmt == kFmtQ4) gemm_q4_kernel<kFmtQ4, 1, 4, 8><<<blocks, 512, 0, s>>>(a);
-    else gemm_q4_kernel<kFmtIq4, 1, 4, 8><<<blocks, 512, 0, s>>>(a);
-    return hipGetLastError();
+    const Shape t = shape_of(a.tiles, batch, num_cu > 0 ? num_cu : 256);
+    a.wg_tiles = t.tiles;
+    a.groups = (a.tiles + t.tiles - 1) / t.tiles;
+    a.items = (batch + t.mt * 16 - 1) / (t.mt * 16);
+    const void* fn = g.fmt == kFmtQ4 ? fn_of<kFmtQ4>(t) : fn_of<kFmtIq4>(t);
+    void* args[] = {&a};
+    return hipLaunchKernel(fn, dim3((a.groups + 7) / 8 * 8 * a.items), dim3(t.rs * t.ks * 64), args, 0, s);
 }
 
 }  // namespace mmhip

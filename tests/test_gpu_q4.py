@@ -4,9 +4,9 @@ products, against 64-bit ones of the exact weights.
 Tolerances, u = 2^-24, S = sum |w x| of a result: one to four vectors enter as
 integers of 31 bits (2^-31 of a block's largest), a block's sum is rounded once,
 and cols / 32 blocks and a few partial sums are added: (cols / 32 + 12) u S. More
-vectors enter the matrix cores as three bf16 numbers that hold 24 bits; each of
-a block's 96 products and its sums is rounded at most by a unit, 2 u: (cols /
-32 + 200) u S.
+vectors enter the matrix cores as two f16 numbers that leave 2^-23 of a value at
+most (2 u), and each of a block's 64 products and its sums is rounded at most by a
+unit, 2 u: (cols / 32 + 200) u S.
 """
 import numpy as np
 import pytest
@@ -161,7 +161,8 @@ def test_several_vectors(ctx, t, layout, batch, rows, cols):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("batch,rows,cols", [(256, 1000, 768), (300, 4100, 256), (64, 16400, 128), (4, 40000, 64), (1000, 130, 8224)])
+@pytest.mark.parametrize("batch,rows,cols", [(256, 1000, 768), (300, 4100, 256), (64, 16400, 128), (4, 40000, 64), (1000, 130, 8224),
+                                             (16, 70001, 96), (29, 40000, 160), (37, 30000, 288), (250, 10250, 544), (513, 5000, 96)])
 def test_large_products(ctx, t, batch, rows, cols):
     rng = np.random.default_rng(batch)
     raw, w = weights(rng, t, rows, cols, 2)
@@ -174,6 +175,34 @@ def test_large_products(ctx, t, batch, rows, cols):
         y = dy.to_numpy(np.float32, batch * rows).reshape(batch, rows)
     wt.free()
     check(y, w[1], x, few=False)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("batch,rows", [(6, 40), (70, 3000), (40, 30000)])
+@pytest.mark.parametrize("where", [100, 321, 600])
+def test_values_that_outgrow_the_first(ctx, t, batch, rows, where):
+    """Values up to 1e6 and 1e30 times as large as a vector's first 64, which set its power of two; first ones of 0."""
+    rng = np.random.default_rng(where)
+    cols = 640
+    raw, w = weights(rng, t, rows, cols)
+    x = rng.standard_normal((batch, cols)).astype(np.float32)
+    x[0, where] = 1e6
+    x[1, where] = -1e30
+    x[2, :where] = 0
+    x[3, :where] *= np.float32(1e-30)
+    x[4, where:where + 32] *= 4000
+    wt = ctx.upload(raw, t, rows, cols)
+    with Buffers(ctx) as d:
+        dy = d.new(batch * rows * 4)
+        ctx.qmm_dev(wt, 0, d.put(x), dy, batch)
+        ctx.synchronize()
+        y = dy.to_numpy(np.float32, batch * rows).reshape(batch, rows)
+    wt.free()
+    x = x.astype(np.float64)
+    want, s = x @ w[0].T, np.abs(x) @ np.abs(w[0]).T
+    # a value below 2^-39 of the vector's largest may be off by that much
+    tol = (cols / 32 + 200) * U * s + 2.0 ** -38 * np.abs(x).max(1, keepdims=True) * np.abs(w[0]).sum(1)
+    assert (np.abs(y - want) <= tol).all()
 
 
 @pytest.mark.parametrize("t", TYPES)
