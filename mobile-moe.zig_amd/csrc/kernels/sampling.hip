@@ -12,6 +12,7 @@
 // computed in 64 bits (weight()) and summed as whole multiples of 2^-shift
 // (44 for up to 2^18 tokens): integer sums have no order.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "kernels.hpp"
@@ -25,7 +26,6 @@ namespace {
 constexpr uint32_t kSmPiece = 256, kSmThreads = 1024, kSmWaves = kSmThreads / 64;
 constexpr uint32_t kSmChunk = 1024;      // logits that a wave takes at a time
 constexpr uint32_t kSmBins = 1024;       // of the row's histogram
-constexpr uint32_t kSmMostPieces = 1024;
 constexpr uint32_t kSmWorkgroups = 2048; // pieces of a call that are enough
 constexpr uint32_t kSmPerThread = 8;     // tokens beside the cut that a thread of the last launch takes
 constexpr uint32_t kSmList = kSmPerThread * kSmThreads;
@@ -43,75 +43,106 @@ __device__ __forceinline__ float key_value(uint64_t k) {
     return __uint_as_float(b & 0x80000000u ? b & 0x7FFFFFFFu : ~b);
 }
 
-// (x - m) / T; 0 for the largest itself, an infinite one too.
-__device__ __forceinline__ double scaled(float x, float m, double inv_t) {
-    return x == m ? 0.0 : ((double)x - (double)m) * inv_t;
+// A weight is 2^(t / 256) with t = (x - m) 256 / (T ln 2), rounded to n + f:
+// 2^(n / 256) is a table's entry and an exponent, 2^(f / 256) a series of four
+// powers (the next is below 4e-17). A fifth of the time of a series alone.
+constexpr uint32_t kSmParts = 256;
+__device__ __forceinline__ void fill_parts(double* parts) {  // by the first 256 threads; a barrier follows
+    if (threadIdx.x >= kSmParts) return;
+    const double f = (int)(threadIdx.x < 128 ? threadIdx.x : threadIdx.x - 256) * (0.6931471805599453 / 256);
+    double p = 1.0, n = 14.0;
+    for (int i = 0; i < 14; ++i, n -= 1.0) p = fma(p, f / n, 1.0);
+    parts[threadIdx.x] = threadIdx.x < 128 ? p : 2.0 * p;
 }
-// exp(z) * 2^shift for z <= 0: 2^n 2^f with |f| <= 1/2, 2^f by its series to the
-// eleventh power (the next term is below 7e-15). From z = -70 on 0 for every shift.
-__device__ __forceinline__ double weight(double z, int shift) {
-    const double t = fmax(z * 1.4426950408889634, -101.0);
-    const double n = rint(t), f = (t - n) * 0.6931471805599453;
-    double p = 1.0 / 39916800.0;
-    p = fma(p, f, 1.0 / 3628800.0);
-    p = fma(p, f, 1.0 / 362880.0);
-    p = fma(p, f, 1.0 / 40320.0);
-    p = fma(p, f, 1.0 / 5040.0);
-    p = fma(p, f, 1.0 / 720.0);
-    p = fma(p, f, 1.0 / 120.0);
-    p = fma(p, f, 1.0 / 24.0);
-    p = fma(p, f, 1.0 / 6.0);
-    p = fma(p, f, 0.5);
-    p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
-    return ldexp(p, (int)n + shift);
+// t; 0 for the largest itself, an infinite one too.
+__device__ __forceinline__ double scaled(float x, float m, double per_t) {
+    return x == m ? 0.0 : ((double)x - (double)m) * per_t;
+}
+// The weight times 2^shift, for t <= 0. From 2^-64 on down as 2^-64, which is 0 for every shift.
+__device__ __forceinline__ double weight(double t, int shift, const double* parts) {
+    constexpr double kLn2 = 0.6931471805599453 / 256;
+    t = fmax(t, -64.0 * 256);
+    const double r = t + 0x1.8p52;  // n in its lowest bits
+    const int n = (int)(uint32_t)__double_as_longlong(r);
+    const double f = t - (r - 0x1.8p52);
+    double p = kLn2 * kLn2 * kLn2 * kLn2 / 24;
+    p = fma(p, f, kLn2 * kLn2 * kLn2 / 6);
+    p = fma(p, f, kLn2 * kLn2 / 2);
+    p = fma(p, f, kLn2);
+    const double part = parts[n & (int)(kSmParts - 1)];
+    return __longlong_as_double(__double_as_longlong(fma(part, p * f, part)) + ((long long)((n >> 8) + shift) << 52));
 }
 // The same as a whole number: at most 2^44, so adding 2^52 rounds it to the
 // lower bits of the sum.
-__device__ __forceinline__ uint64_t whole_weight(double z, int shift) {
-    return __double_as_longlong(weight(z, shift) + 0x1p52) & 0xFFFFFFFFFFFFFull;
+__device__ __forceinline__ uint64_t whole_weight(double t, int shift, const double* parts) {
+    return __double_as_longlong(weight(t, shift, parts) + 0x1p52) & 0xFFFFFFFFFFFFFull;
 }
 
-template <uint32_t WAVES>
-__device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t* red) {
-    __syncthreads();
-    v = wave_scan(v);
-    if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t all = 0;
-    for (uint32_t w = 0; w < WAVES; ++w) all += red[w];
-    return all;
-}
-// Over threads 0 .. this one.
-template <uint32_t WAVES>
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* red, uint64_t& all) {
-    __syncthreads();
-    v = wave_scan(v);
-    if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t before = 0;
-    all = 0;
-    for (uint32_t w = 0; w < WAVES; ++w) {
-        if (w < threadIdx.x >> 6) before += red[w];
-        all += red[w];
-    }
-    return before + v;
-}
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-    for (int off = 32; off; off >>= 1) v = max(v, (uint64_t)__shfl_xor((unsigned long long)v, off, 64));
+// Over lanes 0 .. this one.
+__device__ __forceinline__ uint64_t wave_max_scan(uint64_t v) {
+    v = max(v, moved<0x111, 0xF>(v));
+    v = max(v, moved<0x112, 0xF>(v));
+    v = max(v, moved<0x114, 0xF>(v));
+    v = max(v, moved<0x118, 0xF>(v));
+    v = max(v, moved<0x142, 0xA>(v));
+    v = max(v, moved<0x143, 0xC>(v));
     return v;
 }
+// Sums and maxima of two numbers at once over a workgroup, one barrier each: the
+// memory of one is written again two calls later, when the next one's barrier has
+// shown that all have read it.
 template <uint32_t WAVES>
-__device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* red) {
-    __syncthreads();
-    v = wave_max(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t all = 0;
-    for (uint32_t w = 0; w < WAVES; ++w) all = max(all, red[w]);
-    return all;
-}
+struct Together {
+    uint64_t (*memory)[2][WAVES];  // [2]
+    uint32_t turn = 0;
+    __device__ __forceinline__ void exchange(uint64_t& a, uint64_t& b) {  // lane 63's, to lanes 0 .. WAVES - 1
+        uint64_t(&red)[2][WAVES] = memory[turn & 1];
+        turn += 1;
+        const uint32_t lane = threadIdx.x & 63;
+        if (lane == 63) red[0][threadIdx.x >> 6] = a, red[1][threadIdx.x >> 6] = b;
+        __syncthreads();
+        a = lane < WAVES ? red[0][lane] : 0;
+        b = lane < WAVES ? red[1][lane] : 0;
+    }
+    // a: over threads 0 .. this one, and of all; b: of all.
+    __device__ __forceinline__ uint64_t scan(uint64_t a, uint64_t& all, uint64_t& b) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint64_t mine = wave_scan(a);
+        a = mine;
+        b = wave_scan(b);
+        exchange(a, b);
+        a = wave_scan(a);
+        b = lane_value(wave_scan(b), 63);
+        all = lane_value(a, 63);
+        return mine + (wave ? lane_value(a, wave - 1) : 0);
+    }
+    // Both over threads 0 .. this one.
+    __device__ __forceinline__ void scan2(uint64_t& a, uint64_t& b, uint64_t& all_a, uint64_t& all_b) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint64_t mine_a = wave_scan(a), mine_b = wave_scan(b);
+        a = mine_a;
+        b = mine_b;
+        exchange(a, b);
+        a = wave_scan(a);
+        b = wave_scan(b);
+        all_a = lane_value(a, 63);
+        all_b = lane_value(b, 63);
+        a = mine_a + (wave ? lane_value(a, wave - 1) : 0);
+        b = mine_b + (wave ? lane_value(b, wave - 1) : 0);
+    }
+    __device__ __forceinline__ uint64_t sum(uint64_t a) {
+        uint64_t all, none = 0;
+        scan(a, all, none);
+        return all;
+    }
+    __device__ __forceinline__ void largest(uint64_t& a, uint64_t& b) {
+        a = wave_max_scan(a);
+        b = wave_max_scan(b);
+        exchange(a, b);
+        a = lane_value(wave_max_scan(a), 63);
+        b = lane_value(wave_max_scan(b), 63);
+    }
+};
 
 // What a row asks for.
 enum SmMode : uint32_t { kSmAbsent, kSmNoRow, kSmBadSetting, kSmEmpty, kSmFirst, kSmAll, kSmCut };
@@ -120,7 +151,7 @@ struct RowSettings {
     const float* x;
     uint64_t best;  // the first token's key
     float m, bin_c;
-    double inv_t, least_z;
+    double per_t, least;  // t per logit, and t of min_p
     float p, u;
     uint32_t k;     // 0: no cut by number
     bool by_mass;   // a cut by probability
@@ -132,9 +163,11 @@ struct SmRow {
     uint32_t k_bin, k_rank;    // the cut by number: the bin, and which of its tokens is the last
     uint32_t p_lo, p_hi;       // the cut by probability: the bins that it may be in
     uint64_t k_mass, p_mass;   // of the tokens in bins before k_bin, before p_lo
+    uint64_t mass;             // of all
 };
 struct SmPlan {
     uint32_t chunks, pieces, list;
+    uint32_t per;              // chunks of a piece
     uint64_t* best;            // [rows][pieces]
     float* lowest;             // [rows][pieces]
     unsigned long long* mass;  // [rows][kSmBins]
@@ -143,13 +176,12 @@ struct SmPlan {
     uint32_t* chunk_count;     // [rows][chunks]
     uint64_t* keys;            // [rows][list]
     SmRow* rows;
+    RowSettings* settings;
 };
 constexpr uint32_t kNoBin = 0xFFFFFFFFu;
 
-// A row's settings, from those of its pieces' largest and lowest logits. For the
-// whole workgroup.
-template <uint32_t WAVES>
-__device__ __forceinline__ RowSettings row_settings(const SampleArgs& a, const SmPlan& p, uint32_t out, uint64_t* red) {
+// A row's settings, with its largest token's key and its lowest logit.
+__device__ __forceinline__ RowSettings row_settings(const SampleArgs& a, uint32_t out, uint64_t best, float low) {
     RowSettings s{};
     uint32_t row = out;
     if (a.rows) row = a.rows[out];
@@ -157,14 +189,7 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs& a, const S
     s.p = a.top_p ? a.top_p[out] : 1.0f;
     s.u = a.uniform[out];
     s.k = a.top_k ? a.top_k[out] : 0;
-    uint64_t best = 0;
-    float low = INFINITY;
-    for (uint32_t i = threadIdx.x; i < p.pieces; i += WAVES * 64) {
-        best = max(best, p.best[(uint64_t)out * p.pieces + i]);
-        low = fminf(low, p.lowest[(uint64_t)out * p.pieces + i]);
-    }
-    s.best = block_max<WAVES>(best, red);
-    low = -key_value(block_max<WAVES>(order_bits(-low), red) << 32);
+    s.best = best;
     if (a.rows && row == kNoToken) s.mode = kSmAbsent;
     else if (a.rows && row >= a.n_logits) s.mode = kSmNoRow;
     else if (!(t >= 0.0f && t <= 3.4028235e38f && s.p >= 0.0f && least >= 0.0f && least <= 1.0f && s.u >= 0.0f && s.u < 1.0f))
@@ -179,8 +204,8 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs& a, const S
     if (s.mode < kSmFirst) return s;
     s.x = a.logits + row * a.stride;
     s.m = key_value(s.best);
-    s.inv_t = 1.0 / (double)t;
-    s.least_z = log((double)least);
+    s.per_t = 369.3299304675746 / (double)t;  // 256 / ln 2
+    s.least = 369.3299304675746 * log((double)least);
     s.shift = a.shift;
     // Bins of 1/32 of the temperature next to the largest logit, twice as wide
     // from four temperatures below it on, and so on; narrower ones where the
@@ -209,67 +234,81 @@ __device__ __forceinline__ void load_chunk(const float* x, uint32_t vocab, uint3
         if (i * 64 + lane >= n) v[i] = __builtin_nanf("");
 }
 
+// The row of logits that the row's number names, or null.
+__device__ __forceinline__ const float* row_logits(const SampleArgs& a, uint32_t out) {
+    uint32_t row = out;
+    if (a.rows) row = a.rows[out];
+    return !a.rows || row < a.n_logits ? a.logits + row * a.stride : nullptr;
+}
+
 // The largest and lowest logits of a piece, and the row's memory cleared.
 __global__ __launch_bounds__(kSmPiece) void sample_best_kernel(SampleArgs a, SmPlan p) {
-    __shared__ uint64_t red[2][kSmPiece / 64];
+    __shared__ uint64_t memory[2][2][kSmPiece / 64];
     const uint32_t out = blockIdx.x / p.pieces, piece = blockIdx.x - out * p.pieces;
-    const uint32_t c0 = (uint32_t)((uint64_t)piece * p.chunks / p.pieces), c1 = (uint32_t)((uint64_t)(piece + 1) * p.chunks / p.pieces);
+    const uint32_t c0 = piece * p.per, c1 = min(c0 + p.per, p.chunks);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (uint32_t i = piece * kSmPiece + threadIdx.x; i < kSmBins; i += p.pieces * kSmPiece) {
         p.mass[(uint64_t)out * kSmBins + i] = 0;
         p.count[(uint64_t)out * kSmBins + i] = 0;
     }
     if (piece == 0 && threadIdx.x == 0) p.rows[out].listed = 0;
-    uint32_t row = out;
-    if (a.rows) row = a.rows[out];
-    uint32_t bits = 0, id = 0;
-    float low = INFINITY;
-    if (!a.rows || row < a.n_logits) {
-        const float* x = a.logits + row * a.stride;
+    const float* x = row_logits(a, out);
+    float top = -INFINITY, low = INFINITY;
+    uint32_t id = 0;
+    if (x)
         for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
             float v[kSmChunk / 64];
             load_chunk(x, a.vocab, c, v);
 #pragma unroll
             for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
-                const uint32_t b = order_bits(v[i]);
-                if (b > bits) bits = b, id = c * kSmChunk + i * 64 + lane;
+                if (v[i] > top) top = v[i], id = c * kSmChunk + i * 64 + lane;
                 if (v[i] > -INFINITY) low = fminf(low, v[i]);
             }
         }
-    }
-    const uint64_t best = wave_max((uint64_t)bits << 32 | (0xFFFFFFFFu - id)), lowest = wave_max((uint64_t)order_bits(-low));
-    if (lane == 0) red[0][wave] = best, red[1][wave] = lowest;
-    __syncthreads();
+    uint64_t best = order_key(top, id), lowest = order_bits(-low);
+    Together<kSmPiece / 64> all{memory};
+    all.largest(best, lowest);
     if (threadIdx.x == 0) {
-        uint64_t b = 0, l = 0;
-        for (uint32_t w = 0; w < kSmPiece / 64; ++w) b = max(b, red[0][w]), l = max(l, red[1][w]);
-        p.best[blockIdx.x] = b;
-        p.lowest[blockIdx.x] = -key_value(l << 32);
+        p.best[blockIdx.x] = best;
+        p.lowest[blockIdx.x] = -key_value(lowest << 32);
     }
 }
 
 // How many tokens, and how much of the weights, each bin of the row holds. Rows
-// without a cut: what each chunk keeps.
+// without a cut: what each chunk keeps. The row's settings for the launches behind.
 __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmPlan p) {
-    __shared__ uint64_t red[kSmPiece / 64];
+    __shared__ uint64_t memory[2][2][kSmPiece / 64];
+    __shared__ double parts[kSmParts];
     __shared__ unsigned long long mass[kSmBins];
     __shared__ uint32_t count[kSmBins];
     const uint32_t out = blockIdx.x / p.pieces, piece = blockIdx.x - out * p.pieces;
-    const uint32_t c0 = (uint32_t)((uint64_t)piece * p.chunks / p.pieces), c1 = (uint32_t)((uint64_t)(piece + 1) * p.chunks / p.pieces);
+    const uint32_t c0 = piece * p.per, c1 = min(c0 + p.per, p.chunks);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const RowSettings s = row_settings<kSmPiece / 64>(a, p, out, red);
+    const float* x = row_logits(a, out);
+    float v[kSmChunk / 64];
+    if (x && c0 + wave < c1) load_chunk(x, a.vocab, c0 + wave, v);  // its latency beside the settings'
+    uint64_t best = 0, lowest = 0;
+    for (uint32_t i = threadIdx.x; i < p.pieces; i += kSmPiece) {
+        best = max(best, p.best[(uint64_t)out * p.pieces + i]);
+        lowest = max(lowest, (uint64_t)order_bits(-p.lowest[(uint64_t)out * p.pieces + i]));
+    }
+    fill_parts(parts);
+    for (uint32_t i = threadIdx.x; i < kSmBins; i += kSmPiece) mass[i] = 0, count[i] = 0;
+    Together<kSmPiece / 64> all{memory};
+    all.largest(best, lowest);
+    const RowSettings s = row_settings(a, out, best, -key_value(lowest << 32));
+    if (piece == 0 && threadIdx.x == 0) p.settings[out] = s;
     if (s.mode < kSmAll) return;
     if (s.mode == kSmAll) {
         for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
-            float v[kSmChunk / 64];
-            load_chunk(s.x, a.vocab, c, v);
+            if (c != c0 + wave) load_chunk(x, a.vocab, c, v);
             uint64_t sum = 0;
             uint32_t n = 0;
 #pragma unroll
             for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
-                const double z = scaled(v[i], s.m, s.inv_t);
-                if (v[i] > -INFINITY && z >= s.least_z) {
-                    sum += whole_weight(z, s.shift);
+                const double t = scaled(v[i], s.m, s.per_t);
+                if (v[i] > -INFINITY && t >= s.least) {
+                    sum += whole_weight(t, s.shift, parts);
                     n += 1;
                 }
             }
@@ -282,17 +321,14 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
         }
         return;
     }
-    for (uint32_t i = threadIdx.x; i < kSmBins; i += kSmPiece) mass[i] = 0, count[i] = 0;
-    __syncthreads();
     for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
-        float v[kSmChunk / 64];
-        load_chunk(s.x, a.vocab, c, v);
+        if (c != c0 + wave) load_chunk(x, a.vocab, c, v);
 #pragma unroll
         for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
             if (!(v[i] > -INFINITY)) continue;
             const uint32_t b = bin_of(v[i], s);
             if (s.k) atomicAdd(&count[b], 1u);
-            if (s.by_mass) atomicAdd(&mass[b], (unsigned long long)whole_weight(scaled(v[i], s.m, s.inv_t), s.shift));
+            if (s.by_mass) atomicAdd(&mass[b], (unsigned long long)whole_weight(scaled(v[i], s.m, s.per_t), s.shift, parts));
         }
     }
     __syncthreads();
@@ -306,32 +342,37 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
 // each chunk has in the bins before all of them is kept for certain.
 __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmPlan p) {
     constexpr uint32_t kWaves = kSmPiece / 64, kPer = kSmBins / kSmPiece;
-    __shared__ uint64_t red[kWaves];
+    __shared__ uint64_t memory[2][2][kWaves];
+    __shared__ double parts[kSmParts];
     __shared__ SmRow row;
     __shared__ uint64_t k_here;
     const uint32_t out = blockIdx.x / p.pieces, piece = blockIdx.x - out * p.pieces;
-    const uint32_t c0 = (uint32_t)((uint64_t)piece * p.chunks / p.pieces), c1 = (uint32_t)((uint64_t)(piece + 1) * p.chunks / p.pieces);
+    const uint32_t c0 = piece * p.per, c1 = min(c0 + p.per, p.chunks);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = threadIdx.x;
-    const RowSettings s = row_settings<kWaves>(a, p, out, red);
-    if (s.mode != kSmCut) return;
-    if (tid == 0) {
-        row = SmRow{0, kNoBin, 0, kNoBin, kNoBin, 0, 0};
-        k_here = 0;
-    }
-    uint64_t m[kPer], all_mass = 0, sum = 0;
+    const RowSettings s = p.settings[out];
+    const float* x = row_logits(a, out);
+    float v[kSmChunk / 64];
+    if (x && c0 + wave < c1) load_chunk(x, a.vocab, c0 + wave, v);
+    uint64_t m[kPer], mass_to = 0, all_mass, num_to = 0, all_num;
     uint32_t n[kPer];
-    uint64_t num = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kPer; ++i) {
         m[i] = p.mass[(uint64_t)out * kSmBins + tid * kPer + i];
         n[i] = p.count[(uint64_t)out * kSmBins + tid * kPer + i];
-        sum += m[i];
-        num += n[i];
     }
-    const uint64_t mass_to = block_scan<kWaves>(sum, red, all_mass) - sum;
-    uint64_t all_num;
-    const uint64_t num_to = block_scan<kWaves>(num, red, all_num) - num;
-    __syncthreads();
+    if (s.mode != kSmCut) return;
+    if (tid == 0) {
+        row = SmRow{0, kNoBin, 0, kNoBin, kNoBin, 0, 0, 0};
+        k_here = 0;
+    }
+    fill_parts(parts);
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) mass_to += m[i], num_to += n[i];
+    const uint64_t mass_here = mass_to, num_here = num_to;
+    Together<kWaves> all{memory};
+    all.scan2(mass_to, num_to, all_mass, all_num);
+    mass_to -= mass_here;
+    num_to -= num_here;
     if (s.k && s.k < all_num) {
         uint64_t at = num_to, w = mass_to;
 #pragma unroll
@@ -372,11 +413,11 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
         to->p_hi = r.p_hi;
         to->k_mass = r.k_mass;
         to->p_mass = r.p_mass;
+        to->mass = all_mass;
     }
     const uint32_t sure = min(r.k_bin, r.p_lo);
     for (uint32_t c = c0 + wave; c < c1; c += kWaves) {
-        float v[kSmChunk / 64];
-        load_chunk(s.x, a.vocab, c, v);
+        if (c != c0 + wave) load_chunk(x, a.vocab, c, v);
         uint64_t mine = 0;
         uint32_t kept = 0, to_list = 0;
 #pragma unroll
@@ -384,9 +425,9 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
             if (!(v[i] > -INFINITY)) continue;
             const uint32_t b = bin_of(v[i], s);
             if (b < sure) {
-                const double z = scaled(v[i], s.m, s.inv_t);
-                if (z >= s.least_z) {
-                    mine += whole_weight(z, s.shift);
+                const double t = scaled(v[i], s.m, s.per_t);
+                if (t >= s.least) {
+                    mine += whole_weight(t, s.shift, parts);
                     kept += 1;
                 }
             } else if (b == r.k_bin || (b >= r.p_lo && b <= r.p_hi)) {
@@ -404,7 +445,7 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
         const uint32_t to = (uint32_t)wave_scan(here);
         uint32_t at = 0;
         if (lane == 63) at = atomicAdd(&p.rows[out].listed, to);
-        at = (uint32_t)__shfl((int)at, 63, 64) + to - here;
+        at = (uint32_t)__builtin_amdgcn_readlane(at, 63) + to - here;
 #pragma unroll
         for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
             if (!(to_list >> i & 1u)) continue;
@@ -422,10 +463,13 @@ struct Bins {
     unsigned long long mass[kSmBins];
     uint32_t count[kSmBins];
     uint32_t found, found_n;
-    uint64_t above;
+    uint64_t above, cut;
+    // The keys of a bin that one wave looks through.
+    uint64_t few_key[64], few_weight[64];
+    uint32_t few;
 };
 template <bool MASS>
-__device__ uint64_t find_cut(const RowSettings& s, uint32_t vocab, uint64_t floor, uint64_t target, Bins& b) {
+__device__ uint64_t find_cut(const RowSettings& s, const double* parts, uint32_t vocab, uint64_t floor, uint64_t target, Bins& b) {
     uint64_t prefix = 0, before = 0;
     for (int low = 54, bits = 10;; bits = low < 10 ? 4 : 10, low -= bits) {
         __syncthreads();
@@ -437,7 +481,7 @@ __device__ uint64_t find_cut(const RowSettings& s, uint32_t vocab, uint64_t floo
             if (k < floor || (low < 54 && (k >> (low + bits)) != prefix)) continue;
             const uint32_t at = (uint32_t)(k >> low) & ((1u << bits) - 1);
             atomicAdd(&b.count[at], 1u);
-            if (MASS) atomicAdd(&b.mass[at], (unsigned long long)whole_weight(scaled(v, s.m, s.inv_t), s.shift));
+            if (MASS) atomicAdd(&b.mass[at], (unsigned long long)whole_weight(scaled(v, s.m, s.per_t), s.shift, parts));
         }
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -461,27 +505,39 @@ __device__ uint64_t find_cut(const RowSettings& s, uint32_t vocab, uint64_t floo
     }
 }
 
+// The same among one wave's keys (0: none), each against each.
+template <bool MASS>
+__device__ __forceinline__ uint64_t find_few(uint64_t key, uint64_t w, uint64_t target) {
+    uint64_t to = 0;
+    for (uint64_t left = __ballot(key != 0); left; left &= left - 1) {
+        const uint32_t j = (uint32_t)__builtin_ctzll(left);
+        const uint64_t other = MASS ? lane_value(w, j) : 1;
+        if (lane_value(key, j) >= key) to += other;
+    }
+    const uint64_t at = __ballot(key != 0 && to >= target && to - (MASS ? w : 1) < target);
+    return at ? lane_value(key, (uint32_t)__builtin_ctzll(at)) : 0;
+}
+
 // The same among the keys that a workgroup's threads hold (those of `in`), by
-// their distance from the largest of them: 1024 bins over the distances that are
-// left, until one is left or distances are told apart to the last bit. Ends with
-// what is above the key in *above.
+// their distance from the largest of them: 1024 bins over the distances, then over
+// those of the bin that the key is in, until that holds no more than a wave's.
 template <bool MASS>
 __device__ uint64_t find_listed(const uint64_t (&key)[kSmPerThread], const uint64_t (&w)[kSmPerThread], uint32_t in, uint64_t target,
-                                Bins& b, uint64_t* red, uint64_t& above) {
-    uint64_t top = 0, low = ~0ull;
+                                Bins& b, Together<kSmWaves>& all) {
+    const uint32_t tid = threadIdx.x;
+    uint64_t top = 0, under = 0;  // under: the complement of the smallest
 #pragma unroll
     for (uint32_t i = 0; i < kSmPerThread; ++i)
-        if (in >> i & 1u) top = max(top, key[i]), low = min(low, key[i]);
-    top = block_max<kSmWaves>(top, red);
-    low = ~block_max<kSmWaves>(~low, red);
-    above = 0;
+        if (in >> i & 1u) top = max(top, key[i]), under = max(under, ~key[i]);
+    all.largest(top, under);
+    uint64_t low = ~under, above = 0;
     // Each turn leaves at most a 1024th of the span: seven for 64 bits.
     for (int turn = 0; turn < 7; ++turn) {
         const uint64_t span = top - low;
         const uint32_t sh = span < kSmBins ? 0 : 54 - (uint32_t)__clzll((long long)span);
-        __syncthreads();
-        b.mass[threadIdx.x] = 0;
-        b.count[threadIdx.x] = 0;
+        b.mass[tid] = 0;
+        b.count[tid] = 0;
+        if (tid == 0) b.few = 0;
         __syncthreads();
 #pragma unroll
         for (uint32_t i = 0; i < kSmPerThread; ++i)
@@ -491,25 +547,39 @@ __device__ uint64_t find_listed(const uint64_t (&key)[kSmPerThread], const uint6
                 if (MASS) atomicAdd(&b.mass[at], (unsigned long long)w[i]);
             }
         __syncthreads();
-        const uint64_t here = MASS ? b.mass[threadIdx.x] : b.count[threadIdx.x];
-        uint64_t all;
-        const uint64_t to = above + block_scan<kSmWaves>(here, red, all);
+        const uint32_t num = b.count[tid];
+        const uint64_t here = MASS ? b.mass[tid] : num;
+        uint64_t sum, none = 0;
+        const uint64_t to = above + all.scan(here, sum, none);
         if (to - here < target && target <= to) {
-            b.found = threadIdx.x;
-            b.found_n = b.count[threadIdx.x];
+            b.found = tid;
+            b.found_n = num;
             b.above = to - here;
         }
         __syncthreads();
-        const uint32_t at = b.found;
+        const uint32_t at = b.found, n = b.found_n;
         above = b.above;
         if (sh == 0) return top - at;
-        uint64_t one = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kSmPerThread; ++i) {
-            if ((in >> i & 1u) && (uint32_t)((top - key[i]) >> sh) != at) in &= ~(1u << i);
-            if (in >> i & 1u) one = key[i];
+            if (!(in >> i & 1u)) continue;
+            if ((uint32_t)((top - key[i]) >> sh) != at) {
+                in &= ~(1u << i);
+            } else if (n <= 64) {
+                const uint32_t to_few = atomicAdd(&b.few, 1u);
+                b.few_key[to_few] = key[i];
+                b.few_weight[to_few] = w[i];
+            }
         }
-        if (b.found_n == 1) return block_max<kSmWaves>(one, red);
+        if (n <= 64) {
+            __syncthreads();
+            if (tid < 64) {
+                const uint64_t cut = find_few<MASS>(tid < n ? b.few_key[tid] : 0, tid < n ? b.few_weight[tid] : 0, target - above);
+                if (tid == 0) b.cut = cut;
+            }
+            __syncthreads();
+            return b.cut;
+        }
         const uint64_t end = top - ((uint64_t)at << sh), last = end - (((uint64_t)1 << sh) - 1);
         low = max(low, last);  // (of two different integer types max would go through doubles)
         top = end;
@@ -518,14 +588,30 @@ __device__ uint64_t find_listed(const uint64_t (&key)[kSmPerThread], const uint6
 }
 
 // One workgroup per row: the cut among the listed tokens, the chunk in which the
-// running sum passes u times all, and the token in it.
+// running sum passes u times all, and the token in it. What does not depend on
+// another load is loaded first.
 __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, SmPlan p) {
-    __shared__ uint64_t red[kSmWaves];
+    __shared__ uint64_t memory[2][2][kSmWaves];
+    __shared__ double parts[kSmParts];
     __shared__ Bins bins;
     __shared__ uint32_t found;
     __shared__ uint64_t found_before;
     const uint32_t out = blockIdx.x, tid = threadIdx.x;
-    const RowSettings s = row_settings<kSmWaves>(a, p, out, red);
+    const RowSettings s = p.settings[out];
+    const SmRow r = p.rows[out];
+    // Kept weights by group of chunks, a thread for each group.
+    const uint32_t per = (p.chunks + kSmThreads - 1) / kSmThreads;
+    uint64_t mine = 0, kept = 0;
+    const auto add_chunks = [&] {
+        for (uint32_t c = tid * per; c < min((tid + 1) * per, p.chunks); ++c) {
+            mine += p.chunk_mass[(uint64_t)out * p.chunks + c];
+            kept += p.chunk_count[(uint64_t)out * p.chunks + c];
+        }
+    };
+    if (s.mode >= kSmAll) add_chunks();
+    uint64_t key[kSmPerThread], w[kSmPerThread];
+    key[0] = tid < p.list ? p.keys[(uint64_t)out * p.list + tid] : 0;
+    fill_parts(parts);
     if (s.mode == kSmAbsent) return;
     if (s.mode < kSmAll) {
         if (tid == 0) {
@@ -537,118 +623,125 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
         }
         return;
     }
+    Together<kSmWaves> all{memory};
+    bins.mass[tid] = 0;
+    __syncthreads();
     uint64_t cut = kLeastKey;
-    uint64_t key[kSmPerThread], w[kSmPerThread];
     uint32_t in = 0, in_k = 0, in_p = 0;
-    bool from_chunks = true;  // what the chunks keep for certain is in the workspace
+    bool clear = true;  // are the bins' masses
     if (s.mode == kSmCut) {
-        const SmRow r = p.rows[out];
         if (r.listed <= p.list) {
 #pragma unroll
             for (uint32_t i = 0; i < kSmPerThread; ++i) {
                 const uint32_t at = i * kSmThreads + tid;
-                key[i] = w[i] = 0;
-                if (at >= r.listed) continue;
-                key[i] = p.keys[(uint64_t)out * p.list + at];
+                w[i] = 0;
+                if (at >= r.listed) {
+                    key[i] = 0;
+                    continue;
+                }
+                if (i) key[i] = p.keys[(uint64_t)out * p.list + at];
                 const float v = key_value(key[i]);
                 const uint32_t b = bin_of(v, s);
-                w[i] = whole_weight(scaled(v, s.m, s.inv_t), s.shift);
+                w[i] = whole_weight(scaled(v, s.m, s.per_t), s.shift, parts);
                 in |= 1u << i;
                 in_k |= (uint32_t)(b == r.k_bin) << i;
                 in_p |= (uint32_t)(b >= r.p_lo && b <= r.p_hi) << i;
             }
-            uint64_t above, sum = 0;
+            // Up to 64 are the first wave's.
+            const bool few = r.listed <= 64;
+            const auto find = [&](auto mass, uint32_t among, uint64_t target) -> uint64_t {
+                constexpr bool kMass = decltype(mass)::value;
+                if (!few) {
+                    clear = false;
+                    return find_listed<kMass>(key, w, among, target, bins, all);
+                }
+                if (tid < 64) {
+                    const uint64_t c = find_few<kMass>(among & 1u ? key[0] : 0, w[0], target);
+                    if (tid == 0) bins.cut = c;
+                }
+                __syncthreads();
+                return bins.cut;
+            };
+            uint64_t sum = 0;
             if (r.k_bin != kNoBin) {
-                cut = find_listed<false>(key, w, in_k, r.k_rank, bins, red, above);
+                cut = find(std::false_type(), in_k, r.k_rank);
                 if (s.by_mass) {
 #pragma unroll
                     for (uint32_t i = 0; i < kSmPerThread; ++i)
                         if ((in_k >> i & 1u) && key[i] >= cut) sum += w[i];
-                    sum = r.k_mass + block_sum<kSmWaves>(sum, red);
+                    sum = r.k_mass + all.sum(sum);  // (its barrier: all have read bins.cut)
                 }
-            } else if (s.by_mass) {
-                for (uint32_t i = tid; i < kSmBins; i += kSmThreads) sum += p.mass[(uint64_t)out * kSmBins + i];
-                sum = block_sum<kSmWaves>(sum, red);
+            } else {
+                sum = r.mass;
             }
             if (s.by_mass) {
 #pragma unroll
                 for (uint32_t i = 0; i < kSmPerThread; ++i)
                     if ((in_p >> i & 1u) && key[i] < cut) in_p &= ~(1u << i);
-                cut = max(cut, find_listed<true>(key, w, in_p, mass_target(s.p, sum) - r.p_mass, bins, red, above));
+                cut = max(cut, find(std::true_type(), in_p, mass_target(s.p, sum) - r.p_mass));
             }
         } else {
-            from_chunks = false;
-            in = 0;
-            if (s.k) cut = max(cut, find_cut<false>(s, a.vocab, cut, s.k, bins));
+            // More than the list holds: over all logits again.
+            if (s.k) cut = max(cut, find_cut<false>(s, parts, a.vocab, cut, s.k, bins));
             if (s.by_mass) {
                 uint64_t sum = 0;
                 for (uint32_t i = tid; i < a.vocab; i += kSmThreads) {
                     const float v = s.x[i];
-                    if (order_key(v, i) >= cut) sum += whole_weight(scaled(v, s.m, s.inv_t), s.shift);
+                    if (order_key(v, i) >= cut) sum += whole_weight(scaled(v, s.m, s.per_t), s.shift, parts);
                 }
-                sum = block_sum<kSmWaves>(sum, red);
-                cut = max(cut, find_cut<true>(s, a.vocab, cut, mass_target(s.p, sum), bins));
+                sum = all.sum(sum);
+                cut = max(cut, find_cut<true>(s, parts, a.vocab, cut, mass_target(s.p, sum), bins));
             }
+            // (as the launches over pieces leave them where the list suffices)
+            for (uint32_t c = tid >> 6; c < p.chunks; c += kSmWaves) {
+                uint64_t sum = 0;
+                uint32_t n = 0;
+                for (uint32_t i = c * kSmChunk + (tid & 63); i < min((c + 1) * kSmChunk, a.vocab); i += 64) {
+                    const float v = s.x[i];
+                    const double t = scaled(v, s.m, s.per_t);
+                    if (order_key(v, i) >= cut && t >= s.least) sum += whole_weight(t, s.shift, parts), ++n;
+                }
+                sum = wave_scan(sum);
+                n = (uint32_t)wave_scan(n);
+                if ((tid & 63) == 63) {
+                    p.chunk_mass[(uint64_t)out * p.chunks + c] = sum;
+                    p.chunk_count[(uint64_t)out * p.chunks + c] = n;
+                }
+            }
+            clear = false;
+            __syncthreads();
+            mine = kept = 0;
+            add_chunks();
         }
-    }
-    const auto weight_of = [&](uint32_t i) -> uint64_t {
-        if (i >= a.vocab) return 0;
-        const float v = s.x[i];
-        const double z = scaled(v, s.m, s.inv_t);
-        return order_key(v, i) >= cut && z >= s.least_z ? whole_weight(z, s.shift) : 0;
-    };
-    // Kept weights by group of chunks, a thread for each group.
-    const uint32_t per = (p.chunks + kSmThreads - 1) / kSmThreads;
-    uint64_t mine = 0, kept = 0;
-    if (!from_chunks) {
-        // (as the launches over pieces leave them where the list suffices)
-        for (uint32_t c = tid >> 6; c < p.chunks; c += kSmWaves) {
-            uint64_t sum = 0;
-            uint32_t n = 0;
-            for (uint32_t i = c * kSmChunk + (tid & 63); i < min((c + 1) * kSmChunk, a.vocab); i += 64) {
-                const float v = s.x[i];
-                const double z = scaled(v, s.m, s.inv_t);
-                if (order_key(v, i) >= cut && z >= s.least_z) sum += whole_weight(z, s.shift), ++n;
+        if (!clear) {
+            __syncthreads();
+            bins.mass[tid] = 0;
+            __syncthreads();
+        }
+        // What the list keeps, to its groups.
+#pragma unroll
+        for (uint32_t i = 0; i < kSmPerThread; ++i) {
+            if (!(in >> i & 1u)) continue;
+            if (key[i] < cut || !(scaled(key_value(key[i]), s.m, s.per_t) >= s.least)) {
+                in &= ~(1u << i);
+                continue;
             }
-            sum = wave_scan(sum);
-            n = (uint32_t)wave_scan(n);
-            if ((tid & 63) == 63) {
-                p.chunk_mass[(uint64_t)out * p.chunks + c] = sum;
-                p.chunk_count[(uint64_t)out * p.chunks + c] = n;
-            }
+            ++kept;
+            atomicAdd(&bins.mass[(0xFFFFFFFFu - (uint32_t)key[i]) / kSmChunk / per], (unsigned long long)w[i]);
         }
         __syncthreads();
+        mine += bins.mass[tid];
     }
-    __syncthreads();
-    bins.mass[tid] = 0;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < kSmPerThread; ++i) {
-        if (!(in >> i & 1u)) continue;
-        if (key[i] < cut || !(scaled(key_value(key[i]), s.m, s.inv_t) >= s.least_z)) {
-            in &= ~(1u << i);
-            continue;
-        }
-        ++kept;
-        atomicAdd(&bins.mass[(0xFFFFFFFFu - (uint32_t)key[i]) / kSmChunk / per], (unsigned long long)w[i]);
-    }
-    for (uint32_t c = tid * per; c < min((tid + 1) * per, p.chunks); ++c) {
-        mine += p.chunk_mass[(uint64_t)out * p.chunks + c];
-        kept += p.chunk_count[(uint64_t)out * p.chunks + c];
-    }
-    __syncthreads();
-    mine += bins.mass[tid];
     uint64_t sum;
-    const uint64_t to = block_scan<kSmWaves>(mine, red, sum);
+    const uint64_t to = all.scan(mine, sum, kept);
     const uint64_t target = (uint64_t)((double)s.u * (double)sum);
     if (mine && to > target && to - mine <= target) found = tid, found_before = to - mine;
-    kept = block_sum<kSmWaves>(kept, red);
+    __syncthreads();
     // The chunk of the group.
     const uint32_t group = found;
     uint64_t before = found_before;
     uint32_t chunk = group * per;
     if (per > 1) {
-        __syncthreads();
         bins.mass[tid] = tid < per && chunk + tid < p.chunks ? p.chunk_mass[(uint64_t)out * p.chunks + chunk + tid] : 0;
         __syncthreads();
 #pragma unroll
@@ -663,12 +756,18 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
         }
     }
     const uint32_t id = chunk * kSmChunk + tid;
-    const uint64_t here = weight_of(id);
-    uint64_t all;
-    const uint64_t now = before + block_scan<kSmWaves>(here, red, all);
+    uint64_t here = 0;
+    double t = 0.0;
+    if (id < a.vocab) {
+        const float v = s.x[id];
+        t = scaled(v, s.m, s.per_t);
+        if (order_key(v, id) >= cut && t >= s.least) here = whole_weight(t, s.shift, parts);
+    }
+    uint64_t in_chunk, none = 0;
+    const uint64_t now = before + all.scan(here, in_chunk, none);
     if (here && now > target && now - here <= target) {
         a.tokens[out] = id;
-        if (a.probs) a.probs[out] = (float)(weight(scaled(s.x[id], s.m, s.inv_t), s.shift) / (double)sum);
+        if (a.probs) a.probs[out] = (float)(weight(t, s.shift, parts) / (double)sum);
         if (a.kept) a.kept[out] = (uint32_t)kept;
     }
 }
@@ -676,8 +775,10 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
 SmPlan sm_plan(uint64_t n_rows, uint64_t vocab) {
     SmPlan p{};
     p.chunks = (uint32_t)((vocab + kSmChunk - 1) / kSmChunk);
-    const uint64_t want = (kSmWorkgroups + n_rows - 1) / n_rows, most = (p.chunks + 3) / 4;
-    p.pieces = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(want, kSmMostPieces), most);
+    // Whole chunks for each of a piece's waves, in as few turns as leave enough pieces.
+    const uint64_t fours = (p.chunks + 3) / 4, turns = std::max<uint64_t>(n_rows * fours / kSmWorkgroups, 1);
+    p.per = (uint32_t)std::min(turns, fours) * 4;
+    p.pieces = (p.chunks + p.per - 1) / p.per;
     p.list = (uint32_t)std::min<uint64_t>(kSmList, vocab);
     return p;
 }
@@ -696,6 +797,7 @@ uint64_t sm_layout(SmPlan& p, uint64_t n_rows, uint8_t* base) {
     p.chunk_count = reinterpret_cast<uint32_t*>(take(n_rows * p.chunks * 4));
     p.keys = reinterpret_cast<uint64_t*>(take(n_rows * p.list * 8));
     p.rows = reinterpret_cast<SmRow*>(take(n_rows * sizeof(SmRow)));
+    p.settings = reinterpret_cast<RowSettings*>(take(n_rows * sizeof(RowSettings)));
     return at;
 }
 
