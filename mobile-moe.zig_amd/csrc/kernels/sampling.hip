@@ -4,13 +4,25 @@
 // With m the row's largest logit and T the temperature a token's weight is
 // w = exp((x - m) / T). All three filters keep the front of one order (larger
 // logits first, equal ones by the lower id), so what is kept is every token
-// with a key (rank_key) at or above one cut. The token drawn is the first kept id
+// with a key (order_key) at or above one cut. The token drawn is the first kept id
 // at which the running sum of the kept weights, by id, exceeds u times their
 // sum.
 //
 // A comparison of sums must not depend on how they were taken, so weights are
 // computed in 64 bits (weight()) and summed as whole multiples of 2^-shift
 // (44 for up to 2^18 tokens): integer sums have no order.
+//
+// Four launches: the largest logit (pieces of rows); a histogram of tokens and
+// weights over bins of (m - x) / T; the tokens of the bins that hold the cuts, in a
+// list, and what every 1024 logits keep for certain; the cuts in the list, the 1024
+// logits and the token that u falls on (a workgroup per row). Bound: with few rows
+// the latency of four launches, each two or three dependent trips to memory and a
+// few barriers; with many by vector instructions, about 30 for each logit and
+// weight. Measured with 154880 tokens, us (largest, histogram, list, draw): one
+// row with top-p 4.1, 6.1, 6.3, 7.5, together 25.5; 16 rows with top-k 5.7, 6.2, 7.5,
+// 6.3, together 24.2; 64 rows with settings of their own 10.4, 14.7, 17.2, 11.6, together
+// 52.4 (their logits are 39.7 MB, 8.3 us of copying). One workgroup per row for all
+// of it took 586, 542 and 1036.
 #include <algorithm>
 #include <type_traits>
 
@@ -24,9 +36,14 @@ namespace {
 
 // Threads of the launches over pieces, and of those over rows.
 constexpr uint32_t kSmPiece = 256, kSmThreads = 1024, kSmWaves = kSmThreads / 64;
-constexpr uint32_t kSmChunk = 1024;      // logits that a wave takes at a time
+// Logits that a wave takes at a time, and a lane of it. (256: the histogram's sums in
+// memory meet four times as many workgroups, 16 rows took 37 us for 26.)
+constexpr uint32_t kSmChunk = 1024, kSmEach = kSmChunk / 64;
 constexpr uint32_t kSmBins = 1024;       // of the row's histogram
-constexpr uint32_t kSmWorkgroups = 2048; // pieces of a call that are enough
+// Pieces of a call that are enough: with 64 rows 512, 1024 and 2048 took 57.7, 53.2
+// and 55.7 us.
+constexpr uint32_t kSmWorkgroups = 1024;
+constexpr uint32_t kSmBeside = 4;        // of a lane's logits, worked on beside each other
 constexpr uint32_t kSmPerThread = 8;     // tokens beside the cut that a thread of the last launch takes
 constexpr uint32_t kSmList = kSmPerThread * kSmThreads;
 
@@ -45,32 +62,47 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 
 // A weight is 2^(t / 256) with t = (x - m) 256 / (T ln 2), rounded to n + f:
 // 2^(n / 256) is a table's entry and an exponent, 2^(f / 256) a series of four
-// powers (the next is below 4e-17). A fifth of the time of a series alone.
-constexpr uint32_t kSmParts = 256;
-__device__ __forceinline__ void fill_parts(double* parts) {  // by the first 256 threads; a barrier follows
-    if (threadIdx.x >= kSmParts) return;
-    const double f = (int)(threadIdx.x < 128 ? threadIdx.x : threadIdx.x - 256) * (0.6931471805599453 / 256);
-    double p = 1.0, n = 14.0;
-    for (int i = 0; i < 14; ++i, n -= 1.0) p = fma(p, f / n, 1.0);
-    parts[threadIdx.x] = threadIdx.x < 128 ? p : 2.0 * p;
+// powers (the next is below 4e-17). Half the
+// instructions of a series of eleven powers.
+constexpr int kSmParts = 256;
+struct Parts {
+    double of[kSmParts];
+};
+constexpr Parts make_parts() {
+    Parts t{};
+    for (int i = 0; i < kSmParts; ++i) {
+        const double f = (i < kSmParts / 2 ? i : i - kSmParts) * (0.6931471805599453 / kSmParts);
+        double p = 1.0;
+        for (int n = 14; n > 0; --n) p = 1.0 + p * f / n;
+        t.of[i] = i < kSmParts / 2 ? p : 2.0 * p;
+    }
+    return t;
 }
-// t; 0 for the largest itself, an infinite one too.
-__device__ __forceinline__ double scaled(float x, float m, double per_t) {
-    return x == m ? 0.0 : ((double)x - (double)m) * per_t;
+__constant__ const Parts kParts = make_parts();
+__device__ __forceinline__ void fill_parts(double* parts) {  // by the first 256 threads; a barrier follows
+    if (threadIdx.x < kSmParts) parts[threadIdx.x] = kParts.of[threadIdx.x];
+}
+// (The compiler copies a constant addend to a vector register before each step.)
+__device__ __forceinline__ double fma_to(double a, double b, double addend) {
+    double d;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(addend));
+    return d;
 }
 // The weight times 2^shift, for t <= 0. From 2^-64 on down as 2^-64, which is 0 for every shift.
 __device__ __forceinline__ double weight(double t, int shift, const double* parts) {
-    constexpr double kLn2 = 0.6931471805599453 / 256;
-    t = fmax(t, -64.0 * 256);
-    const double r = t + 0x1.8p52;  // n in its lowest bits
-    const int n = (int)(uint32_t)__double_as_longlong(r);
-    const double f = t - (r - 0x1.8p52);
+    constexpr double kLn2 = 0.6931471805599453 / kSmParts;
+    const double whole = 0x1.8p52 + kSmParts * shift;
+    t = fmax(t, -64.0 * kSmParts);
+    const double r = t + whole;  // n and the shift in its lowest bits
+    const uint32_t n = (uint32_t)__double_as_longlong(r);
+    const double f = t - (r - whole);
     double p = kLn2 * kLn2 * kLn2 * kLn2 / 24;
-    p = fma(p, f, kLn2 * kLn2 * kLn2 / 6);
-    p = fma(p, f, kLn2 * kLn2 / 2);
-    p = fma(p, f, kLn2);
-    const double part = parts[n & (int)(kSmParts - 1)];
-    return __longlong_as_double(__double_as_longlong(fma(part, p * f, part)) + ((long long)((n >> 8) + shift) << 52));
+    p = fma_to(f, p, kLn2 * kLn2 * kLn2 / 6);
+    p = fma_to(p, f, kLn2 * kLn2 / 2);
+    p = fma_to(p, f, kLn2);
+    const double part = parts[n & (uint32_t)(kSmParts - 1)];
+    const double w = fma(part, p * f, part);
+    return __hiloint2double(__double2hiint(w) + ((int)n >> 8 << 20), __double2loint(w));
 }
 // The same as a whole number: at most 2^44, so adding 2^52 rounds it to the
 // lower bits of the sum.
@@ -150,8 +182,9 @@ struct RowSettings {
     SmMode mode;
     const float* x;
     uint64_t best;  // the first token's key
-    float m, bin_c;
-    double per_t, least;  // t per logit, and t of min_p
+    bool far;                // is the largest logit infinite
+    float bin_c, bin_m;
+    double m, per_t, least;  // t per logit, and t of min_p
     float p, u;
     uint32_t k;     // 0: no cut by number
     bool by_mass;   // a cut by probability
@@ -176,12 +209,12 @@ struct SmPlan {
     uint32_t* chunk_count;     // [rows][chunks]
     uint64_t* keys;            // [rows][list]
     SmRow* rows;
-    RowSettings* settings;
+    RowSettings *asked, *settings;
 };
 constexpr uint32_t kNoBin = 0xFFFFFFFFu;
 
-// A row's settings, with its largest token's key and its lowest logit.
-__device__ __forceinline__ RowSettings row_settings(const SampleArgs& a, uint32_t out, uint64_t best, float low) {
+// What a row asks for, as far as that does not depend on its logits.
+__device__ __forceinline__ RowSettings row_asked(const SampleArgs& a, uint32_t out) {
     RowSettings s{};
     uint32_t row = out;
     if (a.rows) row = a.rows[out];
@@ -189,12 +222,10 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs& a, uint32_
     s.p = a.top_p ? a.top_p[out] : 1.0f;
     s.u = a.uniform[out];
     s.k = a.top_k ? a.top_k[out] : 0;
-    s.best = best;
     if (a.rows && row == kNoToken) s.mode = kSmAbsent;
     else if (a.rows && row >= a.n_logits) s.mode = kSmNoRow;
     else if (!(t >= 0.0f && t <= 3.4028235e38f && s.p >= 0.0f && least >= 0.0f && least <= 1.0f && s.u >= 0.0f && s.u < 1.0f))
         s.mode = kSmBadSetting;
-    else if (s.best < kLeastKey) s.mode = kSmEmpty;
     else if (t == 0.0f || s.k == 1) s.mode = kSmFirst;
     else {
         if (s.k >= a.vocab) s.k = 0;
@@ -203,34 +234,58 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs& a, uint32_
     }
     if (s.mode < kSmFirst) return s;
     s.x = a.logits + row * a.stride;
-    s.m = key_value(s.best);
     s.per_t = 369.3299304675746 / (double)t;  // 256 / ln 2
     s.least = 369.3299304675746 * log((double)least);
     s.shift = a.shift;
+    s.bin_c = 0.25f / t;
+    return s;
+}
+// With the row's largest token's key and its lowest logit.
+__device__ __forceinline__ void row_settings(RowSettings& s, const RowSettings& asked, uint64_t best, float low) {
+    const float m = key_value(best);
+    const bool far = m > 3.4028235e38f;
+    s.mode = asked.mode >= kSmFirst && best < kLeastKey ? kSmEmpty : asked.mode;
+    s.x = asked.x;
+    s.best = best;
+    s.far = far;
     // Bins of 1/32 of the temperature next to the largest logit, twice as wide
     // from four temperatures below it on, and so on; narrower ones where the
     // row's logits are closer together than that.
-    s.bin_c = fminf(fmaxf(0.25f / t, 7.0f / (s.m - low)), 1e30f);
-    return s;
+    s.bin_c = fminf(fmaxf(asked.bin_c, 7.0f * __builtin_amdgcn_rcpf(m - low)), 1e30f);
+    s.m = far ? 0.0 : (double)m;
+    s.per_t = far ? 369.3299304675746 : asked.per_t;
+    s.bin_m = fmaf((float)s.m, s.bin_c, 1.0f);
+    s.least = asked.least;
+    s.p = asked.p;
+    s.u = asked.u;
+    s.k = asked.k;
+    s.by_mass = asked.by_mass;
+    s.shift = asked.shift;
 }
-// The bin of a logit: never smaller for a smaller logit.
+// A logit as the weights and bins see it: beside an infinite one no other one
+// weighs anything, so in such a row that is 0 and all others are far below.
+__device__ __forceinline__ float seen(float x, const RowSettings& s) {
+    return !s.far || !(x > -INFINITY) ? x : x > 3.4028235e38f ? 0.0f : -3.4028235e38f;
+}
+// t of a logit.
+__device__ __forceinline__ double scaled(float x, const RowSettings& s) { return ((double)x - s.m) * s.per_t; }
+// The bin of a logit above -infinity: never smaller for a smaller logit.
 __device__ __forceinline__ uint32_t bin_of(float x, const RowSettings& s) {
-    const float d = s.m - x;
-    const float y = x == s.m ? 1.0f : fminf(fmaf(d, s.bin_c, 1.0f), 255.9f);
-    return min((__float_as_uint(y) - 0x3F800000u) >> 16, kSmBins - 1);
+    const float y = __builtin_amdgcn_fmed3f(fmaf(-x, s.bin_c, s.bin_m), 1.0f, 255.9f);
+    return (__float_as_uint(y) - 0x3F800000u) >> 16;
 }
 __device__ __forceinline__ uint64_t mass_target(float p, uint64_t sum) {
     return max((uint64_t)ceil((double)p * (double)sum), (uint64_t)1);
 }
 
 // A wave's chunk: logit i * 64 + lane, NaN where there is none.
-__device__ __forceinline__ void load_chunk(const float* x, uint32_t vocab, uint32_t chunk, float (&v)[kSmChunk / 64]) {
+__device__ __forceinline__ void load_chunk(const float* x, uint32_t vocab, uint32_t chunk, float (&v)[kSmEach]) {
     const uint32_t first = chunk * kSmChunk, n = min(vocab - first, kSmChunk), lane = threadIdx.x & 63;
     const BufRsrc r = make_rsrc(x + first, n * 4);
 #pragma unroll
-    for (uint32_t i = 0; i < kSmChunk / 64; ++i) v[i] = __uint_as_float(buf_load_b32(r, lane * 4, i * 256));
+    for (uint32_t i = 0; i < kSmEach; ++i) v[i] = __uint_as_float(buf_load_b32(r, lane * 4, i * 256));
 #pragma unroll
-    for (uint32_t i = 0; i < kSmChunk / 64; ++i)
+    for (uint32_t i = 0; i < kSmEach; ++i)
         if (i * 64 + lane >= n) v[i] = __builtin_nanf("");
 }
 
@@ -253,18 +308,37 @@ __global__ __launch_bounds__(kSmPiece) void sample_best_kernel(SampleArgs a, SmP
     }
     if (piece == 0 && threadIdx.x == 0) p.rows[out].listed = 0;
     const float* x = row_logits(a, out);
-    float top = -INFINITY, low = INFINITY;
-    uint32_t id = 0;
+    float top = -INFINITY;
+    uint32_t id = 0, under = 0, over = 0xFFFFFFFFu;
+    float v[kSmEach];
+    if (x && c0 + wave < c1) load_chunk(x, a.vocab, c0 + wave, v);
+    if (piece == 0 && threadIdx.x == 0) p.asked[out] = row_asked(a, out);
     if (x)
         for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
-            float v[kSmChunk / 64];
-            load_chunk(x, a.vocab, c, v);
+            if (c != c0 + wave) load_chunk(x, a.vocab, c, v);
+            float here = -INFINITY;
 #pragma unroll
-            for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
-                if (v[i] > top) top = v[i], id = c * kSmChunk + i * 64 + lane;
-                if (v[i] > -INFINITY) low = fminf(low, v[i]);
+            for (uint32_t i = 0; i < kSmEach; i += 2) {
+                const float v0 = v[i] > -INFINITY ? v[i] : -INFINITY, v1 = v[i + 1] > -INFINITY ? v[i + 1] : -INFINITY;
+                here = __builtin_amdgcn_fmed3f(__builtin_amdgcn_fmed3f(here, v0, INFINITY), v1, INFINITY);
+                const uint32_t b0 = __float_as_uint(v0), b1 = __float_as_uint(v1);
+                under = max(under, max(b0 + 0x00800000u, b1 + 0x00800000u));
+                over = min(over, min(b0, b1));
+            }
+            // The wave's largest, at its lowest id.
+            here = key_value(lane_value(wave_max_scan((uint64_t)order_bits(here)), 63) << 32);
+            if (!(here > top)) continue;
+            top = here;
+#pragma unroll
+            for (uint32_t i = kSmEach; i-- > 0;) {
+                const uint64_t at = __ballot(v[i] == here);
+                if (at) id = c * kSmChunk + i * 64 + (uint32_t)__builtin_ctzll(at);
             }
         }
+    // Of finite numbers and +infinity the lowest: a negative one's bits, more for a
+    // lower number, go past those of -infinity with 2^23 added; if there is none, the
+    // least bits are the lowest number's.
+    float low = under >= 0x80800000u ? __uint_as_float(under - 0x00800000u) : over < 0x7F800001u ? __uint_as_float(over) : INFINITY;
     uint64_t best = order_key(top, id), lowest = order_bits(-low);
     Together<kSmPiece / 64> all{memory};
     all.largest(best, lowest);
@@ -285,8 +359,9 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
     const uint32_t c0 = piece * p.per, c1 = min(c0 + p.per, p.chunks);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float* x = row_logits(a, out);
-    float v[kSmChunk / 64];
+    float v[kSmEach];
     if (x && c0 + wave < c1) load_chunk(x, a.vocab, c0 + wave, v);  // its latency beside the settings'
+    const RowSettings& asked = p.asked[out];
     uint64_t best = 0, lowest = 0;
     for (uint32_t i = threadIdx.x; i < p.pieces; i += kSmPiece) {
         best = max(best, p.best[(uint64_t)out * p.pieces + i]);
@@ -296,21 +371,29 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
     for (uint32_t i = threadIdx.x; i < kSmBins; i += kSmPiece) mass[i] = 0, count[i] = 0;
     Together<kSmPiece / 64> all{memory};
     all.largest(best, lowest);
-    const RowSettings s = row_settings(a, out, best, -key_value(lowest << 32));
+    RowSettings s;
+    row_settings(s, asked, best, -key_value(lowest << 32));
     if (piece == 0 && threadIdx.x == 0) p.settings[out] = s;
     if (s.mode < kSmAll) return;
+    const auto next = [&](uint32_t c) {
+        if (c != c0 + wave) load_chunk(x, a.vocab, c, v);
+        if (s.far) {
+#pragma unroll
+            for (uint32_t i = 0; i < kSmEach; ++i) v[i] = seen(v[i], s);
+        }
+    };
     if (s.mode == kSmAll) {
         for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
-            if (c != c0 + wave) load_chunk(x, a.vocab, c, v);
+            next(c);
             uint64_t sum = 0;
             uint32_t n = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
-                const double t = scaled(v[i], s.m, s.per_t);
-                if (v[i] > -INFINITY && t >= s.least) {
-                    sum += whole_weight(t, s.shift, parts);
-                    n += 1;
-                }
+            for (uint32_t i = 0; i < kSmEach; ++i) {
+                const double t = scaled(v[i], s);
+                const uint64_t w = whole_weight(t, s.shift, parts);
+                const bool keep = v[i] > -INFINITY && t >= s.least;
+                sum += keep ? w : 0;
+                n += keep;
             }
             sum = wave_scan(sum);
             n = (uint32_t)wave_scan(n);
@@ -321,16 +404,30 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
         }
         return;
     }
-    for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
-        if (c != c0 + wave) load_chunk(x, a.vocab, c, v);
+    const auto fill = [&](auto by_number, auto by_mass) {
+        for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
+            next(c);
 #pragma unroll
-        for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
-            if (!(v[i] > -INFINITY)) continue;
-            const uint32_t b = bin_of(v[i], s);
-            if (s.k) atomicAdd(&count[b], 1u);
-            if (s.by_mass) atomicAdd(&mass[b], (unsigned long long)whole_weight(scaled(v[i], s.m, s.per_t), s.shift, parts));
+            for (uint32_t i0 = 0; i0 < kSmEach; i0 += kSmBeside) {
+                uint32_t b[kSmBeside];
+                uint64_t w[kSmBeside];
+#pragma unroll
+                for (uint32_t i = 0; i < kSmBeside; ++i) {
+                    b[i] = bin_of(v[i0 + i], s);
+                    if (by_mass()) w[i] = whole_weight(scaled(v[i0 + i], s), s.shift, parts);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kSmBeside; ++i) {
+                    if (!(v[i0 + i] > -INFINITY)) continue;
+                    if (by_number()) atomicAdd(&count[b[i]], 1u);
+                    if (by_mass()) atomicAdd(&mass[b[i]], (unsigned long long)w[i]);
+                }
+            }
         }
-    }
+    };
+    if (!s.by_mass) fill(std::true_type(), std::false_type());
+    else if (!s.k) fill(std::false_type(), std::true_type());
+    else fill(std::true_type(), std::true_type());
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < kSmBins; i += kSmPiece) {
         if (count[i]) atomicAdd(&p.count[(uint64_t)out * kSmBins + i], count[i]);
@@ -340,18 +437,19 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
 
 // The bins that the cuts are in: their tokens go into the row's list, and what
 // each chunk has in the bins before all of them is kept for certain.
-__global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmPlan p) {
+__global__ __launch_bounds__(kSmPiece, 5) void sample_list_kernel(SampleArgs a, SmPlan p) {
     constexpr uint32_t kWaves = kSmPiece / 64, kPer = kSmBins / kSmPiece;
     __shared__ uint64_t memory[2][2][kWaves];
+    __shared__ uint64_t most;
+    __shared__ uint32_t listed, listed_at;
     __shared__ double parts[kSmParts];
     __shared__ SmRow row;
-    __shared__ uint64_t k_here;
     const uint32_t out = blockIdx.x / p.pieces, piece = blockIdx.x - out * p.pieces;
     const uint32_t c0 = piece * p.per, c1 = min(c0 + p.per, p.chunks);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = threadIdx.x;
     const RowSettings s = p.settings[out];
     const float* x = row_logits(a, out);
-    float v[kSmChunk / 64];
+    float v[kSmEach];
     if (x && c0 + wave < c1) load_chunk(x, a.vocab, c0 + wave, v);
     uint64_t m[kPer], mass_to = 0, all_mass, num_to = 0, all_num;
     uint32_t n[kPer];
@@ -363,7 +461,8 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
     if (s.mode != kSmCut) return;
     if (tid == 0) {
         row = SmRow{0, kNoBin, 0, kNoBin, kNoBin, 0, 0, 0};
-        k_here = 0;
+        most = 0;
+        listed = 0;
     }
     fill_parts(parts);
 #pragma unroll
@@ -373,7 +472,8 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
     all.scan2(mass_to, num_to, all_mass, all_num);
     mass_to -= mass_here;
     num_to -= num_here;
-    if (s.k && s.k < all_num) {
+    const bool by_k = s.k && s.k < all_num;
+    if (by_k) {
         uint64_t at = num_to, w = mass_to;
 #pragma unroll
         for (uint32_t i = 0; i < kPer; ++i) {
@@ -381,17 +481,16 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
                 row.k_bin = tid * kPer + i;
                 row.k_rank = (uint32_t)(s.k - at);
                 row.k_mass = w;
-                k_here = m[i];
+                most = w + m[i];
             }
             at += n[i];
             w += m[i];
         }
+        __syncthreads();
     }
-    __syncthreads();
     if (s.by_mass) {
         // The sum that the cut is a part of, at least and at most.
-        const bool by_k = row.k_bin != kNoBin;
-        const uint64_t lo = mass_target(s.p, by_k ? row.k_mass : all_mass), hi = mass_target(s.p, by_k ? row.k_mass + k_here : all_mass);
+        const uint64_t lo = mass_target(s.p, by_k ? row.k_mass : all_mass), hi = mass_target(s.p, by_k ? most : all_mass);
         uint64_t w = mass_to;
 #pragma unroll
         for (uint32_t i = 0; i < kPer; ++i) {
@@ -416,40 +515,66 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
         to->mass = all_mass;
     }
     const uint32_t sure = min(r.k_bin, r.p_lo);
-    for (uint32_t c = c0 + wave; c < c1; c += kWaves) {
-        if (c != c0 + wave) load_chunk(x, a.vocab, c, v);
+    // Every wave takes as many turns: they ask for their tokens' places together.
+    for (uint32_t c = c0 + wave; c < c0 + p.per; c += kWaves) {
+        if (c != c0 + wave && c < c1) load_chunk(x, a.vocab, c, v);
+        if (c >= c1) {
+#pragma unroll
+            for (uint32_t i = 0; i < kSmEach; ++i) v[i] = __builtin_nanf("");
+        }
+        if (s.far) {
+#pragma unroll
+            for (uint32_t i = 0; i < kSmEach; ++i) v[i] = seen(v[i], s);
+        }
         uint64_t mine = 0;
         uint32_t kept = 0, to_list = 0;
+        uint32_t is_sure = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
-            if (!(v[i] > -INFINITY)) continue;
+        for (uint32_t i = 0; i < kSmEach; ++i) {
             const uint32_t b = bin_of(v[i], s);
-            if (b < sure) {
-                const double t = scaled(v[i], s.m, s.per_t);
-                if (t >= s.least) {
-                    mine += whole_weight(t, s.shift, parts);
-                    kept += 1;
+            const bool any = v[i] > -INFINITY;
+            is_sure |= (uint32_t)(any && b < sure) << i;
+            to_list |= (uint32_t)(any && (b == r.k_bin || (b >= r.p_lo && b <= r.p_hi))) << i;
+        }
+        if (__ballot(is_sure != 0)) {
+#pragma unroll
+            for (uint32_t i0 = 0; i0 < kSmEach; i0 += kSmBeside) {
+                if (__ballot((is_sure >> i0 & ((1u << kSmBeside) - 1)) != 0) == 0) continue;
+#pragma unroll
+                for (uint32_t i = i0; i < i0 + kSmBeside; ++i) {
+                    const double t = scaled(v[i], s);
+                    const uint64_t w = whole_weight(t, s.shift, parts);
+                    const bool keep = (is_sure >> i & 1u) && t >= s.least;
+                    mine += keep ? w : 0;
+                    kept += keep;
                 }
-            } else if (b == r.k_bin || (b >= r.p_lo && b <= r.p_hi)) {
-                to_list |= 1u << i;
             }
         }
         mine = wave_scan(mine);
         kept = (uint32_t)wave_scan(kept);
-        if (lane == 63) {
+        if (lane == 63 && c < c1) {
             p.chunk_mass[(uint64_t)out * p.chunks + c] = mine;
             p.chunk_count[(uint64_t)out * p.chunks + c] = kept;
         }
-        const uint32_t here = (uint32_t)__popc(to_list);
-        if (__ballot(here != 0) == 0) continue;
-        const uint32_t to = (uint32_t)wave_scan(here);
+        const uint32_t here = (uint32_t)__popc(to_list), to = (uint32_t)wave_scan(here);
         uint32_t at = 0;
-        if (lane == 63) at = atomicAdd(&p.rows[out].listed, to);
-        at = (uint32_t)__builtin_amdgcn_readlane(at, 63) + to - here;
+        if (lane == 63 && to) at = atomicAdd(&listed, to);
+        __syncthreads();
+        if (tid == 0 && listed) listed_at = atomicAdd(&p.rows[out].listed, listed);
+        __syncthreads();
+        at = listed_at + (uint32_t)__builtin_amdgcn_readlane(at, 63) + to - here;
+        if (c + kWaves < c0 + p.per) {
+            __syncthreads();
+            if (tid == 0) listed = 0;
+            __syncthreads();
+        }
 #pragma unroll
-        for (uint32_t i = 0; i < kSmChunk / 64; ++i) {
+        for (uint32_t i = 0; i < kSmEach; ++i) {
             if (!(to_list >> i & 1u)) continue;
-            if (at < p.list) p.keys[(uint64_t)out * p.list + at] = order_key(v[i], c * kSmChunk + i * 64 + lane);
+            if (at < p.list) {
+                const uint32_t id = c * kSmChunk + i * 64 + lane;
+                p.keys[(uint64_t)out * p.list + at] = order_key(s.far ? x[id] : v[i], id);
+            }
             ++at;
         }
     }
@@ -481,7 +606,7 @@ __device__ uint64_t find_cut(const RowSettings& s, const double* parts, uint32_t
             if (k < floor || (low < 54 && (k >> (low + bits)) != prefix)) continue;
             const uint32_t at = (uint32_t)(k >> low) & ((1u << bits) - 1);
             atomicAdd(&b.count[at], 1u);
-            if (MASS) atomicAdd(&b.mass[at], (unsigned long long)whole_weight(scaled(v, s.m, s.per_t), s.shift, parts));
+            if (MASS) atomicAdd(&b.mass[at], (unsigned long long)whole_weight(scaled(seen(v, s), s), s.shift, parts));
         }
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -640,9 +765,9 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
                     continue;
                 }
                 if (i) key[i] = p.keys[(uint64_t)out * p.list + at];
-                const float v = key_value(key[i]);
+                const float v = seen(key_value(key[i]), s);
                 const uint32_t b = bin_of(v, s);
-                w[i] = whole_weight(scaled(v, s.m, s.per_t), s.shift, parts);
+                w[i] = whole_weight(scaled(v, s), s.shift, parts);
                 in |= 1u << i;
                 in_k |= (uint32_t)(b == r.k_bin) << i;
                 in_p |= (uint32_t)(b >= r.p_lo && b <= r.p_hi) << i;
@@ -687,7 +812,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
                 uint64_t sum = 0;
                 for (uint32_t i = tid; i < a.vocab; i += kSmThreads) {
                     const float v = s.x[i];
-                    if (order_key(v, i) >= cut) sum += whole_weight(scaled(v, s.m, s.per_t), s.shift, parts);
+                    if (order_key(v, i) >= cut) sum += whole_weight(scaled(seen(v, s), s), s.shift, parts);
                 }
                 sum = all.sum(sum);
                 cut = max(cut, find_cut<true>(s, parts, a.vocab, cut, mass_target(s.p, sum), bins));
@@ -698,7 +823,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
                 uint32_t n = 0;
                 for (uint32_t i = c * kSmChunk + (tid & 63); i < min((c + 1) * kSmChunk, a.vocab); i += 64) {
                     const float v = s.x[i];
-                    const double t = scaled(v, s.m, s.per_t);
+                    const double t = scaled(seen(v, s), s);
                     if (order_key(v, i) >= cut && t >= s.least) sum += whole_weight(t, s.shift, parts), ++n;
                 }
                 sum = wave_scan(sum);
@@ -722,7 +847,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
 #pragma unroll
         for (uint32_t i = 0; i < kSmPerThread; ++i) {
             if (!(in >> i & 1u)) continue;
-            if (key[i] < cut || !(scaled(key_value(key[i]), s.m, s.per_t) >= s.least)) {
+            if (key[i] < cut || !(scaled(seen(key_value(key[i]), s), s) >= s.least)) {
                 in &= ~(1u << i);
                 continue;
             }
@@ -760,7 +885,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
     double t = 0.0;
     if (id < a.vocab) {
         const float v = s.x[id];
-        t = scaled(v, s.m, s.per_t);
+        t = scaled(seen(v, s), s);
         if (order_key(v, id) >= cut && t >= s.least) here = whole_weight(t, s.shift, parts);
     }
     uint64_t in_chunk, none = 0;
@@ -797,6 +922,7 @@ uint64_t sm_layout(SmPlan& p, uint64_t n_rows, uint8_t* base) {
     p.chunk_count = reinterpret_cast<uint32_t*>(take(n_rows * p.chunks * 4));
     p.keys = reinterpret_cast<uint64_t*>(take(n_rows * p.list * 8));
     p.rows = reinterpret_cast<SmRow*>(take(n_rows * sizeof(SmRow)));
+    p.asked = reinterpret_cast<RowSettings*>(take(n_rows * sizeof(RowSettings)));
     p.settings = reinterpret_cast<RowSettings*>(take(n_rows * sizeof(RowSettings)));
     return at;
 }
