@@ -12,9 +12,17 @@ namespace mmhip {
 namespace {
 
 constexpr int kEmbedThreads = 256;
+#ifndef EMF
+#define EMF 524288
+#endif
+constexpr uint64_t kEmbedFew = EMF;  // values of a call
 
 __device__ __forceinline__ uint32_t half_at(const uint8_t* p) { return *reinterpret_cast<const uint16_t*>(p); }
-__device__ __forceinline__ uint32_t word_at(const uint8_t* p) { return half_at(p) | half_at(p + 2) << 16; }
+__device__ __forceinline__ uint32_t word_at(const uint8_t* p) {  // at any even address
+    uint32_t v;
+    __builtin_memcpy(&v, __builtin_assume_aligned(p, 2), 4);
+    return v;
+}
 
 enum EmbedType { kEmbF32, kEmbF16, kEmbQ8, kEmbIq2, kEmbQ4, kEmbIq4 };
 
@@ -56,28 +64,56 @@ __device__ __forceinline__ void quad(const uint8_t* row, uint32_t q, uint32_t n,
     }
 }
 
-template <int T>
-__global__ __launch_bounds__(kEmbedThreads) void embed_kernel(EmbedArgs a, uint32_t parts) {
-    const uint64_t t = blockIdx.x / parts;
-    const uint32_t part = blockIdx.x - (uint32_t)(t * parts);
+// A wave takes 64 EACH quads of a row, a lane every 64th, all loads before the first store.
+template <int T, uint32_t EACH>
+__global__ __launch_bounds__(kEmbedThreads) void embed_kernel(EmbedArgs a, uint64_t n_tokens, uint32_t parts) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t unit = (uint64_t)blockIdx.x * (kEmbedThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t t = unit / parts;
+    if (t >= n_tokens) return;
+    const uint32_t part = (uint32_t)(unit - t * parts);
     const uint32_t token = a.tokens[t];
     if (token == kNoToken) return;
     const bool bad = token >= a.rows;
-    if (bad && part == 0 && threadIdx.x == 0) report(a.status, kBadEmbedToken);
+    if (bad && part == 0 && lane == 0) report(a.status, kBadEmbedToken);
     const uint8_t* row = a.table + (bad ? 0 : token) * a.row_bytes;
     float* y = a.y + t * a.y_stride;
-    const uint32_t q = part * kEmbedThreads + threadIdx.x;
-    if (4 * q >= a.cols) return;
-    const uint32_t n = min(a.cols - 4 * q, 4u);
-    float v[4];
-    quad<T>(row, q, n, v);
+    float v[EACH][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = bad ? __builtin_nanf("") : v[e] * a.scale;
-    if (a.vec && n == 4) {
-        *reinterpret_cast<float4*>(y + 4 * q) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-        for (uint32_t e = 0; e < n; ++e) y[4 * q + e] = v[e];
+    for (uint32_t i = 0; i < EACH; ++i) {
+        const uint32_t q = (part * EACH + i) * 64 + lane;
+        if (4 * q < a.cols) quad<T>(row, q, min(a.cols - 4 * q, 4u), v[i]);
     }
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i) {
+        const uint32_t q = (part * EACH + i) * 64 + lane;
+        if (4 * q >= a.cols) return;
+        const uint32_t n = min(a.cols - 4 * q, 4u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = bad ? __builtin_nanf("") : v[i][e] * a.scale;
+        if (a.vec && n == 4) {
+            *reinterpret_cast<float4*>(y + 4 * q) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+        } else {
+            for (uint32_t e = 0; e < n; ++e) y[4 * q + e] = v[i][e];
+        }
+    }
+}
+
+template <uint32_t EACH>
+hipError_t launch_with(const EmbedArgs& a, uint32_t type, uint64_t n_tokens, hipStream_t s) {
+    const uint32_t parts = (a.cols + 256 * EACH - 1) / (256 * EACH);
+    constexpr uint32_t kWaves = kEmbedThreads / 64;
+    const unsigned grid = (unsigned)((n_tokens * parts + kWaves - 1) / kWaves);
+    switch (type) {
+        case 0: embed_kernel<kEmbF32, EACH><<<grid, kEmbedThreads, 0, s>>>(a, n_tokens, parts); break;
+        case 1: embed_kernel<kEmbF16, EACH><<<grid, kEmbedThreads, 0, s>>>(a, n_tokens, parts); break;
+        case 2: embed_kernel<kEmbQ4, EACH><<<grid, kEmbedThreads, 0, s>>>(a, n_tokens, parts); break;
+        case 8: embed_kernel<kEmbQ8, EACH><<<grid, kEmbedThreads, 0, s>>>(a, n_tokens, parts); break;
+        case 16: embed_kernel<kEmbIq2, EACH><<<grid, kEmbedThreads, 0, s>>>(a, n_tokens, parts); break;
+        case 20: embed_kernel<kEmbIq4, EACH><<<grid, kEmbedThreads, 0, s>>>(a, n_tokens, parts); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -85,18 +121,7 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(EmbedArgs a, uint3
 hipError_t launch_embed(const EmbedArgs& a_in, uint32_t type, uint64_t n_tokens, hipStream_t s) {
     EmbedArgs a = a_in;
     a.vec = (reinterpret_cast<uintptr_t>(a.y) & 15u) == 0 && a.y_stride % 4 == 0;
-    const uint32_t parts = ((a.cols + 3) / 4 + kEmbedThreads - 1) / kEmbedThreads;
-    const unsigned grid = (unsigned)(n_tokens * parts);
-    switch (type) {
-        case 0: embed_kernel<kEmbF32><<<grid, kEmbedThreads, 0, s>>>(a, parts); break;
-        case 1: embed_kernel<kEmbF16><<<grid, kEmbedThreads, 0, s>>>(a, parts); break;
-        case 2: embed_kernel<kEmbQ4><<<grid, kEmbedThreads, 0, s>>>(a, parts); break;
-        case 8: embed_kernel<kEmbQ8><<<grid, kEmbedThreads, 0, s>>>(a, parts); break;
-        case 16: embed_kernel<kEmbIq2><<<grid, kEmbedThreads, 0, s>>>(a, parts); break;
-        case 20: embed_kernel<kEmbIq4><<<grid, kEmbedThreads, 0, s>>>(a, parts); break;
-        default: return hipErrorInvalidValue;
-    }
-    return hipGetLastError();
+    return n_tokens * a.cols <= kEmbedFew ? launch_with<1>(a, type, n_tokens, s) : launch_with<4>(a, type, n_tokens, s);
 }
 
 }  // namespace mmhip

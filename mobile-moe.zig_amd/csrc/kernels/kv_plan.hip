@@ -14,23 +14,10 @@ namespace mmhip {
 
 namespace {
 
-constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
-
-// The sum over threads 0 .. this one, and over all. Two barriers.
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* red, uint64_t& all) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t in = wave_scan(v);
-    if (lane == 63) red[wave] = in;
-    __syncthreads();
-    uint64_t before = 0;
-    all = 0;
-    for (uint32_t w = 0; w < kPlanWaves; ++w) {
-        if (w < wave) before += red[w];
-        all += red[w];
-    }
-    __syncthreads();
-    return before + in;
-}
+constexpr uint32_t kPlanThreads = 1024, kPlanFew = 256;  // of the launch over requests; where they are few
+constexpr uint32_t kPlanSmall = 4096;                    // tokens that the same launch writes
+constexpr uint32_t kPlanFill = 256;
+constexpr uint32_t kPlanStarts = 2048;                   // of the requests' first tokens, in LDS
 
 __device__ __forceinline__ uint32_t pages_of(const PlanArgs& a, uint64_t positions) {
     return (uint32_t)((positions + ((1u << a.page_shift) - 1)) >> a.page_shift);
@@ -62,76 +49,92 @@ __device__ __forceinline__ void pad(const PlanArgs& a, uint32_t t) {
     a.seen[t] = 0;
 }
 
-// Token t < the total: the request it belongs to, the last one whose first
-// token is not behind t.
-__device__ __forceinline__ uint32_t request_of(const uint32_t* firsts, uint32_t n, uint32_t t) {
-    uint32_t lo = 0, hi = n;  // firsts[lo] <= t < firsts[hi]
+// The last of n ascending starts that is not behind t; starts[0] is not.
+__device__ __forceinline__ uint32_t last_start(const uint32_t* starts, uint32_t n, uint32_t t) {
+    uint32_t lo = 0, hi = n;
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
-        if (firsts[mid] <= t) lo = mid;
+        if (starts[mid] <= t) lo = mid;
         else hi = mid;
     }
     return lo;
 }
 
-__device__ __forceinline__ void fill_token(const PlanArgs& a, uint32_t t, uint32_t top) {
-    const uint32_t total = a.firsts[a.n_requests];
-    if (t >= total) return pad(a, t);
-    const uint32_t r = request_of(a.firsts, a.n_requests, t);
-    const PlanRow row = a.work[r];
-    const uint32_t pos = row.start + (t - a.firsts[r]);
-    place(a, t, r, pos, pages_of(a, row.start), row, top);
-}
-
 // Gives request r's pages back: free[row.back_at ..).
+__device__ __forceinline__ void give_page(const PlanArgs& a, uint32_t r, const PlanRow& row, uint32_t i) {
+    const uint64_t at = (uint64_t)row.back_at + i;
+    if (at < a.n_pages) a.free[at] = a.tables[(uint64_t)r * a.table_stride + row.back_from + i];
+}
 __device__ __forceinline__ void give_back(const PlanArgs& a, uint32_t r, uint32_t i0, uint32_t step) {
     const PlanRow row = a.work[r];
-    for (uint32_t i = i0; i < row.back; i += step) {
-        const uint64_t at = (uint64_t)row.back_at + i;
-        if (at < a.n_pages) a.free[at] = a.tables[(uint64_t)r * a.table_stride + row.back_from + i];
-    }
+    for (uint32_t i = i0; i < row.back; i += step) give_page(a, r, row, i);
 }
 
-// The requests' running sums: firsts, granted, last, next_lens, the workspace's
-// rows and the new count of free pages. *top: free pages before any is taken.
-__device__ __forceinline__ uint32_t plan_requests(const PlanArgs& a) {
-    __shared__ uint64_t red[kPlanWaves];
+// What one workgroup keeps of its requests where it does the whole call.
+template <uint32_t N>
+struct PlanHeld {
+    PlanRow rows[N];
+    uint32_t starts[N], backs[N];  // the tokens granted and the pages given back before each
+};
+struct PlanTotals {
+    uint32_t top, tokens, backs;  // free pages before any is taken
+};
+
+// The requests' running sums: firsts, granted, last, next_lens, the rows and the
+// new count of free pages. With `held` there are at most THREADS requests, and the
+// rows stay there.
+template <uint32_t THREADS>
+__device__ __forceinline__ PlanTotals plan_requests(const PlanArgs& a, PlanHeld<THREADS>* held) {
+    __shared__ uint64_t memory[2][2][THREADS / 64];
+    Together<THREADS / 64> together{memory};
     const uint64_t capacity = (uint64_t)a.table_pages << a.page_shift;
+    const bool once = held != nullptr;
     uint32_t count = *a.free_count;
+    PlanRow row{};
+    uint32_t add = 0;
+    // Pages that come back, tokens asked for.
+    uint64_t back_all = 0, asked_all = 0;
+    uint32_t fits = 0;  // the last row's
+    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += THREADS) {
+        const uint32_t r = r0 + threadIdx.x;
+        uint64_t len = 0;
+        row = PlanRow{};
+        add = 0;
+        if (r < a.n_requests) {
+            len = a.lens[r];
+            add = a.added[r];
+            const uint32_t release = a.release ? a.release[r] : 0, shared = a.shared ? a.shared[r] : 0;
+            if (len > capacity) report(a.status, kBadPlanLength);
+            if (release) {
+                const uint32_t pages = min(pages_of(a, len), a.table_pages);
+                row.back_from = min(shared, pages);
+                row.back = pages - row.back_from;
+                len = 0;
+            }
+            if (add > 0 && len + add > capacity) {
+                report(a.status, kBadPlanLength);
+                add = 0;
+            }
+        }
+        row.start = (uint32_t)len;
+        uint64_t back = row.back, asked = add, all_back, all_asked;
+        together.scan2(back, asked, all_back, all_asked);
+        if (add && asked_all + asked > a.max_tokens) {
+            add = 0;
+            report(a.status, kBadPlanTokens);
+        }
+        fits = add;
+        const uint64_t before = (uint64_t)min(count, a.n_pages) + back_all + back - row.back;
+        row.back_at = (uint32_t)min(before, (uint64_t)a.n_pages);
+        row.pages = fits;  // until the second sweep
+        if (!once && r < a.n_requests) a.work[r] = row;
+        if (once) held->backs[threadIdx.x] = (uint32_t)(back - row.back);
+        back_all += all_back;
+        asked_all += all_asked;
+    }
     if (count > a.n_pages) {
         if (threadIdx.x == 0) report(a.status, kBadPlanFree);
         count = a.n_pages;
-    }
-    // Pages that come back.
-    uint64_t back_all = 0;
-    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += kPlanThreads) {
-        const uint32_t r = r0 + threadIdx.x;
-        uint32_t back = 0, from = 0;
-        uint64_t len = 0;
-        if (r < a.n_requests) {
-            len = a.lens[r];
-            if (len > capacity) {
-                report(a.status, kBadPlanLength);
-            }
-            if (a.release && a.release[r]) {
-                const uint32_t held = min(pages_of(a, len), a.table_pages);
-                from = a.shared ? min(a.shared[r], held) : 0;
-                back = held - from;
-                len = 0;
-            }
-        }
-        uint64_t all;
-        const uint64_t in = block_scan(back, red, all);
-        if (r < a.n_requests) {
-            PlanRow row;
-            row.start = (uint32_t)len;
-            row.pages = 0;
-            row.back = back;
-            row.back_from = from;
-            row.back_at = (uint32_t)min<uint64_t>(count + back_all + in - back, a.n_pages);
-            a.work[r] = row;
-        }
-        back_all += all;
     }
     uint64_t top64 = count + back_all;
     if (top64 > a.n_pages) {
@@ -139,66 +142,91 @@ __device__ __forceinline__ uint32_t plan_requests(const PlanArgs& a) {
         top64 = a.n_pages;
     }
     const uint32_t top = (uint32_t)top64;
-    // Tokens and pages asked for, tokens granted.
-    uint64_t asked_all = 0, need_all = 0, given_all = 0, taken = 0;
-    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += kPlanThreads) {
+    // Pages asked for, tokens granted and pages taken.
+    uint64_t need_all = 0, given_all = 0, taken = 0;
+    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += THREADS) {
         const uint32_t r = r0 + threadIdx.x;
-        uint64_t len = 0, add = 0;
-        bool ok = false;
-        if (r < a.n_requests) {
-            len = a.work[r].start;
-            add = a.added[r];
-            ok = add > 0 && len + add <= capacity;
-            if (add > 0 && !ok) report(a.status, kBadPlanLength);
+        if (!once) {
+            row = r < a.n_requests ? a.work[r] : PlanRow{};
+            fits = row.pages;
         }
-        uint64_t all;
-        uint64_t in = block_scan(ok ? add : 0, red, all);
-        if (ok && asked_all + in > a.max_tokens) {
-            ok = false;
-            report(a.status, kBadPlanTokens);
-        }
-        asked_all += all;
-        const uint32_t need = ok ? pages_of(a, len + add) - pages_of(a, len) : 0;
-        in = block_scan(need, red, all);
-        if (need && need_all + in > top) ok = false;
-        const uint64_t pages = need_all + in - need;
+        const uint64_t len = row.start;
+        const uint32_t need = fits ? pages_of(a, len + fits) - pages_of(a, len) : 0;
+        uint64_t pages = need, all;
+        uint64_t none = 0;
+        pages = together.scan(pages, all, none);
+        if (need && need_all + pages > top) fits = 0;
+        const uint64_t before = need_all + pages - need;
         need_all += all;
-        const uint64_t mine = (ok && need ? (uint64_t)need << 32 : 0) | (ok ? add : 0);
-        in = block_scan(mine, red, all);
+        uint64_t given = fits, all_given, took = fits ? need : 0;
+        given = together.scan(given, all_given, took);
         if (r < a.n_requests) {
-            const uint32_t first = (uint32_t)(given_all + (uint32_t)(in - mine));
+            const uint32_t first = (uint32_t)(given_all + given - fits);
             a.firsts[r] = first;
-            a.granted[r] = ok;
-            if (a.last) a.last[r] = ok ? first + (uint32_t)add - 1 : kNoToken;
-            a.work[r].pages = (uint32_t)min<uint64_t>(pages, a.n_pages);
-            a.next_lens[r] = (uint32_t)(len + (ok ? add : 0));
+            a.granted[r] = fits != 0;
+            if (a.last) a.last[r] = fits ? first + fits - 1 : kNoToken;
+            row.pages = (uint32_t)min(before, (uint64_t)a.n_pages);
+            if (once) {
+                held->starts[r] = first;
+                held->rows[r] = row;
+            } else {
+                a.work[r] = row;
+            }
+            a.next_lens[r] = (uint32_t)(len + fits);
         }
-        given_all += (uint32_t)all;
-        taken += all >> 32;
+        given_all += all_given;
+        taken += took;
     }
     if (threadIdx.x == 0) {
         a.firsts[a.n_requests] = (uint32_t)given_all;
         *a.next_free_count = top - (uint32_t)taken;
-        *a.top = top;
+        if (!once) *a.top = top;
     }
-    return top;
+    return {top, (uint32_t)given_all, (uint32_t)min(back_all, (uint64_t)0xFFFFFFFFu)};
 }
 
-__global__ __launch_bounds__(kPlanThreads) void plan_small_kernel(PlanArgs a) {
-    const uint32_t top = plan_requests(a);
+template <uint32_t THREADS>
+__global__ __launch_bounds__(THREADS) void plan_small_kernel(PlanArgs a) {
+    __shared__ PlanHeld<THREADS> held;
+    const PlanTotals all = plan_requests<THREADS>(a, &held);
     __syncthreads();
-    if (a.release) {
-        for (uint32_t r = threadIdx.x >> 6; r < a.n_requests; r += kPlanWaves) give_back(a, r, threadIdx.x & 63, 64);
-        __syncthreads();
+    for (uint32_t i = threadIdx.x; i < all.backs; i += THREADS) {
+        const uint32_t r = last_start(held.backs, a.n_requests, i);
+        give_page(a, r, held.rows[r], i - held.backs[r]);
     }
-    for (uint32_t t = threadIdx.x; t < a.max_tokens; t += kPlanThreads) fill_token(a, t, top);
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < a.max_tokens; t += THREADS) {
+        if (t >= all.tokens) {
+            pad(a, t);
+            continue;
+        }
+        const uint32_t r = last_start(held.starts, a.n_requests, t);
+        const PlanRow row = held.rows[r];
+        place(a, t, r, row.start + (t - held.starts[r]), pages_of(a, row.start), row, all.top);
+    }
 }
 
-__global__ __launch_bounds__(kPlanThreads) void plan_requests_kernel(PlanArgs a) { (void)plan_requests(a); }
+__global__ __launch_bounds__(kPlanThreads) void plan_requests_kernel(PlanArgs a) { (void)plan_requests<kPlanThreads>(a, nullptr); }
 __global__ __launch_bounds__(256) void plan_back_kernel(PlanArgs a) { give_back(a, blockIdx.x, threadIdx.x, 256); }
-__global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a) {
-    const uint32_t t = blockIdx.x * 256 + threadIdx.x;
-    if (t < a.max_tokens) fill_token(a, t, *a.top);
+// starts: of requests 0, 1 << shift, ...
+__global__ __launch_bounds__(kPlanFill) void plan_fill_kernel(PlanArgs a, uint32_t shift) {
+    __shared__ uint32_t starts[kPlanStarts];
+    const uint32_t total = a.firsts[a.n_requests], top = *a.top;
+    uint32_t n = 0;
+    if (a.n_requests) n = ((a.n_requests - 1) >> shift) + 1;
+    for (uint32_t i = threadIdx.x; i < n; i += kPlanFill) starts[i] = a.firsts[i << shift];
+    __syncthreads();
+    const uint32_t t = blockIdx.x * kPlanFill + threadIdx.x;
+    if (t >= a.max_tokens) return;
+    if (t >= total) return pad(a, t);
+    uint32_t r = last_start(starts, n, t), first = starts[r];
+    if (shift) {
+        r <<= shift;
+        r += last_start(a.firsts + r, min(1u << shift, a.n_requests - r), t);
+        first = a.firsts[r];
+    }
+    const PlanRow row = a.work[r];
+    place(a, t, r, row.start + (t - first), pages_of(a, row.start), row, top);
 }
 
 }  // namespace
@@ -209,8 +237,12 @@ hipError_t launch_kv_plan(const PlanArgs& a_in, void* work, hipStream_t s) {
     PlanArgs a = a_in;
     a.top = static_cast<uint32_t*>(work);
     a.work = reinterpret_cast<PlanRow*>(static_cast<uint8_t*>(work) + 16);
-    if (a.n_requests <= kPlanThreads && a.max_tokens <= 4096) {
-        plan_small_kernel<<<1, kPlanThreads, 0, s>>>(a);
+    if (a.n_requests <= kPlanFew && a.max_tokens <= kPlanSmall / 4) {
+        plan_small_kernel<kPlanFew><<<1, kPlanFew, 0, s>>>(a);
+        return hipGetLastError();
+    }
+    if (a.n_requests <= kPlanThreads && a.max_tokens <= kPlanSmall) {
+        plan_small_kernel<kPlanThreads><<<1, kPlanThreads, 0, s>>>(a);
         return hipGetLastError();
     }
     plan_requests_kernel<<<1, kPlanThreads, 0, s>>>(a);
@@ -220,7 +252,9 @@ hipError_t launch_kv_plan(const PlanArgs& a_in, void* work, hipStream_t s) {
         e = hipGetLastError();
     }
     if (e == hipSuccess && a.max_tokens) {
-        plan_fill_kernel<<<(unsigned)(((uint64_t)a.max_tokens + 255) / 256), 256, 0, s>>>(a);
+        uint32_t shift = 0;
+        while ((((uint64_t)a.n_requests + (1u << shift) - 1) >> shift) > kPlanStarts) ++shift;
+        plan_fill_kernel<<<(unsigned)(((uint64_t)a.max_tokens + kPlanFill - 1) / kPlanFill), kPlanFill, 0, s>>>(a, shift);
         e = hipGetLastError();
     }
     return e;

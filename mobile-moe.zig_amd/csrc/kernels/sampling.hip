@@ -62,8 +62,7 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 
 // A weight is 2^(t / 256) with t = (x - m) 256 / (T ln 2), rounded to n + f:
 // 2^(n / 256) is a table's entry and an exponent, 2^(f / 256) a series of four
-// powers (the next is below 4e-17). Half the
-// instructions of a series of eleven powers.
+// powers (the next is below 4e-17). Half the instructions of a series of eleven.
 constexpr int kSmParts = 256;
 struct Parts {
     double of[kSmParts];
@@ -109,72 +108,6 @@ __device__ __forceinline__ double weight(double t, int shift, const double* part
 __device__ __forceinline__ uint64_t whole_weight(double t, int shift, const double* parts) {
     return __double_as_longlong(weight(t, shift, parts) + 0x1p52) & 0xFFFFFFFFFFFFFull;
 }
-
-// Over lanes 0 .. this one.
-__device__ __forceinline__ uint64_t wave_max_scan(uint64_t v) {
-    v = max(v, moved<0x111, 0xF>(v));
-    v = max(v, moved<0x112, 0xF>(v));
-    v = max(v, moved<0x114, 0xF>(v));
-    v = max(v, moved<0x118, 0xF>(v));
-    v = max(v, moved<0x142, 0xA>(v));
-    v = max(v, moved<0x143, 0xC>(v));
-    return v;
-}
-// Sums and maxima of two numbers at once over a workgroup, one barrier each: the
-// memory of one is written again two calls later, when the next one's barrier has
-// shown that all have read it.
-template <uint32_t WAVES>
-struct Together {
-    uint64_t (*memory)[2][WAVES];  // [2]
-    uint32_t turn = 0;
-    __device__ __forceinline__ void exchange(uint64_t& a, uint64_t& b) {  // lane 63's, to lanes 0 .. WAVES - 1
-        uint64_t(&red)[2][WAVES] = memory[turn & 1];
-        turn += 1;
-        const uint32_t lane = threadIdx.x & 63;
-        if (lane == 63) red[0][threadIdx.x >> 6] = a, red[1][threadIdx.x >> 6] = b;
-        __syncthreads();
-        a = lane < WAVES ? red[0][lane] : 0;
-        b = lane < WAVES ? red[1][lane] : 0;
-    }
-    // a: over threads 0 .. this one, and of all; b: of all.
-    __device__ __forceinline__ uint64_t scan(uint64_t a, uint64_t& all, uint64_t& b) {
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const uint64_t mine = wave_scan(a);
-        a = mine;
-        b = wave_scan(b);
-        exchange(a, b);
-        a = wave_scan(a);
-        b = lane_value(wave_scan(b), 63);
-        all = lane_value(a, 63);
-        return mine + (wave ? lane_value(a, wave - 1) : 0);
-    }
-    // Both over threads 0 .. this one.
-    __device__ __forceinline__ void scan2(uint64_t& a, uint64_t& b, uint64_t& all_a, uint64_t& all_b) {
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const uint64_t mine_a = wave_scan(a), mine_b = wave_scan(b);
-        a = mine_a;
-        b = mine_b;
-        exchange(a, b);
-        a = wave_scan(a);
-        b = wave_scan(b);
-        all_a = lane_value(a, 63);
-        all_b = lane_value(b, 63);
-        a = mine_a + (wave ? lane_value(a, wave - 1) : 0);
-        b = mine_b + (wave ? lane_value(b, wave - 1) : 0);
-    }
-    __device__ __forceinline__ uint64_t sum(uint64_t a) {
-        uint64_t all, none = 0;
-        scan(a, all, none);
-        return all;
-    }
-    __device__ __forceinline__ void largest(uint64_t& a, uint64_t& b) {
-        a = wave_max_scan(a);
-        b = wave_max_scan(b);
-        exchange(a, b);
-        a = lane_value(wave_max_scan(a), 63);
-        b = lane_value(wave_max_scan(b), 63);
-    }
-};
 
 // What a row asks for.
 enum SmMode : uint32_t { kSmAbsent, kSmNoRow, kSmBadSetting, kSmEmpty, kSmFirst, kSmAll, kSmCut };
