@@ -302,9 +302,9 @@ int mmhip_gemv_grouped_dev(mmhip_ctx* ctx, const mmhip_gemv_group* groups, uint3
  * The kernel, and with it the number format of the activations and the order of
  * the sums, is chosen by shape and batch: a call repeated gives the same bits,
  * but a quantised weight times the same vector in a batch of another size may
- * differ by the error of the coarser form, about 2e-5 of the result. The same
- * holds for mmhip_batch_mat_mul and for the tokens of an MoE layer call (about
- * 1e-4 there). f32 / f16 weights give the same bits at every batch. */
+ * differ by the error of the coarser form, about 2e-5 of the result (4-bit
+ * weights: 1e-6). The same holds for mmhip_batch_mat_mul and for the tokens of
+ * an MoE layer call (about 1e-4 there). f32 / f16 weights give the same bits at every batch. */
 int mmhip_qmm_dev(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat,
                   const float* x_dev, float* y_dev, uint64_t batch,
                   int out_layout);
@@ -619,8 +619,8 @@ int mmhip_kv_plan_dev(mmhip_ctx* ctx, const mmhip_kv_plan* args);
  * -infinity, settings out of range (T outside [0, f32's largest], top_p < 0,
  * min_p or uniform outside [0, 1] and [0, 1), a NaN) and a row number that the
  * logits do not have give MMHIP_NO_TOKEN, NaN and 0, and are reported. Fewer than
- * 2^22 rows; stride in floats, at least vocab. Outputs and workspace overlap neither the inputs nor
- * each other. */
+ * 2^22 rows; stride in floats, at least vocab. Outputs and workspace overlap
+ * neither the inputs nor each other. */
 #define MMHIP_SAMPLE_MAX_VOCAB (1u << 24)
 typedef struct {
     const float* logits_dev;       /* [n_rows or n_logits][stride] */

@@ -403,7 +403,7 @@ int qmm_quantised(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat, const flo
     hipError_t e = hipSuccess;
     if (fmt_4bit(g.fmt)) {
         // One launch reading the f32 activations (qbuf unused): up to four
-        // vectors as the decode kernel takes them, more on the bf16 matrix cores.
+        // vectors as the decode kernel takes them, more on the f16 matrix cores.
         const uint64_t y_slot = out_layout == 0 ? ld : 1, y_row = out_layout == 0 ? 1 : ld;
         TimedLaunch tl(timed ? ctx : nullptr, "qmm");
         if (batch <= 4 && out_layout == 0) {

@@ -446,7 +446,7 @@ int mmhip_embed_dev(mmhip_ctx* ctx, float* y, uint64_t y_stride, const void* tab
         if ((type == kIq2Xxs || type_4bit(type)) && cols % block_size(type))
             return invalid(what, "cols must hold whole blocks of the table's type");
         if (n_tokens > kMostRows) return invalid(what, "2^24 tokens or more");
-        // One workgroup of 256 threads per 1024 values, and fewer than 2^32 threads.
+        // A wave per 512 values, and fewer than 2^32 threads.
         if (n_tokens * (((uint64_t)cols + 1023) / 1024) > kMostRows) return invalid(what, "2^24 pieces of 1024 values or more");
         if (n_tokens == 0) return ctx ? MMHIP_OK : invalid(what, "null context");
         if (!y || !table || !tokens) return invalid(what, "null pointer");

@@ -178,6 +178,52 @@ def test_large_products(ctx, t, batch, rows, cols):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("batch,rows,cols", [(2, 50, 160), (20, 50, 160), (300, 4100, 160), (50, 30000, 96)])
+def test_vectors_at_any_float(ctx, t, batch, rows, cols):
+    """Inputs and outputs that stand four bytes behind what larger accesses like; nothing around the output is written."""
+    rng = np.random.default_rng(batch)
+    raw, w = weights(rng, t, rows, cols)
+    x = rng.standard_normal((batch, cols)).astype(np.float32)
+    wt = ctx.upload(raw, t, rows, cols)
+    with Buffers(ctx) as d:
+        dx, dy = d.put(np.concatenate([[np.float32(np.nan)], x.ravel()])), d.put(np.full(batch * rows + 9, 7.0, np.float32))
+        ctx.qmm_dev(wt, 0, At(dx, 4), At(dy, 4), batch)
+        ctx.synchronize()
+        y = dy.to_numpy(np.float32, batch * rows + 9)
+    wt.free()
+    assert y[0] == 7 and (y[batch * rows + 1:] == 7).all()
+    check(y[1:batch * rows + 1].reshape(batch, rows), w[0], x, few=False)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("layout", [0, 1])
+def test_results_behind_four_gigabytes(ctx, t, layout):
+    """The last ones of [70000 x 32] times 20000 vectors (5.6 GB)."""
+    rng = np.random.default_rng(5)
+    batch, rows, cols = 20000, 70000, 32
+    raw, w = weights(rng, t, rows, cols)
+    x = rng.standard_normal((batch, cols)).astype(np.float32)
+    wt = ctx.upload(raw, t, rows, cols)
+    with Buffers(ctx) as d:
+        y = mm.DeviceArray(ctx, batch * rows * 4)
+        d.held.append(y)
+        ctx.qmm_dev(wt, 0, d.put(x), y, batch, layout)
+        ctx.synchronize()
+        line = rows if layout == 0 else batch
+        take = d.new(4 * line)
+        # the last line, as a row of a table of lines
+        lines = batch if layout == 0 else rows
+        ctx.embed_dev(take, y, mm.F32, lines, line, d.put(np.array([lines - 1], np.uint32)), 1)
+        ctx.synchronize()
+        last = take.to_numpy(np.float32, line)
+    wt.free()
+    if layout == 0:
+        check(last[None], w[0], x[-1:], few=False)
+    else:
+        check(last[:, None], w[0][-1:], x, few=False)
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("batch,rows", [(6, 40), (70, 3000), (40, 30000)])
 @pytest.mark.parametrize("where", [100, 321, 600])
 def test_values_that_outgrow_the_first(ctx, t, batch, rows, where):

@@ -303,6 +303,29 @@ def test_plan_goes_on_from_itself(ctx, n, max_tokens):
             g.free()
 
 
+def test_large_plan_in_place(ctx):
+    """Lengths and the count of free pages in place, several launches and several sweeps over the requests."""
+    rng = np.random.default_rng(4)
+    n, max_tokens = 3000, 9000
+    lens, tables, free, n_pages, table_pages = random_plan(rng, n, 16, 60, 9000)
+    count = 9000
+    with Buffers(ctx) as d:
+        p = Planner(ctx, d, n=n, table_pages=table_pages, pt=16, n_pages=n_pages, max_tokens=max_tokens, aliased=True)
+        p.set(lens=lens, tables=tables, free=free, count=count, shared=np.zeros(n))
+        for _ in range(4):
+            release = rng.random(n) < 0.2
+            new = np.where(rng.random(n) < 0.5, 1, np.where(release, rng.integers(0, 30, n), 0))
+            new = np.minimum(new, table_pages * 16 - np.where(release, 0, lens))
+            new = np.where(np.cumsum(new) <= max_tokens, new, 0)
+            p.set(new=new, release=release)
+            ctx.kv_plan_dev(p.args)
+            ctx.synchronize()
+            want = ref.plan(lens, new, tables, free, count, page_tokens=16, n_pages=n_pages, max_tokens=max_tokens,
+                            release=release, shared=np.zeros(n))
+            p.check(want)
+            lens, tables, free, count = want["next_lens"], want["tables"], want["free"], want["next_free"][0]
+
+
 # ---- sampling -------------------------------------------------------------
 
 def run_sample(ctx, x, u, t=None, k=None, p=None, least=None, pad=0, off=0, rows=None, n_logits=None, times=1):
@@ -424,6 +447,43 @@ def test_nan_and_empty_rows(ctx, vocab):
         clean = np.where(np.isnan(x), -np.inf, x)
         check_sample([g[[0, 3]] for g in got], clean[[0, 3]], u[:2], **settings)
         assert (got[0][1:3] == NONE).all() and np.isnan(got[1][1:3]).all() and (got[2][1:3] == 0).all()
+
+
+@pytest.mark.parametrize("vocab", [70, 20001])
+@pytest.mark.parametrize("settings", [dict(), dict(t=0.0), dict(k=9), dict(t=1.3, p=0.9, least=0.001)], ids=str)
+def test_every_kind_of_nan(ctx, vocab, settings):
+    """Quiet and signalling ones of both signs, beside ordinary logits, infinities and zeros of both signs."""
+    rng = np.random.default_rng(vocab)
+    x = logits_like(rng, 6, vocab)
+    x[3] = -np.abs(x[3])
+    x[4] = np.abs(x[4]) + 1
+    x[5] = np.where(rng.random(vocab) < 0.5, np.float32(-0.0), np.float32(0.0))
+    bits = x.view(np.uint32)
+    for i, nan in enumerate((0x7FC00000, 0xFFC00000, 0x7F800001, 0xFF800001, 0xFFFFFFFF, 0xFF800000)):
+        bits[:, i * 9::64] = nan
+    x[2, 33] = np.inf
+    u = rng.random(6).astype(np.float32)
+    got = run_sample(ctx, x, u, **settings)
+    check_sample(got, np.where(np.isnan(x), np.float32(-np.inf), x), u, **settings)
+
+
+@pytest.mark.parametrize("settings", [dict(t=0.8), dict(k=40), dict(t=0.9, k=300, p=0.95), dict(p=0.9, least=0.01)], ids=str)
+def test_pieces_of_several_turns(ctx, settings):
+    rng = np.random.default_rng(8)
+    x, u = logits_like(rng, 600, 20000), rng.random(600).astype(np.float32)
+    check_sample(run_sample(ctx, x, u, **settings), x, u, **settings)
+
+
+@pytest.mark.parametrize("big,size", [(1e9, 1e-31), (3e38, 1e30), (-1e30, 1e-3), (1e30, 1.0), (65504.0, 0.01)])
+@pytest.mark.parametrize("settings", [dict(), dict(k=6), dict(p=0.7), dict(k=30, p=0.9, least=1e-3)], ids=str)
+def test_logits_far_from_zero(ctx, big, size, settings):
+    """All logits about `big`, a temperature of `size`: nothing of them is lost in their differences from the largest."""
+    rng = np.random.default_rng(11)
+    x = np.full((3, 9000), np.float32(big))
+    for _ in range(5):
+        x = np.where(rng.random(x.shape) < 0.4, np.nextafter(x, np.float32(-np.inf)), x)
+    u = rng.random(3).astype(np.float32)
+    check_sample(run_sample(ctx, x, u, t=size, **settings), x, u, t=size, **settings)
 
 
 def test_settings_out_of_range(ctx):
