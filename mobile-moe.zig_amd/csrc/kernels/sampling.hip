@@ -19,9 +19,9 @@
 // the latency of four launches, each two or three dependent trips to memory and a
 // few barriers; with many by vector instructions, about 30 for each logit and
 // weight. Measured with 154880 tokens, us (largest, histogram, list, draw): one
-// row with top-p 4.1, 6.1, 6.3, 7.5, together 25.5; 16 rows with top-k 5.7, 6.2, 7.5,
-// 6.3, together 24.2; 64 rows with settings of their own 10.4, 14.7, 17.2, 11.6, together
-// 52.4 (their logits are 39.7 MB, 8.3 us of copying). One workgroup per row for all
+// row with top-p 4.1, 6.1, 6.4, 7.4, together 25.6; 16 rows with top-k 5.7, 6.3, 7.8,
+// 6.2, together 24.5; 64 rows with settings of their own 10.3, 14.7, 15.3, 12.1, together
+// 50.6 (their logits are 39.7 MB, 8.3 us of copying). One workgroup per row for all
 // of it took 586, 542 and 1036.
 #include <algorithm>
 #include <type_traits>
@@ -203,10 +203,12 @@ __device__ __forceinline__ float seen(float x, const RowSettings& s) {
 // t of a logit.
 __device__ __forceinline__ double scaled(float x, const RowSettings& s) { return ((double)x - s.m) * s.per_t; }
 // The bin of a logit above -infinity: never smaller for a smaller logit.
-__device__ __forceinline__ uint32_t bin_of(float x, const RowSettings& s) {
-    const float y = __builtin_amdgcn_fmed3f(fmaf(-x, s.bin_c, s.bin_m), 1.0f, 255.9f);
-    return (__float_as_uint(y) - 0x3F800000u) >> 16;
+__device__ __forceinline__ uint32_t bin_bits(float x, const RowSettings& s) {
+    return __float_as_uint(__builtin_amdgcn_fmed3f(fmaf(-x, s.bin_c, s.bin_m), 1.0f, 255.9f));
 }
+__device__ __forceinline__ uint32_t bin_of(float x, const RowSettings& s) { return (bin_bits(x, s) - 0x3F800000u) >> 16; }
+// The least bits of a bin; more than any where there is none.
+__device__ __forceinline__ uint32_t bin_start(uint32_t bin) { return bin < kSmBins ? 0x3F800000u + (bin << 16) : 0x80000000u; }
 __device__ __forceinline__ uint64_t mass_target(float p, uint64_t sum) {
     return max((uint64_t)ceil((double)p * (double)sum), (uint64_t)1);
 }
@@ -370,11 +372,13 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
 
 // The bins that the cuts are in: their tokens go into the row's list, and what
 // each chunk has in the bins before all of them is kept for certain.
-__global__ __launch_bounds__(kSmPiece, 5) void sample_list_kernel(SampleArgs a, SmPlan p) {
+__global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmPlan p) {
     constexpr uint32_t kWaves = kSmPiece / 64, kPer = kSmBins / kSmPiece;
     __shared__ uint64_t memory[2][2][kWaves];
     __shared__ uint64_t most;
     __shared__ uint32_t listed, listed_at;
+    __shared__ float queue[kWaves][kSmChunk];
+    __shared__ uint16_t place[kWaves][kSmChunk];
     __shared__ double parts[kSmParts];
     __shared__ SmRow row;
     const uint32_t out = blockIdx.x / p.pieces, piece = blockIdx.x - out * p.pieces;
@@ -447,10 +451,13 @@ __global__ __launch_bounds__(kSmPiece, 5) void sample_list_kernel(SampleArgs a, 
         to->p_mass = r.p_mass;
         to->mass = all_mass;
     }
-    const uint32_t sure = min(r.k_bin, r.p_lo);
+    // Bits of the bins before all cuts, from the cuts' bins on and how many.
+    const uint32_t sure = bin_start(min(r.k_bin, r.p_lo)), k_from = bin_start(r.k_bin), k_bits = r.k_bin < kSmBins ? 0x10000u : 0u;
+    const uint32_t p_from = bin_start(r.p_lo), p_bits = r.p_lo < kSmBins ? (r.p_hi - r.p_lo + 1) << 16 : 0u;
     // Every wave takes as many turns: they ask for their tokens' places together.
     for (uint32_t c = c0 + wave; c < c0 + p.per; c += kWaves) {
-        if (c != c0 + wave && c < c1) load_chunk(x, a.vocab, c, v);
+        float next[kSmEach];
+        if (c + kWaves < c1) load_chunk(x, a.vocab, c + kWaves, next);
         if (c >= c1) {
 #pragma unroll
             for (uint32_t i = 0; i < kSmEach; ++i) v[i] = __builtin_nanf("");
@@ -460,27 +467,34 @@ __global__ __launch_bounds__(kSmPiece, 5) void sample_list_kernel(SampleArgs a, 
             for (uint32_t i = 0; i < kSmEach; ++i) v[i] = seen(v[i], s);
         }
         uint64_t mine = 0;
-        uint32_t kept = 0, to_list = 0;
-        uint32_t is_sure = 0;
+        uint32_t kept = 0, n_sure = 0, n_list = 0;
+        // Both go to the wave's queue first, what is kept for certain from its front
+        // and what is listed from its end: few lanes have some.
+        const auto before = [](uint64_t which) {
+            return __builtin_amdgcn_mbcnt_hi((uint32_t)(which >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)which, 0));
+        };
 #pragma unroll
         for (uint32_t i = 0; i < kSmEach; ++i) {
-            const uint32_t b = bin_of(v[i], s);
-            const bool any = v[i] > -INFINITY;
-            is_sure |= (uint32_t)(any && b < sure) << i;
-            to_list |= (uint32_t)(any && (b == r.k_bin || (b >= r.p_lo && b <= r.p_hi))) << i;
+            const uint32_t bits = bin_bits(v[i], s);
+            const bool there = v[i] > -INFINITY, is_sure = there && bits < sure;
+            const bool in_list = there && (bits - k_from < k_bits || bits - p_from < p_bits);
+            const uint64_t sures = __ballot(is_sure), lists = __ballot(in_list);
+            if (sures) {
+                if (is_sure) queue[wave][n_sure + before(sures)] = v[i];
+                n_sure += (uint32_t)__popcll(sures);
+            }
+            if (lists) {
+                const uint32_t to = kSmChunk - 1 - (n_list + before(lists));
+                if (in_list) queue[wave][to] = v[i], place[wave][to] = (uint16_t)(i * 64 + lane);
+                n_list += (uint32_t)__popcll(lists);
+            }
         }
-        if (__ballot(is_sure != 0)) {
-#pragma unroll
-            for (uint32_t i0 = 0; i0 < kSmEach; i0 += kSmBeside) {
-                if (__ballot((is_sure >> i0 & ((1u << kSmBeside) - 1)) != 0) == 0) continue;
-#pragma unroll
-                for (uint32_t i = i0; i < i0 + kSmBeside; ++i) {
-                    const double t = scaled(v[i], s);
-                    const uint64_t w = whole_weight(t, s.shift, parts);
-                    const bool keep = (is_sure >> i & 1u) && t >= s.least;
-                    mine += keep ? w : 0;
-                    kept += keep;
-                }
+        __builtin_amdgcn_wave_barrier();
+        for (uint32_t i = lane; i < n_sure; i += 64) {
+            const double t = scaled(queue[wave][i], s);
+            if (t >= s.least) {
+                mine += whole_weight(t, s.shift, parts);
+                kept += 1;
             }
         }
         mine = wave_scan(mine);
@@ -489,27 +503,24 @@ __global__ __launch_bounds__(kSmPiece, 5) void sample_list_kernel(SampleArgs a, 
             p.chunk_mass[(uint64_t)out * p.chunks + c] = mine;
             p.chunk_count[(uint64_t)out * p.chunks + c] = kept;
         }
-        const uint32_t here = (uint32_t)__popc(to_list), to = (uint32_t)wave_scan(here);
         uint32_t at = 0;
-        if (lane == 63 && to) at = atomicAdd(&listed, to);
+        if (lane == 0 && n_list) at = atomicAdd(&listed, n_list);
         __syncthreads();
         if (tid == 0 && listed) listed_at = atomicAdd(&p.rows[out].listed, listed);
         __syncthreads();
-        at = listed_at + (uint32_t)__builtin_amdgcn_readlane(at, 63) + to - here;
+        at = listed_at + (uint32_t)__builtin_amdgcn_readfirstlane(at);
+        for (uint32_t i = lane; i < n_list; i += 64) {
+            if (at + i >= p.list) break;
+            const uint32_t from = kSmChunk - 1 - i, id = c * kSmChunk + place[wave][from];
+            p.keys[(uint64_t)out * p.list + at + i] = order_key(s.far ? x[id] : queue[wave][from], id);
+        }
         if (c + kWaves < c0 + p.per) {
             __syncthreads();
             if (tid == 0) listed = 0;
             __syncthreads();
         }
 #pragma unroll
-        for (uint32_t i = 0; i < kSmEach; ++i) {
-            if (!(to_list >> i & 1u)) continue;
-            if (at < p.list) {
-                const uint32_t id = c * kSmChunk + i * 64 + lane;
-                p.keys[(uint64_t)out * p.list + at] = order_key(s.far ? x[id] : v[i], id);
-            }
-            ++at;
-        }
+        for (uint32_t i = 0; i < kSmEach; ++i) v[i] = next[i];
     }
 }
 
