@@ -329,6 +329,7 @@ struct Shape {
 template <int FMT>
 const void* fn_of(const Shape& t) {
     if (t.mt == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 4, 2, 8, 1>);
+    if (t.mt == 2 && t.ks == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 1, 8, 2>);
     if (t.mt == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 2, 8, 1>);
     if (t.ks == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 4, 4>);
     if (t.ks == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 2>);
@@ -337,34 +338,37 @@ const void* fn_of(const Shape& t) {
 
 // By the number of 16 x 16 tiles of the result. Few: sixteen waves a workgroup in
 // four groups of columns, up to a workgroup per CU; then larger tiles and fewer
-// groups; many: as many vectors to a weight as there are. Measured, us, with
-// {1,1,4,4} / {1,2,4,2} / {1,2,4,1} / {2,2,8,1} / {4,2,8,1}: [2048 x 2560] times 16
-// (128 tiles) 9.8 / 14.4 / 19.9 / 29.0 / 38, times 128 (1024) 10.7 / 15.2 / 21.6 /
-// 30.2 / 39, times 256 (2048) 19.0 / 15.4 / 21.7 / 30.3 / 39; [10240 x 2048] times 256
-// (10240) 74.7 / 42.9 / 41.1 / 39.7 / 33.9; [154880 x 2048] times 16 (9680) 89 / 55 /
-// 51 / 66 / 125, times 32 (19360) 154 / 92 / 86 / 74 / 127.
+// groups. Measured, us, with {1,1,4,4} / {1,2,4,2} / {2,1,8,2} / {2,2,8,1} / {4,2,8,1}:
+// [2048 x 2560] times 16 (128 tiles) 10.0 / 14.6 / 18.7 / 29.0 / 48, times 128 (1024)
+// 10.6 / 15.2 / 19.0 / 30.3 / 50, times 256 (2048) 19.0 / 15.6 / 19.2 / 30.3 / 51; [3840 x
+// 768] times 256 (3840) 21.7 / 10.2 / 9.3 / 12.2 / 19.0; [10240 x 2048] times 64 (2560)
+// 23.9 / 18.8 / 16.4 / 25.2 / 41, times 256 (10240) 75 / 42.4 / 45.6 / 39.8 / 33.9.
 //
-// The largest tile takes as many weight tiles as cost least: rounds of one
-// workgroup per CU, times the tiles of a SIMD's two waves ([10240 x 2048] times 256
-// with 10 tiles, one round of 256 workgroups, 33.9 us, with 16 tiles 42.4, with 8
-// 55.0).
+// Many: the two largest tiles by what they cost, rounds of one workgroup per CU
+// times a round's time, in hundredths of a microsecond a unit (fitted to the above
+// and: times 128 25.6 / 28.8, times 512 61.6 / 66.4; [3840 x 768] times 512 13.0 /
+// 14.7, {2,2,8,1} before {4,2,8,1}). The largest takes as many weight tiles as cost
+// least: a SIMD's two waves have a quarter of them. Up to 32 vectors leave it no
+// choice, and up to 16 the smallest tile is ahead: [154880 x 2048] times 16 {1,2,4,1}
+// 51, {1,2,4,2} 55, {2,2,8,1} 66; times 32 86 / 92 / 74.
 Shape shape_of(uint32_t tiles, uint32_t batch, uint32_t cus) {
     const uint64_t results = (uint64_t)tiles * ((batch + 15) / 16);
     if (results <= 4ull * cus) return Shape{1, 1, 4, 4, 4};
-    if (results <= 16ull * cus) return Shape{1, 2, 4, 2, 8};
+    if (results <= 16ull * cus) return results > 8ull * cus && batch > 16 ? Shape{2, 1, 8, 2, 8} : Shape{1, 2, 4, 2, 8};
     if (batch <= 16) return Shape{1, 2, 4, 1, 8};
-    if (batch <= 32) return Shape{2, 2, 8, 1, 16};
-    uint32_t best = 16;
-    uint64_t least = ~0ull;
-    for (uint32_t t = 16; t >= 8; --t) {
-        const uint64_t groups = (uint64_t)((tiles + t - 1) / t) * ((batch + 63) / 64);
-        const uint64_t cost = (groups + cus - 1) / cus * ((t + 3) / 4);
+    const auto rounds = [&](uint32_t t, uint32_t vecs) {
+        return ((uint64_t)((tiles + t - 1) / t) * ((batch + vecs - 1) / vecs) + cus - 1) / cus;
+    };
+    Shape best{2, 2, 8, 1, 16};
+    uint64_t least = 30 + 110 * rounds(16, 32);
+    for (uint32_t t = 16; t >= 8 && batch > 32; --t) {
+        const uint64_t cost = rounds(t, 64) * (70 + 42 * ((t + 3) / 4));
         if (cost < least) {
             least = cost;
-            best = t;
+            best = Shape{4, 2, 8, 1, t};
         }
     }
-    return Shape{4, 2, 8, 1, best};
+    return best;
 }
 
 }  // namespace

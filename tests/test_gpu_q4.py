@@ -162,7 +162,8 @@ def test_several_vectors(ctx, t, layout, batch, rows, cols):
 
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("batch,rows,cols", [(256, 1000, 768), (300, 4100, 256), (64, 16400, 128), (4, 40000, 64), (1000, 130, 8224),
-                                             (16, 70001, 96), (29, 40000, 160), (37, 30000, 288), (250, 10250, 544), (513, 5000, 96)])
+                                             (16, 70001, 96), (29, 40000, 160), (37, 30000, 288), (250, 10250, 544), (513, 5000, 96), (40, 16000, 544), (100, 6000, 96),
+                                             (77, 7001, 2176)])
 def test_large_products(ctx, t, batch, rows, cols):
     rng = np.random.default_rng(batch)
     raw, w = weights(rng, t, rows, cols, 2)
@@ -224,7 +225,7 @@ def test_results_behind_four_gigabytes(ctx, t, layout):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("batch,rows", [(6, 40), (70, 3000), (40, 30000)])
+@pytest.mark.parametrize("batch,rows", [(6, 40), (70, 3000), (70, 9000), (40, 30000)])
 @pytest.mark.parametrize("where", [100, 321, 600])
 def test_values_that_outgrow_the_first(ctx, t, batch, rows, where):
     """Values up to 1e6 and 1e30 times as large as a vector's first 64, which set its power of two; first ones of 0."""
