@@ -1,4 +1,5 @@
-// 4-bit weights (q4_ops.hpp) times one to four vectors on gfx950: decode.
+// 4-bit weights (q4_ops.hpp) times one to four vectors, or a few fours, on gfx950:
+// decode.
 //
 // y[t][r] = sum_b d[r][b] sum_{i < 32} v[r][32 b + i] x[t][32 b + i]. A vector's
 // block of 32 becomes integers of 31 bits with the block's own power of two

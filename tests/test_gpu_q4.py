@@ -1,7 +1,7 @@
 """4-bit weights with group scales (Q4_0, IQ4_NL) through the library's
 products, against 64-bit ones of the exact weights.
 
-Tolerances, u = 2^-24, S = sum |w x| of a result: one to four vectors enter as
+Tolerances, u = 2^-24, S = sum |w x| of a result: few vectors (one to four here) enter as
 integers of 31 bits (2^-31 of a block's largest), a block's sum is rounded once,
 and cols / 32 blocks and a few partial sums are added: (cols / 32 + 12) u S. More
 vectors enter the matrix cores as two f16 numbers that leave 2^-23 of a value at
