@@ -10,7 +10,7 @@
 // first) and one multiply-add per output with the block's scale.
 //
 // Bound: vector instructions (per value of x two conversions, per eight weights
-// 11 or 21 operations, per output and block one multiply-add) beside the matrix
+// 9 or 21 operations, per output and block one multiply-add) beside the matrix
 // cores. A workgroup's waves share the x tile in LDS: each converts its part of
 // the next 64 columns while the matrix cores work on the last ones, and a wave
 // unpacks weights of its own rows straight from their records. Waves may also
@@ -47,7 +47,7 @@ struct GemmQ4Args {
 };
 
 // Eight weights as f16, in the order of columns 0 2, 4 6, 1 3, 5 7: 0x6400 | u is
-// 1024 + u.
+// 1024 + u, 0x5400 | u << 4 is 64 + u.
 __device__ __forceinline__ uint32_t f16_less(uint32_t h, float by) {
     const f16x2 b = {(_Float16)by, (_Float16)by};
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, h) - b);
@@ -58,7 +58,11 @@ __device__ __forceinline__ f16x8 q4_bop_f16(uint32_t d) {
     if constexpr (FMT == kFmtQ4) {
         // (the stored codes have their top bit flipped)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) h[k] = f16_less(((d >> (4 * k)) & 0x000F000Fu) ^ 0x64086408u, 1032.0f);
+        for (int k = 0; k < 4; k += 2) {
+            const uint32_t e = d >> (4 * k);
+            h[k] = f16_less((e & 0x000F000Fu) ^ 0x64086408u, 1032.0f);
+            h[k + 1] = f16_less((e & 0x00F000F0u) ^ 0x54805480u, 72.0f);
+        }
     } else {
         uint32_t w[2];
         q4_words<FMT>(d, w[0], w[1]);
