@@ -62,8 +62,7 @@ __device__ __forceinline__ uint32_t last_start(const uint32_t* starts, uint32_t 
 
 // Gives request r's pages back: free[row.back_at ..).
 __device__ __forceinline__ void give_page(const PlanArgs& a, uint32_t r, const PlanRow& row, uint32_t i) {
-    const uint64_t at = (uint64_t)row.back_at + i;
-    if (at < a.n_pages) a.free[at] = a.tables[(uint64_t)r * a.table_stride + row.back_from + i];
+    a.free[row.back_at + i] = a.tables[(uint64_t)r * a.table_stride + row.back_from + i];
 }
 __device__ __forceinline__ void give_back(const PlanArgs& a, uint32_t r, uint32_t i0, uint32_t step) {
     const PlanRow row = a.work[r];
@@ -124,11 +123,13 @@ __device__ __forceinline__ PlanTotals plan_requests(const PlanArgs& a, PlanHeld<
             report(a.status, kBadPlanTokens);
         }
         fits = add;
-        const uint64_t before = (uint64_t)min(count, a.n_pages) + back_all + back - row.back;
+        // No more than the stack holds (a length may name more pages than the pool has).
+        const uint64_t backs = back_all + back - row.back, before = (uint64_t)min(count, a.n_pages) + backs;
         row.back_at = (uint32_t)min(before, (uint64_t)a.n_pages);
+        row.back = min(row.back, a.n_pages - row.back_at);
         row.pages = fits;  // until the second sweep
         if (!once && r < a.n_requests) a.work[r] = row;
-        if (once) held->backs[threadIdx.x] = (uint32_t)(back - row.back);
+        if (once) held->backs[threadIdx.x] = (uint32_t)min(backs, (uint64_t)0xFFFFFFFFu);
         back_all += all_back;
         asked_all += all_asked;
     }
@@ -182,7 +183,7 @@ __device__ __forceinline__ PlanTotals plan_requests(const PlanArgs& a, PlanHeld<
         *a.next_free_count = top - (uint32_t)taken;
         if (!once) *a.top = top;
     }
-    return {top, (uint32_t)given_all, (uint32_t)min(back_all, (uint64_t)0xFFFFFFFFu)};
+    return {top, (uint32_t)given_all, top - count};
 }
 
 template <uint32_t THREADS>

@@ -303,6 +303,36 @@ def test_plan_goes_on_from_itself(ctx, n, max_tokens):
             g.free()
 
 
+@pytest.mark.parametrize("n,max_tokens", [(17, 40), (17, 5000)])
+def test_more_pages_given_back_than_there_are(ctx, n, max_tokens):
+    """Lengths of 2^32 - 16 in tables of 2^28 - 1 entries, 2^32 of them together: those that the stack holds come back."""
+    pt, tp, n_pages, count = 16, (1 << 28) - 1, 20, 4
+    with Buffers(ctx) as d:
+        tables = mm.DeviceArray(ctx, n * tp * 4)  # only what comes back is read
+        d.held.append(tables)
+        put_into(ctx, tables, np.arange(100, 140, dtype=np.int32))
+        put_into(ctx, At(tables, (n - 1) * tp * 4), np.arange(200, 210, dtype=np.int32))
+        ints = lambda k: d.put(np.zeros(k, np.uint32))  # noqa: E731
+        free, next_free = d.put(np.arange(n_pages, dtype=np.int32)), ints(1)
+        out = {k: ints(max_tokens) for k in ("positions", "slots", "table_of", "seen")}
+        new = np.zeros(n, np.uint32)
+        new[n - 1] = 18  # in the row that begins anew: two pages, the two last ones that came back
+        release = np.ones(n, np.uint32)
+        args = ctx.kv_plan_args(
+            n_requests=n, lens=d.put(np.full(n, pt * tp, np.uint32)), new=d.put(new), release=d.put(release), shared=None,
+            next_lens=ints(n), tables=tables, table_pages=tp, table_stride=tp, page_tokens=pt, n_pages=n_pages, free=free,
+            free_count=d.put(np.array([count], np.uint32)), next_free_count=next_free, max_tokens=max_tokens, firsts=ints(n + 1),
+            granted=ints(n), last=None, workspace=d.new(ctx.kv_plan_workspace(n)), **out)
+        ctx.kv_plan_dev(args)
+        with pytest.raises(mm.MmhipError):  # the pages' numbers are wrong too
+            ctx.synchronize()
+        ctx.synchronize()
+        assert free.to_numpy(np.int32, n_pages).tolist() == [0, 1, 2, 3] + list(range(100, 116))
+        assert next_free.to_numpy(np.uint32, 1)[0] == n_pages - 2
+        slots = out["slots"].to_numpy(np.int32, max_tokens)
+        assert (slots == -1).all()  # pages 115 and 114 are not of the pool
+
+
 def test_large_plan_in_place(ctx):
     """Lengths and the count of free pages in place, several launches and several sweeps over the requests."""
     rng = np.random.default_rng(4)
