@@ -538,34 +538,39 @@ struct Bins {
     uint32_t few;
 };
 template <bool MASS>
-__device__ uint64_t find_cut(const RowSettings& s, const double* parts, uint32_t vocab, uint64_t floor, uint64_t target, Bins& b) {
+__device__ uint64_t find_cut(const RowSettings& s, const double* parts, uint32_t vocab, uint64_t floor, uint64_t target, Bins& b,
+                             Together<kSmWaves>& all) {
+    const uint32_t tid = threadIdx.x;
     uint64_t prefix = 0, before = 0;
     for (int low = 54, bits = 10;; bits = low < 10 ? 4 : 10, low -= bits) {
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < kSmBins; i += kSmThreads) b.mass[i] = 0, b.count[i] = 0;
+        b.mass[tid] = 0;
+        b.count[tid] = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < vocab; i += kSmThreads) {
-            const float v = s.x[i];
+        const auto add = [&](float v, uint32_t i) {
             const uint64_t k = order_key(v, i);
-            if (k < floor || (low < 54 && (k >> (low + bits)) != prefix)) continue;
-            const uint32_t at = (uint32_t)(k >> low) & ((1u << bits) - 1);
+            if (k < floor || (low < 54 && (k >> (low + bits)) != prefix)) return;
+            const uint32_t at = (1u << bits) - 1 - ((uint32_t)(k >> low) & ((1u << bits) - 1));  // larger ones first
             atomicAdd(&b.count[at], 1u);
             if (MASS) atomicAdd(&b.mass[at], (unsigned long long)whole_weight(scaled(seen(v, s), s), s.shift, parts));
+        };
+        uint32_t i = tid;
+        for (; i + 7 * kSmThreads < vocab; i += 8 * kSmThreads) {
+            float v[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) v[e] = s.x[i + e * kSmThreads];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) add(v[e], i + e * kSmThreads);
         }
+        for (; i < vocab; i += kSmThreads) add(s.x[i], i);
         __syncthreads();
-        if (threadIdx.x == 0) {
-            // The last digit there is where all of them fall short.
-            uint32_t last = 0;
-            uint64_t sum = before, above = before;
-            for (uint32_t at = 1u << bits; at-- > 0;) {
-                if (b.count[at] == 0) continue;
-                last = at;
-                above = sum;
-                sum += MASS ? b.mass[at] : b.count[at];
-                if (sum >= target) break;
-            }
-            b.found = last;
-            b.above = above;
+        const uint64_t here = MASS ? b.mass[tid] : b.count[tid];
+        uint64_t sum, none = 0;
+        const uint64_t to = before + all.scan(here, sum, none);
+        target = min(target, before + sum);  // where all of them fall short the last one is it
+        if (to - here < target && target <= to) {
+            b.found = (1u << bits) - 1 - tid;
+            b.above = to - here;
         }
         __syncthreads();
         prefix = prefix << bits | b.found;
@@ -751,7 +756,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
             }
         } else {
             // More than the list holds: over all logits again.
-            if (s.k) cut = max(cut, find_cut<false>(s, parts, a.vocab, cut, s.k, bins));
+            if (s.k) cut = max(cut, find_cut<false>(s, parts, a.vocab, cut, s.k, bins, all));
             if (s.by_mass) {
                 uint64_t sum = 0;
                 for (uint32_t i = tid; i < a.vocab; i += kSmThreads) {
@@ -759,7 +764,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
                     if (order_key(v, i) >= cut) sum += whole_weight(scaled(seen(v, s), s), s.shift, parts);
                 }
                 sum = all.sum(sum);
-                cut = max(cut, find_cut<true>(s, parts, a.vocab, cut, mass_target(s.p, sum), bins));
+                cut = max(cut, find_cut<true>(s, parts, a.vocab, cut, mass_target(s.p, sum), bins, all));
             }
             // (as the launches over pieces leave them where the list suffices)
             for (uint32_t c = tid >> 6; c < p.chunks; c += kSmWaves) {
