@@ -14,14 +14,14 @@
 //
 // Four launches: the largest logit (pieces of rows); a histogram of tokens and
 // weights over bins of (m - x) / T; the tokens of the bins that hold the cuts, in a
-// list, and what every 1024 logits keep for certain; the cuts in the list, the 1024
-// logits and the token that u falls on (a workgroup per row). Bound: with few rows
+// list, and what each chunk of logits keeps for certain; the cuts in the list, the
+// chunk and the token that u falls on (a workgroup per row). Bound: with few rows
 // the latency of four launches, each two or three dependent trips to memory and a
 // few barriers; with many by vector instructions, about 30 for each logit and
 // weight. Measured with 154880 tokens, us (largest, histogram, list, draw): one
-// row with top-p 4.1, 6.1, 6.4, 7.4, together 25.6; 16 rows with top-k 5.7, 6.3, 7.8,
-// 6.2, together 24.5; 64 rows with settings of their own 10.3, 14.7, 15.3, 12.1, together
-// 50.6 (their logits are 39.7 MB, 8.3 us of copying). One workgroup per row for all
+// row with top-p 3.8, 5.5, 5.7, 7.5, together 23.7; 16 rows with top-k 6.1, 6.6, 7.8,
+// 5.7, together 24.8; 64 rows with settings of their own 10.4, 14.8, 15.1, 11.9, together
+// 50.8 (their logits are 39.7 MB, 8.3 us of copying). One workgroup per row for all
 // of it took 586, 542 and 1036.
 #include <algorithm>
 #include <type_traits>
@@ -34,17 +34,19 @@ namespace mmhip {
 
 namespace {
 
-// Threads of the launches over pieces, and of those over rows.
-constexpr uint32_t kSmPiece = 256, kSmThreads = 1024, kSmWaves = kSmThreads / 64;
-// Logits that a wave takes at a time, and a lane of it. (256: the histogram's sums in
-// memory meet four times as many workgroups, 16 rows took 37 us for 26.)
-constexpr uint32_t kSmChunk = 1024, kSmEach = kSmChunk / 64;
-constexpr uint32_t kSmBins = 1024;       // of the row's histogram
+constexpr uint32_t kSmThreads = 1024, kSmWaves = kSmThreads / 64;  // of the launch over rows
+// Logits of a piece's turn, and the waves that share them. Eight waves with half as
+// many each, up to a piece per workgroup of the limit below, are 2 us faster for few
+// rows (1 row 23.7 against 25.9 us, 8 rows 29.2 and 31.2, 16 rows 32.3 and 32.8) and 1
+// slower for many (64 rows 51.8 and 50.7). (More workgroups instead of wider ones: the
+// histogram's sums in memory meet as many more of them, 16 rows took 37 us for 26.)
+constexpr uint32_t kSmTurn = 4096, kSmWide = 8, kSmNarrow = 4;
+constexpr uint32_t kSmBins = 1024;  // of the row's histogram
 // Pieces of a call that are enough: with 64 rows 512, 1024 and 2048 took 57.7, 53.2
 // and 55.7 us.
 constexpr uint32_t kSmWorkgroups = 1024;
-constexpr uint32_t kSmBeside = 4;        // of a lane's logits, worked on beside each other
-constexpr uint32_t kSmPerThread = 8;     // tokens beside the cut that a thread of the last launch takes
+constexpr uint32_t kSmBeside = 4;  // of a lane's logits, worked on beside each other
+constexpr uint32_t kSmPerThread = 8;  // tokens beside the cut that a thread of the last launch takes
 constexpr uint32_t kSmList = kSmPerThread * kSmThreads;
 
 // A logit's place in the order: larger is earlier, equal ones by the lower id.
@@ -133,7 +135,8 @@ struct SmRow {
 };
 struct SmPlan {
     uint32_t chunks, pieces, list;
-    uint32_t per;              // chunks of a piece
+    uint32_t chunk, per;       // logits of a chunk, chunks of a piece
+    uint32_t waves;            // of a piece
     uint64_t* best;            // [rows][pieces]
     float* lowest;             // [rows][pieces]
     unsigned long long* mass;  // [rows][kSmBins]
@@ -214,13 +217,14 @@ __device__ __forceinline__ uint64_t mass_target(float p, uint64_t sum) {
 }
 
 // A wave's chunk: logit i * 64 + lane, NaN where there is none.
-__device__ __forceinline__ void load_chunk(const float* x, uint32_t vocab, uint32_t chunk, float (&v)[kSmEach]) {
-    const uint32_t first = chunk * kSmChunk, n = min(vocab - first, kSmChunk), lane = threadIdx.x & 63;
+template <uint32_t EACH>
+__device__ __forceinline__ void load_chunk(const float* x, uint32_t vocab, uint32_t chunk, float (&v)[EACH]) {
+    const uint32_t first = chunk * (EACH * 64), n = min(vocab - first, EACH * 64), lane = threadIdx.x & 63;
     const BufRsrc r = make_rsrc(x + first, n * 4);
 #pragma unroll
-    for (uint32_t i = 0; i < kSmEach; ++i) v[i] = __uint_as_float(buf_load_b32(r, lane * 4, i * 256));
+    for (uint32_t i = 0; i < EACH; ++i) v[i] = __uint_as_float(buf_load_b32(r, lane * 4, i * 256));
 #pragma unroll
-    for (uint32_t i = 0; i < kSmEach; ++i)
+    for (uint32_t i = 0; i < EACH; ++i)
         if (i * 64 + lane >= n) v[i] = __builtin_nanf("");
 }
 
@@ -232,12 +236,13 @@ __device__ __forceinline__ const float* row_logits(const SampleArgs& a, uint32_t
 }
 
 // The largest and lowest logits of a piece, and the row's memory cleared.
-__global__ __launch_bounds__(kSmPiece) void sample_best_kernel(SampleArgs a, SmPlan p) {
-    __shared__ uint64_t memory[2][2][kSmPiece / 64];
+template <uint32_t WAVES, uint32_t EACH>
+__global__ __launch_bounds__(WAVES * 64) void sample_best_kernel(SampleArgs a, SmPlan p) {
+    __shared__ uint64_t memory[2][2][WAVES];
     const uint32_t out = blockIdx.x / p.pieces, piece = blockIdx.x - out * p.pieces;
     const uint32_t c0 = piece * p.per, c1 = min(c0 + p.per, p.chunks);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (uint32_t i = piece * kSmPiece + threadIdx.x; i < kSmBins; i += p.pieces * kSmPiece) {
+    for (uint32_t i = piece * WAVES * 64 + threadIdx.x; i < kSmBins; i += p.pieces * WAVES * 64) {
         p.mass[(uint64_t)out * kSmBins + i] = 0;
         p.count[(uint64_t)out * kSmBins + i] = 0;
     }
@@ -245,15 +250,15 @@ __global__ __launch_bounds__(kSmPiece) void sample_best_kernel(SampleArgs a, SmP
     const float* x = row_logits(a, out);
     float top = -INFINITY;
     uint32_t id = 0, under = 0, over = 0xFFFFFFFFu;
-    float v[kSmEach];
+    float v[EACH];
     if (x && c0 + wave < c1) load_chunk(x, a.vocab, c0 + wave, v);
     if (piece == 0 && threadIdx.x == 0) p.asked[out] = row_asked(a, out);
     if (x)
-        for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
+        for (uint32_t c = c0 + wave; c < c1; c += WAVES) {
             if (c != c0 + wave) load_chunk(x, a.vocab, c, v);
             float here = -INFINITY;
 #pragma unroll
-            for (uint32_t i = 0; i < kSmEach; i += 2) {
+            for (uint32_t i = 0; i < EACH; i += 2) {
                 const float v0 = v[i] > -INFINITY ? v[i] : -INFINITY, v1 = v[i + 1] > -INFINITY ? v[i + 1] : -INFINITY;
                 here = __builtin_amdgcn_fmed3f(__builtin_amdgcn_fmed3f(here, v0, INFINITY), v1, INFINITY);
                 const uint32_t b0 = __float_as_uint(v0), b1 = __float_as_uint(v1);
@@ -265,9 +270,9 @@ __global__ __launch_bounds__(kSmPiece) void sample_best_kernel(SampleArgs a, SmP
             if (!(here > top)) continue;
             top = here;
 #pragma unroll
-            for (uint32_t i = kSmEach; i-- > 0;) {
+            for (uint32_t i = EACH; i-- > 0;) {
                 const uint64_t at = __ballot(v[i] == here);
-                if (at) id = c * kSmChunk + i * 64 + (uint32_t)__builtin_ctzll(at);
+                if (at) id = c * (EACH * 64) + i * 64 + (uint32_t)__builtin_ctzll(at);
             }
         }
     // Of finite numbers and +infinity the lowest: a negative one's bits, more for a
@@ -275,7 +280,7 @@ __global__ __launch_bounds__(kSmPiece) void sample_best_kernel(SampleArgs a, SmP
     // least bits are the lowest number's.
     float low = under >= 0x80800000u ? __uint_as_float(under - 0x00800000u) : over < 0x7F800001u ? __uint_as_float(over) : INFINITY;
     uint64_t best = order_key(top, id), lowest = order_bits(-low);
-    Together<kSmPiece / 64> all{memory};
+    Together<WAVES> all{memory};
     all.largest(best, lowest);
     if (threadIdx.x == 0) {
         p.best[blockIdx.x] = best;
@@ -285,8 +290,9 @@ __global__ __launch_bounds__(kSmPiece) void sample_best_kernel(SampleArgs a, SmP
 
 // How many tokens, and how much of the weights, each bin of the row holds. Rows
 // without a cut: what each chunk keeps. The row's settings for the launches behind.
-__global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmPlan p) {
-    __shared__ uint64_t memory[2][2][kSmPiece / 64];
+template <uint32_t WAVES, uint32_t EACH>
+__global__ __launch_bounds__(WAVES * 64) void sample_bins_kernel(SampleArgs a, SmPlan p) {
+    __shared__ uint64_t memory[2][2][WAVES];
     __shared__ double parts[kSmParts];
     __shared__ unsigned long long mass[kSmBins];
     __shared__ uint32_t count[kSmBins];
@@ -294,17 +300,17 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
     const uint32_t c0 = piece * p.per, c1 = min(c0 + p.per, p.chunks);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float* x = row_logits(a, out);
-    float v[kSmEach];
+    float v[EACH];
     if (x && c0 + wave < c1) load_chunk(x, a.vocab, c0 + wave, v);  // its latency beside the settings'
     const RowSettings& asked = p.asked[out];
     uint64_t best = 0, lowest = 0;
-    for (uint32_t i = threadIdx.x; i < p.pieces; i += kSmPiece) {
+    for (uint32_t i = threadIdx.x; i < p.pieces; i += WAVES * 64) {
         best = max(best, p.best[(uint64_t)out * p.pieces + i]);
         lowest = max(lowest, (uint64_t)order_bits(-p.lowest[(uint64_t)out * p.pieces + i]));
     }
     fill_parts(parts);
-    for (uint32_t i = threadIdx.x; i < kSmBins; i += kSmPiece) mass[i] = 0, count[i] = 0;
-    Together<kSmPiece / 64> all{memory};
+    for (uint32_t i = threadIdx.x; i < kSmBins; i += WAVES * 64) mass[i] = 0, count[i] = 0;
+    Together<WAVES> all{memory};
     all.largest(best, lowest);
     RowSettings s;
     row_settings(s, asked, best, -key_value(lowest << 32));
@@ -314,16 +320,16 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
         if (c != c0 + wave) load_chunk(x, a.vocab, c, v);
         if (s.far) {
 #pragma unroll
-            for (uint32_t i = 0; i < kSmEach; ++i) v[i] = seen(v[i], s);
+            for (uint32_t i = 0; i < EACH; ++i) v[i] = seen(v[i], s);
         }
     };
     if (s.mode == kSmAll) {
-        for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
+        for (uint32_t c = c0 + wave; c < c1; c += WAVES) {
             next(c);
             uint64_t sum = 0;
             uint32_t n = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < kSmEach; ++i) {
+            for (uint32_t i = 0; i < EACH; ++i) {
                 const double t = scaled(v[i], s);
                 const uint64_t w = whole_weight(t, s.shift, parts);
                 const bool keep = v[i] > -INFINITY && t >= s.least;
@@ -340,10 +346,10 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
         return;
     }
     const auto fill = [&](auto by_number, auto by_mass) {
-        for (uint32_t c = c0 + wave; c < c1; c += kSmPiece / 64) {
+        for (uint32_t c = c0 + wave; c < c1; c += WAVES) {
             next(c);
 #pragma unroll
-            for (uint32_t i0 = 0; i0 < kSmEach; i0 += kSmBeside) {
+            for (uint32_t i0 = 0; i0 < EACH; i0 += kSmBeside) {
                 uint32_t b[kSmBeside];
                 uint64_t w[kSmBeside];
 #pragma unroll
@@ -364,7 +370,7 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
     else if (!s.k) fill(std::false_type(), std::true_type());
     else fill(std::true_type(), std::true_type());
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kSmBins; i += kSmPiece) {
+    for (uint32_t i = threadIdx.x; i < kSmBins; i += WAVES * 64) {
         if (count[i]) atomicAdd(&p.count[(uint64_t)out * kSmBins + i], count[i]);
         if (mass[i]) atomicAdd(&p.mass[(uint64_t)out * kSmBins + i], mass[i]);
     }
@@ -372,13 +378,14 @@ __global__ __launch_bounds__(kSmPiece) void sample_bins_kernel(SampleArgs a, SmP
 
 // The bins that the cuts are in: their tokens go into the row's list, and what
 // each chunk has in the bins before all of them is kept for certain.
-__global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmPlan p) {
-    constexpr uint32_t kWaves = kSmPiece / 64, kPer = kSmBins / kSmPiece;
-    __shared__ uint64_t memory[2][2][kWaves];
+template <uint32_t WAVES, uint32_t EACH>
+__global__ __launch_bounds__(WAVES * 64) void sample_list_kernel(SampleArgs a, SmPlan p) {
+    constexpr uint32_t kPer = kSmBins / (WAVES * 64);
+    __shared__ uint64_t memory[2][2][WAVES];
     __shared__ uint64_t most;
     __shared__ uint32_t listed, listed_at;
-    __shared__ float queue[kWaves][kSmChunk];
-    __shared__ uint16_t place[kWaves][kSmChunk];
+    __shared__ float queue[WAVES][EACH * 64];
+    __shared__ uint16_t place[WAVES][EACH * 64];
     __shared__ double parts[kSmParts];
     __shared__ SmRow row;
     const uint32_t out = blockIdx.x / p.pieces, piece = blockIdx.x - out * p.pieces;
@@ -386,7 +393,7 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = threadIdx.x;
     const RowSettings s = p.settings[out];
     const float* x = row_logits(a, out);
-    float v[kSmEach];
+    float v[EACH];
     if (x && c0 + wave < c1) load_chunk(x, a.vocab, c0 + wave, v);
     uint64_t m[kPer], mass_to = 0, all_mass, num_to = 0, all_num;
     uint32_t n[kPer];
@@ -405,7 +412,7 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
 #pragma unroll
     for (uint32_t i = 0; i < kPer; ++i) mass_to += m[i], num_to += n[i];
     const uint64_t mass_here = mass_to, num_here = num_to;
-    Together<kWaves> all{memory};
+    Together<WAVES> all{memory};
     all.scan2(mass_to, num_to, all_mass, all_num);
     mass_to -= mass_here;
     num_to -= num_here;
@@ -455,16 +462,16 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
     const uint32_t sure = bin_start(min(r.k_bin, r.p_lo)), k_from = bin_start(r.k_bin), k_bits = r.k_bin < kSmBins ? 0x10000u : 0u;
     const uint32_t p_from = bin_start(r.p_lo), p_bits = r.p_lo < kSmBins ? (r.p_hi - r.p_lo + 1) << 16 : 0u;
     // Every wave takes as many turns: they ask for their tokens' places together.
-    for (uint32_t c = c0 + wave; c < c0 + p.per; c += kWaves) {
-        float next[kSmEach];
-        if (c + kWaves < c1) load_chunk(x, a.vocab, c + kWaves, next);
+    for (uint32_t c = c0 + wave; c < c0 + p.per; c += WAVES) {
+        float next[EACH];
+        if (c + WAVES < c1) load_chunk(x, a.vocab, c + WAVES, next);
         if (c >= c1) {
 #pragma unroll
-            for (uint32_t i = 0; i < kSmEach; ++i) v[i] = __builtin_nanf("");
+            for (uint32_t i = 0; i < EACH; ++i) v[i] = __builtin_nanf("");
         }
         if (s.far) {
 #pragma unroll
-            for (uint32_t i = 0; i < kSmEach; ++i) v[i] = seen(v[i], s);
+            for (uint32_t i = 0; i < EACH; ++i) v[i] = seen(v[i], s);
         }
         uint64_t mine = 0;
         uint32_t kept = 0, n_sure = 0, n_list = 0;
@@ -474,7 +481,7 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
             return __builtin_amdgcn_mbcnt_hi((uint32_t)(which >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)which, 0));
         };
 #pragma unroll
-        for (uint32_t i = 0; i < kSmEach; ++i) {
+        for (uint32_t i = 0; i < EACH; ++i) {
             const uint32_t bits = bin_bits(v[i], s);
             const bool there = v[i] > -INFINITY, is_sure = there && bits < sure;
             const bool in_list = there && (bits - k_from < k_bits || bits - p_from < p_bits);
@@ -484,7 +491,7 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
                 n_sure += (uint32_t)__popcll(sures);
             }
             if (lists) {
-                const uint32_t to = kSmChunk - 1 - (n_list + before(lists));
+                const uint32_t to = EACH * 64 - 1 - (n_list + before(lists));
                 if (in_list) queue[wave][to] = v[i], place[wave][to] = (uint16_t)(i * 64 + lane);
                 n_list += (uint32_t)__popcll(lists);
             }
@@ -511,16 +518,16 @@ __global__ __launch_bounds__(kSmPiece) void sample_list_kernel(SampleArgs a, SmP
         at = listed_at + (uint32_t)__builtin_amdgcn_readfirstlane(at);
         for (uint32_t i = lane; i < n_list; i += 64) {
             if (at + i >= p.list) break;
-            const uint32_t from = kSmChunk - 1 - i, id = c * kSmChunk + place[wave][from];
+            const uint32_t from = EACH * 64 - 1 - i, id = c * (EACH * 64) + place[wave][from];
             p.keys[(uint64_t)out * p.list + at + i] = order_key(s.far ? x[id] : queue[wave][from], id);
         }
-        if (c + kWaves < c0 + p.per) {
+        if (c + WAVES < c0 + p.per) {
             __syncthreads();
             if (tid == 0) listed = 0;
             __syncthreads();
         }
 #pragma unroll
-        for (uint32_t i = 0; i < kSmEach; ++i) v[i] = next[i];
+        for (uint32_t i = 0; i < EACH; ++i) v[i] = next[i];
     }
 }
 
@@ -770,7 +777,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
             for (uint32_t c = tid >> 6; c < p.chunks; c += kSmWaves) {
                 uint64_t sum = 0;
                 uint32_t n = 0;
-                for (uint32_t i = c * kSmChunk + (tid & 63); i < min((c + 1) * kSmChunk, a.vocab); i += 64) {
+                for (uint32_t i = c * p.chunk + (tid & 63); i < min((c + 1) * p.chunk, a.vocab); i += 64) {
                     const float v = s.x[i];
                     const double t = scaled(seen(v, s), s);
                     if (order_key(v, i) >= cut && t >= s.least) sum += whole_weight(t, s.shift, parts), ++n;
@@ -801,7 +808,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
                 continue;
             }
             ++kept;
-            atomicAdd(&bins.mass[(0xFFFFFFFFu - (uint32_t)key[i]) / kSmChunk / per], (unsigned long long)w[i]);
+            atomicAdd(&bins.mass[(0xFFFFFFFFu - (uint32_t)key[i]) / p.chunk / per], (unsigned long long)w[i]);
         }
         __syncthreads();
         mine += bins.mass[tid];
@@ -820,7 +827,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
         __syncthreads();
 #pragma unroll
         for (uint32_t i = 0; i < kSmPerThread; ++i) {
-            const uint32_t c = (0xFFFFFFFFu - (uint32_t)key[i]) / kSmChunk;
+            const uint32_t c = (0xFFFFFFFFu - (uint32_t)key[i]) / p.chunk;
             if ((in >> i & 1u) && c / per == group) atomicAdd(&bins.mass[c - chunk], (unsigned long long)w[i]);
         }
         __syncthreads();
@@ -829,10 +836,10 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
             ++chunk;
         }
     }
-    const uint32_t id = chunk * kSmChunk + tid;
+    const uint32_t id = chunk * p.chunk + tid;
     uint64_t here = 0;
     double t = 0.0;
-    if (id < a.vocab) {
+    if (tid < p.chunk && id < a.vocab) {
         const float v = s.x[id];
         t = scaled(seen(v, s), s);
         if (order_key(v, id) >= cut && t >= s.least) here = whole_weight(t, s.shift, parts);
@@ -848,10 +855,13 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
 
 SmPlan sm_plan(uint64_t n_rows, uint64_t vocab) {
     SmPlan p{};
-    p.chunks = (uint32_t)((vocab + kSmChunk - 1) / kSmChunk);
     // Whole chunks for each of a piece's waves, in as few turns as leave enough pieces.
-    const uint64_t fours = (p.chunks + 3) / 4, turns = std::max<uint64_t>(n_rows * fours / kSmWorkgroups, 1);
-    p.per = (uint32_t)std::min(turns, fours) * 4;
+    const uint64_t most = (vocab + kSmTurn - 1) / kSmTurn;
+    const uint64_t turns = std::max<uint64_t>(n_rows * most / kSmWorkgroups, 1);
+    p.waves = n_rows * most <= kSmWorkgroups ? kSmWide : kSmNarrow;
+    p.chunk = kSmTurn / p.waves;
+    p.chunks = (uint32_t)((vocab + p.chunk - 1) / p.chunk);
+    p.per = (uint32_t)std::min(turns, most) * p.waves;
     p.pieces = (p.chunks + p.per - 1) / p.per;
     p.list = (uint32_t)std::min<uint64_t>(kSmList, vocab);
     return p;
@@ -893,12 +903,17 @@ hipError_t launch_sample(const SampleArgs& a_in, uint64_t n_rows, hipStream_t s)
     SmPlan p = sm_plan(n_rows, a.vocab);
     sm_layout(p, n_rows, static_cast<uint8_t*>(a.work));
     const unsigned grid = (unsigned)(n_rows * p.pieces);
-    sample_best_kernel<<<grid, kSmPiece, 0, s>>>(a, p);
+    const bool wide = p.waves == kSmWide;
+    const unsigned threads = p.waves * 64;
+    (wide ? sample_best_kernel<kSmWide, kSmTurn / kSmWide / 64> : sample_best_kernel<kSmNarrow, kSmTurn / kSmNarrow / 64>)
+        <<<grid, threads, 0, s>>>(a, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    sample_bins_kernel<<<grid, kSmPiece, 0, s>>>(a, p);
+    (wide ? sample_bins_kernel<kSmWide, kSmTurn / kSmWide / 64> : sample_bins_kernel<kSmNarrow, kSmTurn / kSmNarrow / 64>)
+        <<<grid, threads, 0, s>>>(a, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    sample_list_kernel<<<grid, kSmPiece, 0, s>>>(a, p);
+    (wide ? sample_list_kernel<kSmWide, kSmTurn / kSmWide / 64> : sample_list_kernel<kSmNarrow, kSmTurn / kSmNarrow / 64>)
+        <<<grid, threads, 0, s>>>(a, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     sample_draw_kernel<<<(unsigned)n_rows, kSmThreads, 0, s>>>(a, p);
     return hipGetLastError();
