@@ -404,15 +404,15 @@ int qmm_quantised(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat, const flo
     if (fmt_4bit(g.fmt)) {
         // One launch reading the f32 activations (qbuf unused): as the decode kernel
         // takes them, four vectors to a reading of the weights, or on the f16 matrix
-        // cores. The first is ahead up to two workgroups per CU, whose chain is the
-        // shorter one: [768 x 2048] times 16 vectors 5.6 us against 8.7, times 40 7.3
-        // against 8.8, times 64 (beyond) 10.2 against 8.8; [2048 x 2560] times 16 7.8
-        // against 10.0; [3840 x 768] times 8 6.2 against 6.5, times 12 (beyond) 8.5
-        // against 6.5.
+        // cores. The first is ahead up to two workgroups per CU, one where rows are
+        // short: [768 x 2048] times 16 vectors 5.6 us against 7.5, times 40 7.3 against
+        // 7.6, times 64 (beyond) 10.2 against 7.5; [2048 x 2560] times 16 7.8 against 8.7;
+        // [3840 x 768] times 8 (beyond) 6.2 against 5.7.
         const uint64_t y_slot = out_layout == 0 ? ld : 1, y_row = out_layout == 0 ? 1 : ld;
         TimedLaunch tl(timed ? ctx : nullptr, "qmm");
         const uint64_t in_fours = (batch + 3) / 4;
-        if (out_layout == 0 && (batch <= 4 || g.tiles * in_fours <= 2ull * (uint64_t)(ctx->num_cu > 0 ? ctx->num_cu : 256))) {
+        const uint64_t cus = ctx->num_cu > 0 ? ctx->num_cu : 256;
+        if (out_layout == 0 && (batch <= 4 || g.tiles * in_fours <= (g.units >= 12 ? 2 : 1) * cus)) {
             e = launch_gemv_q4_vecs(gemv_args(w, mat, 1, x, w->cols, y, ld), (uint32_t)batch, g.fmt, ctx->num_cu, ctx->stream);
             return e == hipSuccess ? MMHIP_OK : hip_fail(e, "qmm: launch");
         }

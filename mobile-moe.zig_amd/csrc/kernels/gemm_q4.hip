@@ -335,14 +335,19 @@ const void* fn_of(const Shape& t) {
     if (t.mt == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 4, 2, 8, 1>);
     if (t.mt == 2 && t.ks == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 1, 8, 2>);
     if (t.mt == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 2, 8, 1>);
+    if (t.ks == 8) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 1, 8>);
+    if (t.ks == 4 && t.rs == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 2, 4>);
     if (t.ks == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 4, 4>);
     if (t.ks == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 2>);
     return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 1>);
 }
 
-// By the number of 16 x 16 tiles of the result. Few: sixteen waves a workgroup in
-// four groups of columns, up to a workgroup per CU; then larger tiles and fewer
-// groups. Measured, us, with {1,1,4,4} / {1,2,4,2} / {2,1,8,2} / {2,2,8,1} / {4,2,8,1}:
+// By the number of 16 x 16 tiles of the result. Few: up to a workgroup per CU with
+// four groups of columns and two or four tiles (or eight groups, where rows are long
+// and one tile makes enough workgroups). {1,1,1,8} / {1,1,2,4} / {1,1,4,4}, us:
+// [768 x 8192] times 64 (192 tiles) 16.1 / 19.7 / 23.3, [2048 x 2560] times 20 (256) 8.9 /
+// 8.7 / 10.0, times 64 (512) 13.1 / 8.9 / 10.1, times 100 (896) - / 12.6 / 10.4,
+// [3840 x 768] times 32 (480) 8.1 / 5.9 / 6.6. Then larger tiles and fewer groups. Measured, us, with {1,1,4,4} / {1,2,4,2} / {2,1,8,2} / {2,2,8,1} / {4,2,8,1}:
 // [2048 x 2560] times 16 (128 tiles) 10.0 / 14.6 / 18.7 / 29.0 / 48, times 128 (1024)
 // 10.6 / 15.2 / 19.0 / 30.3 / 50, times 256 (2048) 19.0 / 15.6 / 19.2 / 30.3 / 51; [3840 x
 // 768] times 256 (3840) 21.7 / 10.2 / 9.3 / 12.2 / 19.0; [10240 x 2048] times 64 (2560)
@@ -355,8 +360,10 @@ const void* fn_of(const Shape& t) {
 // least: a SIMD's two waves have a quarter of them. Up to 32 vectors leave it no
 // choice, and up to 16 the smallest tile is ahead: [154880 x 2048] times 16 {1,2,4,1}
 // 51, {1,2,4,2} 55, {2,2,8,1} 66; times 32 86 / 92 / 74.
-Shape shape_of(uint32_t tiles, uint32_t batch, uint32_t cus) {
+Shape shape_of(uint32_t tiles, uint32_t units, uint32_t batch, uint32_t cus) {
     const uint64_t results = (uint64_t)tiles * ((batch + 15) / 16);
+    if (results <= cus && units >= 32) return Shape{1, 1, 1, 8, 1};
+    if (results <= 2ull * cus) return Shape{1, 1, 2, 4, 2};
     if (results <= 4ull * cus) return Shape{1, 1, 4, 4, 4};
     if (results <= 16ull * cus) return results > 8ull * cus && batch > 16 ? Shape{2, 1, 8, 2, 8} : Shape{1, 2, 4, 2, 8};
     if (batch <= 16) return Shape{1, 2, 4, 1, 8};
@@ -404,7 +411,7 @@ hipError_t launch_gemm_q4(const uint4* recs, const uint16_t* dvals, const TileGe
     a.units = (uint32_t)g.units;
     a.rows = (uint32_t)g.rows;
     a.d_row = (uint32_t)g.d_row;
-    const Shape t = shape_of(a.tiles, batch, num_cu > 0 ? num_cu : 256);
+    const Shape t = shape_of(a.tiles, a.units, batch, num_cu > 0 ? num_cu : 256);
     a.wg_tiles = t.tiles;
     a.groups = (a.tiles + t.tiles - 1) / t.tiles;
     a.items = (batch + t.mt * 16 - 1) / (t.mt * 16);
