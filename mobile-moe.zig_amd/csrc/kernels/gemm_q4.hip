@@ -16,7 +16,7 @@
 // unpacks weights of its own rows straight from their records. Waves may also
 // split the columns (KS groups), their sums added at the end.
 //
-// Measured: [10240 x 2048] times 256 vectors 34.8 us (309 Tflop/s of products; the
+// Measured: [10240 x 2048] times 256 vectors 34.4 us (312 Tflop/s of products; the
 // two matrix instructions per product alone would take 17 us), [3840 x 768] times
 // 77 vectors 7.7 us; with bf16 parts (three instructions per product, four
 // conversions) 74 and 10.9 us.

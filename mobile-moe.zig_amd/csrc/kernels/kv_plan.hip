@@ -6,6 +6,12 @@
 // pages asked for, tokens granted. One workgroup takes them; small calls write
 // the step's tokens in the same launch, larger ones in a second one over the
 // whole chip. All counts are integers: nothing depends on timing.
+//
+// Bound: latency. One workgroup's chain is a trip to memory for the lengths, three
+// sums (a barrier each), a trip for the pages that come back and one for the
+// tables, about a microsecond each: 4 requests 3.8 us, 64 4.8 to 6.1, 500 with 2400
+// tokens 8.7. 512 requests with 64 prompts (110 thousand tokens) take three
+// dependent launches: 4.5, 2.4 and 4.3, together 11.1.
 #include "device_common.hpp"
 #include "kernels.hpp"
 #include "lanes.hpp"
@@ -14,8 +20,13 @@ namespace mmhip {
 
 namespace {
 
-constexpr uint32_t kPlanThreads = 1024, kPlanFew = 256;  // of the launch over requests; where they are few
-constexpr uint32_t kPlanSmall = 4096;                    // tokens that the same launch writes
+// Threads of the launch over requests; where there are few requests and tokens fewer
+// of them, whose barriers are shorter (4 requests 3.8 against 5.2 us, 64 with 93 tokens
+// 4.8 and 6.1, with 64 both 6.1; beyond, 250 requests 7.5 and 6.9).
+constexpr uint32_t kPlanThreads = 1024, kPlanFew = 256;
+// Tokens that the same launch writes: 500 requests with 2387 tokens 8.7 us, in three
+// launches 10.1 to 11.5; 900 with 6092 (beyond) 13.2 and 11.4.
+constexpr uint32_t kPlanSmall = 4096;
 constexpr uint32_t kPlanFill = 256;
 constexpr uint32_t kPlanStarts = 2048;                   // of the requests' first tokens, in LDS
 
@@ -238,7 +249,7 @@ hipError_t launch_kv_plan(const PlanArgs& a_in, void* work, hipStream_t s) {
     PlanArgs a = a_in;
     a.top = static_cast<uint32_t*>(work);
     a.work = reinterpret_cast<PlanRow*>(static_cast<uint8_t*>(work) + 16);
-    if (a.n_requests <= kPlanFew && a.max_tokens <= kPlanSmall / 4) {
+    if (a.n_requests <= kPlanFew / 2 && a.max_tokens <= kPlanFew) {
         plan_small_kernel<kPlanFew><<<1, kPlanFew, 0, s>>>(a);
         return hipGetLastError();
     }
