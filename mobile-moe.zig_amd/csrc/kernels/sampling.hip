@@ -19,9 +19,9 @@
 // the latency of four launches, each two or three dependent trips to memory and a
 // few barriers; with many by vector instructions, about 30 for each logit and
 // weight. Measured with 154880 tokens, us (largest, histogram, list, draw): one
-// row with top-p 3.8, 5.5, 5.7, 7.5, together 23.7; 16 rows with top-k 6.1, 6.6, 7.8,
-// 5.7, together 24.8; 64 rows with settings of their own 10.4, 14.8, 15.1, 11.9, together
-// 50.8 (their logits are 39.7 MB, 8.3 us of copying). One workgroup per row for all
+// row with top-p 3.7, 5.1, 6.0, 7.1, together 22.6; 16 rows with top-k 5.6, 6.0, 7.8,
+// 6.0, together 24.1; 64 rows with settings of their own 10.1, 14.2, 14.6, 11.6, together
+// 49.9 (their logits are 39.7 MB, 8.3 us of copying). One workgroup per row for all
 // of it took 586, 542 and 1036.
 #include <algorithm>
 #include <type_traits>
@@ -216,16 +216,28 @@ __device__ __forceinline__ uint64_t mass_target(float p, uint64_t sum) {
     return max((uint64_t)ceil((double)p * (double)sum), (uint64_t)1);
 }
 
-// A wave's chunk: logit i * 64 + lane, NaN where there is none.
+// A wave's chunk: a lane's i-th logit stands at place_of(i), NaN where there is none.
+__device__ __forceinline__ uint32_t place_of(uint32_t i) { return (i >> 2) * 256 + (threadIdx.x & 63) * 4 + (i & 3); }
 template <uint32_t EACH>
 __device__ __forceinline__ void load_chunk(const float* x, uint32_t vocab, uint32_t chunk, float (&v)[EACH]) {
     const uint32_t first = chunk * (EACH * 64), n = min(vocab - first, EACH * 64), lane = threadIdx.x & 63;
     const BufRsrc r = make_rsrc(x + first, n * 4);
+    if (n == EACH * 64) {
 #pragma unroll
-    for (uint32_t i = 0; i < EACH; ++i) v[i] = __uint_as_float(buf_load_b32(r, lane * 4, i * 256));
+        for (uint32_t j = 0; j < EACH / 4; ++j) {
+            const uint4 q = buf_load_b128(r, lane * 16, j * 1024);
+            v[4 * j] = __uint_as_float(q.x);
+            v[4 * j + 1] = __uint_as_float(q.y);
+            v[4 * j + 2] = __uint_as_float(q.z);
+            v[4 * j + 3] = __uint_as_float(q.w);
+        }
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < EACH; ++i)
-        if (i * 64 + lane >= n) v[i] = __builtin_nanf("");
+        for (uint32_t i = 0; i < EACH; ++i) v[i] = __uint_as_float(buf_load_b32(r, lane * 16, (i >> 2) * 1024 + (i & 3) * 4));
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i)
+            if (place_of(i) >= n) v[i] = __builtin_nanf("");
+    }
 }
 
 // The row of logits that the row's number names, or null.
@@ -270,9 +282,14 @@ __global__ __launch_bounds__(WAVES * 64) void sample_best_kernel(SampleArgs a, S
             if (!(here > top)) continue;
             top = here;
 #pragma unroll
-            for (uint32_t i = EACH; i-- > 0;) {
-                const uint64_t at = __ballot(v[i] == here);
-                if (at) id = c * (EACH * 64) + i * 64 + (uint32_t)__builtin_ctzll(at);
+            for (uint32_t j = EACH / 4; j-- > 0;) {
+                uint32_t lowest_place = 256;
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const uint64_t at = __ballot(v[4 * j + e] == here);
+                    if (at) lowest_place = min(lowest_place, (uint32_t)__builtin_ctzll(at) * 4 + e);
+                }
+                if (lowest_place < 256) id = c * (EACH * 64) + j * 256 + lowest_place;
             }
         }
     // Of finite numbers and +infinity the lowest: a negative one's bits, more for a
@@ -492,7 +509,7 @@ __global__ __launch_bounds__(WAVES * 64) void sample_list_kernel(SampleArgs a, S
             }
             if (lists) {
                 const uint32_t to = EACH * 64 - 1 - (n_list + before(lists));
-                if (in_list) queue[wave][to] = v[i], place[wave][to] = (uint16_t)(i * 64 + lane);
+                if (in_list) queue[wave][to] = v[i], place[wave][to] = (uint16_t)place_of(i);
                 n_list += (uint32_t)__popcll(lists);
             }
         }
@@ -602,9 +619,10 @@ __device__ __forceinline__ uint64_t find_few(uint64_t key, uint64_t w, uint64_t 
 // The same among the keys that a workgroup's threads hold (those of `in`), by
 // their distance from the largest of them: 1024 bins over the distances, then over
 // those of the bin that the key is in, until that holds no more than a wave's.
+// clear: the bins are.
 template <bool MASS>
 __device__ uint64_t find_listed(const uint64_t (&key)[kSmPerThread], const uint64_t (&w)[kSmPerThread], uint32_t in, uint64_t target,
-                                Bins& b, Together<kSmWaves>& all) {
+                                Bins& b, bool& clear, Together<kSmWaves>& all) {
     const uint32_t tid = threadIdx.x;
     uint64_t top = 0, under = 0;  // under: the complement of the smallest
 #pragma unroll
@@ -616,10 +634,13 @@ __device__ uint64_t find_listed(const uint64_t (&key)[kSmPerThread], const uint6
     for (int turn = 0; turn < 7; ++turn) {
         const uint64_t span = top - low;
         const uint32_t sh = span < kSmBins ? 0 : 54 - (uint32_t)__clzll((long long)span);
-        b.mass[tid] = 0;
-        b.count[tid] = 0;
-        if (tid == 0) b.few = 0;
-        __syncthreads();
+        if (!clear) {
+            b.mass[tid] = 0;
+            b.count[tid] = 0;
+            if (tid == 0) b.few = 0;
+            __syncthreads();
+        }
+        clear = false;
 #pragma unroll
         for (uint32_t i = 0; i < kSmPerThread; ++i)
             if (in >> i & 1u) {
@@ -675,6 +696,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
     __shared__ uint64_t memory[2][2][kSmWaves];
     __shared__ double parts[kSmParts];
     __shared__ Bins bins;
+    __shared__ unsigned long long in_chunks[kSmThreads];  // the list's kept weights, by group of chunks
     __shared__ uint32_t found;
     __shared__ uint64_t found_before;
     const uint32_t out = blockIdx.x, tid = threadIdx.x;
@@ -706,10 +728,13 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
     }
     Together<kSmWaves> all{memory};
     bins.mass[tid] = 0;
+    bins.count[tid] = 0;
+    in_chunks[tid] = 0;
+    if (tid == 0) bins.few = 0;
     __syncthreads();
     uint64_t cut = kLeastKey;
     uint32_t in = 0, in_k = 0, in_p = 0;
-    bool clear = true;  // are the bins' masses
+    bool clear = true;  // the bins are
     if (s.mode == kSmCut) {
         if (r.listed <= p.list) {
 #pragma unroll
@@ -732,10 +757,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
             const bool few = r.listed <= 64;
             const auto find = [&](auto mass, uint32_t among, uint64_t target) -> uint64_t {
                 constexpr bool kMass = decltype(mass)::value;
-                if (!few) {
-                    clear = false;
-                    return find_listed<kMass>(key, w, among, target, bins, all);
-                }
+                if (!few) return find_listed<kMass>(key, w, among, target, bins, clear, all);
                 if (tid < 64) {
                     const uint64_t c = find_few<kMass>(among & 1u ? key[0] : 0, w[0], target);
                     if (tid == 0) bins.cut = c;
@@ -789,15 +811,9 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
                     p.chunk_count[(uint64_t)out * p.chunks + c] = n;
                 }
             }
-            clear = false;
             __syncthreads();
             mine = kept = 0;
             add_chunks();
-        }
-        if (!clear) {
-            __syncthreads();
-            bins.mass[tid] = 0;
-            __syncthreads();
         }
         // What the list keeps, to its groups.
 #pragma unroll
@@ -808,10 +824,10 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a, S
                 continue;
             }
             ++kept;
-            atomicAdd(&bins.mass[(0xFFFFFFFFu - (uint32_t)key[i]) / p.chunk / per], (unsigned long long)w[i]);
+            atomicAdd(&in_chunks[(0xFFFFFFFFu - (uint32_t)key[i]) / p.chunk / per], (unsigned long long)w[i]);
         }
         __syncthreads();
-        mine += bins.mass[tid];
+        mine += in_chunks[tid];
     }
     uint64_t sum;
     const uint64_t to = all.scan(mine, sum, kept);
