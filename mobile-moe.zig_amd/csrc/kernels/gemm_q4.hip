@@ -337,6 +337,7 @@ const void* fn_of(const Shape& t) {
     if (t.mt == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 2, 8, 1>);
     if (t.ks == 8) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 1, 8>);
     if (t.ks == 4 && t.rs == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 2, 4>);
+    if (t.ks == 4 && t.nj == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 4>);
     if (t.ks == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 4, 4>);
     if (t.ks == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 2>);
     return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 1>);
@@ -347,11 +348,16 @@ const void* fn_of(const Shape& t) {
 // and one tile makes enough workgroups). {1,1,1,8} / {1,1,2,4} / {1,1,4,4}, us:
 // [768 x 8192] times 64 (192 tiles) 16.1 / 19.7 / 23.3, [2048 x 2560] times 20 (256) 8.9 /
 // 8.7 / 10.0, times 64 (512) 13.1 / 8.9 / 10.1, times 100 (896) - / 12.6 / 10.4,
-// [3840 x 768] times 32 (480) 8.1 / 5.9 / 6.6. Then larger tiles and fewer groups. Measured, us, with {1,1,4,4} / {1,2,4,2} / {2,1,8,2} / {2,2,8,1} / {4,2,8,1}:
-// [2048 x 2560] times 16 (128 tiles) 10.0 / 14.6 / 18.7 / 29.0 / 48, times 128 (1024)
+// [3840 x 768] times 32 (480) 8.1 / 5.9 / 6.6.
+//
+// Then larger tiles and fewer groups. {1,1,4,4} / {1,2,4,2} / {2,1,8,2} / {2,2,8,1} /
+// {4,2,8,1}: [2048 x 2560] times 16 (128 tiles) 10.0 / 14.6 / 18.7 / 29.0 / 48, times 128 (1024)
 // 10.6 / 15.2 / 19.0 / 30.3 / 50, times 256 (2048) 19.0 / 15.6 / 19.2 / 30.3 / 51; [3840 x
 // 768] times 256 (3840) 21.7 / 10.2 / 9.3 / 12.2 / 19.0; [10240 x 2048] times 64 (2560)
 // 23.9 / 18.8 / 16.4 / 25.2 / 41, times 256 (10240) 75 / 42.4 / 45.6 / 39.8 / 33.9.
+// Between four and eight tiles per CU {1,2,4,4} is ahead of {1,2,4,2} where rows are
+// long: [3840 x 2048] times 77 11.7 / 12.8, [1536 x 4096] times 256 18.7 / 21.6, but [5120
+// x 1664] times 64 13.9 / 12.9.
 //
 // Many: the two largest tiles by what they cost, rounds of one workgroup per CU
 // times a round's time, in hundredths of a microsecond a unit (fitted to the above
@@ -365,6 +371,7 @@ Shape shape_of(uint32_t tiles, uint32_t units, uint32_t batch, uint32_t cus) {
     if (results <= cus && units >= 32) return Shape{1, 1, 1, 8, 1};
     if (results <= 2ull * cus) return Shape{1, 1, 2, 4, 2};
     if (results <= 4ull * cus) return Shape{1, 1, 4, 4, 4};
+    if (results <= 8ull * cus && units >= 16) return Shape{1, 2, 4, 4, 8};
     if (results <= 16ull * cus) return results > 8ull * cus && batch > 16 ? Shape{2, 1, 8, 2, 8} : Shape{1, 2, 4, 2, 8};
     if (batch <= 16) return Shape{1, 2, 4, 1, 8};
     const auto rounds = [&](uint32_t t, uint32_t vecs) {

@@ -164,7 +164,7 @@ def test_several_vectors(ctx, t, layout, batch, rows, cols):
 @pytest.mark.parametrize("batch,rows,cols", [(256, 1000, 768), (300, 4100, 256), (64, 16400, 128), (4, 40000, 64), (1000, 130, 8224),
                                              (16, 70001, 96), (29, 40000, 160), (37, 30000, 288), (250, 10250, 544), (513, 5000, 96), (40, 16000, 544), (100, 6000, 96),
                                              (77, 7001, 2176), (64, 768, 4352), (64, 1000, 768),
-                                             (100, 1000, 2176)])
+                                             (100, 1000, 2176), (77, 4000, 2112)])
 def test_large_products(ctx, t, batch, rows, cols):
     rng = np.random.default_rng(batch)
     raw, w = weights(rng, t, rows, cols, 2)
@@ -226,7 +226,7 @@ def test_results_behind_four_gigabytes(ctx, t, layout):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("batch,rows,cols", [(6, 40, 640), (64, 500, 640), (70, 3000, 640), (70, 9000, 640), (40, 30000, 640), (64, 768, 4352)])
+@pytest.mark.parametrize("batch,rows,cols", [(6, 40, 640), (64, 500, 640), (70, 3000, 640), (70, 9000, 640), (40, 30000, 640), (64, 768, 4352), (77, 4000, 2112)])
 @pytest.mark.parametrize("where", [100, 321, 600])
 def test_values_that_outgrow_the_first(ctx, t, batch, rows, cols, where):
     """Values up to 1e6 and 1e30 times as large as a vector's first 64, which set its power of two; first ones of 0."""
