@@ -1,13 +1,16 @@
 // 4-bit weights (q4_ops.hpp) times many f32 vectors on gfx950's f16 matrix
 // cores: prompts.
 //
-// The integer weights are exact in f16. A vector's value, times a power of two
-// that keeps the vector's largest below 2^15, is the sum of two f16 numbers: the
-// nearest one, and the nearest to what that leaves, off by 2^-23 of the value at
-// most (where that is more, by 2^-28 of the largest of its first 64 or by 2^-39
-// of the vector's largest). A 32-column block of 16
-// weight rows times 16 vectors is two v_mfma_f32_16x16x32_f16 (the smaller parts
-// first) and one multiply-add per output with the block's scale.
+// The integer weights are exact in f16. A vector's value, times a power of two, is
+// the sum of two f16 numbers: the nearest one, and the nearest to what that leaves.
+// That is off by 2^-23 of the value at most, or by half of f16's smallest step, 2^-25,
+// where that is more. So the power of two goes with the vector's values: the largest
+// of every 128 columns lies in [2^6, 2^15) (the last step is at most 2^-31 of it), and
+// where the power changes the sums so far change with it. It stays within 2^64 of its
+// smallest, which keeps the sums in range: beside a value 2^64 and more times as large
+// a value may be off by 2^-95 of that. A 32-column block of 16 weight rows times 16
+// vectors is two v_mfma_f32_16x16x32_f16 (the smaller parts first) and one
+// multiply-add per output with the block's scale.
 //
 // Bound: vector instructions (per value of x two conversions, per eight weights
 // 9 or 21 operations, per output and block one multiply-add) beside the matrix
@@ -16,9 +19,9 @@
 // unpacks weights of its own rows straight from their records. Waves may also
 // split the columns (KS groups), their sums added at the end.
 //
-// Measured: [10240 x 2048] times 256 vectors 34.4 us (312 Tflop/s of products; the
+// Measured: [10240 x 2048] times 256 vectors 33.4 us (321 Tflop/s of products; the
 // two matrix instructions per product alone would take 17 us), [3840 x 768] times
-// 77 vectors 7.7 us; with bf16 parts (three instructions per product, four
+// 77 vectors 7.4 us; with bf16 parts (three instructions per product, four
 // conversions) 74 and 10.9 us.
 #include <type_traits>
 
@@ -83,31 +86,44 @@ __device__ __forceinline__ uint32_t run_place(uint32_t vec, uint32_t group) {
     return (vec & 15) ^ ((0x2130u >> (4 * group) & 3u) << 2);  // 0 3 1 2 fours for groups 0 1 2 3
 }
 
-// A vector's power of two: its largest |x| becomes at least 2^at and less than
-// twice that. Below 2^-95 as 2^-95.
-__device__ __forceinline__ float fit(float most, uint32_t at) {
-    const uint32_t e = min(max(__float_as_uint(most) >> 23, 32u), 254u);
-    return __uint_as_float((254 + at - e) << 23);
-}
-constexpr float kQ4Fits = 32768.0f;
+// The power of two that takes a largest |x| into [2^12, 2^13), or as near to that as
+// f32 has one: room for values four times as large, and for a 64th.
+__device__ __forceinline__ int fit(float most) { return 139 - (int)min(max(__float_as_uint(most) >> 23, 12u), 254u); }
+__device__ __forceinline__ float power_of_two(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
+constexpr float kQ4Fits = 32768.0f, kQ4Low = 64.0f;
+constexpr int kQ4Up = 64;
 __device__ __forceinline__ float row_max(float m) {  // over 16 lanes
     m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0xB1, 0xF, 0xF, false)));
     m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x4E, 0xF, 0xF, false)));
     m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x141, 0xF, 0xF, false)));
     return fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x140, 0xF, 0xF, false)));
 }
-// max(m, |a|, |b|), NaN left out (fmaxf would quiet each operand first).
-__device__ __forceinline__ void max_abs2(float& m, uint32_t a, uint32_t b) {
-    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(a), "v"(b));
+// The largest of eight |x|, NaN left out (fmaxf would quiet each operand first).
+__device__ __forceinline__ float max_abs(const uint4& v, const uint4& w) {
+    float m;
+    asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(m) : "v"(v.x), "v"(v.y), "v"(v.z));
+    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(v.w), "v"(w.x));
+    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(w.y), "v"(w.z));
+    asm("v_max_f32 %0, %0, |%1|" : "+v"(m) : "v"(w.w));
+    return m;
+}
+// Of 64 lanes' truth values, one bit for each 16: is one of them true.
+__device__ __forceinline__ uint32_t any_of_rows(uint64_t which) {
+    uint64_t b;
+    asm("s_quadmask_b64 %0, %1\n\ts_quadmask_b64 %0, %0" : "=&s"(b) : "s"(which) : "scc");
+    return (uint32_t)b;
 }
 
 // MT: 16 vectors each; NJ: 16 weight rows each of a wave; RS waves share an x
 // tile, KS groups of them the columns.
 //
-// A vector's power of two comes from its first 64 columns, with room for values
-// 2048 times as large; where one is larger still, which shows at the end, the
-// workgroup goes over its columns a second time with what it knows then. So the
-// loop has no case for it.
+// The wave that stages a unit's values looks at their largest before. Where one has
+// left the range of its vector's power of two, the wave takes another one and says so
+// in LDS, and the waves that read the values change their sums before that unit;
+// otherwise nothing of this is in the loop but seven vector instructions for eight
+// columns and two branches a unit. (For values of a normal distribution the power
+// stays as the first unit sets it. A branch each 64 columns instead of 128 costs
+// [10240 x 2048] times 256 2 us.)
 template <int FMT, int MT, int NJ, int RS, int KS>
 __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_kernel(GemmQ4Args a) {
     constexpr int kQuads = MT * 4 / RS;                              // of x, a thread and half step
@@ -117,8 +133,10 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
     constexpr uint32_t kRed = KS > 1 ? RS * KS * kSlot * 4 : 0, kMain = KS * 2 * kBuf;
     constexpr int kAhead = 2;
     __shared__ __align__(16) uint8_t lds[kRed > kMain ? kRed : kMain];
-    __shared__ float undo[KS][MT * 16];
-    __shared__ uint32_t again;
+    // For two turns: how much the vectors' powers of two have grown, and the turn for which
+    // each staging wave (any of them) has said so. In the end, the powers undone.
+    __shared__ __align__(16) int grown[KS][2][MT * 16];
+    __shared__ uint32_t grown_at[KS][2][RS], any_at[KS][2];
     // Tile group tg runs on XCD tg % 8, its groups of vectors one after the other:
     // each XCD's L2 holds an eighth of the matrix, read once.
     const uint32_t r8 = blockIdx.x >> 3, item = r8 % a.items, tg = r8 / a.items * 8 + (blockIdx.x & 7);
@@ -133,7 +151,7 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
     // Its tiles, as evenly over the waves as they go.
     const uint32_t each = a.wg_tiles / RS, more = a.wg_tiles % RS;
     const uint32_t tile0 = tg * a.wg_tiles + rw * each + min(rw, more), n_tiles = each + (rw < more);
-    if (threadIdx.x == 0) again = 0;
+    if (lane < 2) grown_at[kg][lane][rw] = any_at[kg][lane] = 0;
 
     // Units of this group; all groups take as many turns.
     const uint32_t u0 = a.units * kg / KS, u1 = a.units * (kg + 1) / KS, turns = (a.units + KS - 1) / KS;
@@ -152,17 +170,20 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
     for (int i = 0; i < 4; ++i) place[i] = run_place(r0 + 4 * RS * i, (n >> 1) & 3) * 16;
 
     f32x4 acc[MT][NJ];
-    float pow2[kQuads], most[kQuads];
-    // Loads in flight: of x a unit ahead (each half when the last one's is in
-    // LDS), of the weights kAhead.
-    uint4 xv[2][kQuads], wv[kAhead][NJ];
+    int power[kQuads], least[kQuads];  // a vector's power of two, and the smallest it has had
+    float absent[kQuads];              // in range where there is no vector, otherwise 0
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) absent[i] = r0 + 4 * RS * i < count ? 0.0f : kQ4Low;
+    // Loads in flight: of x one unit's first half and two units' second ones (a unit's
+    // largest is looked at before its first half goes to LDS), of the weights kAhead units.
+    uint4 x0[kQuads], x1[2][kQuads], wv[kAhead][NJ];
     uint32_t dv[kAhead][NJ];
-    const auto load_x = [&](uint32_t u, int h) {
+    const auto load_x = [&](uint32_t u, int h, uint4 (&to)[kQuads]) {
         const uint32_t col = u * kQ4UnitCols + 64 * h;
         const uint32_t part = u < u1 && col + 32 == a.cols ? upper : 0;
         const uint32_t soff = u < u1 && col < a.cols ? col * 4 : kBufOob;
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) xv[h][i] = buf_load_b128(x_r, x_voff[i] | part, soff);
+        for (int i = 0; i < kQuads; ++i) to[i] = buf_load_b128(x_r, x_voff[i] | part, soff);
     };
     const auto load_w = [&](auto nj, uint32_t u, uint4 (&wq)[NJ], uint32_t (&dq)[NJ]) {
 #pragma unroll
@@ -173,15 +194,54 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
             dq[j] = buf_load_b16(d_r, lane * 8, ok ? t * a.d_row * 32 + (u >> 2) * kQ4StepScaleBytes + (u & 3) * 2 : kBufOob);
         }
     };
-    // Half h's loaded values into its buffer.
-    const auto stage = [&](int h) {
+    // Are the largest of a unit, as loaded, out of range of the last one's power of two?
+    // (Yes also where a lane has not one of all its vectors in range: adapt() tells.)
+    const auto out_of_range = [&](uint32_t u, int q) {
+        float low = kQ4Low, most = kQ4Low;
 #pragma unroll
         for (int i = 0; i < kQuads; ++i) {
-            const float s = pow2[i];
-            max_abs2(most[i], xv[h][i].x, xv[h][i].y);
-            max_abs2(most[i], xv[h][i].z, xv[h][i].w);
-            const float v[4] = {__uint_as_float(xv[h][i].x), __uint_as_float(xv[h][i].y), __uint_as_float(xv[h][i].z),
-                                __uint_as_float(xv[h][i].w)};
+            const float at = fmaf(max_abs(x0[i], x1[q][i]), power_of_two(power[i]), absent[i]);
+            low = i ? fminf(low, at) : at;
+            most = i ? fmaxf(most, at) : at;
+        }
+        const bool out = (__ballot(most >= kQ4Fits) != 0) | (any_of_rows(__ballot(low >= kQ4Low)) != 15);
+        return out && u < u1;
+    };
+    // The powers of two for it, the turn-th.
+    const auto adapt = [&](uint32_t turn, int q) {
+        bool changed = false;
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+            const float m = row_max(max_abs(x0[i], x1[q][i])), at = m * power_of_two(power[i]);
+            int by = 0;
+            if (at >= kQ4Fits || (m > 0.0f && at < kQ4Low)) by = min(fit(m), least[i] + kQ4Up) - power[i];
+            power[i] += by;
+            least[i] = min(least[i], power[i]);
+            changed |= by != 0;
+            if (n == 0) grown[kg][turn & 1][r0 + 4 * RS * i] = by;
+        }
+        if (__any(changed) && lane == 0) grown_at[kg][turn & 1][rw] = any_at[kg][turn & 1] = turn;
+    };
+    // The sums so far, as the turn-th unit wants them.
+    const auto follow = [&](uint32_t turn) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int4 by = *reinterpret_cast<const int4*>(&grown[kg][turn & 1][m * 16 + 4 * g]);
+            const bool said = grown_at[kg][turn & 1][(4 * m + g) % RS] == turn;
+            const int b[4] = {said ? by.x : 0, said ? by.y : 0, said ? by.z : 0, said ? by.w : 0};
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[m][j][e] = ldexpf(acc[m][j][e], b[e]);
+        }
+    };
+    // Half h's loaded values into its buffer.
+    const auto stage = [&](int h, const uint4 (&from)[kQuads]) {
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+            const float s = power_of_two(power[i]);
+            const float v[4] = {__uint_as_float(from[i].x), __uint_as_float(from[i].y), __uint_as_float(from[i].z),
+                                __uint_as_float(from[i].w)};
             _Float16 hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -221,77 +281,83 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
         }
     };
 
+    // A wave that shares its tile with no other needs only the order of its own accesses
+    // ([768 x 8192] times 64 15.9 us, with barriers 19.0).
+    const auto staged = [] {
+        if constexpr (RS == 1) wave_lds_order();
+        else lds_barrier();
+    };
+    // Sums that the compiler does not put off beyond a branch: of the largest tile a fourth,
+    // or its products do not fit the registers (1.3 us of 34).
+    const auto settle = [&](auto nj) {
+        if constexpr (MT >= 4) {
+#pragma unroll
+            for (int j = 0; j < nj(); ++j) {
+                f32x4& sums = acc[0][j];
+                asm volatile("" : "+v"(sums));
+            }
+        }
+    };
     // All columns, for a wave with so many tiles. As many barriers whatever it has.
-    const auto sweep = [&](auto nj, bool begin) {
-        load_x(u0, 0);
+    const auto sweep = [&](auto nj) {
+        load_x(u0, 0, x0);
+        load_x(u0, 1, x1[0]);
 #pragma unroll
         for (int q = 0; q < kAhead; ++q) load_w(nj, u0 + q, wv[q], dv[q]);
-        load_x(u0, 1);
+        load_x(u0 + 1, 1, x1[1]);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int j = 0; j < NJ; ++j) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (begin) {
 #pragma unroll
-            for (int i = 0; i < kQuads; ++i) {
-                most[i] = 0.0f;
-                max_abs2(most[i], xv[0][i].x, xv[0][i].y);
-                max_abs2(most[i], xv[0][i].z, xv[0][i].w);
-                pow2[i] = fit(row_max(most[i]), 3);
-            }
-        }
-        stage(0);
-        load_x(u0 + 1, 0);
-        lds_barrier();
+        for (int i = 0; i < kQuads; ++i) power[i] = least[i] = fit(row_max(max_abs(x0[i], x1[0][i])));
+        stage(0, x0);
+        load_x(u0 + 1, 0, x0);
+        staged();
+        bool said = false;
         for (uint32_t k = 0; k < turns; k += kAhead) {
 #pragma unroll
             for (int q = 0; q < kAhead; ++q) {
                 if (k + q >= turns) break;  // for the whole workgroup
                 const uint32_t u = u0 + k + q;
+                if (said) follow(k + q);
                 float c[NJ][4];
 #pragma unroll
                 for (int j = 0; j < nj(); ++j) broadcast_rows4(f16_scale((uint16_t)dv[q][j]), c[j]);
-                stage(1);
-                load_x(u + 1, 1);
+                stage(1, x1[q]);
+                load_x(u + 2, 1, x1[q]);
                 products(nj, 0, wv[q], c);
-                lds_barrier();
-                stage(0);
-                load_x(u + 2, 0);
+                settle(nj);
+                if (out_of_range(u + 1, q ^ 1)) adapt(k + q + 1, q ^ 1);
+                staged();
+                const uint32_t any = any_at[kg][q ^ 1];
+                stage(0, x0);
+                load_x(u + 2, 0, x0);
                 products(nj, 1, wv[q], c);
                 load_w(nj, u + kAhead, wv[q], dv[q]);
-                lds_barrier();
+                settle(nj);
+                said = (uint32_t)__builtin_amdgcn_readfirstlane(any) == k + q + 1;
+                staged();
             }
         }
     };
-    for (int pass = 0; pass < 2; ++pass) {
-        if (NJ > 1 && n_tiles < NJ) sweep(std::integral_constant<int, (NJ > 1 ? NJ - 1 : 1)>(), pass == 0);
-        else sweep(std::integral_constant<int, NJ>(), pass == 0);
-        // Did all of them fit?
-        bool far = false;
-#pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
-            const float m = row_max(most[i]);
-            far |= m * pow2[i] >= kQ4Fits;
-            if (pass == 0 && m * pow2[i] >= kQ4Fits) pow2[i] = fit(m, 14);
-        }
-        if (pass == 0 && __any(far) && lane == 0) again = 1;
-        lds_barrier();
-        if (!again) break;
-    }
+    if (NJ > 1 && n_tiles < NJ) sweep(std::integral_constant<int, (NJ > 1 ? NJ - 1 : 1)>());
+    else sweep(std::integral_constant<int, NJ>());
 
     // The vectors' powers of two, undone.
 #pragma unroll
     for (int i = 0; i < kQuads; ++i)
-        if (n == 0) undo[kg][r0 + 4 * RS * i] = 1.0f / pow2[i];
+        if (n == 0) grown[kg][0][r0 + 4 * RS * i] = -power[i];
     lds_barrier();
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m) {
+        const int4 by = *reinterpret_cast<const int4*>(&grown[kg][0][m * 16 + 4 * g]);
+        const int b[4] = {by.x, by.y, by.z, by.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float f = undo[kg][m * 16 + 4 * g + e];
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) acc[m][j][e] *= f;
-        }
+            for (int j = 0; j < NJ; ++j) acc[m][j][e] = ldexpf(acc[m][j][e], b[e]);
+    }
     const auto put = [&](uint32_t m, uint32_t j, uint32_t e, float v) {
         const uint32_t t = m * 16 + 4 * g + e, row = (tile0 + j) * 16 + n;
         if (j < n_tiles && t < count && row < a.rows) a.y[(uint64_t)(first + t) * a.y_slot + (uint64_t)row * a.y_row] = v;

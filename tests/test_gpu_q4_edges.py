@@ -1,0 +1,110 @@
+"""4-bit products where they can lose what counts: vectors with a few large values
+beside small ones, tiny vectors, values that are not finite, on every tile of the
+matrix-core kernel and in the decode kernel.
+
+Tolerances, u = 2^-24. The matrix-core kernel (every product with the outputs' rows
+first, layout 1) takes a value as two f16 numbers after a power of two that puts the
+largest of its 128 columns at 2^6 or more: off by 2^-23 of it, or by half a step of
+2^-24, 2^-31 of that largest; where the power is kept within 2^64 of the one that put
+the vector's largest there, by 2^-(25 + 64 + 6) of that. The decode kernel takes integers of at most 2^30 for a block whose largest value
+is at least 2^29 of them: off by half a step, 2^-30 of the block's largest. A row with a single weight of 1 gives the value itself: both, and a unit
+for the sum of the two parts; nothing of the other columns' sizes.
+"""
+import numpy as np
+import pytest
+
+import mmhip as mm
+import step_ends_reference as ref
+from step_reference import At, Buffers, U
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [mm.Q4_0, mm.IQ4_NL]
+# A (vectors, rows, columns) for each tile of the matrix-core kernel on 256 CUs: vectors in 16s, weight tiles a wave, waves
+# that share x, groups of columns.
+TILES = {"1118": (6, 64, 4128), "1124": (20, 64, 2176), "1144": (16, 8200, 672), "1244": (40, 5500, 2048),
+         "1242": (40, 5500, 672), "2182": (40, 11000, 672), "1241": (16, 65600, 352), "2281": (40, 22000, 352),
+         "4281": (250, 10250, 352)}
+
+
+def product(ctx, raw, t, x, rows, layout):
+    """[batch, rows]"""
+    batch, cols = x.shape
+    wt = ctx.upload(raw, t, rows, cols)
+    with Buffers(ctx) as d:
+        dy = d.put(np.full(batch * rows, 7.0, np.float32))
+        ctx.qmm_dev(wt, 0, d.put(x), dy, batch, layout)
+        ctx.synchronize()
+        y = dy.to_numpy(np.float32, batch * rows)
+    wt.free()
+    return y.reshape(batch, rows) if layout == 0 else np.ascontiguousarray(y.reshape(rows, batch).T)
+
+
+def picking(t, rows, cols):
+    """Weights of which row r has a single 1, at column at[r] (Q4_0), or 1 in the block around it (IQ4_NL, which has no 0)."""
+    at = np.arange(rows) * 37 % cols
+    blk = np.zeros((rows, cols // 32, 18), np.uint8)
+    one = np.array([1.0], np.float16).view(np.uint8)
+    if t == mm.Q4_0:
+        blk[..., :2], blk[..., 2:] = one, 0x88
+        j = at % 32
+        blk[np.arange(rows), at // 32, 2 + j % 16] = np.where(j < 16, 0x89, 0x98)
+    else:
+        blk[..., 2:] = 0x88
+        blk[np.arange(rows), at // 32, :2] = one
+    return blk.reshape(-1), at
+
+
+def largest_of(x, n):
+    """|x|'s largest in each run of n columns, for every column."""
+    pad = -(-x.shape[1] // n) * n
+    b = np.zeros((len(x), pad))
+    b[:, :x.shape[1]] = np.abs(x)
+    return np.repeat(b.reshape(len(x), -1, n).max(-1), n, 1)[:, :x.shape[1]]
+
+
+def check_picked(y, x, t, at, run, step):
+    """y against the values (or block sums) that the rows pick; run columns share a step of `step` of their largest."""
+    x = x.astype(np.float64)
+    off = 2 * U * np.abs(x) + step * largest_of(x, run) + 2.0 ** -95 * np.abs(x).max(1, keepdims=True)
+    if t == mm.Q4_0:
+        want, tol = x[:, at], off[:, at] + U * np.abs(x[:, at])
+    else:  # 32 values: 64 parts summed, each sum rounded by a unit at most
+        want = x.reshape(len(x), -1, 32).sum(-1)[:, at // 32]
+        tol = (off + 66 * U * np.abs(x)).reshape(len(x), -1, 32).sum(-1)[:, at // 32]
+    err, tol = np.abs(y - want), tol + 2.0 ** -149
+    assert (err <= tol).all(), (err / tol).max()
+
+
+def uneven(rng, batch, cols):
+    """Vectors with one value 10^3 to 10^25 times as large as the rest, first ones among them, and some with several."""
+    x = rng.standard_normal((batch, cols)).astype(np.float32)
+    where = [3, 40, 63, 64, 100, cols - 1, cols // 2, 130]
+    size = [1e3, 1e4, 1e5, 1e6, 1e9, 1e25]
+    for b in range(1, batch):
+        x[b, where[b % 8]] = size[b % 6] * (-1) ** (b // 3)
+        if b % 5 == 0:
+            x[b, where[(b + 3) % 8]] = -size[(b + 1) % 6]
+        if b % 7 == 0:
+            x[b, :64] *= np.float32(1e-6)
+        if b % 11 == 0:
+            x[b, 64:192] = 0
+    return x
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tile", sorted(TILES))
+def test_large_values_cost_others_nothing(ctx, t, tile):
+    batch, rows, cols = TILES[tile]
+    x = uneven(np.random.default_rng(batch), batch, cols)
+    raw, at = picking(t, rows, cols)
+    check_picked(product(ctx, raw, t, x, rows, 1), x, t, at, 128, 2.0 ** -31)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("batch", [1, 3, 4, 21])
+def test_large_values_in_the_decode_kernel(ctx, t, batch):
+    rows, cols = 500, 2080
+    x = uneven(np.random.default_rng(batch), batch, cols)
+    raw, at = picking(t, rows, cols)
+    check_picked(product(ctx, raw, t, x, rows, 0), x, t, at, 32, 2.0 ** -30)
