@@ -2,9 +2,9 @@
 // decode.
 //
 // y[t][r] = sum_b d[r][b] sum_{i < 32} v[r][32 b + i] x[t][32 b + i]. A vector's
-// block of 32 becomes integers of 31 bits with the block's own power of two
-// (exact down to 2^-7 of the block's largest value, below that off by at most
-// 2^-31 of it), cut into four int8 digits. The digits are rows of the A
+// block of 32 becomes integers of up to 2^30 with the block's own power of two
+// (exact down to 2^-6 of the block's largest value, below that off by at most
+// 2^-30 of it), cut into four int8 digits. The digits are rows of the A
 // operand of v_mfma_i32_16x16x32_i8, which has sixteen: one product per block
 // and 16 weight rows gives the exact integer sums of all four digits of up to
 // four vectors, so the weights are read and unpacked once for all of them and
@@ -44,10 +44,10 @@ constexpr uint32_t q4_unit_bytes() { return TOK == 1 ? 64 * 8 : 64 * 32; }
 
 // The four digits of four columns' integers (digit 0 the highest), a word per
 // digit, column e in byte e.
-__device__ __forceinline__ void digits4(const float (&v)[4], float inv, uint32_t (&out)[4]) {
+__device__ __forceinline__ void digits4(const float (&v)[4], int up, uint32_t (&out)[4]) {
     uint32_t q[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = ((uint32_t)(int)rintf(v[e] * inv) + 0x00808080u) ^ 0x00808080u;
+    for (int e = 0; e < 4; ++e) q[e] = ((uint32_t)(int)rintf(ldexpf(v[e], up)) + 0x00808080u) ^ 0x00808080u;
     const uint32_t a = __builtin_amdgcn_perm(q[1], q[0], 0x05010400u);  // bytes 0 0 1 1 of q0, q1
     const uint32_t b = __builtin_amdgcn_perm(q[3], q[2], 0x05010400u);
     const uint32_t c = __builtin_amdgcn_perm(q[1], q[0], 0x07030602u);  // bytes 2 2 3 3
@@ -58,13 +58,12 @@ __device__ __forceinline__ void digits4(const float (&v)[4], float inv, uint32_t
     out[0] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
-// A block's scale and its inverse, powers of two, from the bits of its largest
-// |x|: integers of at most 2^30. Values below 2^-97 keep steps of 2^-126; a
+// A block's scale, a power of two, and the power that undoes it, from the bits of its
+// largest |x|: integers of at most 2^30, and no steps below f32's own, 2^-149. A
 // block with an infinity or NaN gets a NaN scale.
-__device__ __forceinline__ float block_scale(uint32_t m_bits, float& inv) {
-    const uint32_t e = max(m_bits >> 23, 30u);
-    inv = __uint_as_float((283u - e) << 23);
-    return m_bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float((e - 29u) << 23);
+__device__ __forceinline__ float block_scale(uint32_t m_bits, int& up) {
+    up = 156 - (int)max(m_bits >> 23, 7u);
+    return m_bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : ldexpf(1.0f, -up);
 }
 
 // A quarter block of a vector, four columns per lane, into the LDS digits.
@@ -75,10 +74,10 @@ __device__ __forceinline__ void store_digits(const float (&v)[4], uint32_t tok, 
     m = umax_dpp<0xB1>(m);
     m = umax_dpp<0x4E>(m);
     m = umax_dpp<0x141>(m);
-    float inv;
-    const float s = block_scale(m, inv);
+    int up;
+    const float s = block_scale(m, up);
     uint32_t d[4];
-    digits4(v, m >= 0x7F800000u ? 0.0f : inv, d);
+    digits4(v, up, d);
     const uint32_t g = jq >> 1, half = jq & 1;
     uint8_t* const unit = aq + (blk >> 2) * q4_unit_bytes<TOK>();
 #pragma unroll
@@ -90,9 +89,10 @@ __device__ __forceinline__ void store_digits(const float (&v)[4], uint32_t tok, 
     if (jq == 0) xs[TOK == 1 ? blk : (blk >> 2) * 16 + tok * 4 + (blk & 3)] = s;
 }
 
-// Four digits' sums as one number, rounded once. Times the weights' scale first
-// (at most 2^59) and the vector's last: no product of scales that could leave
-// f32's normal numbers.
+// Four digits' sums as one number: the upper two's and the lower two's (below 2^28)
+// are rounded to f32 where they have more than 24 bits, and their sum once more.
+// Times the weights' scale first (at most 2^60) and the vector's last: no product of
+// scales that could leave f32's normal numbers.
 __device__ __forceinline__ float digits_value(int t1, int t2) { return fmaf((float)t1, 65536.0f, (float)t2); }
 
 struct Q4Args {

@@ -108,3 +108,18 @@ def test_large_values_in_the_decode_kernel(ctx, t, batch):
     x = uneven(np.random.default_rng(batch), batch, cols)
     raw, at = picking(t, rows, cols)
     check_picked(product(ctx, raw, t, x, rows, 0), x, t, at, 32, 2.0 ** -30)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("layout,batch", [(0, 1), (0, 4), (0, 22), (1, 1), (1, 22), (1, 70)])
+@pytest.mark.parametrize("size", [1e-30, 1e-36, 1e-38, 1e-42])
+def test_tiny_vectors(ctx, t, layout, batch, size):
+    """Down to f32's subnormal numbers, of which the last has 10 bits: nothing is flushed."""
+    rng = np.random.default_rng(batch)
+    rows, cols = 300, 1056
+    x = (rng.standard_normal((batch, cols)) * size).astype(np.float32)
+    x[:, 32:64] = 0
+    x[:, 64:128] *= np.float32(1e-2)
+    x[batch // 2, :256] = 0
+    raw, at = picking(t, rows, cols)
+    check_picked(product(ctx, raw, t, x, rows, layout), x, t, at, 128 if layout else 32, 2.0 ** (-31 if layout else -30))
