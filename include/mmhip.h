@@ -302,9 +302,18 @@ int mmhip_gemv_grouped_dev(mmhip_ctx* ctx, const mmhip_gemv_group* groups, uint3
  * The kernel, and with it the number format of the activations and the order of
  * the sums, is chosen by shape and batch: a call repeated gives the same bits,
  * but a quantised weight times the same vector in a batch of another size may
- * differ by the error of the coarser form, about 2e-5 of the result (4-bit
- * weights: 1e-6). The same holds for mmhip_batch_mat_mul and for the tokens of
- * an MoE layer call (about 1e-4 there). f32 / f16 weights give the same bits at every batch. */
+ * differ by the error of the coarser form, about 2e-5 of the result. The same holds
+ * for mmhip_batch_mat_mul and for the tokens of an MoE layer call (about 1e-4
+ * there). f32 / f16 weights give the same bits at every batch.
+ * 4-bit weights, at every batch: a result is off by the rounding of f32 sums, and by
+ * what its vector's values are off: 2^-23 of themselves, or up to four vectors (more
+ * of small matrices) 2^-30 of the largest of their 32 columns, otherwise 2^-31 of
+ * the largest of their 128 (2^-95 of the vector's). So batches of different sizes agree
+ * to about 1e-6 unless a value is some 10^5 times as large as those beside it.
+ * Infinities and NaN in vectors or scales: results that they take part in are not
+ * finite; with 4-bit weights they are what the sum over the columns gives in 64 bits
+ * (an infinity of either sign, or NaN), found more slowly, and so is a result whose
+ * sum leaves f32's range on the way. */
 int mmhip_qmm_dev(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat,
                   const float* x_dev, float* y_dev, uint64_t batch,
                   int out_layout);

@@ -358,9 +358,15 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
 #pragma unroll
             for (int j = 0; j < NJ; ++j) acc[m][j][e] = ldexpf(acc[m][j][e], b[e]);
     }
+    float odd = 0.0f;  // NaN once a result is infinite or NaN
+    const auto place_in_y = [&](uint32_t m, uint32_t j, uint32_t e) -> float* {
+        const uint32_t t = m * 16 + 4 * g + e, row = (tile0 + j) * 16 + n;
+        return j < n_tiles && t < count && row < a.rows ? a.y + ((uint64_t)(first + t) * a.y_slot + (uint64_t)row * a.y_row) : nullptr;
+    };
     const auto put = [&](uint32_t m, uint32_t j, uint32_t e, float v) {
         const uint32_t t = m * 16 + 4 * g + e, row = (tile0 + j) * 16 + n;
         if (j < n_tiles && t < count && row < a.rows) a.y[(uint64_t)(first + t) * a.y_slot + (uint64_t)row * a.y_row] = v;
+        odd = fmaf(v, 0.0f, odd);
     };
     if constexpr (KS == 1) {
 #pragma unroll
@@ -388,6 +394,16 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
             }
         }
     }
+    if (odd == odd) return;
+#pragma unroll 1
+    for (uint32_t q = KS > 1 ? kg : 0; q < MT * NJ; q += KS)
+#pragma unroll 1
+        for (uint32_t e = 0; e < 4; ++e) {
+            float* const y = place_in_y(q / NJ, q % NJ, e);
+            if (y && !(fabsf(*y) < INFINITY))
+                *y = q4_defined<FMT>(a.recs, a.dvals, a.units, a.d_row, a.cols, (tile0 + q % NJ) * 16 + n,
+                                     a.x + (uint64_t)(first + q / NJ * 16 + 4 * g + e) * a.x_stride);
+        }
 }
 
 // A launch's tile: 16 mt vectors by `tiles` weight tiles (at most nj for each of

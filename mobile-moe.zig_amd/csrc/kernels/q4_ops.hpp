@@ -60,6 +60,30 @@ __device__ __forceinline__ int q4_code(uint32_t c) {
     return NL ? (int)(int8_t)((c & 8u ? 0x7159453526190D01ull : 0xF6EADDCFBFAD9881ull) >> (8 * (c & 7u))) : (int)c - 8;
 }
 
+// A row's product with a vector by its definition, in 64 bits, one column after the
+// other: for results that the fast forms left infinite or NaN, which an infinity or NaN
+// spreads over (digits and parts of one are NaN), or sums beyond f32 on the way.
+template <int FMT>
+__device__ __forceinline__ float q4_defined(const uint4* recs, const uint16_t* dvals, uint32_t units, uint32_t d_row, uint32_t cols,
+                                            uint32_t row, const float* x) {
+    const uint32_t n = row & 15;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(recs + (uint64_t)(row >> 4) * units * 64 + n);
+    const uint16_t* d = dvals + (uint64_t)(row >> 4) * 16 * d_row + n * 4;
+    double sum = 0.0;
+#pragma unroll 1
+    for (uint32_t c = 0; c < cols; c += 8) {
+        const uint32_t u = c >> 7, b = (c >> 5) & 3, g = (c >> 3) & 3;
+        const double scale = f16_bits_to_f32(d[(u >> 2) * 256 + b * 64 + (u & 3)]);
+        uint32_t codes = w[(uint64_t)u * 256 + g * 64 + b];
+        if (FMT == kFmtQ4) codes ^= 0x88888888u;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+            sum += scale * q4_code<FMT == kFmtIq4>((codes >> (8 * (i & 3) + 4 * (i >> 2))) & 15u) * (double)x[c + i];
+        if (sum != sum) break;
+    }
+    return (float)sum;
+}
+
 // Where a step's scales of a tile begin, in bytes (steps: of a tile).
 constexpr uint32_t kQ4StepScaleBytes = 64 * 4 * 2;
 

@@ -123,3 +123,52 @@ def test_tiny_vectors(ctx, t, layout, batch, size):
     x[batch // 2, :256] = 0
     raw, at = picking(t, rows, cols)
     check_picked(product(ctx, raw, t, x, rows, layout), x, t, at, 128 if layout else 32, 2.0 ** (-31 if layout else -30))
+
+
+def definition(x, w):
+    """The sums of w x, and of |w x|: x [batch, cols], w [rows, cols] in 64 bits, of which some are not finite."""
+    at = ~(np.isfinite(x).all(0) & np.isfinite(w).all(0))
+    fx, fw = np.where(at, 0.0, x), np.where(at, 0.0, w)
+    y, s = fx @ fw.T, np.abs(fx) @ np.abs(fw).T
+    for c in np.flatnonzero(at):
+        term = x[:, c, None] * w[:, c]
+        y, s = y + term, s + np.abs(term)
+    return y, s
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tile", sorted(TILES) + ["decode1", "decode4", "fours"])
+def test_what_is_not_finite_follows_the_definition(ctx, t, tile):
+    """Infinite values times weights of either sign and 0, infinite and NaN scales, sums that only 64 bits hold: the
+    definition's infinity or NaN in their results, and nothing of them in the others."""
+    batch, rows, cols = TILES.get(tile) or {"decode1": (1, 700, 2080), "decode4": (4, 700, 2080), "fours": (22, 700, 544)}[tile]
+    rng = np.random.default_rng(rows)
+    raw = mm.make_weight(rng, t, rows, cols).reshape(rows, cols // 32, 18)
+    big = np.array([65504.0], np.float16).view(np.uint8)
+    raw[3, 1, :2] = np.array([np.inf], np.float16).view(np.uint8)
+    raw[20 % rows, 2, :2] = np.array([-np.inf], np.float16).view(np.uint8)
+    raw[37 % rows, 0, :2] = np.array([np.nan], np.float16).view(np.uint8)
+    raw[40:44, :, :2], raw[40:44, :, 2:] = big, rng.integers(0, 256, (4, 1, 16))  # rows of alike blocks
+    x = rng.standard_normal((batch, cols)).astype(np.float32)
+    odd = [lambda v: v.__setitem__(5, np.inf), lambda v: v.__setitem__(cols - 1, -np.inf), lambda v: v.__setitem__(64, np.nan),
+           lambda v: v.__setitem__([70, 90], np.inf), lambda v: v.__setitem__([3, 99], [np.inf, -np.inf]),
+           # the first half's values again with the other sign: sums beyond f32 that cancel in rows of alike blocks
+           lambda v: (v.__setitem__(slice(None), 0), v.__setitem__(slice(0, 32), 3e38), v.__setitem__(slice(64, 96), -3e38))]
+    with np.errstate(invalid="ignore"):
+        for b in range(batch):
+            if batch == 1 or b % 3 == 1:
+                odd[(b // 3 + rows) % 6](x[b])
+    w = ref.values_4bit(raw, t).reshape(rows, cols)
+    y = product(ctx, raw.reshape(-1), t, x, rows, 1 if tile in TILES else 0)
+    with np.errstate(over="ignore", invalid="ignore"):
+        want, s = definition(x.astype(np.float64), w)
+        want32 = want.astype(np.float32)
+    fine = np.isfinite(want32)
+    assert np.array_equal(np.isnan(y), np.isnan(want32))
+    assert np.array_equal(y[~fine & ~np.isnan(y)], want32[~fine & ~np.isnan(want32)])
+    tol = (cols / 32 + 200) * U * s + 2.0 ** -30 * cols * np.abs(x).max(1, keepdims=True, where=np.isfinite(x), initial=0) * np.max(
+        np.where(np.isfinite(w), np.abs(w), 0), 1)
+    with np.errstate(invalid="ignore"):
+        err = np.where(fine, np.abs(y - want), 0)
+    bad = fine & ~(err <= tol)
+    assert (fine.any() or batch == 1) and not bad.any(), [(i, y[tuple(i)], want[tuple(i)], s[tuple(i)], tol[tuple(i)]) for i in np.argwhere(bad)[:9]]
