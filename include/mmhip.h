@@ -558,9 +558,9 @@ int mmhip_embed_dev(mmhip_ctx* ctx, float* y_dev, uint64_t y_stride, const void*
  *     tables name too; shared_dev NULL: none), go onto the stack, requests and
  *     pages in order, and the row begins anew with no positions.
  *  2. A request gets its tokens where its table has the pages for all of its
- *     positions, where the tokens asked for by it and all before it are at
+ *     positions, where the tokens asked for by it and all such ones before it are at
  *     most max_tokens, and where it needs no new page or the new pages needed by
- *     it and all before it are at most those on the stack. granted[r] is 1
+ *     it and all such ones before it are at most those on the stack. granted[r] is 1
  *     there and 0 elsewhere; a request that gets none keeps its positions.
  *  3. New pages are taken from the top of the stack, requests and positions in
  *     order, and written to the tables. next_lens[r] and next_free_count are the
@@ -573,10 +573,11 @@ int mmhip_embed_dev(mmhip_ctx* ctx, float* y_dev, uint64_t y_stride, const void*
  *     NULL). Behind the last token, up to max_tokens, stand slot -1 and zeros.
  * next_lens_dev may be lens_dev and next_free_count_dev may be free_count_dev, so
  * that a captured step goes on from itself; no other buffers overlap. Shared
- * pages have to be full. A length or a request beyond its table and tokens
- * beyond max_tokens are reported; so is a page number on the stack or in a table
- * that the pool does not have (its positions get slot -1) and a stack that
- * would hold more than n_pages pages (it is cut there). Too few free pages are no
+ * pages have to be full; shared_dev needs release_dev. A length beyond its table
+ * (where its row is released it counts as that of a full table, otherwise its request
+ * gets nothing), a request beyond it and tokens beyond max_tokens are reported; so is
+ * a page number on the stack or in a table that the pool does not have (its positions
+ * get slot -1) and a stack that would hold more than n_pages pages (it is cut there). Too few free pages are no
  * fault: granted says so. n_requests below 2^24, max_tokens below 2^31;
  * page_tokens, n_pages as in mmhip_kv_cache, table_pages as in mmhip_mla_attention. */
 typedef struct {

@@ -46,7 +46,7 @@ int check_step_status(mmhip_ctx* ctx, const char* what) {
                                       "mla_attention: a page that the pool does not have (left out)",
                                       "logprobs: a token outside the vocabulary (NaN)",
                                       "embed: a token outside the table (NaN)",
-                                      "kv_plan: a length beyond a table's pages (its request got nothing)",
+                                      "kv_plan: a length beyond a table's pages (a released one cut there, otherwise its request got nothing)",
                                       "kv_plan: more tokens than max_tokens (the requests behind them got nothing)",
                                       "kv_plan: a page that the pool does not have (its positions got no slot)",
                                       "kv_plan: more free pages than the pool has (cut there)",
