@@ -172,3 +172,68 @@ def test_what_is_not_finite_follows_the_definition(ctx, t, tile):
         err = np.where(fine, np.abs(y - want), 0)
     bad = fine & ~(err <= tol)
     assert (fine.any() or batch == 1) and not bad.any(), [(i, y[tuple(i)], want[tuple(i)], s[tuple(i)], tol[tuple(i)]) for i in np.argwhere(bad)[:9]]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("layout,batch", [(0, 1), (0, 3), (0, 24), (1, 1), (1, 24), (1, 100)])
+def test_all_bits_of_a_value(ctx, t, layout, batch):
+    """One value of 23 bits in each block: it comes out as it is. (Two f16 numbers hold it: of the values' 4096 .. 8191 the
+    nearest multiple of 4, and what that leaves, at most 2 in steps of 2^-10; a block's integers hold 30 bits.)"""
+    rng = np.random.default_rng(batch)
+    rows, cols = 320, 1056
+    x = np.zeros((batch, cols), np.float32)
+    x[:, rng.integers(0, 32, cols // 32) + np.arange(0, cols, 32)] = (
+        rng.integers(1 << 22, 1 << 23, (batch, cols // 32)) * np.float32(2.0 ** -22) * rng.choice([-1, 1], (batch, cols // 32)))
+    raw, at = picking(mm.IQ4_NL, rows, cols)  # whole blocks of ones
+    if t == mm.Q4_0:
+        raw = raw.reshape(rows, -1, 18)
+        raw[..., 2:] = 0x99
+        raw = raw.reshape(-1)
+    assert np.array_equal(product(ctx, raw, t, x, rows, layout), x.reshape(batch, -1, 32).sum(-1)[:, at // 32])
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("batch", [2, 4, 5, 7, 15, 16, 17, 32, 33, 40])
+@pytest.mark.parametrize("rows,cols", [(17, 96), (100, 544), (64, 2176), (500, 4128)])
+def test_fours_are_as_exact_as_one_vector(ctx, t, batch, rows, cols):
+    """Shapes of up to two workgroups per CU. A block's sum: two roundings of the digits' sums, one of both together, one
+    with its scale, one with the others, the last one in up to cols / 32 blocks, eight waves' parts and three chunks one after
+    the other; the values themselves are off by 2^-30 of their block's largest."""
+    rng = np.random.default_rng(batch * 31 + rows)
+    raw = mm.make_weight(rng, t, rows, cols)
+    w = np.abs(ref.values_4bit(raw, t).reshape(rows, cols))
+    x = rng.standard_normal((batch, cols)).astype(np.float32)
+    x[:, rng.integers(0, cols, cols // 32)] *= 300
+    y = product(ctx, raw, t, x, rows, 0)
+    x = x.astype(np.float64)
+    want = x @ ref.values_4bit(raw, t).reshape(rows, cols).T
+    tol = (cols / 32 + 4 + 8 + 3) * U * (np.abs(x) @ w.T) + (2.0 ** -30 + 2.0 ** -38) * (largest_of(x, 32) @ w.T)
+    err = np.abs(y - want)
+    assert (err <= tol).all(), (err / tol).max()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("batch", [1, 20, 70])
+@pytest.mark.parametrize("size", [1e-38, 1.0, 1e30, 1e38])
+def test_sizes_of_vectors_and_scales_on_the_matrix_cores(ctx, t, batch, size):
+    """Scales of 0, of f16's largest and smallest, beside vectors of all sizes; results beyond f32 are infinite."""
+    rng = np.random.default_rng(9)
+    rows, cols = 500, 1056
+    raw = mm.make_weight(rng, t, rows, cols).reshape(rows, cols // 32, 18)
+    for r, d in ((3, 65504.0), (5, 6e-8), (7, 0.0)):
+        raw[r, 4:6, :2] = np.array([d], np.float16).view(np.uint8)
+    w = ref.values_4bit(raw, t).reshape(rows, cols)
+    x = (rng.standard_normal((batch, cols)) * size).clip(-3e38, 3e38).astype(np.float32)
+    x[:, 32:64] = 0
+    x[:, 64:96] *= np.float32(1e-3)
+    y = product(ctx, raw.reshape(-1), t, x, rows, 1)
+    x = x.astype(np.float64)
+    want, s = x @ w.T, np.abs(x) @ np.abs(w).T
+    # each of a block's 64 products and its sums is rounded by a unit at most, as each block's sum; subnormal results by 2^-150
+    tol = (cols / 32 + 200) * U * s + 2.0 ** -31 * (largest_of(x, 128) @ np.abs(w).T) + 2.0 ** -149
+    with np.errstate(over="ignore"):
+        inf = np.abs(want.astype(np.float32)) == np.inf
+    sure = np.abs(np.abs(want) - 2.0 ** 128) > tol
+    assert np.array_equal((np.abs(y) == np.inf)[sure], inf[sure])
+    ok = ~inf & np.isfinite(y)
+    assert (np.abs(y.astype(np.float64) - want)[ok] <= tol[ok]).all()
