@@ -298,7 +298,7 @@ void weight_destroy(mmhip_weight* w) {
 int gemv_device(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t first, uint64_t n, const float* x,
                 uint64_t x_stride, float* y, uint64_t y_stride, DevBuf* qscratch) {
     if (n == 0) return MMHIP_OK;
-    if (first + n > w->count) {
+    if (n > w->count || first > w->count - n) {
         set_error(MMHIP_ERR_INVALID, "gemv: matrix index out of range");
         return MMHIP_ERR_INVALID;
     }

@@ -237,3 +237,18 @@ def test_sizes_of_vectors_and_scales_on_the_matrix_cores(ctx, t, batch, size):
     assert np.array_equal((np.abs(y) == np.inf)[sure], inf[sure])
     ok = ~inf & np.isfinite(y)
     assert (np.abs(y.astype(np.float64) - want)[ok] <= tol[ok]).all()
+
+
+@pytest.mark.parametrize("t", [mm.Q4_0, mm.IQ4_NL, mm.Q8_0, mm.F32])
+def test_ranges_of_matrices_that_wrap(ctx, t):
+    """A first matrix whose sum with their number goes round 2^64 is refused like any other beyond the stack."""
+    wt = ctx.upload(mm.make_weight(np.random.default_rng(1), t, 16, 64, 3), t, 16, 64, 3)
+    with Buffers(ctx) as d:
+        x, y = d.new(64 * 4, 0), d.put(np.full(3 * 16, 7.0, np.float32))
+        for first, n in ((2 ** 64 - 1, 1), (2 ** 64 - 2, 3), (2, 2 ** 64 - 1), (3, 1), (0, 4), (2 ** 63, 2 ** 63)):
+            with pytest.raises(mm.MmhipError, match="out of range") as e:
+                ctx.gemv_batched_dev(wt, first, n, x, 0, y, 16)
+            assert e.value.code == mm.ERR_INVALID
+        ctx.synchronize()
+        assert (y.to_numpy(np.float32, 48) == 7).all()
+    wt.free()
