@@ -115,7 +115,7 @@ __device__ __forceinline__ uint32_t any_of_rows(uint64_t which) {
 }
 
 // MT: 16 vectors each; NJ: 16 weight rows each of a wave; RS waves share an x
-// tile, KS groups of them the columns.
+// tile, KS groups of them the columns. WAVES of a SIMD fit its registers.
 //
 // The wave that stages a unit's values looks at their largest before. Where one has
 // left the range of its vector's power of two, the wave takes another one and says so
@@ -124,8 +124,8 @@ __device__ __forceinline__ uint32_t any_of_rows(uint64_t which) {
 // columns and two branches a unit. (For values of a normal distribution the power
 // stays as the first unit sets it. A branch each 64 columns instead of 128 costs
 // [10240 x 2048] times 256 2 us.)
-template <int FMT, int MT, int NJ, int RS, int KS>
-__global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_kernel(GemmQ4Args a) {
+template <int FMT, int MT, int NJ, int RS, int KS, int WAVES>
+__global__ __launch_bounds__(RS * KS * 64, WAVES) void gemm_q4_kernel(GemmQ4Args a) {
     constexpr int kQuads = MT * 4 / RS;                              // of x, a thread and half step
     static_assert(kQuads >= 1 && MT * 4 % RS == 0, "a wave stages whole rows of four vectors");
     constexpr uint32_t kBuf = MT * 2 * kQ4Part;
@@ -287,16 +287,18 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
         if constexpr (RS == 1) wave_lds_order();
         else lds_barrier();
     };
-    // Sums that the compiler does not put off beyond a branch: of the largest tile a fourth,
-    // or its products do not fit the registers (1.3 us of 34).
-    const auto settle = [&](auto nj) {
-        if constexpr (MT >= 4) {
+    // Sums that the compiler does not put off beyond a branch, where a wave's products
+    // would not fit the registers otherwise: [10240 x 2048] times 256 33.4 us, without them
+    // 34.7; times 512 with four waves a SIMD 61.8 and 107.
+    constexpr int kSettleFirst = MT >= 4 ? 1 : MT * NJ == 4 && WAVES == 4 ? 2 : 0, kSettleSecond = MT >= 4 ? 1 : 0;
+    const auto settle = [&](auto nj, auto count) {
+#pragma unroll
+        for (int m = 0; m < count(); ++m)
 #pragma unroll
             for (int j = 0; j < nj(); ++j) {
-                f32x4& sums = acc[0][j];
+                f32x4& sums = acc[m][j];
                 asm volatile("" : "+v"(sums));
             }
-        }
     };
     // All columns, for a wave with so many tiles. As many barriers whatever it has.
     const auto sweep = [&](auto nj) {
@@ -327,7 +329,7 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
                 stage(1, x1[q]);
                 load_x(u + 2, 1, x1[q]);
                 products(nj, 0, wv[q], c);
-                settle(nj);
+                settle(nj, std::integral_constant<int, kSettleFirst>());
                 if (out_of_range(u + 1, q ^ 1)) adapt(k + q + 1, q ^ 1);
                 staged();
                 const uint32_t any = any_at[kg][q ^ 1];
@@ -335,7 +337,7 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
                 load_x(u + 2, 0, x0);
                 products(nj, 1, wv[q], c);
                 load_w(nj, u + kAhead, wv[q], dv[q]);
-                settle(nj);
+                settle(nj, std::integral_constant<int, kSettleSecond>());
                 said = (uint32_t)__builtin_amdgcn_readfirstlane(any) == k + q + 1;
                 staged();
             }
@@ -407,47 +409,49 @@ __global__ __launch_bounds__(RS * KS * 64, RS * KS >= 16 ? 4 : 2) void gemm_q4_k
 }
 
 // A launch's tile: 16 mt vectors by `tiles` weight tiles (at most nj for each of
-// rs waves), ks groups of columns.
+// rs waves), ks groups of columns; waves a SIMD.
 struct Shape {
     int mt, nj, rs, ks;
     uint32_t tiles;
+    int waves = 2;
 };
 template <int FMT>
 const void* fn_of(const Shape& t) {
-    if (t.mt == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 4, 2, 8, 1>);
-    if (t.mt == 2 && t.ks == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 1, 8, 2>);
-    if (t.mt == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 2, 8, 1>);
-    if (t.ks == 8) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 1, 8>);
-    if (t.ks == 4 && t.rs == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 2, 4>);
-    if (t.ks == 4 && t.nj == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 4>);
-    if (t.ks == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 4, 4>);
-    if (t.ks == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 2>);
-    return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 1>);
+    if (t.mt == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 4, 2, 8, 1, 2>);
+    if (t.mt == 2 && t.ks == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 1, 8, 2, 4>);
+    if (t.mt == 2 && t.waves == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 2, 8, 1, 2>);
+    if (t.mt == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 2, 2, 8, 1, 4>);
+    if (t.ks == 8) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 1, 8, 2>);
+    if (t.ks == 4 && t.rs == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 2, 4, 2>);
+    if (t.ks == 4 && t.nj == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 4, 4>);
+    if (t.ks == 4) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 1, 4, 4, 4>);
+    if (t.ks == 2) return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 2, 2>);
+    return reinterpret_cast<const void*>(&gemm_q4_kernel<FMT, 1, 2, 4, 1, 2>);
 }
 
 // By the number of 16 x 16 tiles of the result. Few: up to a workgroup per CU with
 // four groups of columns and two or four tiles (or eight groups, where rows are long
 // and one tile makes enough workgroups). {1,1,1,8} / {1,1,2,4} / {1,1,4,4}, us:
-// [768 x 8192] times 64 (192 tiles) 16.1 / 19.7 / 23.3, [2048 x 2560] times 20 (256) 8.9 /
-// 8.7 / 10.0, times 64 (512) 13.1 / 8.9 / 10.1, times 100 (896) - / 12.6 / 10.4,
-// [3840 x 768] times 32 (480) 8.1 / 5.9 / 6.6.
+// [768 x 8192] times 64 (192 tiles) 15.2 / 20.6 / 23.1, [2048 x 2560] times 20 (256) 8.3 /
+// 8.6 / 9.9, times 64 (512) 14.8 / 8.7 / 9.9, times 100 (896) 27.2 / 12.7 / 10.0,
+// [3840 x 768] times 32 (480) 9.0 / 5.4 / 6.3.
 //
 // Then larger tiles and fewer groups. {1,1,4,4} / {1,2,4,2} / {2,1,8,2} / {2,2,8,1} /
-// {4,2,8,1}: [2048 x 2560] times 16 (128 tiles) 10.0 / 14.6 / 18.7 / 29.0 / 48, times 128 (1024)
-// 10.6 / 15.2 / 19.0 / 30.3 / 50, times 256 (2048) 19.0 / 15.6 / 19.2 / 30.3 / 51; [3840 x
-// 768] times 256 (3840) 21.7 / 10.2 / 9.3 / 12.2 / 19.0; [10240 x 2048] times 64 (2560)
-// 23.9 / 18.8 / 16.4 / 25.2 / 41, times 256 (10240) 75 / 42.4 / 45.6 / 39.8 / 33.9.
+// {4,2,8,1}: [2048 x 2560] times 128 (1024 tiles) 10.5 / 14.9 / 19.7 / 30.0 / 34.6, times
+// 256 (2048) 18.7 / 15.1 / 19.9 / 30.2 / 34.9; [3840 x 768] times 256 (3840) 20.5 / 10.0 /
+// 9.3 / 12.0 / 13.9; [10240 x 2048] times 64 (2560) 23.0 / 18.3 / 16.8 / 25.0 / 29.1, times
+// 256 (10240) 72 / 42.7 / 46.9 / 40.2 / 33.3.
 // Between four and eight tiles per CU {1,2,4,4} is ahead of {1,2,4,2} where rows are
-// long: [3840 x 2048] times 77 11.7 / 12.8, [1536 x 4096] times 256 18.7 / 21.6, but [5120
-// x 1664] times 64 13.9 / 12.9.
+// long: [3840 x 2048] times 77 11.7 / 12.5, [1536 x 4096] times 256 19.7 / 21.7, but [5120
+// x 1664] times 64 11.6 / 11.4.
 //
 // Many: the two largest tiles by what they cost, rounds of one workgroup per CU
 // times a round's time, in hundredths of a microsecond a unit (fitted to the above
-// and: times 128 25.6 / 28.8, times 512 61.6 / 66.4; [3840 x 768] times 512 13.0 /
-// 14.7, {2,2,8,1} before {4,2,8,1}). The largest takes as many weight tiles as cost
+// and, {2,2,8,1} before {4,2,8,1}: times 128 25.4 / 29.5, times 512 61.9 / 63.6; [3840 x
+// 768] times 512 12.7 / 14.7). The largest takes as many weight tiles as cost
 // least: a SIMD's two waves have a quarter of them. Up to 32 vectors leave it no
 // choice, and up to 16 the smallest tile is ahead: [154880 x 2048] times 16 {1,2,4,1}
-// 51, {1,2,4,2} 55, {2,2,8,1} 66; times 32 86 / 92 / 74.
+// 50, {1,2,4,2} 54, {2,2,8,1} 67; times 32 84, 91, 72.
 Shape shape_of(uint32_t tiles, uint32_t units, uint32_t batch, uint32_t cus) {
     const uint64_t results = (uint64_t)tiles * ((batch + 15) / 16);
     if (results <= cus && units >= 32) return Shape{1, 1, 1, 8, 1};
@@ -459,7 +463,9 @@ Shape shape_of(uint32_t tiles, uint32_t units, uint32_t batch, uint32_t cus) {
     const auto rounds = [&](uint32_t t, uint32_t vecs) {
         return ((uint64_t)((tiles + t - 1) / t) * ((batch + vecs - 1) / vecs) + cus - 1) / cus;
     };
-    Shape best{2, 2, 8, 1, 16};
+    // (In a second round a CU has room for two workgroups: [10240 x 2048] times 512 61.8
+    // us, with one 72.8; times 128, one round, 26.8 and 25.4.)
+    Shape best{2, 2, 8, 1, 16, rounds(16, 32) > 1 ? 4 : 2};
     uint64_t least = 30 + 110 * rounds(16, 32);
     for (uint32_t t = 16; t >= 8 && batch > 32; --t) {
         const uint64_t cost = rounds(t, 64) * (70 + 42 * ((t + 3) / 4));
