@@ -405,9 +405,11 @@ int qmm_quantised(mmhip_ctx* ctx, const mmhip_weight* w, uint64_t mat, const flo
         // One launch reading the f32 activations (qbuf unused): as the decode kernel
         // takes them, four vectors to a reading of the weights, or on the f16 matrix
         // cores. The first is ahead up to two workgroups per CU, one where rows are
-        // short: [768 x 2048] times 16 vectors 5.6 us against 7.5, times 40 7.3 against
-        // 7.6, times 64 (beyond) 10.2 against 7.5; [2048 x 2560] times 16 7.8 against 8.7;
-        // [3840 x 768] times 8 (beyond) 6.2 against 5.7.
+        // short: [768 x 2048] times 16 vectors 5.7 us against 7.4, times 40 7.4 against
+        // 7.5, times 64 (beyond) 10.3 against 7.5; with two workgroups per CU [2048 x 2560]
+        // times 16 7.9 against 8.6, [2048 x 1536] 6.5 both, [2048 x 1024] 6.4 against 5.4; with
+        // one [1024 x 1280] times 16 5.2 against 6.4, [3840 x 768] times 4 4.9 against 5.4,
+        // times 8 (beyond) 6.3 against 5.4.
         const uint64_t y_slot = out_layout == 0 ? ld : 1, y_row = out_layout == 0 ? 1 : ld;
         TimedLaunch tl(timed ? ctx : nullptr, "qmm");
         const uint64_t in_fours = (batch + 3) / 4;

@@ -13,15 +13,15 @@
 // multiply-add per output with the block's scale.
 //
 // Bound: vector instructions (per value of x two conversions, per eight weights
-// 9 or 21 operations, per output and block one multiply-add) beside the matrix
-// cores. A workgroup's waves share the x tile in LDS: each converts its part of
+// 9 or 21 operations, per output and block one multiply-add), matrix cores and LDS
+// together: of a large prompt's time they take 46, 34 and 47 hundredths. A workgroup's waves share the x tile in LDS: each converts its part of
 // the next 64 columns while the matrix cores work on the last ones, and a wave
 // unpacks weights of its own rows straight from their records. Waves may also
 // split the columns (KS groups), their sums added at the end.
 //
-// Measured: [10240 x 2048] times 256 vectors 33.4 us (321 Tflop/s of products; the
+// Measured: [10240 x 2048] times 256 vectors 33.0 us (325 Tflop/s of products; the
 // two matrix instructions per product alone would take 17 us), [3840 x 768] times
-// 77 vectors 7.4 us; with bf16 parts (three instructions per product, four
+// 77 vectors 7.5 us; with bf16 parts (three instructions per product, four
 // conversions) 74 and 10.9 us.
 #include <type_traits>
 
@@ -288,8 +288,8 @@ __global__ __launch_bounds__(RS * KS * 64, WAVES) void gemm_q4_kernel(GemmQ4Args
         else lds_barrier();
     };
     // Sums that the compiler does not put off beyond a branch, where a wave's products
-    // would not fit the registers otherwise: [10240 x 2048] times 256 33.4 us, without them
-    // 34.7; times 512 with four waves a SIMD 61.8 and 107.
+    // would not fit the registers otherwise: [10240 x 2048] times 256 33.0 us, without them
+    // 34.3; times 512 with four waves a SIMD 61.8 and 107.
     constexpr int kSettleFirst = MT >= 4 ? 1 : MT * NJ == 4 && WAVES == 4 ? 2 : 0, kSettleSecond = MT >= 4 ? 1 : 0;
     const auto settle = [&](auto nj, auto count) {
 #pragma unroll

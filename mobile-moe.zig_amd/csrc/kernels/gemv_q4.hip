@@ -15,8 +15,9 @@
 // contiguous part, with the next steps' loads in flight. Tiles that two waves
 // share are joined in wave order, so the result does not depend on timing.
 // Measured: 64 IQ4_NL matrices of [1536 x 2048], one vector each, 21.0 us (5.4
-// TB/s); Q4_0 [154880 x 2048] times four vectors 32.3 us (5.6 TB/s); [768 x 2048]
-// times one 4.1 us, a launch's time.
+// TB/s); [154880 x 2048] times four vectors 32.1 us (5.6 TB/s), in IQ4_NL, whose
+// lookups take more instructions than Q4_0's unpacking, 38.1 (4.8); times one 29.2 and
+// 31.7; [768 x 2048] times one 4.1 us, a launch's time.
 #include "device_common.hpp"
 #include "gemm_tile_ops.hpp"
 #include "kernels.hpp"
